@@ -74,7 +74,8 @@ PLA_API const char* pla_status_string(int status);
 PLA_API const char* pla_last_cuda_error(void);
 
 /* Library ABI version: (major << 16) | minor.  1.1 added pla_depthwise_forward,
- * 1.2 pla_depthwise7x7_layernorm_nhwc, 1.3 pla_depthwise7x7_forward_many. */
+ * 1.2 pla_depthwise7x7_layernorm_nhwc, 1.3 pla_depthwise7x7_forward_many, 1.4 the
+ * sequence operators. */
 PLA_API int pla_version(void);
 
 /*
@@ -298,6 +299,168 @@ PLA_API int pla_stencil7x7_band_step_halo(const void* in, const float* taps, con
                                           unsigned int* flags, unsigned int* up_flags,
                                           unsigned int* down_flags, unsigned int* counters,
                                           unsigned int step, pla_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Sequence operators: the layers of a sequence block built from the same
+ * pieces as above (depthwise convolution, fused norm, a state updated
+ * linearly).  No reference counterpart.  dtype is f32 / bf16 / f16; sums,
+ * norms and states are fp32.  Strides are in elements; the innermost
+ * dimension is dense.  Outputs are dense and must not overlap an input.
+ *
+ * A ragged batch is one batch row (batch == 1) of `tokens` tokens cut by
+ * cu_seqlens, an int32 device array of sequences + 1 ascending entries that
+ * starts at 0: sequence i holds tokens [cu_seqlens[i], cu_seqlens[i + 1]).
+ * Entries are clamped to [0, tokens] on the device, so wrong ones give wrong
+ * results but touch nothing outside the tensors.  Output rows that belong to
+ * no sequence are zero.  cu_seqlens NULL: every batch row is one sequence
+ * (sequences == batch).
+ * ------------------------------------------------------------------------ */
+
+/*
+ * Causal depthwise convolution along time, channels last:
+ *     p[t] = b + sum_{j < taps} w[c, j] x[t - taps + 1 + j],  taps in 2..4
+ *     y[t] = silu ? p[t] / (1 + e^-p[t]) : p[t].
+ * x [batch, tokens, channels]; w [channels, taps]; b [channels] or NULL.
+ * state_in [sequences, taps - 1, channels] holds the inputs before each
+ * sequence, oldest first (NULL: zeros); state_out, if not NULL, receives the
+ * last taps - 1 inputs (it may not be state_in).
+ */
+typedef struct pla_causal {
+  const void* x;
+  int64_t x_batch, x_token;
+  const void* w;
+  const void* b;
+  const int* cu_seqlens;
+  const void* state_in;
+  void* state_out;
+  void* y;
+  int batch, tokens, channels, taps, sequences, silu, dtype;
+} pla_causal;
+PLA_API int pla_causal_depthwise_forward(const pla_causal* a, pla_stream_t stream);
+
+/*
+ * Gradients of pla_causal_depthwise_forward (a->y and a->state_out unused):
+ * dx (dense) from dy and, if not NULL, dstate_out; dw, db and dstate_in each
+ * if not NULL.  workspace holds pla_causal_depthwise_workspace(a) bytes,
+ * 16-byte aligned, needed when dw or db is wanted.  No atomics: the same
+ * inputs give the same bits.
+ */
+typedef struct pla_causal_gradient {
+  const void* dy;
+  int64_t dy_batch, dy_token;
+  const void* dstate_out;
+  void* dx;
+  void* dw;
+  void* db;
+  void* dstate_in;
+  void* workspace;
+  size_t workspace_bytes;
+} pla_causal_gradient;
+PLA_API size_t pla_causal_depthwise_workspace(const pla_causal* a);
+PLA_API int pla_causal_depthwise_backward(const pla_causal* a, const pla_causal_gradient* g, pla_stream_t stream);
+
+/* One more token for each of n sequences: x [n, channels] (row stride x_row),
+ * state [n, taps - 1, channels] (row stride state_row) moved up in place, y
+ * dense. */
+PLA_API int pla_causal_depthwise_step(const void* x, int64_t x_row, void* state, int64_t state_row, const void* w,
+                                      const void* b, void* y, int n, int channels, int taps, int silu, int dtype,
+                                      pla_stream_t stream);
+
+/*
+ * Norm of queries and keys for each head, then the position rotation, in one
+ * pass: n = x w / sqrt(mean(x^2) + eps) (l2 == 0) or x w / sqrt(sum(x^2) +
+ * eps) (l2 == 1; w usually NULL); the first `rot` features are rotated in
+ * pairs (a, b) -> (a c - b s, b c + a s) with c, s from row m of the fp32
+ * tables cos_table / sin_table [table_rows, rot / 2] (NULL: no rotation),
+ * pairs (2i, 2i + 1) if interleaved, else (i, i + rot / 2).  m is the token's
+ * entry of `positions` ([batch, tokens], 4- or 8-byte integers, row stride
+ * position_batch) or, if NULL, its number.  A position outside the tables
+ * reads nothing and makes the rotated features NaN.  dim <= 256, rot even.
+ */
+typedef struct pla_norm_side {
+  const void* x; /* [batch, tokens, heads, dim] */
+  int64_t x_batch, x_token, x_head;
+  const void* w; /* [dim] or NULL */
+  void* y;       /* dense; backward: the gradient of x */
+  const void* dy; /* backward */
+  int64_t dy_batch, dy_token, dy_head;
+  void* dw;      /* backward: [dim] or NULL */
+  int heads;
+} pla_norm_side;
+typedef struct pla_qk_norm {
+  pla_norm_side q, k;
+  const float* cos_table;
+  const float* sin_table;
+  const void* positions;
+  int64_t position_batch;
+  int position_bytes, table_rows, batch, tokens, dim, rot, interleaved, l2;
+  float eps;
+  int dtype;
+} pla_qk_norm;
+PLA_API int pla_qk_norm_rotate_forward(const pla_qk_norm* a, pla_stream_t stream);
+/* workspace: pla_qk_norm_rotate_workspace(a) bytes, needed when a dw is wanted. */
+PLA_API size_t pla_qk_norm_rotate_workspace(const pla_qk_norm* a);
+PLA_API int pla_qk_norm_rotate_backward(const pla_qk_norm* a, void* workspace, size_t workspace_bytes,
+                                        pla_stream_t stream);
+
+/*
+ * Gated delta rule: per value head h (key head h / (hv / hk)) the state
+ * S [dk, dv] starts as state_in[sequence, h] (fp32, NULL: zeros) and follows
+ *     S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q.
+ * q, k [batch, tokens, hk, dk]; v [batch, tokens, hv, dv]; g, beta [batch,
+ * tokens, hv], both of dtype or both fp32 (gates32); o dense like v;
+ * state_out [sequences, hv, dk, dv] fp32 or NULL.  dk, dv <= 128, hv a
+ * multiple of hk.  It is stable for |k| up to about 1 and beta in [0, 2]; a g
+ * below -200 is taken as -200 (its decay is 0 in fp32 either way).
+ * workspace: pla_gated_delta_rule_workspace(a, 0) bytes, 256-byte aligned.
+ */
+typedef struct pla_delta {
+  const void *q, *k, *v, *g, *beta;
+  int64_t q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head;
+  int64_t g_batch, g_token, g_head, beta_batch, beta_token, beta_head;
+  const int* cu_seqlens;
+  const float* state_in;
+  float* state_out;
+  void* o;
+  int batch, tokens, sequences, hk, hv, dk, dv, gates32, dtype;
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+} pla_delta;
+PLA_API size_t pla_gated_delta_rule_workspace(const pla_delta* a, int backward);
+PLA_API int pla_gated_delta_rule_forward(const pla_delta* a, pla_stream_t stream);
+
+/*
+ * Gradients of pla_gated_delta_rule_forward (a->o and a->state_out unused;
+ * the chunks' states are computed again): from d_o and, if not NULL,
+ * dstate_out, all of dq, dk, dv, dg, dbeta (dense, of their input's type) and,
+ * if not NULL, dstate_in.  workspace: pla_gated_delta_rule_workspace(a, 1).
+ */
+typedef struct pla_delta_gradient {
+  const void* d_o;
+  int64_t do_batch, do_token, do_head;
+  const float* dstate_out;
+  float* dstate_in;
+  void *dq, *dk, *dv, *dg, *dbeta;
+} pla_delta_gradient;
+PLA_API int pla_gated_delta_rule_backward(const pla_delta* a, const pla_delta_gradient* g, pla_stream_t stream);
+
+/*
+ * One more token for each of n sequences, the state updated in place:
+ * q, k [n, hk, dk], v [n, hv, dv], g, beta [n, hv], state [n, hv, dk, dv]
+ * fp32 (state_row elements between sequences), o [n, hv, dv] dense.
+ * dk <= 256, dv any.
+ */
+typedef struct pla_delta_step {
+  const void *q, *k, *v, *g, *beta;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, g_row, g_head, beta_row, beta_head;
+  float* state;
+  int64_t state_row;
+  void* o;
+  int n, hk, hv, dk, dv, gates32, dtype;
+  float scale;
+} pla_delta_step;
+PLA_API int pla_gated_delta_rule_step(const pla_delta_step* a, pla_stream_t stream);
 
 /* CUDA IPC: export a device pointer as (64-byte handle of its allocation,
  * byte offset), import it in another process (peer access enabled lazily),

@@ -50,6 +50,17 @@ SIGNATURES = {
     "pla_ipc_export": ([_vp, _vp, ctypes.POINTER(ctypes.c_uint64)], _i32),
     "pla_ipc_import": ([_vp, ctypes.c_uint64, ctypes.POINTER(ctypes.c_void_p)], _i32),
     "pla_ipc_close": ([_vp, ctypes.c_uint64], _i32),
+    "pla_causal_depthwise_forward": ([_vp, _vp], _i32),
+    "pla_causal_depthwise_workspace": ([_vp], ctypes.c_size_t),
+    "pla_causal_depthwise_backward": ([_vp, _vp, _vp], _i32),
+    "pla_causal_depthwise_step": ([_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp], _i32),
+    "pla_qk_norm_rotate_forward": ([_vp, _vp], _i32),
+    "pla_qk_norm_rotate_workspace": ([_vp], ctypes.c_size_t),
+    "pla_qk_norm_rotate_backward": ([_vp, _vp, ctypes.c_size_t, _vp], _i32),
+    "pla_gated_delta_rule_workspace": ([_vp, _i32], ctypes.c_size_t),
+    "pla_gated_delta_rule_forward": ([_vp, _vp], _i32),
+    "pla_gated_delta_rule_backward": ([_vp, _vp, _vp], _i32),
+    "pla_gated_delta_rule_step": ([_vp, _vp], _i32),
     "pla_read_device_faults": ([_u32p], _i32),
     "pla_clear_device_faults": ([], _i32),
 }
@@ -59,6 +70,46 @@ class DwProblem(ctypes.Structure):
 
     _fields_ = [("x", ctypes.c_void_p), ("w", ctypes.c_void_p), ("b", ctypes.c_void_p), ("y", ctypes.c_void_p),
                 ("n", ctypes.c_int), ("c", ctypes.c_int), ("h", ctypes.c_int), ("width", ctypes.c_int)]
+
+
+def _fields(pointers="", strides="", ints="", floats="", sizes=""):
+    return ([(n, ctypes.c_void_p) for n in pointers.split()], [(n, ctypes.c_int64) for n in strides.split()],
+            [(n, ctypes.c_int) for n in ints.split()], [(n, ctypes.c_float) for n in floats.split()],
+            [(n, ctypes.c_size_t) for n in sizes.split()])
+
+
+def _struct(name, doc, *groups):
+    """A C struct of include/pla_b200.h: groups of fields in the header's order."""
+    return type(name, (ctypes.Structure,), {"__doc__": doc, "_fields_": [f for g in groups for part in g for f in part]})
+
+
+Causal = _struct("Causal", "pla_causal", _fields("x", "x_batch x_token"),
+                 _fields("w b cu_seqlens state_in state_out y", "", "batch tokens channels taps sequences silu dtype"))
+CausalGradient = _struct("CausalGradient", "pla_causal_gradient", _fields("dy", "dy_batch dy_token"),
+                         _fields("dstate_out dx dw db dstate_in workspace", sizes="workspace_bytes"))
+NormSide = _struct("NormSide", "pla_norm_side", _fields("x", "x_batch x_token x_head"),
+                   _fields("w y dy", "dy_batch dy_token dy_head"), _fields("dw", "", "heads"))
+
+
+class QkNorm(ctypes.Structure):
+    """pla_qk_norm"""
+
+    _fields_ = [("q", NormSide), ("k", NormSide), ("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p), ("position_batch", ctypes.c_int64)] + [
+                    (n, ctypes.c_int) for n in ("position_bytes", "table_rows", "batch", "tokens", "dim", "rot",
+                                                "interleaved", "l2")] + [("eps", ctypes.c_float), ("dtype", ctypes.c_int)]
+
+
+Delta = _struct("Delta", "pla_delta",
+                _fields("q k v g beta", "q_batch q_token q_head k_batch k_token k_head v_batch v_token v_head "
+                        "g_batch g_token g_head beta_batch beta_token beta_head"),
+                _fields("cu_seqlens state_in state_out o", "", "batch tokens sequences hk hv dk dv gates32 dtype", "scale"),
+                _fields("workspace", sizes="workspace_bytes"))
+DeltaGradient = _struct("DeltaGradient", "pla_delta_gradient", _fields("d_o", "do_batch do_token do_head"),
+                        _fields("dstate_out dstate_in dq dk dv dg dbeta"))
+DeltaStep = _struct("DeltaStep", "pla_delta_step",
+                    _fields("q k v g beta", "q_row q_head k_row k_head v_row v_head g_row g_head beta_row beta_head"),
+                    _fields("state", "state_row"), _fields("o", "", "n hk hv dk dv gates32 dtype", "scale"))
 
 
 _lib = None

@@ -6,17 +6,19 @@
   (include/pla_b200.h).  nvcc cross-compiles without a GPU; this is what the
   Python package and any C/C++ host load.
 * ``libpla_b200_torch.so``: the torch custom ops (``torch.ops.pla_b200.*``,
-  csrc/torch_ops.cpp), plain C++ over that C ABI, compiled with g++ against
-  the installed torch's headers and linked to ``libpla_b200.so`` by rpath.
+  csrc/*.cpp), plain C++ over that C ABI, compiled with g++ against the
+  installed torch's headers and linked to ``libpla_b200.so`` by rpath.
 """
 from __future__ import annotations
 
 import argparse
+import concurrent.futures
 import glob
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -28,8 +30,8 @@ NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-    "-shared", "-Xlinker", "-soname=libpla_b200.so",
 ]
+LINK_FLAGS = ["-shared", "-Xlinker", "-soname=libpla_b200.so"]
 
 
 def _nvcc() -> str:
@@ -39,13 +41,22 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
+def units() -> list[str]:
+    """The CUDA translation units (compiled side by side, then linked)."""
+    return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
+
+
 def sources() -> list[str]:
-    return sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))
+    return sorted(units() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h"))
                   + [os.path.join(ROOT, "include", "pla_b200.h")])
 
 
+def torch_units() -> list[str]:
+    return sorted(glob.glob(os.path.join(CSRC, "*.cpp")))
+
+
 def torch_sources() -> list[str]:
-    return [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(ROOT, "include", "pla_b200.h")]
+    return torch_units() + [os.path.join(ROOT, "include", "pla_b200.h")]
 
 
 def up_to_date(out: str = OUT, srcs: list[str] | None = None) -> bool:
@@ -64,26 +75,37 @@ def _run(cmd: list[str], out: str, verbose: bool) -> None:
     os.replace(out + ".tmp", out)
 
 
-def torch_cmd() -> list[str]:
-    """g++ command for libpla_b200_torch.so (torch's headers, ABI flag and libraries)."""
+def _compile_units(cmd: list[str], srcs: list[str], where: str, verbose: bool) -> list[str]:
+    """One object per source under ``where``, the compilers running side by side."""
+    objs = [os.path.join(where, os.path.basename(s) + ".o") for s in srcs]
+    with concurrent.futures.ThreadPoolExecutor(len(srcs)) as pool:
+        for job in [pool.submit(_run, [*cmd, "-c", s, "-o", o + ".tmp"], o, verbose) for s, o in zip(srcs, objs)]:
+            job.result()
+    return objs
+
+
+def torch_cmds() -> tuple[list[str], list[str]]:
+    """g++ compile command and link flags of libpla_b200_torch.so (torch's headers, ABI flag and libraries)."""
     import torch
     from torch.utils import cpp_extension
 
     cuda_home = cpp_extension.CUDA_HOME or "/usr/local/cuda"
-    cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+    cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     cmd += [f"-I{p}" for p in cpp_extension.include_paths()] + [f"-I{os.path.join(cuda_home, 'include')}"]
-    cmd += ["-o", TORCH_OUT + ".tmp", os.path.join(CSRC, "torch_ops.cpp")]
-    cmd += [f"-L{p}" for p in cpp_extension.library_paths()] + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch"]
-    cmd += [f"-L{HERE}", "-lpla_b200", "-Wl,-rpath,$ORIGIN"]
-    return cmd
+    link = [f"-L{p}" for p in cpp_extension.library_paths()] + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch"]
+    return cmd, link + [f"-L{HERE}", "-lpla_b200", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if force or not up_to_date():
-        _run([_nvcc(), *NVCC_FLAGS, "-o", OUT + ".tmp", os.path.join(CSRC, "pla_capi.cu")], OUT, verbose)
-    if force or not up_to_date(TORCH_OUT, torch_sources() + [OUT]):
-        _run(torch_cmd(), TORCH_OUT, verbose)
+    with tempfile.TemporaryDirectory(prefix="pla_b200_build_") as where:
+        if force or not up_to_date():
+            objs = _compile_units([_nvcc(), *NVCC_FLAGS], units(), where, verbose)
+            _run([_nvcc(), *NVCC_FLAGS, *LINK_FLAGS, "-o", OUT + ".tmp", *objs], OUT, verbose)
+        if force or not up_to_date(TORCH_OUT, torch_sources() + [OUT]):
+            cmd, link = torch_cmds()
+            objs = _compile_units(cmd, torch_units(), where, verbose)
+            _run([cmd[0], "-shared", "-o", TORCH_OUT + ".tmp", *objs, *link], TORCH_OUT, verbose)
     return OUT
 
 

@@ -1,0 +1,262 @@
+// Gated delta rule: what its kernels share.
+//
+// A head's state S [Dk, Dv] follows, token by token,
+//     S <- e^g S,   u = beta (v - S^T k),   S <- S + k u^T,   o = scale S^T q.
+// Over a chunk of 64 tokens, with G the running sum of g, the same is
+//     M_ij = e^{G_i - G_j} k_i . k_j (i > j)     P_ij = e^{G_i - G_j} q_i . k_j (i >= j)
+//     X = beta (V - e^G (K S0))                  U = T X,  T = (1 + diag(beta) M)^-1
+//     O = scale (e^G (Q S0) + P U)               S = e^{G_C} S0 + K^T (e^{G_C - G} U),
+// which turns 64 dependent steps into matrix products.  delta_prepare builds
+// T and P of every chunk in parallel; delta_sweep walks the chunks of a
+// sequence with S in registers.
+//
+// Products run on the tensor cores in fp16 with fp32 accumulators.  An fp32
+// operand is split into planes, hi = fp16(x f), lo = fp16(x f - hi), after
+// multiplying by a power of two f that brings its row's largest value near
+// 2^12: f is exact, nothing overflows whatever the inputs' range, and hi + lo
+// keep 22 bits of a value (values 2^-26 below the row's largest keep fewer,
+// with an error below 2^-38 of the largest).  16-bit inputs fit one plane: a
+// bfloat16 has 8 bits, so only values 2^-22 below the row's largest lose any.
+// Products of two lo planes are below 2^-22 and left out.  bf16 planes would
+// need three of them for the same precision.
+#pragma once
+
+#include "seq_common.cuh"
+
+namespace pla {
+namespace seq {
+
+constexpr int kChunk = 64;
+
+// Per-chunk, per-head coefficients over the chunk's tokens (rows of 64 floats).
+enum DeltaCoef {
+  kBeta = 0,   // beta
+  kDown = 1,   // beta e^G f_k: weight of K S0 in X
+  kTail = 2,   // e^{G_C - G} f_k: weight of U in the state's update
+  kTRow = 3,   // scale of the rows of T's planes
+  kOutQ = 4,   // scale e^G f_q: weight of Q S0 in O
+  kOutP = 5,   // scale * scale of the rows of P's planes
+  kSumHi = 6,  // G as an unevaluated sum of two floats
+  kSumLo = 7,
+  kKRow = 8,   // f_k, f_q: what a row of the K / Q planes is to be multiplied by
+  kQRow = 9,
+  kDecay = 10, // e^{G_C} in every place
+  kCoefs = 11
+};
+
+struct DeltaParams {
+  const void *q, *k, *v, *g, *beta;
+  long long q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head;
+  long long g_batch, g_token, g_head, beta_batch, beta_token, beta_head;
+  const int* cu;
+  const float* state_in;
+  float* state_out;
+  void* o;  // dense
+  int batch, tokens, sequences, hk, hv, dk, dv, gates32;
+  float scale;
+  int row_chunks;    // dense: chunks of a batch row
+  int chunk_bound;   // chunks the workspace has room for
+  int* plan;         // ragged: lo [N], len [N], first chunk [N + 1]
+  char* tiles;       // K, Q planes of every (chunk, key head)
+  char* heads;       // T, P planes and coefficients of every (chunk, value head)
+  float* states;     // backward: S at every chunk's start, fragment order
+  float* us;         // backward: U
+  // backward
+  const void* d_o;
+  long long do_batch, do_token, do_head;
+  const float* dstate_out;
+  float* dstate_in;
+  float* dstates;    // dS at every chunk's end, fragment order
+  float* dxs;        // dX
+  void *dq, *dk_out, *dv_out, *dg, *dbeta;
+  int slabs;         // ceil(dv / 16)
+  int vec_qk, vec_v, vec_o, vec_do;
+};
+
+struct ChunkAt {
+  int sequence, batch, token, len;  // first token and number of tokens
+};
+
+__device__ __forceinline__ bool chunk_at(const DeltaParams& p, int chunk, ChunkAt* c) {
+  if (!p.cu) {
+    c->sequence = c->batch = chunk / p.row_chunks;
+    c->token = (chunk % p.row_chunks) * kChunk;
+    c->len = min(kChunk, p.tokens - c->token);
+    return true;
+  }
+  const int n = p.sequences;
+  const int s = find_sequence(p.plan + 2 * n, n, chunk);
+  if (s < 0) return false;
+  const int at = (chunk - p.plan[2 * n + s]) * kChunk;
+  c->sequence = s;
+  c->batch = 0;
+  c->token = p.plan[s] + at;
+  c->len = min(kChunk, p.plan[n + s] - at);
+  return true;
+}
+
+// Ragged batches: first token, length and first chunk of every sequence.  A
+// running maximum over the clamped entries keeps sequences in order and apart
+// whatever cu_seqlens holds, so their chunks never exceed tokens / 64 + N.
+__global__ void __launch_bounds__(1024) delta_plan(const int* cu, int tokens, int n, int* plan) {
+  __shared__ int scan[1024];
+  __shared__ int carry_max, carry_sum;
+  const int i = threadIdx.x;
+  if (i == 0) {
+    carry_max = clamp_token(cu[0], tokens);
+    carry_sum = 0;
+  }
+  __syncthreads();
+  for (int base = 0; base < n; base += 1024) {
+    const int s = base + i;
+    scan[i] = s < n ? clamp_token(cu[s + 1], tokens) : 0;
+    __syncthreads();
+    for (int o = 1; o < 1024; o <<= 1) {
+      const int v = i >= o ? scan[i - o] : 0;
+      __syncthreads();
+      scan[i] = max(scan[i], v);
+      __syncthreads();
+    }
+    const int hi = max(scan[i], carry_max), lo = i ? max(scan[i - 1], carry_max) : carry_max;
+    __syncthreads();
+    const int chunks = s < n ? (hi - lo + kChunk - 1) / kChunk : 0;
+    scan[i] = chunks;
+    __syncthreads();
+    for (int o = 1; o < 1024; o <<= 1) {
+      const int v = i >= o ? scan[i - o] : 0;
+      __syncthreads();
+      scan[i] += v;
+      __syncthreads();
+    }
+    if (s < n) {
+      plan[s] = lo;
+      plan[n + s] = hi - lo;
+      plan[2 * n + s] = carry_sum + scan[i] - chunks;
+      if (s == n - 1) plan[3 * n] = carry_sum + scan[i];
+    }
+    __syncthreads();
+    if (i == 1023) {
+      carry_max = hi;
+      carry_sum += scan[i];
+    }
+    __syncthreads();
+  }
+}
+
+// ---- planes ----------------------------------------------------------------
+// Power of two that brings `largest` into [2^12, 2^13), and its inverse; both
+// finite for every input (zero, subnormal, infinite or NaN too).
+struct Pow2 {
+  float f, inverse;
+};
+__device__ __forceinline__ Pow2 pow2_for(float largest) {
+  int e = static_cast<int>((__float_as_uint(largest) >> 23) & 0xff);
+  e = min(max(e, 32), 240);  // f in [2^-101, 2^107]
+  return {__int_as_float((127 + 12 - e + 127) << 23), __int_as_float((e - 12) << 23)};
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// hi and, with two planes, lo of a pair of values that are already scaled.
+template <int PLANES>
+__device__ __forceinline__ void split(float a, float b, uint32_t* hi, uint32_t* lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  *hi = *reinterpret_cast<const uint32_t*>(&h);
+  if (PLANES > 1) {
+    const float2 back = __half22float2(h);
+    *lo = pack_half2(a - back.x, b - back.y);
+  }
+}
+
+__device__ __forceinline__ uint32_t shared_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// D += A B, A 16 x 16 row-major, B 16 x 8 column-major, fp16 with fp32 sums.
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at));
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at));
+}
+
+// Tiles of fp16 rows of W features (64 or 128): 16-byte units of a row are
+// permuted by the row number so that eight rows at one column, and one row's
+// neighbours, fall into different banks.
+template <int W>
+__device__ __forceinline__ uint32_t tile_at(int row, int unit) {
+  return static_cast<uint32_t>(row * W * 2 + ((unit ^ (row & 7)) << 4));
+}
+// B fragments of two 8-wide column tiles: B[k][n] = tile[n0 + n][k0 + k] ...
+template <int W>
+__device__ __forceinline__ uint32_t at_nk(int lane, int n0, int k0) {
+  const int m = lane >> 3;
+  return tile_at<W>(n0 + (m >> 1) * 8 + (lane & 7), (k0 >> 3) + (m & 1));
+}
+// ... or B[k][n] = tile[k0 + k][n0 + n] (transposing loads).
+template <int W>
+__device__ __forceinline__ uint32_t at_kn(int lane, int n0, int k0) {
+  const int m = lane >> 3;
+  return tile_at<W>(k0 + (m & 1) * 8 + (lane & 7), (n0 >> 3) + (m >> 1));
+}
+// A fragment (16 x 16): A[m][k] = tile[m0 + m][k0 + k].
+template <int W>
+__device__ __forceinline__ uint32_t at_mk(int lane, int m0, int k0) {
+  const int m = lane >> 3;
+  return tile_at<W>(m0 + (m & 1) * 8 + (lane & 7), (k0 >> 3) + (m >> 1));
+}
+
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+
+// e^(hi + lo), lo below half a unit of hi's last place.
+__device__ __forceinline__ float exp_sum(float hi, float lo) {
+  const float e = expf(hi);
+  return fmaf(e, lo, e);
+}
+
+// What the kernels of a type hold: planes of the inputs, of T and the states,
+// of P and the operands that only an output of the type sees.
+template <typename T>
+struct DeltaType {
+  static constexpr int kIn = sizeof(T) == 4 ? 2 : 1;
+  static constexpr int kState = 2;
+  static constexpr int kOut = 2;
+};
+template <>
+struct DeltaType<__nv_bfloat16> {
+  static constexpr int kIn = 1;
+  static constexpr int kState = 2;
+  // one fp16 plane adds an error of 2^-12 to results that are rounded by 2^-9
+  static constexpr int kOut = 1;
+};
+
+template <typename T, int DK>
+struct DeltaLayout {
+  static constexpr int kIn = DeltaType<T>::kIn;
+  static constexpr uint32_t kTile = kChunk * DK * 2;
+  static constexpr uint32_t kTiles = 2 * kIn * kTile;            // K planes, Q planes
+  static constexpr uint32_t kSquare = kChunk * kChunk * 2;
+  static constexpr uint32_t kT = DeltaType<T>::kState * kSquare;
+  static constexpr uint32_t kP = DeltaType<T>::kOut * kSquare;
+  static constexpr uint32_t kCoef = kCoefs * kChunk * 4;
+  static constexpr uint32_t kHead = kT + kP + kCoef;
+  static constexpr uint32_t kStage = kTiles + kHead;
+};
+
+}  // namespace seq
+}  // namespace pla

@@ -14,6 +14,7 @@
 #include "../../include/pla_b200.h"
 #include "cm_kernel.cuh"
 #include "generic_kernel.cuh"
+#include "host_shared.h"
 #include "nhwc_tile_kernel.cuh"
 #include "pair_kernel.cuh"
 #include "pla_common.cuh"
@@ -1050,6 +1051,15 @@ int dw_check(const void* x, const void* w, const void* y, int n, int c, int h, i
 }
 
 }  // namespace
+
+int record_cuda_error(cudaError_t e, const char* where) { return cuda_fail(e, where); }
+
+int current_sm100(int* sms) {
+  int st;
+  const DeviceInfo* d = device_info(&st);
+  if (d) *sms = d->sms;
+  return st;
+}
 }  // namespace pla
 
 using namespace pla;
@@ -1073,7 +1083,7 @@ const char* pla_last_cuda_error(void) { return g_last_cuda_error; }
 
 // 1.1: pla_depthwise_forward (k x k); 1.2: pla_depthwise7x7_layernorm_nhwc;
 // 1.3: pla_depthwise7x7_forward_many
-int pla_version(void) { return (1 << 16) | 3; }
+int pla_version(void) { return (1 << 16) | 4; }
 
 int pla_stencil7x7_forward(const void* x, const void* w, const void* b, void* y, int n, int h, int width,
                            int64_t sn, int64_t sh, int64_t sw, int dtype, pla_stream_t stream) {
@@ -1372,12 +1382,16 @@ int pla_ipc_close(void* ptr, uint64_t offset) {
 int pla_read_device_faults(unsigned int* faults) {
   if (!faults) return PLA_ERR_INVALID_ARGUMENT;
   PLA_CUDA(cudaMemcpyFromSymbol(faults, g_device_faults, sizeof(unsigned int)));
+  unsigned int more = 0;
+  PLA_CUDA(pla::sequence_faults(&more, false));
+  *faults |= more;
   return PLA_OK;
 }
 
 int pla_clear_device_faults(void) {
   const unsigned int zero = 0;
   PLA_CUDA(cudaMemcpyToSymbol(g_device_faults, &zero, sizeof(unsigned int)));
+  PLA_CUDA(pla::sequence_faults(nullptr, true));
   return PLA_OK;
 }
 

@@ -1,0 +1,334 @@
+// Norms of queries and keys for each head, with the position rotation in the
+// same pass.  For a head x of D features at position m:
+//     r = 1 / sqrt(sum x^2 / count + eps)     count = D (rms) or 1 (l2)
+//     n = x r w                               w = 1 without a weight
+//     the first `rot` features of n are rotated in pairs by the angle whose
+//     cosine and sine the tables hold at row m:
+//         (a, b) -> (a cos - b sin, b cos + a sin),
+//     pairs (2i, 2i + 1) or (i, i + rot / 2); the others pass through.
+// Backward, dn = dy rotated back:
+//     h = dn w,  dx = r (h - xhat sum(h xhat) / count),  xhat = x r,  dw = sum dn xhat.
+//
+// Bound by HBM: queries and keys are read and written once (backward: read
+// twice, written once), about 8 flops an element.  A group of 8, 16 or 32
+// lanes owns a head; a lane holds pairs in the layout the rotation needs, so
+// the partner is in the same lane and the sum of squares is the only exchange
+// (shuffles).  A group takes several heads of one token at a time: their loads
+// are in flight together and share the token's cosines and sines.  All
+// arithmetic is fp32 with one rounding at the end.
+#pragma once
+
+#include "seq_common.cuh"
+
+namespace pla {
+namespace seq {
+
+struct NormSide {
+  const void* x;
+  long long x_batch, x_token, x_head;
+  const void* w;  // [D] or nullptr
+  void* y;        // dense [batch, tokens, heads, D]; backward: the gradient of x
+  const void* dy;
+  long long dy_batch, dy_token, dy_head;
+  int heads;
+};
+
+struct NormParams {
+  NormSide side[2];        // queries, keys
+  const float* cos;        // [table_rows, rot / 2]; nullptr: no rotation
+  const float* sin;
+  const void* positions;   // [batch, tokens] (position_batch stride), nullptr: the token's number
+  long long position_batch;
+  int position_bytes;      // 4 or 8
+  int table_rows;
+  int batch, tokens, dim, rot, interleaved, l2;
+  float eps;
+  int units[2];            // groups of heads of a token, per side
+  float* partial;          // backward: [blocks of a side][D] twice, or nullptr
+  int side_blocks[2];
+};
+
+// A lane's NC chunks of CH pairs of a head's features.  CH = 4 needs rot / 2
+// and (D - rot) / 2 to be multiples of 4 and 16-byte rows; CH = 1 takes any D.
+template <int CH, int NC>
+struct PairMap {
+  int first[NC], second[NC];  // first feature of each chunk's a and b parts
+  bool turned[NC], there[NC], adjacent[NC], single[NC];
+  int angle[NC];
+  __device__ __forceinline__ PairMap(int lane, int lanes, int D, int rot, int interleaved) {
+    const int half = rot >> 1, rest = D - rot, rest_half = rest >> 1;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int p = (n * lanes + lane) * CH;  // pair number
+      turned[n] = p < half;
+      adjacent[n] = turned[n] && interleaved;
+      angle[n] = p;
+      const int q = p - half;
+      single[n] = CH == 1 && !turned[n] && q == rest_half && (rest & 1);
+      there[n] = turned[n] || q < rest_half || single[n];
+      first[n] = turned[n] ? (interleaved ? 2 * p : p) : (single[n] ? D - 1 : rot + q);
+      second[n] = turned[n] ? (interleaved ? 2 * p + CH : p + half) : rot + rest_half + q;
+    }
+  }
+};
+
+template <typename T, int CH>
+__device__ __forceinline__ void load_pairs(const T* x, int first, int second, bool adjacent, bool single, float (&a)[CH],
+                                           float (&b)[CH]) {
+  float f[CH], s[CH] = {};
+  load<T, CH>(x + first, f);
+  if (!single) load<T, CH>(x + (CH == 1 && adjacent ? first + 1 : second), s);
+  if (CH > 1 && adjacent) {  // 2 CH neighbours: even ones are a, odd ones b
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      a[i] = 2 * i < CH ? f[(2 * i) % CH] : s[(2 * i) % CH];
+      b[i] = 2 * i < CH ? f[(2 * i + 1) % CH] : s[(2 * i + 1) % CH];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) a[i] = f[i], b[i] = s[i];
+  }
+}
+
+template <typename T, int CH>
+__device__ __forceinline__ void store_pairs(T* y, int first, int second, bool adjacent, bool single, const float (&a)[CH],
+                                            const float (&b)[CH]) {
+  float f[CH], s[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    if (CH > 1 && adjacent) {
+      f[i] = i % 2 == 0 ? a[i / 2] : b[i / 2];
+      s[i] = i % 2 == 0 ? a[(CH + i) / 2] : b[(CH + i) / 2];
+    } else {
+      f[i] = a[i];
+      s[i] = b[i];
+    }
+  }
+  store<T, CH>(y + first, f);
+  if (!single) store<T, CH>(y + (CH == 1 && adjacent ? first + 1 : second), s);
+}
+
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Row of the tables for a token; -1 if the position is outside them.
+__device__ __forceinline__ long long table_row(const NormParams& p, int b, int t) {
+  long long m = t;
+  if (p.positions) {
+    const long long at = b * p.position_batch + t;
+    m = p.position_bytes == 8 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
+  }
+  return m >= 0 && m < p.table_rows ? m : -1;
+}
+
+// A position outside the tables reads nothing: its rotated features are NaN.
+template <int CH, int NC>
+__device__ __forceinline__ void load_angles(const NormParams& p, const PairMap<CH, NC>& map, int b, int t, float (&c)[NC][CH],
+                                            float (&s)[NC][CH]) {
+  const long long m = p.cos ? table_row(p, b, t) : 0;
+  const float nan = __int_as_float(0x7fc00000);
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) c[n][i] = map.turned[n] ? nan : 1.f, s[n][i] = map.turned[n] ? nan : 0.f;
+    if (map.turned[n] && m >= 0) {
+      load<float, CH>(p.cos + m * (p.rot >> 1) + map.angle[n], c[n]);
+      load<float, CH>(p.sin + m * (p.rot >> 1) + map.angle[n], s[n]);
+    }
+  }
+}
+
+constexpr int kNormThreads = 256;
+
+template <typename T, int CH, int NC, int LANES, int HB>
+__global__ void __launch_bounds__(kNormThreads) qk_norm_forward(NormParams p) {
+  const int lane = threadIdx.x % LANES;
+  const long long group = (static_cast<long long>(blockIdx.x) * kNormThreads + threadIdx.x) / LANES;
+  const int units = p.units[0] + p.units[1];
+  const long long token = group / units;
+  int unit = static_cast<int>(group % units);
+  const bool live = token < static_cast<long long>(p.batch) * p.tokens;  // whole groups: every lane still shuffles
+  const int b = live ? static_cast<int>(token / p.tokens) : 0, t = live ? static_cast<int>(token % p.tokens) : 0;
+  const int which = unit >= p.units[0];
+  if (which) unit -= p.units[0];
+  const NormSide& side = p.side[which];
+  const PairMap<CH, NC> map(lane, LANES, p.dim, p.rot, p.interleaved);
+  const T* x = static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token;
+  T* y = static_cast<T*>(side.y) + (static_cast<long long>(b) * p.tokens + t) * side.heads * p.dim;
+  const int h0 = unit * HB;
+
+  float xa[HB][NC][CH], xb[HB][NC][CH];
+#pragma unroll
+  for (int h = 0; h < HB; ++h)
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) xa[h][n][i] = xb[h][n][i] = 0.f;
+      if (live && h0 + h < side.heads && map.there[n])
+        load_pairs<T, CH>(x + (h0 + h) * side.x_head, map.first[n], map.second[n], map.adjacent[n], map.single[n],
+                          xa[h][n], xb[h][n]);
+    }
+  float c[NC][CH], s[NC][CH], wa[NC][CH], wb[NC][CH];
+  if (live) load_angles<CH, NC>(p, map, b, t, c, s);
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) wa[n][i] = wb[n][i] = 1.f;
+    if (side.w && map.there[n])
+      load_pairs<T, CH>(static_cast<const T*>(side.w), map.first[n], map.second[n], map.adjacent[n], map.single[n], wa[n],
+                        wb[n]);
+  }
+  const float per = p.l2 ? 1.f : 1.f / p.dim;
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int i = 0; i < CH; ++i) sum = fmaf(xa[h][n][i], xa[h][n][i], fmaf(xb[h][n][i], xb[h][n][i], sum));
+    const float r = 1.f / sqrtf(fmaf(group_sum<LANES>(sum), per, p.eps));
+    if (!live || h0 + h >= side.heads) continue;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      if (!map.there[n]) continue;
+      float oa[CH], ob[CH];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const float na = xa[h][n][i] * r * wa[n][i], nb = xb[h][n][i] * r * wb[n][i];
+        oa[i] = map.turned[n] ? fmaf(na, c[n][i], -nb * s[n][i]) : na;
+        ob[i] = map.turned[n] ? fmaf(nb, c[n][i], na * s[n][i]) : nb;
+      }
+      store_pairs<T, CH>(y + (h0 + h) * static_cast<long long>(p.dim), map.first[n], map.second[n], map.adjacent[n],
+                         map.single[n], oa, ob);
+    }
+  }
+}
+
+// dx, and the block's sums for dw: a group walks tokens of one side with dw
+// in registers, the groups of a block are added in shared memory, the blocks
+// in qk_norm_reduce, all in a fixed order.
+template <typename T, int CH, int NC, int LANES>
+__global__ void __launch_bounds__(kNormThreads) qk_norm_backward(NormParams p) {
+  constexpr int GROUPS = kNormThreads / LANES;
+  __shared__ float part[GROUPS][2 * CH * NC][LANES + 1];
+  const int lane = threadIdx.x % LANES, in_block = threadIdx.x / LANES;
+  const int which = static_cast<int>(blockIdx.x) >= p.side_blocks[0];
+  const NormSide& side = p.side[which];
+  const int block = which ? blockIdx.x - p.side_blocks[0] : blockIdx.x;
+  const PairMap<CH, NC> map(lane, LANES, p.dim, p.rot, p.interleaved);
+  float wa[NC][CH], wb[NC][CH], ga[NC][CH] = {}, gb[NC][CH] = {};
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) wa[n][i] = wb[n][i] = 1.f;
+    if (side.w && map.there[n])
+      load_pairs<T, CH>(static_cast<const T*>(side.w), map.first[n], map.second[n], map.adjacent[n], map.single[n], wa[n],
+                        wb[n]);
+  }
+  const float per = p.l2 ? 1.f : 1.f / p.dim;
+  const long long rows = static_cast<long long>(p.batch) * p.tokens * side.heads;
+  const long long step = static_cast<long long>(p.side_blocks[which]) * GROUPS;
+  // every group of the block makes the same number of turns: all lanes shuffle
+  for (long long base = static_cast<long long>(block) * GROUPS; base < rows; base += step) {
+    const long long row = base + in_block;
+    const bool live = row < rows;
+    const long long token = live ? row / side.heads : 0;
+    const int h = live ? static_cast<int>(row % side.heads) : 0;
+    const int b = static_cast<int>(token / p.tokens), t = static_cast<int>(token % p.tokens);
+    const T* x = static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token + h * side.x_head;
+    const T* dy = static_cast<const T*>(side.dy) + b * side.dy_batch + t * side.dy_token + h * side.dy_head;
+    float xa[NC][CH] = {}, xb[NC][CH] = {}, da[NC][CH] = {}, db[NC][CH] = {}, c[NC][CH], s[NC][CH];
+    if (live) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        if (map.there[n]) {
+          load_pairs<T, CH>(x, map.first[n], map.second[n], map.adjacent[n], map.single[n], xa[n], xb[n]);
+          load_pairs<T, CH>(dy, map.first[n], map.second[n], map.adjacent[n], map.single[n], da[n], db[n]);
+        }
+      load_angles<CH, NC>(p, map, b, t, c, s);
+    }
+    float square = 0.f, dot = 0.f;
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        if (live && map.turned[n]) {  // rotate back
+          const float ya = da[n][i], yb = db[n][i];
+          da[n][i] = fmaf(ya, c[n][i], yb * s[n][i]);
+          db[n][i] = fmaf(yb, c[n][i], -ya * s[n][i]);
+        }
+        square = fmaf(xa[n][i], xa[n][i], fmaf(xb[n][i], xb[n][i], square));
+        dot = fmaf(da[n][i] * wa[n][i], xa[n][i], fmaf(db[n][i] * wb[n][i], xb[n][i], dot));
+      }
+    square = group_sum<LANES>(square);
+    dot = group_sum<LANES>(dot);
+    if (!live) continue;
+    const float r = 1.f / sqrtf(fmaf(square, per, p.eps));
+    const float back = dot * r * r * per;  // sum(h xhat) r / count
+    T* dx = static_cast<T*>(side.y) + row * p.dim;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      if (!map.there[n]) continue;
+      float oa[CH], ob[CH];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        oa[i] = r * fmaf(-back, xa[n][i], da[n][i] * wa[n][i]);
+        ob[i] = r * fmaf(-back, xb[n][i], db[n][i] * wb[n][i]);
+        ga[n][i] = fmaf(da[n][i], xa[n][i] * r, ga[n][i]);
+        gb[n][i] = fmaf(db[n][i], xb[n][i] * r, gb[n][i]);
+      }
+      store_pairs<T, CH>(dx, map.first[n], map.second[n], map.adjacent[n], map.single[n], oa, ob);
+    }
+  }
+  if (!p.partial || !side.w) return;
+#pragma unroll
+  for (int n = 0; n < NC; ++n)
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      part[in_block][2 * (n * CH + i)][lane] = ga[n][i];
+      part[in_block][2 * (n * CH + i) + 1][lane] = gb[n][i];
+    }
+  __syncthreads();
+  if (in_block) return;
+  float* out = p.partial + static_cast<long long>(blockIdx.x) * p.dim;
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    if (!map.there[n]) continue;
+    float a[CH] = {}, b[CH] = {};
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        a[i] += part[g][2 * (n * CH + i)][lane];
+        b[i] += part[g][2 * (n * CH + i) + 1][lane];
+      }
+    store_pairs<float, CH>(out, map.first[n], map.second[n], map.adjacent[n], map.single[n], a, b);
+  }
+}
+
+// dw of one side: blocks' sums in eight interleaved parts, the parts pairwise.
+template <typename T>
+__global__ void __launch_bounds__(256) qk_norm_reduce(const float* partial, int blocks_q, int blocks_k, int dim, T* dwq, T* dwk) {
+  __shared__ float part[8][33];
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int d = blockIdx.x * 32 + lane;
+  const int blocks = blockIdx.y ? blocks_k : blocks_q;
+  const float* from = partial + (blockIdx.y ? static_cast<long long>(blocks_q) * dim : 0);
+  T* to = blockIdx.y ? dwk : dwq;
+  if (!to) return;
+  float sum = 0.f;
+  if (d < dim)
+    for (int i = row; i < blocks; i += 8) sum += from[static_cast<long long>(i) * dim + d];
+  part[row][lane] = sum;
+  __syncthreads();
+  if (row || d >= dim) return;
+  sum = ((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane])) +
+        ((part[4][lane] + part[5][lane]) + (part[6][lane] + part[7][lane]));
+  to[d] = down<T>(sum);
+}
+
+}  // namespace seq
+}  // namespace pla

@@ -1,0 +1,65 @@
+// Shared device helpers of the sequence operators (causal depthwise
+// convolution, query / key norm with rotation, gated delta rule).
+//
+// Tensors are addressed as base + batch * stride + token * stride + ..., with
+// 64-bit element offsets.  A ragged batch is one row of `tokens` tokens cut
+// by cu_seqlens[0 .. sequences]; the entries come from device memory, so the
+// kernels clamp them to [0, tokens] and never index by an unchecked one.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace pla {
+namespace seq {
+
+__device__ __forceinline__ float up(float v) { return v; }
+__device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float up(__half v) { return __half2float(v); }
+
+// One rounding to the nearest value of the output type.
+template <typename T> __device__ __forceinline__ T down(float v);
+template <> __device__ __forceinline__ float down<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 down<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half down<__half>(float v) { return __float2half_rn(v); }
+
+// V consecutive elements moved by one access (V * sizeof(T) <= 16 bytes, a power of two).
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T e[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ void load(const T* p, float (&f)[V]) {
+  const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = up(v.e[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&f)[V]) {
+  Vec<T, V> v;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v.e[i] = down<T>(f[i]);
+  *reinterpret_cast<Vec<T, V>*>(p) = v;
+}
+
+// 1 / (1 + e^-p).  16-bit results take the hardware exponential and divide
+// (relative error below 2^-20, their own rounding is 2^-12 at best).
+template <typename T> __device__ __forceinline__ float sigmoid(float p) { return __fdividef(1.f, 1.f + __expf(-p)); }
+template <> __device__ __forceinline__ float sigmoid<float>(float p) { return 1.f / (1.f + expf(-p)); }
+
+__device__ __forceinline__ int clamp_token(int v, int tokens) { return v < 0 ? 0 : (v > tokens ? tokens : v); }
+
+// The sequence a token belongs to: cu[i] <= t < cu[i + 1], by bisection; -1 if none.
+__device__ __forceinline__ int find_sequence(const int* cu, int sequences, int t) {
+  int lo = 0, hi = sequences;  // first index in (0, sequences] with cu > t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid + 1] > t) hi = mid; else lo = mid + 1;
+  }
+  return lo < sequences && cu[lo] <= t ? lo : -1;
+}
+
+}  // namespace seq
+}  // namespace pla

@@ -1,0 +1,110 @@
+"""Sequence operators: causal depthwise convolution, query / key norm with
+position rotation, gated delta rule, and the block that chains them.
+
+They are the layers of a delta-rule sequence block, built from the pieces the
+library has for images: a depthwise convolution (here along time), a norm
+fused to its neighbour (here over a head, with the rotation) and a linearly
+updated state.  No reference counterpart (the reference's operator is the
+depthwise convolution of data/depthwise_conv_7x7.py:15-29).
+
+* ``causal_depthwise()`` / ``causal_depthwise_step()``
+* ``qk_norm_rotate()``
+* ``gated_delta_rule()`` / ``gated_delta_rule_step()``
+* ``DeltaMixer``: projections, the three operators, output projection
+
+The first form of each runs over whole sequences, has a gradient, and takes
+ragged batches: ``cu_seqlens`` is an int32 CUDA vector of N + 1 ascending
+token offsets starting at 0 that cuts one batch row into N sequences (rows in
+no sequence come back zero).  ``state=`` is what precedes each sequence and
+``return_state=True`` also returns what follows it.  The ``_step`` forms
+advance every sequence by one token and update ``state`` in place; they have
+no gradient.
+
+Dtypes: float32, bfloat16, float16; sums, norms and delta-rule states are
+fp32.  Every call runs as ``torch.ops.pla_b200.*`` on the current stream and
+can be captured in a CUDA graph.  A CPU tensor raises: there is no fallback.
+A second derivative raises.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+
+def _cuda(t, op: str):
+    if not isinstance(t, torch.Tensor) or not (t.is_cuda or t.is_meta):
+        raise ValueError(f"{op} requires CUDA inputs")
+    return _lib.ops()
+
+
+def causal_depthwise(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, silu: bool = False,
+                     cu_seqlens: torch.Tensor | None = None, state: torch.Tensor | None = None,
+                     return_state: bool = False):
+    """``y[t] = act(bias + sum_j weight[:, j] * x[t - K + 1 + j])`` for x [B, T, C], weight [C, K] or [C, 1, K].
+
+    K is 2 to 4 taps; ``silu`` applies ``p * sigmoid(p)``.  ``state``
+    [N, K - 1, C] holds the inputs before each sequence, oldest first (zeros
+    if None).  Returns y, or (y, state after the sequences).  Differentiable
+    in x, weight, bias and state.
+    """
+    y, last = _cuda(x, "causal_depthwise").causal_depthwise.default(x, weight, bias, silu, cu_seqlens, state, return_state)
+    return (y, last) if return_state else y
+
+
+def causal_depthwise_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                          silu: bool = False) -> torch.Tensor:
+    """One token of ``causal_depthwise`` for x [N, C]; ``state`` [N, K - 1, C] moves up by one row in place."""
+    return _cuda(x, "causal_depthwise_step").causal_depthwise_step.default(x, state, weight, bias, silu)
+
+
+def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None = None,
+                   k_weight: torch.Tensor | None = None, cos: torch.Tensor | None = None,
+                   sin: torch.Tensor | None = None, positions: torch.Tensor | None = None, norm: str = "rms",
+                   eps: float = 1e-6, interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norm of every head of q [B, T, Hq, D] and k [B, T, Hk, D], then the rotation of its first features.
+
+    ``norm="rms"``: ``x / sqrt(mean(x^2) + eps) * weight``; ``norm="l2"``:
+    ``x / sqrt(sum(x^2) + eps) * weight``; weights [D] or None.  ``cos`` and
+    ``sin`` are float32 tables [P, R / 2]: the first R features are rotated in
+    pairs (i, i + R / 2), or (2i, 2i + 1) with ``interleaved``, by row
+    ``positions`` ([T], [1, T] or [B, T] integers; the token's number if
+    None).  A position outside the tables gives NaN in the rotated features.
+    D is at most 256.  Differentiable in q, k and the weights.
+    """
+    if norm not in ("rms", "l2"):
+        raise ValueError('norm must be "rms" or "l2"')
+    return _cuda(q, "qk_norm_rotate").qk_norm_rotate.default(q, k, q_weight, k_weight, cos, sin, positions, norm == "l2",
+                                                             eps, interleaved)
+
+
+def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                     scale: float | None = None, cu_seqlens: torch.Tensor | None = None,
+                     state: torch.Tensor | None = None, return_state: bool = False):
+    """Token by token, for every value head: ``S = exp(g) S; u = beta (v - S^T k); S = S + k u^T; o = scale S^T q``.
+
+    q, k [B, T, Hk, Dk], v [B, T, Hv, Dv], g and beta [B, T, Hv] (both of v's
+    dtype, or both float32); value head h reads key head ``h // (Hv // Hk)``.
+    ``g`` is the log of the decay (0 keeps the state, -inf clears it), ``scale``
+    is ``Dk ** -0.5`` if None.  ``state`` is float32 [N, Hv, Dk, Dv] (zeros if
+    None).  Dk and Dv are at most 128.  Keys are expected normalised
+    (``qk_norm_rotate(..., norm="l2")``): the rule is stable for
+    ``beta * |k|^2 <= 2``.  Returns o, or (o, state after the sequences).
+    Differentiable in q, k, v, g, beta and state; the backward pass computes
+    the states again and keeps only the inputs.
+    """
+    ops = _cuda(q, "gated_delta_rule")
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    o, last = ops.gated_delta_rule.default(q, k, v, g, beta, scale, cu_seqlens, state, return_state)
+    return (o, last) if return_state else o
+
+
+def gated_delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                          state: torch.Tensor, scale: float | None = None) -> torch.Tensor:
+    """One token of ``gated_delta_rule``: q, k [N, Hk, Dk], v [N, Hv, Dv], g, beta [N, Hv].
+
+    ``state``, float32 [N, Hv, Dk, Dv], is updated in place.  Dk is at most
+    256.  Returns o [N, Hv, Dv].
+    """
+    ops = _cuda(q, "gated_delta_rule_step")
+    return ops.gated_delta_rule_step.default(q, k, v, g, beta, state, q.shape[-1] ** -0.5 if scale is None else scale)
