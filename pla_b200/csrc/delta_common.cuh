@@ -68,6 +68,7 @@ struct DeltaParams {
   float* dstate_in;
   float* dstates;    // dS at every chunk's end, fragment order
   float* dxs;        // dX
+  float* largest;    // of S, dS, U, dX in every (chunk, value head, slab): 4 floats
   void *dq, *dk_out, *dv_out, *dg, *dbeta;
   int slabs;         // ceil(dv / 16)
   int vec_qk, vec_v, vec_o, vec_do;
@@ -218,6 +219,13 @@ __device__ __forceinline__ uint32_t at_mk(int lane, int m0, int k0) {
   return tile_at<W>(m0 + (m & 1) * 8 + (lane & 7), (k0 >> 3) + (m >> 1));
 }
 
+// A fragment from a tile that holds the transpose: A[m][k] = tile[k0 + k][m0 + m] (transposing loads).
+template <int W>
+__device__ __forceinline__ uint32_t at_km(int lane, int m0, int k0) {
+  const int m = lane >> 3;
+  return tile_at<W>(k0 + (m >> 1) * 8 + (lane & 7), (m0 >> 3) + (m & 1));
+}
+
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -229,30 +237,22 @@ __device__ __forceinline__ float exp_sum(float hi, float lo) {
   return fmaf(e, lo, e);
 }
 
-// What the kernels of a type hold: planes of the inputs, of T and the states,
-// of P and the operands that only an output of the type sees.
+// Planes of the inputs of a type.
 template <typename T>
 struct DeltaType {
   static constexpr int kIn = sizeof(T) == 4 ? 2 : 1;
-  static constexpr int kState = 2;
-  static constexpr int kOut = 2;
-};
-template <>
-struct DeltaType<__nv_bfloat16> {
-  static constexpr int kIn = 1;
-  static constexpr int kState = 2;
-  // one fp16 plane adds an error of 2^-12 to results that are rounded by 2^-9
-  static constexpr int kOut = 1;
 };
 
-template <typename T, int DK>
+// Workspace of a chunk.  PS: planes of T and of the states, X and U where they
+// are operands; PO: planes of P and of what only a result of type T sees.
+template <typename T, int DK, int PS, int PO>
 struct DeltaLayout {
-  static constexpr int kIn = DeltaType<T>::kIn;
+  static constexpr int kIn = DeltaType<T>::kIn, kState = PS, kOut = PO;
   static constexpr uint32_t kTile = kChunk * DK * 2;
-  static constexpr uint32_t kTiles = 2 * kIn * kTile;            // K planes, Q planes
+  static constexpr uint32_t kTiles = 2 * kIn * kTile;  // K planes, Q planes
   static constexpr uint32_t kSquare = kChunk * kChunk * 2;
-  static constexpr uint32_t kT = DeltaType<T>::kState * kSquare;
-  static constexpr uint32_t kP = DeltaType<T>::kOut * kSquare;
+  static constexpr uint32_t kT = PS * kSquare;
+  static constexpr uint32_t kP = PO * kSquare;
   static constexpr uint32_t kCoef = kCoefs * kChunk * 4;
   static constexpr uint32_t kHead = kT + kP + kCoef;
   static constexpr uint32_t kStage = kTiles + kHead;

@@ -80,9 +80,9 @@ __device__ __forceinline__ float store_square_row(char* out, int row, int lane, 
   return s.inverse;
 }
 
-template <typename T, int DK>
+template <typename T, int DK, int PS, int PO>
 __global__ void __launch_bounds__(kPrepThreads) delta_prepare(DeltaParams p) {
-  using L = DeltaLayout<T, DK>;
+  using L = DeltaLayout<T, DK, PS, PO>;
   extern __shared__ char shared_bytes[];
   PrepShared<T, DK>& s = *reinterpret_cast<PrepShared<T, DK>*>(shared_bytes);
   const int chunk = blockIdx.x / p.hk, kh = blockIdx.x % p.hk;
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prepare(DeltaParams p) {
         pv[e] = j <= row ? decay * s.qk[row][j] : 0.f;
         s.a[row][j] = j < row ? s.beta[row] * (decay * s.kk[row][j]) : 0.f;
       }
-      const float back = store_square_row<DeltaType<T>::kOut>(to_p, row, lane, pv[0], pv[1]);
+      const float back = store_square_row<PO>(to_p, row, lane, pv[0], pv[1]);
       if (lane == 0) coef[kOutP * kChunk + row] = p.scale * back;
     }
     __syncthreads();
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prepare(DeltaParams p) {
     for (int i = 0; i < kChunk / 4; ++i) {
       const int row = warp * (kChunk / 4) + i;
       const float2 v = *reinterpret_cast<const float2*>(&s.a[row][2 * lane]);
-      const float back = store_square_row<DeltaType<T>::kState>(head, row, lane, v.x, v.y);
+      const float back = store_square_row<PS>(head, row, lane, v.x, v.y);
       if (lane == 0) coef[kTRow * kChunk + row] = back;
     }
     if (tid < kChunk) {

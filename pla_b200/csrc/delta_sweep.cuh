@@ -181,6 +181,13 @@ __device__ __forceinline__ void row_max(const float (&f)[N][4], float (&m)[2]) {
   m[1] = quad_max(m[1]);
 }
 
+// Over the quads of a warp, of what row_max gives.
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
 // Accumulators of column tiles 2k, 2k + 1, times their rows' factors, as the
 // left operand of step k of the next product.
 template <int PLANES>
@@ -321,10 +328,10 @@ __device__ __forceinline__ float2 coef_at(const char* head, int which, int n, in
 constexpr int kSweepRing = 128;  // bytes of the ring's barriers
 
 // KEEP: store S at every chunk's start and U for the backward pass instead of O.
-template <typename T, int DK, bool KEEP>
+template <typename T, int DK, int PS, int PO, bool KEEP>
 __global__ void __launch_bounds__(256) delta_sweep(DeltaParams p, int stages) {
-  using L = DeltaLayout<T, DK>;
-  constexpr int IN = DeltaType<T>::kIn, OUT = DeltaType<T>::kOut;
+  using L = DeltaLayout<T, DK, PS, PO>;
+  constexpr int IN = L::kIn;
   extern __shared__ __align__(128) char shared_bytes[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const SweepAt a = sweep_at(p, warps, warp);
@@ -362,22 +369,26 @@ __global__ void __launch_bounds__(256) delta_sweep(DeltaParams p, int stages) {
     if (mine) {
       const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
       const char* coef = stage + L::kTiles + L::kT + L::kP;
-      if (KEEP)
-        fragments_store(p.states + ((static_cast<long long>(a.first + c) * p.hv + a.vh) * p.slabs + a.slab) * 16 * DK, lane, s);
+      const long long slab_at = (static_cast<long long>(a.first + c) * p.hv + a.vh) * p.slabs + a.slab;
+      if (KEEP) fragments_store(p.states + slab_at * 16 * DK, lane, s);
       float top[2];
       row_max(s, top);
+      if (KEEP) {
+        const float most = warp_max(fmaxf(top[0], top[1]));
+        if (lane == 0) p.largest[slab_at * 4] = most;
+      }
       const Pow2 ss[2] = {pow2_for(top[0]), pow2_for(top[1])};
       float x[8][4] = {}, o_acc[8][4] = {};
       // (K S)^T and (Q S)^T
 #pragma unroll
       for (int kk = 0; kk < DK / 16; ++kk) {
         uint32_t hi[4], lo[4];
-        as_operand<2>(s[2 * kk], s[2 * kk + 1], ss, hi, lo);
+        as_operand<PS>(s[2 * kk], s[2 * kk + 1], ss, hi, lo);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const uint32_t at = at_nk<DK>(lane, n * 16, kk * 16);
-          product<2, IN, false>(x[2 * n], x[2 * n + 1], hi, lo, kt + at, L::kTile);
-          if (!KEEP) product<OUT, IN, false>(o_acc[2 * n], o_acc[2 * n + 1], hi, lo, qt + at, L::kTile);
+          product<PS, IN, false>(x[2 * n], x[2 * n + 1], hi, lo, kt + at, L::kTile);
+          if (!KEEP) product<PO, IN, false>(o_acc[2 * n], o_acc[2 * n + 1], hi, lo, qt + at, L::kTile);
         }
       }
       // X = beta v - beta e^G K S
@@ -406,10 +417,10 @@ __global__ void __launch_bounds__(256) delta_sweep(DeltaParams p, int stages) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           uint32_t hi[4], lo[4];
-          as_operand<2>(x[2 * kk], x[2 * kk + 1], sx, hi, lo);
+          as_operand<PS>(x[2 * kk], x[2 * kk + 1], sx, hi, lo);
 #pragma unroll
           for (int n = kk; n < 4; ++n)
-            product<2, 2, false>(u[2 * n], u[2 * n + 1], hi, lo, tt + at_nk<kChunk>(lane, n * 16, kk * 16), L::kSquare);
+            product<PS, PS, false>(u[2 * n], u[2 * n + 1], hi, lo, tt + at_nk<kChunk>(lane, n * 16, kk * 16), L::kSquare);
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
@@ -421,7 +432,10 @@ __global__ void __launch_bounds__(256) delta_sweep(DeltaParams p, int stages) {
         }
       }
       if (KEEP) {
-        fragments_store(p.us + ((static_cast<long long>(a.first + c) * p.hv + a.vh) * p.slabs + a.slab) * 16 * kChunk, lane, u);
+        fragments_store(p.us + slab_at * 16 * kChunk, lane, u);
+        row_max(u, top);
+        const float most = warp_max(fmaxf(top[0], top[1]));
+        if (lane == 0) p.largest[slab_at * 4 + 2] = most;
       } else {  // O^T = (Q S)^T + U^T P^T, each with its weights
         row_max(u, top);
         const Pow2 su[2] = {pow2_for(top[0]), pow2_for(top[1])};
@@ -429,10 +443,10 @@ __global__ void __launch_bounds__(256) delta_sweep(DeltaParams p, int stages) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           uint32_t hi[4], lo[4];
-          as_operand<OUT>(u[2 * kk], u[2 * kk + 1], su, hi, lo);
+          as_operand<PO>(u[2 * kk], u[2 * kk + 1], su, hi, lo);
 #pragma unroll
           for (int n = kk; n < 4; ++n)
-            product<OUT, OUT, false>(pu[2 * n], pu[2 * n + 1], hi, lo, pt + at_nk<kChunk>(lane, n * 16, kk * 16), L::kSquare);
+            product<PO, PO, false>(pu[2 * n], pu[2 * n + 1], hi, lo, pt + at_nk<kChunk>(lane, n * 16, kk * 16), L::kSquare);
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
@@ -473,10 +487,10 @@ __global__ void __launch_bounds__(256) delta_sweep(DeltaParams p, int stages) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           uint32_t hi[4], lo[4];
-          as_operand<2>(u[2 * kk], u[2 * kk + 1], sc, hi, lo);
+          as_operand<PS>(u[2 * kk], u[2 * kk + 1], sc, hi, lo);
 #pragma unroll
           for (int n = 0; n < DK / 16; ++n)
-            product<2, IN, true>(s[2 * n], s[2 * n + 1], hi, lo, kt + at_kn<DK>(lane, n * 16, kk * 16), L::kTile);
+            product<PS, IN, true>(s[2 * n], s[2 * n + 1], hi, lo, kt + at_kn<DK>(lane, n * 16, kk * 16), L::kTile);
         }
 #pragma unroll
         for (int n = 0; n < DK / 8; ++n) {

@@ -5,9 +5,11 @@
 #include <atomic>
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/pla_b200.h"
 #include "causal_kernel.cuh"
+#include "delta_backward.cuh"
 #include "delta_prepare.cuh"
 #include "delta_step.cuh"
 #include "delta_sweep.cuh"
@@ -271,13 +273,13 @@ int check_delta(const pla_delta* a) {
 
 struct DeltaSizes {
   long long chunks = 0;
-  size_t plan = 0, tiles = 0, heads = 0, states = 0, us = 0, total = 0;
+  size_t plan = 0, tiles = 0, heads = 0, states = 0, us = 0, largest = 0, total = 0;
 };
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-template <typename T, int DK>
+template <typename T, int DK, int PS, int PO>
 DeltaSizes delta_sizes_of(const pla_delta* a, bool backward) {
-  using L = DeltaLayout<T, DK>;
+  using L = DeltaLayout<T, DK, PS, PO>;
   DeltaSizes s;
   s.chunks = a->cu_seqlens ? a->tokens / kChunk + static_cast<long long>(a->sequences)
                            : static_cast<long long>(a->batch) * ((a->tokens + kChunk - 1) / kChunk);
@@ -288,14 +290,33 @@ DeltaSizes delta_sizes_of(const pla_delta* a, bool backward) {
     const size_t columns = static_cast<size_t>(s.chunks) * a->hv * ((a->dv + 15) / 16) * 16;
     s.states = up256(columns * DK * sizeof(float));
     s.us = up256(columns * kChunk * sizeof(float));
+    s.largest = up256(columns / 16 * 4 * sizeof(float));
   }
-  s.total = s.plan + s.tiles + s.heads + 2 * s.states + 2 * s.us;
+  s.total = s.plan + s.tiles + s.heads + 2 * s.states + 2 * s.us + s.largest;
   return s;
 }
 
+// f(element type, padded Dk, planes of states, planes of outputs).  Forward:
+// states come back in fp32, so their operands keep 22 bits; what only a bf16
+// output sees takes one fp16 plane (2^-12 beside a rounding of 2^-9).
 template <typename F>
 int with_delta(const pla_delta* a, F&& f) {
-  return with_type(a->dtype, [&](auto zero) { return a->dk <= 64 ? f(zero, Int<64>{}) : f(zero, Int<128>{}); });
+  return with_type(a->dtype, [&](auto zero) {
+    using T = decltype(zero);
+    constexpr int PO = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
+    return a->dk <= 64 ? f(zero, Int<64>{}, Int<2>{}, Int<PO>{}) : f(zero, Int<128>{}, Int<2>{}, Int<PO>{});
+  });
+}
+// Backward: one plane everywhere if every gradient is rounded to bf16, else two.
+template <typename F>
+int with_delta_gradient(const pla_delta* a, bool fp32_result, F&& f) {
+  return with_type(a->dtype, [&](auto zero) {
+    using T = decltype(zero);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      if (!fp32_result)
+        return a->dk <= 64 ? f(zero, Int<64>{}, Int<1>{}, Int<1>{}) : f(zero, Int<128>{}, Int<1>{}, Int<1>{});
+    return a->dk <= 64 ? f(zero, Int<64>{}, Int<2>{}, Int<2>{}) : f(zero, Int<128>{}, Int<2>{}, Int<2>{});
+  });
 }
 
 DeltaParams delta_params(const pla_delta* a, const DeltaSizes& s) {
@@ -340,6 +361,8 @@ DeltaParams delta_params(const pla_delta* a, const DeltaSizes& s) {
   p.us = reinterpret_cast<float*>(w);
   w += s.us;
   p.dxs = reinterpret_cast<float*>(w);
+  w += s.us;
+  p.largest = reinterpret_cast<float*>(w);
   const size_t es = type_size(a->dtype);
   const int whole = static_cast<int>(16 / es);
   p.vec_qk = a->dk % 4 == 0 && aligned_to(a->q, 4 * es) && aligned_to(a->k, 4 * es) &&
@@ -349,7 +372,7 @@ DeltaParams delta_params(const pla_delta* a, const DeltaSizes& s) {
   return p;
 }
 
-template <typename T, int DK>
+template <typename T, int DK, int PS, int PO>
 int launch_prepare(const DeltaParams& p, cudaStream_t stream) {
   if (p.cu) {
     delta_plan<<<1, 1024, 0, stream>>>(p.cu, p.tokens, p.sequences, p.plan);
@@ -359,9 +382,9 @@ int launch_prepare(const DeltaParams& p, cudaStream_t stream) {
   if (static_cast<long long>(p.chunk_bound) * p.hk > kMaxGrid) return PLA_ERR_TOO_LARGE;
   if (!p.chunk_bound) return PLA_OK;
   const size_t shared = sizeof(PrepShared<T, DK>);
-  const int st = allow_shared<delta_prepare<T, DK>>(shared);
+  const int st = allow_shared<delta_prepare<T, DK, PS, PO>>(shared);
   if (st != PLA_OK) return st;
-  delta_prepare<T, DK><<<p.chunk_bound * p.hk, kPrepThreads, shared, stream>>>(p);
+  delta_prepare<T, DK, PS, PO><<<p.chunk_bound * p.hk, kPrepThreads, shared, stream>>>(p);
   return launched("delta_prepare");
 }
 
@@ -375,20 +398,48 @@ int sweep_warps(const DeltaParams& p, int sms) {
   return warps;
 }
 
-template <typename T, int DK, bool KEEP>
+// Stages of the ring, shared memory and grid of a sweep.
+template <typename T, typename L>
+struct SweepShape {
+  int warps, stages;
+  long long grid;
+  size_t shared;
+  SweepShape(const DeltaParams& p, int sms) {
+    warps = sweep_warps(p, sms);
+    grid = static_cast<long long>(p.sequences) * p.hv * ((p.slabs + warps - 1) / warps);
+    const size_t slabs = static_cast<size_t>(warps) * 2 * Slab<T>::kBytes;
+    stages = static_cast<int>(std::min<size_t>(3, (227 * 1024 - kSweepRing - slabs) / L::kStage));
+    shared = kSweepRing + stages * L::kStage + slabs;
+  }
+};
+
+template <typename T, int DK, int PS, int PO, bool KEEP>
 int launch_sweep(const DeltaParams& p, int sms, cudaStream_t stream) {
-  using L = DeltaLayout<T, DK>;
-  const int warps = sweep_warps(p, sms);
-  const long long grid = static_cast<long long>(p.sequences) * p.hv * ((p.slabs + warps - 1) / warps);
-  if (grid > kMaxGrid) return PLA_ERR_TOO_LARGE;
-  if (!grid) return PLA_OK;
-  const size_t slabs = static_cast<size_t>(warps) * 2 * Slab<T>::kBytes;
-  const int stages = static_cast<int>(std::min<size_t>(3, (227 * 1024 - kSweepRing - slabs) / L::kStage));
-  const size_t shared = kSweepRing + stages * L::kStage + slabs;
-  const int st = allow_shared<delta_sweep<T, DK, KEEP>>(shared);
+  const SweepShape<T, DeltaLayout<T, DK, PS, PO>> at(p, sms);
+  if (at.grid > kMaxGrid) return PLA_ERR_TOO_LARGE;
+  if (!at.grid) return PLA_OK;
+  const int st = allow_shared<delta_sweep<T, DK, PS, PO, KEEP>>(at.shared);
   if (st != PLA_OK) return st;
-  delta_sweep<T, DK, KEEP><<<static_cast<int>(grid), warps * 32, shared, stream>>>(p, stages);
+  delta_sweep<T, DK, PS, PO, KEEP><<<static_cast<int>(at.grid), at.warps * 32, at.shared, stream>>>(p, at.stages);
   return launched("delta_sweep");
+}
+
+template <typename T, int DK, int PS, int PO>
+int launch_gradient(const DeltaParams& p, int sms, cudaStream_t stream) {
+  const SweepShape<T, DeltaLayout<T, DK, PS, PO>> at(p, sms);
+  int st = allow_shared<delta_sweep_back<T, DK, PS, PO>>(at.shared);
+  if (st != PLA_OK) return st;
+  delta_sweep_back<T, DK, PS, PO><<<static_cast<int>(at.grid), at.warps * 32, at.shared, stream>>>(p, at.stages);
+  if ((st = launched("delta_sweep_back")) != PLA_OK) return st;
+  if (p.cu) {
+    delta_clear_rows<T><<<std::min(p.tokens + 1, 4 * sms), 256, 0, stream>>>(p);
+    if ((st = launched("delta_clear_rows")) != PLA_OK) return st;
+  }
+  if (!p.chunk_bound) return PLA_OK;
+  const size_t shared = sizeof(GradShared<T, DK, PS>);
+  if ((st = allow_shared<delta_gradient<T, DK, PS, PO>>(shared)) != PLA_OK) return st;
+  delta_gradient<T, DK, PS, PO><<<p.chunk_bound * p.hk, kGradThreads, shared, stream>>>(p);
+  return launched("delta_gradient");
 }
 
 }  // namespace
@@ -606,10 +657,14 @@ int pla_qk_norm_rotate_backward(const pla_qk_norm* a, void* workspace, size_t wo
 size_t pla_gated_delta_rule_workspace(const pla_delta* a, int backward) {
   if (check_delta(a) != PLA_OK) return 0;
   size_t bytes = 0;
-  with_delta(a, [&](auto zero, auto dk) {
-    bytes = delta_sizes_of<decltype(zero), decltype(dk)::value>(a, backward != 0).total;
+  const auto size = [&](auto zero, auto dk, auto ps, auto po) {
+    bytes = delta_sizes_of<decltype(zero), decltype(dk)::value, decltype(ps)::value, decltype(po)::value>(a, backward != 0).total;
     return 0;
-  });
+  };
+  if (backward)
+    with_delta_gradient(a, true, size);
+  else
+    with_delta(a, size);
   return bytes;
 }
 
@@ -632,25 +687,68 @@ int pla_gated_delta_rule_forward(const pla_delta* a, pla_stream_t stream) {
   if (!a->hv || !a->dv || !a->sequences) return PLA_OK;
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
-  return with_delta(a, [&](auto zero, auto dk) {
+  return with_delta(a, [&](auto zero, auto dk, auto ps, auto po) {
     using T = decltype(zero);
-    constexpr int DK = decltype(dk)::value;
-    const DeltaSizes s = delta_sizes_of<T, DK>(a, false);
+    constexpr int DK = decltype(dk)::value, PS = decltype(ps)::value, PO = decltype(po)::value;
+    const DeltaSizes s = delta_sizes_of<T, DK, PS, PO>(a, false);
     if (s.chunks > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
     if (s.total && (a->workspace_bytes < s.total || !a->workspace || !aligned_to(a->workspace, 256)))
       return static_cast<int>(PLA_ERR_INVALID_ARGUMENT);
     const DeltaParams p = delta_params(a, s);
-    const int st = launch_prepare<T, DK>(p, as_stream(stream));
+    const int st = launch_prepare<T, DK, PS, PO>(p, as_stream(stream));
     if (st != PLA_OK) return st;
-    return launch_sweep<T, DK, false>(p, sms, as_stream(stream));
+    return launch_sweep<T, DK, PS, PO, false>(p, sms, as_stream(stream));
   });
 }
 
 int pla_gated_delta_rule_backward(const pla_delta* a, const pla_delta_gradient* g, pla_stream_t stream) {
-  const int st = check_delta(a);
+  int st = check_delta(a);
   if (st != PLA_OK) return st;
   if (!g) return PLA_ERR_INVALID_ARGUMENT;
-  return PLA_ERR_UNSUPPORTED;
+  const size_t es = type_size(a->dtype);
+  const bool work = a->batch && a->tokens && a->hv && a->dv;
+  if (work && (!g->d_o || !g->dq || !g->dk || !g->dv || !g->dg || !g->dbeta)) return PLA_ERR_INVALID_ARGUMENT;
+  const long long tokens = static_cast<long long>(a->batch) * a->tokens;
+  const Bytes written[3] = {dense(g->dq, tokens * a->hk * a->dk, es), dense(g->dk, tokens * a->hk * a->dk, es),
+                            dense(g->dv, tokens * a->hv * a->dv, es)};
+  const Bytes read[4] = {
+      strided(a->q, es, {{a->dk, 1}, {a->hk, a->q_head}, {a->tokens, a->q_token}, {a->batch, a->q_batch}}),
+      strided(a->k, es, {{a->dk, 1}, {a->hk, a->k_head}, {a->tokens, a->k_token}, {a->batch, a->k_batch}}),
+      strided(a->v, es, {{a->dv, 1}, {a->hv, a->v_head}, {a->tokens, a->v_token}, {a->batch, a->v_batch}}),
+      strided(g->d_o, es, {{a->dv, 1}, {a->hv, g->do_head}, {a->tokens, g->do_token}, {a->batch, g->do_batch}})};
+  for (const Bytes& w : written)
+    for (const Bytes& r : read)
+      if (meets(w, r)) return PLA_ERR_INVALID_ARGUMENT;
+  const long long held = static_cast<long long>(a->sequences) * a->hv * a->dk * a->dv;
+  if (meets(dense(g->dstate_in, held, 4), dense(g->dstate_out, held, 4)) ||
+      meets(dense(g->dstate_in, held, 4), dense(a->state_in, held, 4)))
+    return PLA_ERR_INVALID_ARGUMENT;
+  if (!a->hv || !a->dv || !a->sequences) return PLA_OK;
+  int sms;
+  if ((st = current_sm100(&sms)) != PLA_OK) return st;
+  const bool fp32_result = a->gates32 || g->dstate_in || g->dstate_out;
+  return with_delta_gradient(a, fp32_result, [&](auto zero, auto dk, auto ps, auto po) {
+    using T = decltype(zero);
+    constexpr int DK = decltype(dk)::value, PS = decltype(ps)::value, PO = decltype(po)::value;
+    const DeltaSizes s = delta_sizes_of<T, DK, PS, PO>(a, true);
+    if (s.chunks > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
+    if (s.total && (a->workspace_bytes < s.total || !a->workspace || !aligned_to(a->workspace, 256)))
+      return static_cast<int>(PLA_ERR_INVALID_ARGUMENT);
+    DeltaParams p = delta_params(a, s);
+    p.d_o = g->d_o;
+    p.do_batch = g->do_batch, p.do_token = g->do_token, p.do_head = g->do_head;
+    p.dstate_out = g->dstate_out;
+    p.dstate_in = g->dstate_in;
+    p.dq = g->dq, p.dk_out = g->dk, p.dv_out = g->dv, p.dg = g->dg, p.dbeta = g->dbeta;
+    const int whole = static_cast<int>(16 / es);
+    p.vec_do = aligned_to(g->d_o, 16) && !((g->do_batch | g->do_token | g->do_head) % whole);
+    p.vec_o = aligned_to(g->dv, 16) && a->dv % whole == 0;
+    p.state_out = nullptr;
+    int st = launch_prepare<T, DK, PS, PO>(p, as_stream(stream));
+    if (st != PLA_OK) return st;
+    if ((st = launch_sweep<T, DK, PS, PO, true>(p, sms, as_stream(stream))) != PLA_OK) return st;
+    return launch_gradient<T, DK, PS, PO>(p, sms, as_stream(stream));
+  });
 }
 
 int pla_gated_delta_rule_step(const pla_delta_step* a, pla_stream_t stream) {

@@ -405,3 +405,118 @@ def test_sequence_offsets_that_do_not_ascend_stay_in_bounds():
         y, last = P.causal_depthwise(x, w, cu_seqlens=cu, return_state=True)
         for t in (o, state, y, last):
             assert bool(torch.isfinite(t).all())
+
+
+# ---- gated delta rule, backward --------------------------------------------
+def delta_gradients(case, dtype, seed, with_state, change=None):
+    q, k, v, g, beta, s, cu = delta_inputs(case, dtype, seed=seed)
+    if change:
+        change(q, k, v, g, beta)
+    gen = torch.Generator().manual_seed(seed + 1)
+    d_o = rand(gen, *v.shape, dtype=dtype)
+    leaves = [f64(t, True) for t in (q, k, v, g, beta)]
+    s64 = f64(s, True)
+    o, last = R.gated_delta_rule(*leaves, cu=cu, state=s64)
+    ds = rand(gen, *last.shape, scale=0.5) if with_state else None
+    inputs = leaves + ([s64] if s is not None and with_state else [])
+    outs = ((o, last), (f64(d_o), f64(ds))) if with_state else ((o,), (f64(d_o),))
+    want = torch.autograd.grad(outs[0], inputs, outs[1], allow_unused=True)
+    want = [torch.zeros_like(i) if w is None else w for w, i in zip(want, inputs)]
+    mine = [gpu(t).requires_grad_() for t in (q, k, v, g, beta)]
+    sm = None if s is None else gpu(s).requires_grad_(with_state)
+    o, last = P.gated_delta_rule(*mine, cu_seqlens=gpu(cu), state=sm, return_state=True)
+    inputs = mine + ([sm] if s is not None and with_state else [])
+    outs = ((o, last), (gpu(d_o), gpu(ds))) if with_state else ((o,), (gpu(d_o),))
+    got = torch.autograd.grad(outs[0], inputs, outs[1], retain_graph=True)
+    again = torch.autograd.grad(outs[0], inputs, outs[1])
+    assert all(torch.equal(a, b) for a, b in zip(got, again))  # no atomics in any sum
+    return got, want
+
+
+def check_delta_gradients(got, want, dtype, gates, plain):
+    """plain: one plane everywhere (every gradient bf16)."""
+    for name, a, b in zip("q k v g beta state".split(), got, want):
+        fp32 = name == "state" or (name in ("g", "beta") and gates == F32)
+        tol = BACKWARD[F32 if fp32 else dtype if plain or dtype != BF16 else BF16]
+        if name in ("g", "beta"):
+            # dg sums products over the rest of the sequence and its parts cancel: relative to the largest of a head
+            a, b = a.transpose(1, 2), b.transpose(1, 2)
+            tol = 4 * tol
+        token_norms(a, b, tol, "d" + name)
+
+
+@pytest.mark.parametrize("with_state", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("case", DELTA)
+def test_delta_gradients(case, dtype, with_state):
+    got, want = delta_gradients(case, dtype, 21, with_state)
+    check_delta_gradients(got, want, dtype, case[8] or dtype, not with_state and case[8] is None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_delta_gradients_at_resets_and_zero_gates(dtype):
+    def change(q, k, v, g, beta):
+        g[0, 40] = -float("inf")
+        g[0, 64] = -90.0
+        beta[0, ::7] = 0
+        beta[0, 3::11] = 2
+        q[0, 10], k[0, 11] = 0, 0
+        v[..., 5] *= 1e3
+
+    got, want = delta_gradients((1, 150, 1, 2, 64, 32, True, None, F32), dtype, 31, True, change)
+    want = [torch.nan_to_num(w, nan=0.0) for w in want]  # exp's slope at -inf times 0
+    check_delta_gradients(got, want, dtype, F32, False)
+
+
+def test_delta_gradient_against_differences():
+    q, k, v, g, beta, s, cu = delta_inputs((1, 100, 1, 2, 64, 32, True, [0, 30, 100], F32), F32, seed=41)
+    leaves = [gpu(t).requires_grad_() for t in (q, k, v, g, beta, s)]
+    f = lambda a: P.gated_delta_rule(*a[:5], cu_seqlens=gpu(cu), state=a[5])  # noqa: E731
+    o = f(leaves)
+    d_o = gpu(rand(torch.Generator().manual_seed(42), *o.shape))
+    for i, grad in enumerate(torch.autograd.grad(o, leaves, d_o)):
+        step = gpu(rand(torch.Generator().manual_seed(43 + i), *leaves[i].shape)) * (0.1 if i in (0, 1) else 1)
+        e = 2 ** -9
+        moved = [[t.detach() + sign * e * step if j == i else t.detach() for j, t in enumerate(leaves)] for sign in (1, -1)]
+        up_, down_ = f(moved[0]).double(), f(moved[1]).double()
+        slope = float(((up_ - down_) / (2 * e) * d_o.double()).sum())
+        want = float((grad.double() * step.double()).sum())
+        # o's errors of 2^-16 (see the tolerances) over 2 e, as random terms, and the cubic rest, e^2 of a sum of its size
+        noise = 2 ** -16 / e * float(o.detach().double().norm() * d_o.double().norm() / o.numel() ** 0.5)
+        cubic = 40 * e * e * float(((up_ - down_) / (2 * e)).norm() * d_o.double().norm())
+        assert abs(slope - want) <= noise + cubic, (i, slope, want, noise, cubic)
+
+
+def test_backward_passes_replay_in_a_graph():
+    q, k, v, g, beta, _, _ = (gpu(t) for t in delta_inputs((1, 200, 2, 2, 64, 64, False, None, None), BF16, seed=51))
+    x, w, b, _, _ = (gpu(t) for t in conv_inputs((1, 200, 64, 4, True, True, False, None), BF16, seed=52))
+
+    def passes(leaves):
+        q, k, v, g, beta, x, w, b = leaves
+        y = P.causal_depthwise(x, w, b, silu=True)
+        qn, kn = P.qk_norm_rotate(q, k, norm="l2")
+        o = P.gated_delta_rule(qn, kn, v, g, beta)
+        return [y.detach(), o.detach(), *torch.autograd.grad((y, o), leaves, (x.detach(), v.detach()))]
+
+    fresh = lambda: [t.detach().clone().requires_grad_() for t in (q, k, v, g, beta, x, w, b)]  # noqa: E731
+    want = passes(fresh())
+    leaves = fresh()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        passes(leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = passes(leaves)
+    for _ in range(2):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_second_derivatives_raise():
+    x = torch.randn(1, 8, 16, device=DEV, requires_grad=True)
+    w = torch.randn(16, 4, device=DEV, requires_grad=True)
+    (dx,) = torch.autograd.grad(P.causal_depthwise(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
