@@ -3,8 +3,7 @@
 //     dU = P^T do' + e^{G_C - G} (K D)          dX = T^T dU          dv = beta dX
 //     dS0 = e^{G_C} D + Q^T (e^G do') - K^T (beta e^G dX)
 // is the reverse of the forward's chain and runs like it (delta_sweep_back:
-// 16 value features a warp, D in registers, chunks from the last to the
-// first).  What remains has no dependence between chunks (delta_gradient):
+// D in registers, chunks from the last to the first).  What remains has no dependence between chunks (delta_gradient):
 //     dP = tril(do' U^T)       dA = -stril(dX U^T)
 //     N = Gamma . dP           B = beta Gamma . dA          Gamma_ij = e^{G_i - G_j}
 //     dq = e^G (do' S0^T) + N K
@@ -22,192 +21,153 @@
 namespace pla {
 namespace seq {
 
-template <typename T, int DK, int PS, int PO>
-__global__ void __launch_bounds__(256) delta_sweep_back(DeltaParams p, int stages) {
+template <typename T, int DK, int PS, int PO, int VB>
+__global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int stages) {
   using L = DeltaLayout<T, DK, PS, PO>;
-  constexpr int IN = L::kIn;
+  using M = SweepShared<T, DK, PS, PO, VB, true>;
+  constexpr int IN = L::kIn, QN = DK / 32;
   extern __shared__ __align__(128) char shared_bytes[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const SweepAt a = sweep_at(p, warps, warp);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wm = warp % (VB / 16), wn = warp / (VB / 16), m0 = wm * 16;
+  const SweepAt a = sweep_at(p, VB);
   Ring<L> ring;
-  ring.begin(shared_bytes, stages, warps);
-  char* slabs = shared_bytes + kSweepRing + stages * L::kStage + warp * 2 * Slab<T>::kBytes;
-  const T* d_o = static_cast<const T*>(p.d_o) + a.batch * p.do_batch + a.lo * p.do_token + a.vh * p.do_head + a.slab * 16;
+  ring.begin(shared_bytes, stages, VB / 4);
+  M& m = *reinterpret_cast<M*>(shared_bytes + kSweepRing + stages * L::kStage);
+  const uint32_t dt = shared_u32(m.s), yt = shared_u32(m.a), xt = shared_u32(m.b), wt = shared_u32(m.c), ft = shared_u32(m.d);
+  const T* d_o = static_cast<const T*>(p.d_o) + a.batch * p.do_batch + a.lo * p.do_token + a.vh * p.do_head + a.column;
   const long long dv_step = static_cast<long long>(p.hv) * p.dv;
   T* dv = static_cast<T*>(p.dv_out) + (static_cast<long long>(a.batch) * p.tokens + a.lo) * dv_step +
-          static_cast<long long>(a.vh) * p.dv + a.slab * 16;
-  const bool mine = a.width > 0;
-  float d[DK / 8][4];
-  state_load<DK>(mine ? p.dstate_out : nullptr, p, a, lane, d);
+          static_cast<long long>(a.vh) * p.dv + a.column;
   if (threadIdx.x == 0)
     for (int i = 0; i < stages && i < a.chunks; ++i) ring.fill(p, i, a.first + a.chunks - 1 - i, a.kh, a.vh);
-  if (mine && a.chunks)
-    slab_fetch<T>(slabs, d_o + (a.chunks - 1) * kChunk * p.do_token, p.do_token, a.len - (a.chunks - 1) * kChunk, a.width,
-                  p.vec_do, lane);
+  if (a.chunks)
+    slab_fetch<T, VB>(m.slab[0], d_o + (a.chunks - 1) * kChunk * p.do_token, p.do_token, a.len - (a.chunks - 1) * kChunk,
+                      a.width, p.vec_do);
+  const Walk dw(dt + at_mk<DK>(lane, m0, 0)), yw(yt + at_mk<kChunk>(lane, m0, 0));  // planes of D and Y; the others follow Y's
+  const Walk kw(at_nk<DK>(lane, wn * 16, 0));                                       // in K
+  const uint32_t ts = at_kn<kChunk>(lane, wn * 16, 0);                              // in T and P
+  uint32_t ks[QN / 2];                                                              // in K and Q, for the state's update
+#pragma unroll
+  for (int n = 0; n < QN / 2; ++n) ks[n] = at_kn<DK>(lane, wn * (DK / 4) + n * 16, 0);
+  float d[QN][4];
+  state_load(p.dstate_out, p, a, m0, wn * (DK / 4), lane, d);
+  tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, &m.scale[0][wn][m0]);
 
   for (int turn = 0; turn < a.chunks; ++turn) {
     const int c = a.chunks - 1 - turn, len = min(kChunk, a.len - c * kChunk);
-    char* slab = slabs + (turn & 1) * Slab<T>::kBytes;
-    if (mine && c > 0)
-      slab_fetch<T>(slabs + (~turn & 1) * Slab<T>::kBytes, d_o + (c - 1) * kChunk * p.do_token, p.do_token, kChunk, a.width,
-                    p.vec_do, lane);
+    const long long slab_at = (static_cast<long long>(a.first + c) * p.hv + a.vh) * p.slabs + a.column / 16 + wm;
+    const bool kept = m0 < a.width;
+    if (kept) fragments_store(p.dstates + slab_at * 16 * DK, p.largest + (slab_at * 4 + wn) * 4 + 1, wn * QN, lane, d);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     const char* stage = ring.wait(turn);
-    if (mine) {
-      const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
-      const char* coef = stage + L::kTiles + L::kT + L::kP;
-      const long long slab_at = (static_cast<long long>(a.first + c) * p.hv + a.vh) * p.slabs + a.slab;
-      fragments_store(p.dstates + slab_at * 16 * DK, lane, d);
-      float top[2];
-      row_max(d, top);
-      const float most = warp_max(fmaxf(top[0], top[1]));
-      if (lane == 0) p.largest[slab_at * 4 + 1] = most;
-      // (K D)^T
-      float du[8][4] = {};
-      {
-        const Pow2 sd[2] = {pow2_for(top[0]), pow2_for(top[1])};
+    __syncthreads();  // planes of D and this chunk's do are there; the other slab is free
+    if (c > 0)
+      slab_fetch<T, VB>(m.slab[~turn & 1], d_o + (c - 1) * kChunk * p.do_token, p.do_token, kChunk, a.width, p.vec_do);
+    const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
+    const char* coef = stage + L::kTiles + L::kT + L::kP;
+    float2 w[2];
+    {  // do' with the weights of P's rows and with e^G
+      float f[2][4], g[2][4];
+      slab_read<T, VB>(m.slab[turn & 1], wn * 16, m0, lane, f);
 #pragma unroll
-        for (int kk = 0; kk < DK / 16; ++kk) {
-          uint32_t hi[4], lo[4];
-          as_operand<PS>(d[2 * kk], d[2 * kk + 1], sd, hi, lo);
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-            product<PS, IN, false>(du[2 * n], du[2 * n + 1], hi, lo, kt + at_nk<DK>(lane, n * 16, kk * 16), L::kTile);
-        }
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float2 w = coef_at(coef, kTail, n, lane);
-          du[n][0] *= w.x * sd[0].inverse;
-          du[n][1] *= w.y * sd[0].inverse;
-          du[n][2] *= w.x * sd[1].inverse;
-          du[n][3] *= w.y * sd[1].inverse;
-        }
-      }
-      if (c > 0)
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-      __syncwarp();
-      float f[8][4], x[8][4];
-      // + (P^T do')^T: tokens j take from i >= j
-      slab_read<T>(slab, lane, f);
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const float2 w = coef_at(coef, kOutP, n, lane);
-        f[n][0] *= w.x;
-        f[n][1] *= w.y;
-        f[n][2] *= w.x;
-        f[n][3] *= w.y;
-      }
-      {
-        row_max(f, top);
-        const Pow2 sf[2] = {pow2_for(top[0]), pow2_for(top[1])};
-#pragma unroll
-        for (int n = 0; n < 8; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t hi[4], lo[4];
-          as_operand<PO>(f[2 * kk], f[2 * kk + 1], sf, hi, lo);
-#pragma unroll
-          for (int n = 0; n <= kk; ++n)
-            product<PO, PO, true>(x[2 * n], x[2 * n + 1], hi, lo, pt + at_kn<kChunk>(lane, n * 16, kk * 16), L::kSquare);
-        }
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {  // dU, then times the scales of T's rows
-          const float2 w = coef_at(coef, kTRow, n, lane);
-          du[n][0] = (du[n][0] + x[n][0] * sf[0].inverse) * w.x;
-          du[n][1] = (du[n][1] + x[n][1] * sf[0].inverse) * w.y;
-          du[n][2] = (du[n][2] + x[n][2] * sf[1].inverse) * w.x;
-          du[n][3] = (du[n][3] + x[n][3] * sf[1].inverse) * w.y;
-        }
-      }
-      // dX^T = (T^T dU)^T
-      {
-        row_max(du, top);
-        const Pow2 su[2] = {pow2_for(top[0]), pow2_for(top[1])};
-#pragma unroll
-        for (int n = 0; n < 8; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t hi[4], lo[4];
-          as_operand<PS>(du[2 * kk], du[2 * kk + 1], su, hi, lo);
-#pragma unroll
-          for (int n = 0; n <= kk; ++n)
-            product<PS, PS, true>(x[2 * n], x[2 * n + 1], hi, lo, tt + at_kn<kChunk>(lane, n * 16, kk * 16), L::kSquare);
-        }
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          x[n][0] *= su[0].inverse;
-          x[n][1] *= su[0].inverse;
-          x[n][2] *= su[1].inverse;
-          x[n][3] *= su[1].inverse;
-        }
-      }
-      fragments_store(p.dxs + slab_at * 16 * kChunk, lane, x);
-      row_max(x, top);
-      const float most_x = warp_max(fmaxf(top[0], top[1]));
-      if (lane == 0) p.largest[slab_at * 4 + 3] = most_x;
-      // D = e^{G_C} D + (e^G do')^T Q - (beta e^G dX)^T K, all at one scale
-      slab_read<T>(slab, lane, f);
-      __syncwarp();
-      {
-        float out[8][4];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float2 b = coef_at(coef, kBeta, n, lane), wq = coef_at(coef, kOutQ, n, lane), wk = coef_at(coef, kDown, n, lane);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            out[n][e] = (e & 1 ? b.y : b.x) * x[n][e];
-            f[n][e] *= e & 1 ? wq.y : wq.x;
-            x[n][e] *= e & 1 ? -wk.y : -wk.x;
-          }
-        }
-        slab_write<T>(slab, lane, out);
-        __syncwarp();
-        slab_store<T>(slab, dv + c * kChunk * dv_step, dv_step, len, a.width, p.vec_o, lane);
-        __syncwarp();
-      }
-      {
-        const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
-        float td[2], tx[2];
-        row_max(f, top);
-        row_max(x, tx);
-        row_max(d, td);
-        const Pow2 sc[2] = {pow2_for(fmaxf(fmaxf(top[0], tx[0]), decay * td[0])),
-                            pow2_for(fmaxf(fmaxf(top[1], tx[1]), decay * td[1]))};
-#pragma unroll
-        for (int n = 0; n < DK / 8; ++n) {
-          d[n][0] *= decay * sc[0].f;
-          d[n][1] *= decay * sc[0].f;
-          d[n][2] *= decay * sc[1].f;
-          d[n][3] *= decay * sc[1].f;
-        }
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t hi[4], lo[4];
-          as_operand<PS>(f[2 * kk], f[2 * kk + 1], sc, hi, lo);
-#pragma unroll
-          for (int n = 0; n < DK / 16; ++n)
-            product<PS, IN, true>(d[2 * n], d[2 * n + 1], hi, lo, qt + at_kn<DK>(lane, n * 16, kk * 16), L::kTile);
-          as_operand<PS>(x[2 * kk], x[2 * kk + 1], sc, hi, lo);
-#pragma unroll
-          for (int n = 0; n < DK / 16; ++n)
-            product<PS, IN, true>(d[2 * n], d[2 * n + 1], hi, lo, kt + at_kn<DK>(lane, n * 16, kk * 16), L::kTile);
-        }
-#pragma unroll
-        for (int n = 0; n < DK / 8; ++n) {
-          d[n][0] *= sc[0].inverse;
-          d[n][1] *= sc[0].inverse;
-          d[n][2] *= sc[1].inverse;
-          d[n][3] *= sc[1].inverse;
-        }
-      }
+        for (int e = 0; e < 4; ++e) g[n][e] = f[n][e];
+      coef_read(coef, kOutP, wn * 2, lane, w);
+      scale_columns(f, w);
+      tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, f, &m.scale[3][wn][m0]);
+      coef_read(coef, kOutQ, wn * 2, lane, w);
+      scale_columns(g, w);
+      tile_write<PS, kChunk>(m.d, M::kNarrow, m0, wn * 16, lane, g, &m.scale[4][wn][m0]);
     }
+    // (K D)^T
+    float du[2][4] = {};
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      float bx[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < DK / 64; ++k) {
+        const int kk = b * (DK / 64) + k;
+        uint32_t hi[4], lo[4];
+        tile_operand<PS>(dw[kk], M::kWide, hi, lo);
+        product<PS, IN, false>(bx[0], bx[1], hi, lo, kt + kw[kk], L::kTile);
+      }
+      add_scaled(du, bx, &m.scale[0][b][m0], lane);
+    }
+    coef_read(coef, kTail, wn * 2, lane, w);
+    scale_columns(du, w);
+    __syncthreads();
+    // dU = P^T do' + e^{G_C - G} (K D): tokens j take from i >= j
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      if (VB == 64 && kk < wn) continue;  // the other blocks are zero
+      uint32_t hi[4], lo[4];
+      float bx[2][4] = {};
+      tile_operand<PO>(yw[kk] + (wt - yt), M::kNarrow, hi, lo);
+      product<PO, PO, true>(bx[0], bx[1], hi, lo, pt + ts + kk * 16 * kChunk * 2, L::kSquare);
+      add_scaled(du, bx, &m.scale[3][kk][m0], lane);
+    }
+    coef_read(coef, kTRow, wn * 2, lane, w);
+    scale_columns(du, w);
+    tile_write<PS, kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, du, &m.scale[1][wn][m0]);
+    __syncthreads();
+    // dX^T = (T^T dU)^T
+    float x[2][4] = {};
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      if (VB == 64 && kk < wn) continue;  // the other blocks are zero
+      uint32_t hi[4], lo[4];
+      float bx[2][4] = {};
+      tile_operand<PS>(yw[kk], M::kNarrow, hi, lo);
+      product<PS, PS, true>(bx[0], bx[1], hi, lo, tt + ts + kk * 16 * kChunk * 2, L::kSquare);
+      add_scaled(x, bx, &m.scale[1][kk][m0], lane);
+    }
+    if (kept) fragments_store(p.dxs + slab_at * 16 * kChunk, p.largest + (slab_at * 4 + wn) * 4 + 3, wn * 2, lane, x);
+    {
+      float out[2][4], minus[2][4];
+      float2 b[2];
+      coef_read(coef, kBeta, wn * 2, lane, b);
+      coef_read(coef, kDown, wn * 2, lane, w);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          out[n][e] = (e & 1 ? b[n].y : b[n].x) * x[n][e];
+          minus[n][e] = (e & 1 ? -w[n].y : -w[n].x) * x[n][e];
+        }
+      tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, minus, &m.scale[2][wn][m0]);
+      strip_store<T>(m.strip[warp], lane, out, dv + (c * kChunk + wn * 16) * dv_step + m0, dv_step, len - wn * 16, a.width - m0,
+                     p.vec_o);
+    }
+    __syncthreads();
+    // D = e^{G_C} D + (e^G do')^T Q - (beta e^G dX)^T K
+    const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
+#pragma unroll
+    for (int n = 0; n < QN; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[n][e] *= decay;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      uint32_t hi[4], lo[4];
+      float bs[QN][4] = {}, bt[QN][4] = {};
+      tile_operand<PS>(yw[kk] + (ft - yt), M::kNarrow, hi, lo);
+#pragma unroll
+      for (int n = 0; n < QN / 2; ++n)
+        product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, qt + ks[n] + kk * 16 * DK * 2, L::kTile);
+      add_scaled(d, bs, &m.scale[4][kk][m0], lane);
+      tile_operand<PS>(yw[kk] + (xt - yt), M::kNarrow, hi, lo);
+#pragma unroll
+      for (int n = 0; n < QN / 2; ++n)
+        product<PS, IN, true>(bt[2 * n], bt[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile);
+      add_scaled(d, bt, &m.scale[2][kk][m0], lane);
+    }
+    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, &m.scale[0][wn][m0]);
     ring.done(turn, lane);
     if (threadIdx.x == 0 && turn + stages < a.chunks)
       ring.fill(p, turn + stages, a.first + a.chunks - 1 - turn - stages, a.kh, a.vh);
     __syncwarp();
   }
-  if (mine && p.dstate_in) state_store<DK>(p.dstate_in, p, a, lane, d);
+  if (p.dstate_in) state_store(p.dstate_in, p, a, m0, wn * (DK / 4), lane, d);
 }
 
 // ---- what is left, in parallel over chunks ---------------------------------
@@ -343,8 +303,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_gradient(DeltaParams p) {
     if (tid < 4) s.most[tid] = 0;
     const float decay = coef[kDecay * kChunk];
     float most[4] = {};
-    for (int i = 0; i < p.slabs; ++i) {
-      const float4 m = *reinterpret_cast<const float4*>(p.largest + (head_at * p.slabs + i) * 4);
+    for (int i = 0; i < p.slabs * 4; ++i) {
+      const float4 m = *reinterpret_cast<const float4*>(p.largest + (head_at * p.slabs * 4 + i) * 4);
       most[0] = fmaxf(most[0], m.x);
       most[1] = fmaxf(most[1], m.y);
       most[2] = fmaxf(most[2], m.z);

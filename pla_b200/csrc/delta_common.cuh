@@ -68,7 +68,7 @@ struct DeltaParams {
   float* dstate_in;
   float* dstates;    // dS at every chunk's end, fragment order
   float* dxs;        // dX
-  float* largest;    // of S, dS, U, dX in every (chunk, value head, slab): 4 floats
+  float* largest;    // magnitudes of S, dS, U, dX: [chunk, value head, slab, warp, 4]
   void *dq, *dk_out, *dv_out, *dg, *dbeta;
   int slabs;         // ceil(dv / 16)
   int vec_qk, vec_v, vec_o, vec_do;
@@ -225,6 +225,19 @@ __device__ __forceinline__ uint32_t at_km(int lane, int m0, int k0) {
   const int m = lane >> 3;
   return tile_at<W>(k0 + (m >> 1) * 8 + (lane & 7), (m0 >> 3) + (m & 1));
 }
+
+// A lane's ldmatrix addresses walk a tile along a row by 16 columns a step:
+// step k's address is (base ^ 32 (k % 4)) + 128 (k / 4), because the unit
+// permutation only touches address bits 4 to 6.  The four permuted bases are
+// computed once, the rest are instruction offsets.
+struct Walk {
+  uint32_t at[4];
+  __device__ __forceinline__ explicit Walk(uint32_t base) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i] = base ^ (i << 5);
+  }
+  __device__ __forceinline__ uint32_t operator[](int k) const { return at[k & 3] + (k >> 2) * 128; }
+};
 
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));

@@ -1,16 +1,24 @@
 // delta_sweep: walks the chunks of a sequence with the state in registers
 // (delta_common.cuh has the mathematics).
 //
-// The columns of S (one per value feature) never meet, so a warp takes 16 of
-// them through the whole sequence on its own: it holds S^T [16, Dk] as the
-// accumulators of m16n8k16 products.  Every product of a chunk has the value
-// features as its 16 rows,
+// The columns of S (one per value feature) never meet, so a block takes VB of
+// them (16, 32 or 64) through the whole sequence on its own.  Every product of
+// a chunk has the value features as its rows,
 //     (K S)^T = S^T K^T,  U^T = X^T T^T,  O^T = S^T Q^T + U^T P^T,  S^T += U^T K,
-// and the accumulator of one is, register for register, the left operand of
-// the next: state, X and U never leave the registers.  K, Q, T and P are the
-// right operands, read from shared memory by ldmatrix; the warps of a block
-// share them.  They lie in the workspace as whole tiles, already in the
-// shared-memory order, and come by bulk copies a few chunks ahead.
+// so that K, Q, T and P are always the right operand, read by ldmatrix from
+// tiles that lie in the workspace in shared-memory order and come by bulk
+// copies a chunk or two ahead.  The chain of a chunk is three dependent
+// products, and a sequence is hundreds of chunks: its time is latency.  Four
+// warps share 16 value features: warp wn computes 16 of the 64 tokens of K S,
+// X, U and O and a quarter of the features of S, so each step is a few dozen
+// instructions a warp, and operands pass between the warps through shared
+// memory as planes (one barrier a step).  One warp that kept all of S^T in
+// registers instead needed no barrier, but its 400 products and 1500 other
+// instructions a chunk took 8.6 us where this takes KSWEEP us (bf16, Dk = 128).
+//
+// Planes are scaled per row and per 16 tokens (or per quarter of Dk), as each
+// warp knows them; the products of such a block are scaled back and added in
+// fp32 registers, which also keeps the tensor cores' accumulations short.
 #pragma once
 
 #include "delta_common.cuh"
@@ -61,109 +69,108 @@ __device__ __forceinline__ void bulk_copy(void* to, const void* from, uint32_t b
                "l"(from), "r"(bytes), "r"(shared_u32(bar))
                : "memory");
 }
-__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
 
-// The 64 x 16 part of v (or do, or o) that a warp works on, in its own shared
-// memory: rows of 16 features, the pitch spreads eight rows over the banks.
-template <typename T>
+// A chunk's 64 x VB part of v (or do) in shared memory; the pitch spreads
+// eight rows over the banks.
+template <typename T, int VB>
 struct Slab {
-  static constexpr int kPitch = 16 * sizeof(T) + 16;
+  static constexpr int kPitch = VB * sizeof(T) + 16;
   static constexpr int kBytes = kChunk * kPitch;
 };
 
-// Starts the copy of rows [0, len) of a slab; zeros elsewhere.  16-byte
-// copies if the rows allow it, single elements otherwise.
-template <typename T>
-__device__ __forceinline__ void slab_fetch(char* to, const T* from, long long step, int len, int width, int vec, int lane) {
-  constexpr int UNIT = 16 / sizeof(T), PER = 16 / UNIT;  // units of a row
-  if (vec && width == 16 && len == kChunk) {
+// Starts the copy of rows [0, len) and columns [0, width) by the whole block;
+// zeros elsewhere.  16-byte copies if the rows allow it, single elements otherwise.
+template <typename T, int VB>
+__device__ __forceinline__ void slab_fetch(char* to, const T* from, long long step, int len, int width, int vec) {
+  constexpr int UNIT = 16 / sizeof(T), PER = VB / UNIT, THREADS = VB * 8;
+  if (vec) {
 #pragma unroll
-    for (int i = 0; i < kChunk * PER / 32; ++i) {
-      const int at = i * 32 + lane, row = at / PER, u = at % PER;
-      copy16(shared_u32(to) + row * Slab<T>::kPitch + u * 16, from + row * step + u * UNIT);
+    for (int i = 0; i < kChunk * PER / THREADS; ++i) {
+      const int at = i * THREADS + threadIdx.x, row = at / PER, u = at % PER;
+      const bool there = row < len && u * UNIT < width;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_u32(to) + row * Slab<T, VB>::kPitch + u * 16),
+                   "l"(there ? from + row * step + u * UNIT : from), "r"(there ? 16 : 0)
+                   : "memory");
     }
   } else {
-    for (int at = lane; at < kChunk * 16; at += 32) {
-      const int row = at >> 4, col = at & 15;
-      reinterpret_cast<T*>(to + row * Slab<T>::kPitch)[col] =
+    for (int at = threadIdx.x; at < kChunk * VB; at += THREADS) {
+      const int row = at / VB, col = at % VB;
+      reinterpret_cast<T*>(to + row * Slab<T, VB>::kPitch)[col] =
           row < len && col < width ? from[row * step + col] : down<T>(0.f);
     }
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
-// A slab as accumulators of [features x tokens]: f[n][e] of token tile n.
-template <typename T>
-__device__ __forceinline__ void slab_read(const char* from, int lane, float (&f)[8][4]) {
+// 16 tokens x 16 features of a slab as accumulators of [features x tokens].
+template <typename T, int VB>
+__device__ __forceinline__ void slab_read(const char* from, int t0, int f0, int lane, float (&f)[2][4]) {
   if constexpr (sizeof(T) == 2) {
     const int m = lane >> 3;
+    uint32_t r[4];  // tokens 0-7, 8-15; features 0-7 and 8-15 of each
+    ldsm_t(r, shared_u32(from) + (t0 + (m >> 1) * 8 + (lane & 7)) * Slab<T, VB>::kPitch + f0 * 2 + (m & 1) * 16);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      uint32_t r[4];  // token tiles 2n, 2n + 1, features 0-7 and 8-15
-      ldsm_t(r, shared_u32(from) + (n * 16 + (m >> 1) * 8 + (lane & 7)) * Slab<T>::kPitch + (m & 1) * 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const Vec<T, 2> v = *reinterpret_cast<const Vec<T, 2>*>(&r[i]);
-        f[2 * n + (i >> 1)][(i & 1) * 2] = up(v.e[0]);
-        f[2 * n + (i >> 1)][(i & 1) * 2 + 1] = up(v.e[1]);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const Vec<T, 2> v = *reinterpret_cast<const Vec<T, 2>*>(&r[i]);
+      f[i >> 1][(i & 1) * 2] = up(v.e[0]);
+      f[i >> 1][(i & 1) * 2 + 1] = up(v.e[1]);
     }
   } else {
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        f[n][e] = up(reinterpret_cast<const T*>(from + (n * 8 + (lane & 3) * 2 + (e & 1)) *
-                                                           Slab<T>::kPitch)[(lane >> 2) + (e >> 1) * 8]);
+        f[n][e] = up(reinterpret_cast<const T*>(from + (t0 + n * 8 + (lane & 3) * 2 + (e & 1)) *
+                                                           Slab<T, VB>::kPitch)[f0 + (lane >> 2) + (e >> 1) * 8]);
   }
 }
 
+// Accumulators of [16 features x 16 tokens] to rows of a tensor, through 16
+// rows of the warp's own shared memory.
 template <typename T>
-__device__ __forceinline__ void slab_write(char* to, int lane, const float (&f)[8][4]) {
+struct Strip {
+  static constexpr int kPitch = 16 * sizeof(T) + 16;
+  static constexpr int kBytes = 16 * kPitch;
+};
+template <typename T>
+__device__ __forceinline__ void strip_store(char* buffer, int lane, const float (&f)[2][4], T* to, long long step, int len,
+                                            int width, int vec) {
+  constexpr int PITCH = Strip<T>::kPitch;
+  __syncwarp();
   if constexpr (sizeof(T) == 2) {
     const int m = lane >> 3;
+    uint32_t r[4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      uint32_t r[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        Vec<T, 2> v;
-        v.e[0] = down<T>(f[2 * n + (i >> 1)][(i & 1) * 2]);
-        v.e[1] = down<T>(f[2 * n + (i >> 1)][(i & 1) * 2 + 1]);
-        r[i] = *reinterpret_cast<const uint32_t*>(&v);
-      }
-      asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
-                       shared_u32(to) + (n * 16 + (m >> 1) * 8 + (lane & 7)) * Slab<T>::kPitch + (m & 1) * 16),
-                   "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-                   : "memory");
+    for (int i = 0; i < 4; ++i) {
+      Vec<T, 2> v;
+      v.e[0] = down<T>(f[i >> 1][(i & 1) * 2]);
+      v.e[1] = down<T>(f[i >> 1][(i & 1) * 2 + 1]);
+      r[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
+                     shared_u32(buffer) + ((m >> 1) * 8 + (lane & 7)) * PITCH + (m & 1) * 16),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
   } else {
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        reinterpret_cast<T*>(to + (n * 8 + (lane & 3) * 2 + (e & 1)) * Slab<T>::kPitch)[(lane >> 2) + (e >> 1) * 8] =
-            down<T>(f[n][e]);
+        reinterpret_cast<T*>(buffer + (n * 8 + (lane & 3) * 2 + (e & 1)) * PITCH)[(lane >> 2) + (e >> 1) * 8] = down<T>(f[n][e]);
   }
-}
-
-template <typename T>
-__device__ __forceinline__ void slab_store(const char* from, T* to, long long step, int len, int width, int vec, int lane) {
+  __syncwarp();
   constexpr int UNIT = 16 / sizeof(T), PER = 16 / UNIT;
-  if (vec && width == 16) {
+  if (vec) {
 #pragma unroll
-    for (int i = 0; i < kChunk * PER / 32; ++i) {
+    for (int i = 0; i < 16 * PER / 32; ++i) {
       const int at = i * 32 + lane, row = at / PER, u = at % PER;
-      if (row < len)
-        *reinterpret_cast<uint4*>(to + row * step + u * UNIT) =
-            *reinterpret_cast<const uint4*>(from + row * Slab<T>::kPitch + u * 16);
+      if (row < len && u * UNIT < width)
+        *reinterpret_cast<uint4*>(to + row * step + u * UNIT) = *reinterpret_cast<const uint4*>(buffer + row * PITCH + u * 16);
     }
   } else {
-    for (int at = lane; at < kChunk * 16; at += 32) {
+    for (int at = lane; at < 256; at += 32) {
       const int row = at >> 4, col = at & 15;
-      if (row < len && col < width) to[row * step + col] = reinterpret_cast<const T*>(from + row * Slab<T>::kPitch)[col];
+      if (row < len && col < width) to[row * step + col] = reinterpret_cast<const T*>(buffer + row * PITCH)[col];
     }
   }
 }
@@ -188,15 +195,59 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Accumulators of column tiles 2k, 2k + 1, times their rows' factors, as the
-// left operand of step k of the next product.
+// Accumulators of 16 rows x 8 N columns as planes of a tile of W columns, at
+// one scale for each row; the inverses go to `inverse` (16 of them).
+template <int PLANES, int W, int N>
+__device__ __forceinline__ void tile_write(char* tile, uint32_t plane, int row0, int col0, int lane, const float (&f)[N][4],
+                                           float* inverse) {
+  float m[2];
+  row_max(f, m);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const Pow2 s = pow2_for(m[h]);
+    const int row = row0 + (lane >> 2) + h * 8;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      uint32_t hi, lo;
+      split<PLANES>(f[n][2 * h] * s.f, f[n][2 * h + 1] * s.f, &hi, &lo);
+      const uint32_t at = tile_at<W>(row, (col0 >> 3) + n) + (lane & 3) * 4;
+      *reinterpret_cast<uint32_t*>(tile + at) = hi;
+      if (PLANES > 1) *reinterpret_cast<uint32_t*>(tile + plane + at) = lo;
+    }
+    if ((lane & 3) == 0) inverse[(lane >> 2) + h * 8] = s.inverse;
+  }
+}
+
+// Left operand: 16 x 16 of a tile's planes.
 template <int PLANES>
-__device__ __forceinline__ void as_operand(const float (&x)[4], const float (&y)[4], const Pow2 (&s)[2], uint32_t (&hi)[4],
-                                           uint32_t (&lo)[4]) {
-  split<PLANES>(x[0] * s[0].f, x[1] * s[0].f, &hi[0], &lo[0]);
-  split<PLANES>(x[2] * s[1].f, x[3] * s[1].f, &hi[1], &lo[1]);
-  split<PLANES>(y[0] * s[0].f, y[1] * s[0].f, &hi[2], &lo[2]);
-  split<PLANES>(y[2] * s[1].f, y[3] * s[1].f, &hi[3], &lo[3]);
+__device__ __forceinline__ void tile_operand(uint32_t at, uint32_t plane, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  ldsm(hi, at);
+  if (PLANES > 1) ldsm(lo, at + plane);
+}
+
+// f += g, row by row times the inverse of a block's scale.
+template <int N>
+__device__ __forceinline__ void add_scaled(float (&f)[N][4], const float (&g)[N][4], const float* inverse, int lane) {
+  const float a = inverse[lane >> 2], b = inverse[(lane >> 2) + 8];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    f[n][0] = fmaf(g[n][0], a, f[n][0]);
+    f[n][1] = fmaf(g[n][1], a, f[n][1]);
+    f[n][2] = fmaf(g[n][2], b, f[n][2]);
+    f[n][3] = fmaf(g[n][3], b, f[n][3]);
+  }
+}
+
+// Columns (tokens) times their coefficients.
+template <int N>
+__device__ __forceinline__ void scale_columns(float (&f)[N][4], const float2 (&w)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    f[n][0] *= w[n].x;
+    f[n][1] *= w[n].y;
+    f[n][2] *= w[n].x;
+    f[n][3] *= w[n].y;
+  }
 }
 
 // d0, d1 += A B for two column tiles: A in PA planes (hi, lo), B in PB planes
@@ -258,15 +309,15 @@ struct Ring {
   }
 };
 
-// What a block of a sweep works on: value head and slabs of one sequence.
+// What a block of a sweep works on: VB value features of one head of one sequence.
 struct SweepAt {
-  int sequence, vh, kh, slab, batch, lo, len, first, chunks, width;
+  int sequence, vh, kh, column, batch, lo, len, first, chunks, width;
 };
-__device__ __forceinline__ SweepAt sweep_at(const DeltaParams& p, int warps, int warp) {
+__device__ __forceinline__ SweepAt sweep_at(const DeltaParams& p, int vb) {
   SweepAt a;
-  const int parts = (p.slabs + warps - 1) / warps;
+  const int parts = (p.dv + vb - 1) / vb;
   int b = blockIdx.x;
-  a.slab = (b % parts) * warps + warp;
+  a.column = (b % parts) * vb;
   b /= parts;
   a.vh = b % p.hv;
   a.sequence = b / p.hv;
@@ -283,229 +334,225 @@ __device__ __forceinline__ SweepAt sweep_at(const DeltaParams& p, int warps, int
     a.first = a.sequence * p.row_chunks;
   }
   a.chunks = (a.len + kChunk - 1) / kChunk;
-  a.width = min(16, p.dv - a.slab * 16);  // <= 0: a warp without columns only keeps the ring going
+  a.width = min(vb, p.dv - a.column);
   return a;
 }
 
-// S^T of a slab from or to [Dk, Dv] fp32.
-template <int DK>
-__device__ __forceinline__ void state_load(const float* from, const DeltaParams& p, const SweepAt& a, int lane, float (&s)[DK / 8][4]) {
+// A warp's part of S^T, features [col0, col0 + 16) of the block and 8 N of Dk
+// from dk0, from or to [Dk, Dv] fp32.
+template <int N>
+__device__ __forceinline__ void state_load(const float* from, const DeltaParams& p, const SweepAt& a, int col0, int dk0, int lane,
+                                           float (&s)[N][4]) {
 #pragma unroll
-  for (int n = 0; n < DK / 8; ++n)
+  for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int dk = n * 8 + (lane & 3) * 2 + (e & 1), dv = (lane >> 2) + (e >> 1) * 8;
+      const int dk = dk0 + n * 8 + (lane & 3) * 2 + (e & 1), dv = col0 + (lane >> 2) + (e >> 1) * 8;
       s[n][e] = from && dk < p.dk && dv < a.width
-                    ? from[(static_cast<long long>(a.sequence) * p.hv + a.vh) * p.dk * p.dv + static_cast<long long>(dk) * p.dv +
-                           a.slab * 16 + dv]
+                    ? from[((static_cast<long long>(a.sequence) * p.hv + a.vh) * p.dk + dk) * p.dv + a.column + dv]
                     : 0.f;
     }
 }
-template <int DK>
-__device__ __forceinline__ void state_store(float* to, const DeltaParams& p, const SweepAt& a, int lane, const float (&s)[DK / 8][4]) {
-#pragma unroll
-  for (int n = 0; n < DK / 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int dk = n * 8 + (lane & 3) * 2 + (e & 1), dv = (lane >> 2) + (e >> 1) * 8;
-      if (dk < p.dk && dv < a.width)
-        to[(static_cast<long long>(a.sequence) * p.hv + a.vh) * p.dk * p.dv + static_cast<long long>(dk) * p.dv + a.slab * 16 +
-           dv] = s[n][e];
-    }
-}
-// Accumulators in fragment order: [.., column tile, lane, 4].
 template <int N>
-__device__ __forceinline__ void fragments_store(float* to, int lane, const float (&f)[N][4]) {
+__device__ __forceinline__ void state_store(float* to, const DeltaParams& p, const SweepAt& a, int col0, int dk0, int lane,
+                                            const float (&s)[N][4]) {
 #pragma unroll
   for (int n = 0; n < N; ++n)
-    *reinterpret_cast<float4*>(to + (n * 32 + lane) * 4) = make_float4(f[n][0], f[n][1], f[n][2], f[n][3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int dk = dk0 + n * 8 + (lane & 3) * 2 + (e & 1), dv = col0 + (lane >> 2) + (e >> 1) * 8;
+      if (dk < p.dk && dv < a.width)
+        to[((static_cast<long long>(a.sequence) * p.hv + a.vh) * p.dk + dk) * p.dv + a.column + dv] = s[n][e];
+    }
+}
+// Accumulators in fragment order [.., column tile, lane, 4], and the warp's
+// largest magnitude.
+template <int N>
+__device__ __forceinline__ void fragments_store(float* to, float* largest, int tile, int lane, const float (&f)[N][4]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    *reinterpret_cast<float4*>(to + ((tile + n) * 32 + lane) * 4) = make_float4(f[n][0], f[n][1], f[n][2], f[n][3]);
+  float m[2];
+  row_max(f, m);
+  const float most = warp_max(fmaxf(m[0], m[1]));
+  if (lane == 0) *largest = most;
 }
 
-__device__ __forceinline__ float2 coef_at(const char* head, int which, int n, int lane) {
-  return *reinterpret_cast<const float2*>(head + (which * kChunk + n * 8 + (lane & 3) * 2) * 4);
+template <int N>
+__device__ __forceinline__ void coef_read(const char* coef, int which, int tile, int lane, float2 (&w)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    w[n] = *reinterpret_cast<const float2*>(coef + (which * kChunk + (tile + n) * 8 + (lane & 3) * 2) * 4);
 }
 
 constexpr int kSweepRing = 128;  // bytes of the ring's barriers
 
-// KEEP: store S at every chunk's start and U for the backward pass instead of O.
-template <typename T, int DK, int PS, int PO, bool KEEP>
-__global__ void __launch_bounds__(256) delta_sweep(DeltaParams p, int stages) {
-  using L = DeltaLayout<T, DK, PS, PO>;
-  constexpr int IN = L::kIn;
-  extern __shared__ __align__(128) char shared_bytes[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const SweepAt a = sweep_at(p, warps, warp);
-  Ring<L> ring;
-  ring.begin(shared_bytes, stages, warps);
-  char* slabs = shared_bytes + kSweepRing + stages * L::kStage + warp * 2 * Slab<T>::kBytes;
+// Shared memory of a sweep behind the ring: planes of S, X, U and what else
+// the steps hand on, with the inverses of their scales.
+template <typename T, int DK, int PS, int PO, int VB, bool BACK>
+struct SweepShared {
+  static constexpr uint32_t kWide = VB * DK * 2, kNarrow = VB * kChunk * 2;
+  alignas(128) char s[PS * kWide];
+  char a[PS * kNarrow];  // X; back: Y
+  char b[PS * kNarrow];  // e^{G_C - G} U; back: beta e^G dX
+  char c[PO * kNarrow];  // U; back: do' with P's weights
+  char d[BACK ? PS * kNarrow : 128];  // back: e^G do'
+  float scale[BACK ? 5 : 4][4][VB];
+  alignas(16) char slab[2][Slab<T, VB>::kBytes];
+  char strip[VB / 4][Strip<T>::kBytes];
+};
 
-  const T* v = static_cast<const T*>(p.v) + a.batch * p.v_batch + a.lo * p.v_token + a.vh * p.v_head + a.slab * 16;
+// KEEP: store S at every chunk's start and U for the backward pass instead of O.
+template <typename T, int DK, int PS, int PO, int VB, bool KEEP>
+__global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p, int stages) {
+  using L = DeltaLayout<T, DK, PS, PO>;
+  using M = SweepShared<T, DK, PS, PO, VB, false>;
+  constexpr int IN = L::kIn, QN = DK / 32;  // column tiles of a quarter of Dk
+  extern __shared__ __align__(128) char shared_bytes[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wm = warp % (VB / 16), wn = warp / (VB / 16), m0 = wm * 16;
+  const SweepAt a = sweep_at(p, VB);
+  Ring<L> ring;
+  ring.begin(shared_bytes, stages, VB / 4);
+  M& m = *reinterpret_cast<M*>(shared_bytes + kSweepRing + stages * L::kStage);
+  const uint32_t st = shared_u32(m.s), xt = shared_u32(m.a), ut = shared_u32(m.b), vt = shared_u32(m.c);
+
+  const T* v = static_cast<const T*>(p.v) + a.batch * p.v_batch + a.lo * p.v_token + a.vh * p.v_head + a.column;
   const long long o_step = static_cast<long long>(p.hv) * p.dv;
   T* o = KEEP ? nullptr
               : static_cast<T*>(p.o) + (static_cast<long long>(a.batch) * p.tokens + a.lo) * o_step +
-                    static_cast<long long>(a.vh) * p.dv + a.slab * 16;
-  const bool mine = a.width > 0;
-  if (!KEEP && p.cu && mine) {  // rows of no sequence: zero
+                    static_cast<long long>(a.vh) * p.dv + a.column;
+  if (!KEEP && p.cu) {  // rows of no sequence: zero
     if (a.sequence == 0)
-      for (int at = lane; at < a.lo * 16; at += 32)
-        if ((at & 15) < a.width) o[((at >> 4) - a.lo) * o_step + (at & 15)] = down<T>(0.f);
+      for (long long at = threadIdx.x; at < a.lo * static_cast<long long>(VB); at += VB * 8)
+        if (at % VB < a.width) o[(at / VB - a.lo) * o_step + at % VB] = down<T>(0.f);
     if (a.sequence == p.sequences - 1)
-      for (long long at = lane; at < (p.tokens - a.lo - a.len) * 16ll; at += 32)
-        if ((at & 15) < a.width) o[(a.len + (at >> 4)) * o_step + (at & 15)] = down<T>(0.f);
+      for (long long at = threadIdx.x; at < (p.tokens - a.lo - a.len) * static_cast<long long>(VB); at += VB * 8)
+        if (at % VB < a.width) o[(a.len + at / VB) * o_step + at % VB] = down<T>(0.f);
   }
-  float s[DK / 8][4];
-  state_load<DK>(mine ? p.state_in : nullptr, p, a, lane, s);
   if (threadIdx.x == 0)
     for (int i = 0; i < stages && i < a.chunks; ++i) ring.fill(p, i, a.first + i, a.kh, a.vh);
-  if (mine && a.chunks) slab_fetch<T>(slabs, v, p.v_token, min(a.len, kChunk), a.width, p.vec_v, lane);
+  if (a.chunks) slab_fetch<T, VB>(m.slab[0], v, p.v_token, min(a.len, kChunk), a.width, p.vec_v);
+  const Walk sw(st + at_mk<DK>(lane, m0, 0)), xw(xt + at_mk<kChunk>(lane, m0, 0));  // planes of S and X; U's follow X's
+  const Walk kw(at_nk<DK>(lane, wn * 16, 0)), tw(at_nk<kChunk>(lane, wn * 16, 0));  // in K and Q; in T and P
+  uint32_t ks[QN / 2];  // in K, for the state's update
+#pragma unroll
+  for (int n = 0; n < QN / 2; ++n) ks[n] = at_kn<DK>(lane, wn * (DK / 4) + n * 16, 0);
+  float s[QN][4];
+  state_load(p.state_in, p, a, m0, wn * (DK / 4), lane, s);
+  tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, &m.scale[0][wn][m0]);
 
   for (int c = 0; c < a.chunks; ++c) {
     const int len = min(kChunk, a.len - c * kChunk);
-    char* slab = slabs + (c & 1) * Slab<T>::kBytes;
-    if (mine && c + 1 < a.chunks)
-      slab_fetch<T>(slabs + (~c & 1) * Slab<T>::kBytes, v + (c + 1) * kChunk * p.v_token, p.v_token,
-                    min(kChunk, a.len - (c + 1) * kChunk), a.width, p.vec_v, lane);
+    const long long slab_at = (static_cast<long long>(a.first + c) * p.hv + a.vh) * p.slabs + a.column / 16 + wm;
+    const bool kept = m0 < a.width;
+    if (KEEP && kept)
+      fragments_store(p.states + slab_at * 16 * DK, p.largest + (slab_at * 4 + wn) * 4, wn * QN, lane, s);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     const char* stage = ring.wait(c);
-    if (mine) {
-      const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
-      const char* coef = stage + L::kTiles + L::kT + L::kP;
-      const long long slab_at = (static_cast<long long>(a.first + c) * p.hv + a.vh) * p.slabs + a.slab;
-      if (KEEP) fragments_store(p.states + slab_at * 16 * DK, lane, s);
-      float top[2];
-      row_max(s, top);
-      if (KEEP) {
-        const float most = warp_max(fmaxf(top[0], top[1]));
-        if (lane == 0) p.largest[slab_at * 4] = most;
-      }
-      const Pow2 ss[2] = {pow2_for(top[0]), pow2_for(top[1])};
-      float x[8][4] = {}, o_acc[8][4] = {};
-      // (K S)^T and (Q S)^T
+    __syncthreads();  // planes of S and this chunk's v are there; the other slab is free
+    if (c + 1 < a.chunks)
+      slab_fetch<T, VB>(m.slab[~c & 1], v + (c + 1) * kChunk * p.v_token, p.v_token, min(kChunk, a.len - (c + 1) * kChunk),
+                        a.width, p.vec_v);
+    const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
+    const char* coef = stage + L::kTiles + L::kT + L::kP;
+    float x[2][4] = {}, q[2][4] = {};
+    float2 w[2];
+    // (K S)^T and (Q S)^T
 #pragma unroll
-      for (int kk = 0; kk < DK / 16; ++kk) {
+    for (int b = 0; b < 4; ++b) {
+      float bx[2][4] = {}, bq[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < DK / 64; ++k) {
+        const int kk = b * (DK / 64) + k;
         uint32_t hi[4], lo[4];
-        as_operand<PS>(s[2 * kk], s[2 * kk + 1], ss, hi, lo);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint32_t at = at_nk<DK>(lane, n * 16, kk * 16);
-          product<PS, IN, false>(x[2 * n], x[2 * n + 1], hi, lo, kt + at, L::kTile);
-          if (!KEEP) product<PO, IN, false>(o_acc[2 * n], o_acc[2 * n + 1], hi, lo, qt + at, L::kTile);
-        }
+        tile_operand<PS>(sw[kk], M::kWide, hi, lo);
+        product<PS, IN, false>(bx[0], bx[1], hi, lo, kt + kw[kk], L::kTile);
+        if (!KEEP) product<PO, IN, false>(bq[0], bq[1], hi, lo, qt + kw[kk], L::kTile);
       }
-      // X = beta v - beta e^G K S
-      if (c + 1 < a.chunks)
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-      __syncwarp();
-      {
-        float vv[8][4];
-        slab_read<T>(slab, lane, vv);
+      add_scaled(x, bx, &m.scale[0][b][m0], lane);
+      if (!KEEP) add_scaled(q, bq, &m.scale[0][b][m0], lane);
+    }
+    {  // X = beta v - beta e^G K S
+      float vv[2][4];
+      slab_read<T, VB>(m.slab[c & 1], wn * 16, m0, lane, vv);
+      float2 b[2];
+      coef_read(coef, kBeta, wn * 2, lane, b);
+      coef_read(coef, kDown, wn * 2, lane, w);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float2 b = coef_at(coef, kBeta, n, lane), w = coef_at(coef, kDown, n, lane);
-          x[n][0] = b.x * vv[n][0] - w.x * (x[n][0] * ss[0].inverse);
-          x[n][1] = b.y * vv[n][1] - w.y * (x[n][1] * ss[0].inverse);
-          x[n][2] = b.x * vv[n][2] - w.x * (x[n][2] * ss[1].inverse);
-          x[n][3] = b.y * vv[n][3] - w.y * (x[n][3] * ss[1].inverse);
-        }
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[n][e] = (e & 1 ? b[n].y : b[n].x) * vv[n][e] - (e & 1 ? w[n].y : w[n].x) * x[n][e];
+    }
+    tile_write<PS, kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, x, &m.scale[1][wn][m0]);
+    __syncthreads();
+    // U^T = X^T T^T, T lower triangular
+    float u[2][4] = {};
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      if (VB == 64 && kk > wn) break;  // T's other blocks are zero
+      uint32_t hi[4], lo[4];
+      float bu[2][4] = {};
+      tile_operand<PS>(xw[kk], M::kNarrow, hi, lo);
+      product<PS, PS, false>(bu[0], bu[1], hi, lo, tt + tw[kk], L::kSquare);
+      add_scaled(u, bu, &m.scale[1][kk][m0], lane);
+    }
+    coef_read(coef, kTRow, wn * 2, lane, w);
+    scale_columns(u, w);
+    if (KEEP) {
+      if (kept) fragments_store(p.us + slab_at * 16 * kChunk, p.largest + (slab_at * 4 + wn) * 4 + 2, wn * 2, lane, u);
+    } else {
+      tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, u, &m.scale[3][wn][m0]);
+    }
+    coef_read(coef, kTail, wn * 2, lane, w);
+    scale_columns(u, w);
+    tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, u, &m.scale[2][wn][m0]);
+    __syncthreads();
+    // S^T = e^{G_C} S^T + (e^{G_C - G} U)^T K
+    const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
+#pragma unroll
+    for (int n = 0; n < QN; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] *= decay;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      uint32_t hi[4], lo[4];
+      float bs[QN][4] = {};
+      tile_operand<PS>(xw[kk] + (ut - xt), M::kNarrow, hi, lo);
+#pragma unroll
+      for (int n = 0; n < QN / 2; ++n)
+        product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile);
+      add_scaled(s, bs, &m.scale[2][kk][m0], lane);
+    }
+    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, &m.scale[0][wn][m0]);
+    if (!KEEP) {  // O^T = (Q S)^T + U^T P^T, each with its weights
+      float pu[2][4] = {};
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        if (VB == 64 && kk > wn) break;
+        uint32_t hi[4], lo[4];
+        float bu[2][4] = {};
+        tile_operand<PO>(xw[kk] + (vt - xt), M::kNarrow, hi, lo);
+        product<PO, PO, false>(bu[0], bu[1], hi, lo, pt + tw[kk], L::kSquare);
+        add_scaled(pu, bu, &m.scale[3][kk][m0], lane);
       }
-      // U^T = X^T T^T, T lower triangular
-      float u[8][4] = {};
-      {
-        row_max(x, top);
-        const Pow2 sx[2] = {pow2_for(top[0]), pow2_for(top[1])};
+      float2 wq[2];
+      coef_read(coef, kOutQ, wn * 2, lane, wq);
+      coef_read(coef, kOutP, wn * 2, lane, w);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t hi[4], lo[4];
-          as_operand<PS>(x[2 * kk], x[2 * kk + 1], sx, hi, lo);
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int n = kk; n < 4; ++n)
-            product<PS, PS, false>(u[2 * n], u[2 * n + 1], hi, lo, tt + at_nk<kChunk>(lane, n * 16, kk * 16), L::kSquare);
-        }
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float2 w = coef_at(coef, kTRow, n, lane);
-          u[n][0] *= w.x * sx[0].inverse;
-          u[n][1] *= w.y * sx[0].inverse;
-          u[n][2] *= w.x * sx[1].inverse;
-          u[n][3] *= w.y * sx[1].inverse;
-        }
-      }
-      if (KEEP) {
-        fragments_store(p.us + slab_at * 16 * kChunk, lane, u);
-        row_max(u, top);
-        const float most = warp_max(fmaxf(top[0], top[1]));
-        if (lane == 0) p.largest[slab_at * 4 + 2] = most;
-      } else {  // O^T = (Q S)^T + U^T P^T, each with its weights
-        row_max(u, top);
-        const Pow2 su[2] = {pow2_for(top[0]), pow2_for(top[1])};
-        float pu[8][4] = {};
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t hi[4], lo[4];
-          as_operand<PO>(u[2 * kk], u[2 * kk + 1], su, hi, lo);
-#pragma unroll
-          for (int n = kk; n < 4; ++n)
-            product<PO, PO, false>(pu[2 * n], pu[2 * n + 1], hi, lo, pt + at_nk<kChunk>(lane, n * 16, kk * 16), L::kSquare);
-        }
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float2 wq = coef_at(coef, kOutQ, n, lane), wp = coef_at(coef, kOutP, n, lane);
-          o_acc[n][0] = wq.x * (o_acc[n][0] * ss[0].inverse) + wp.x * (pu[n][0] * su[0].inverse);
-          o_acc[n][1] = wq.y * (o_acc[n][1] * ss[0].inverse) + wp.y * (pu[n][1] * su[0].inverse);
-          o_acc[n][2] = wq.x * (o_acc[n][2] * ss[1].inverse) + wp.x * (pu[n][2] * su[1].inverse);
-          o_acc[n][3] = wq.y * (o_acc[n][3] * ss[1].inverse) + wp.y * (pu[n][3] * su[1].inverse);
-        }
-        __syncwarp();
-        slab_write<T>(slab, lane, o_acc);
-        __syncwarp();
-        slab_store<T>(slab, o + c * kChunk * o_step, o_step, len, a.width, p.vec_o, lane);
-        __syncwarp();
-      }
-      // S^T = e^{G_C} S^T + (e^{G_C - G} U)^T K: both at one scale
-      {
-        const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
-        float su[2], sd[2];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float2 w = coef_at(coef, kTail, n, lane);
-          u[n][0] *= w.x;
-          u[n][1] *= w.y;
-          u[n][2] *= w.x;
-          u[n][3] *= w.y;
-        }
-        row_max(u, su);
-        row_max(s, sd);
-        const Pow2 sc[2] = {pow2_for(fmaxf(su[0], decay * sd[0])), pow2_for(fmaxf(su[1], decay * sd[1]))};
-#pragma unroll
-        for (int n = 0; n < DK / 8; ++n) {
-          s[n][0] *= decay * sc[0].f;
-          s[n][1] *= decay * sc[0].f;
-          s[n][2] *= decay * sc[1].f;
-          s[n][3] *= decay * sc[1].f;
-        }
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t hi[4], lo[4];
-          as_operand<PS>(u[2 * kk], u[2 * kk + 1], sc, hi, lo);
-#pragma unroll
-          for (int n = 0; n < DK / 16; ++n)
-            product<PS, IN, true>(s[2 * n], s[2 * n + 1], hi, lo, kt + at_kn<DK>(lane, n * 16, kk * 16), L::kTile);
-        }
-#pragma unroll
-        for (int n = 0; n < DK / 8; ++n) {
-          s[n][0] *= sc[0].inverse;
-          s[n][1] *= sc[0].inverse;
-          s[n][2] *= sc[1].inverse;
-          s[n][3] *= sc[1].inverse;
-        }
-      }
+        for (int e = 0; e < 4; ++e)
+          q[n][e] = (e & 1 ? wq[n].y : wq[n].x) * q[n][e] + (e & 1 ? w[n].y : w[n].x) * pu[n][e];
+      strip_store<T>(m.strip[warp], lane, q, o + (c * kChunk + wn * 16) * o_step + m0, o_step, len - wn * 16, a.width - m0,
+                     p.vec_o);
     }
     ring.done(c, lane);
     if (threadIdx.x == 0 && c + stages < a.chunks) ring.fill(p, c + stages, a.first + c + stages, a.kh, a.vh);
     __syncwarp();
   }
-  if (mine && p.state_out) state_store<DK>(p.state_out, p, a, lane, s);
+  if (p.state_out) state_store(p.state_out, p, a, m0, wn * (DK / 4), lane, s);
 }
 
 }  // namespace seq

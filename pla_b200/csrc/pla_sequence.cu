@@ -290,7 +290,7 @@ DeltaSizes delta_sizes_of(const pla_delta* a, bool backward) {
     const size_t columns = static_cast<size_t>(s.chunks) * a->hv * ((a->dv + 15) / 16) * 16;
     s.states = up256(columns * DK * sizeof(float));
     s.us = up256(columns * kChunk * sizeof(float));
-    s.largest = up256(columns / 16 * 4 * sizeof(float));
+    s.largest = up256(columns * sizeof(float));
   }
   s.total = s.plan + s.tiles + s.heads + 2 * s.states + 2 * s.us + s.largest;
   return s;
@@ -367,7 +367,7 @@ DeltaParams delta_params(const pla_delta* a, const DeltaSizes& s) {
   const int whole = static_cast<int>(16 / es);
   p.vec_qk = a->dk % 4 == 0 && aligned_to(a->q, 4 * es) && aligned_to(a->k, 4 * es) &&
              !((a->q_batch | a->q_token | a->q_head | a->k_batch | a->k_token | a->k_head) % 4);
-  p.vec_v = aligned_to(a->v, 16) && !((a->v_batch | a->v_token | a->v_head) % whole);
+  p.vec_v = a->dv % whole == 0 && aligned_to(a->v, 16) && !((a->v_batch | a->v_token | a->v_head) % whole);
   p.vec_o = aligned_to(a->o, 16) && a->dv % whole == 0;
   return p;
 }
@@ -388,49 +388,59 @@ int launch_prepare(const DeltaParams& p, cudaStream_t stream) {
   return launched("delta_prepare");
 }
 
-// Warps of a block share the chunk's tiles, but a block is one SM's: few
-// warps a block while that leaves SMs without one.
-int sweep_warps(const DeltaParams& p, int sms) {
-  int warps = std::min(8, p.slabs);
-  while (warps > 1 &&
-         static_cast<long long>(p.sequences) * p.hv * ((p.slabs + warps - 1) / warps) < sms)
-    warps = (warps + 1) / 2;
-  return warps;
-}
-
-// Stages of the ring, shared memory and grid of a sweep.
-template <typename T, typename L>
+// Stages of the ring and shared memory of a sweep.
+template <typename T, int DK, int PS, int PO, int VB, bool BACK>
 struct SweepShape {
-  int warps, stages;
-  long long grid;
-  size_t shared;
-  SweepShape(const DeltaParams& p, int sms) {
-    warps = sweep_warps(p, sms);
-    grid = static_cast<long long>(p.sequences) * p.hv * ((p.slabs + warps - 1) / warps);
-    const size_t slabs = static_cast<size_t>(warps) * 2 * Slab<T>::kBytes;
-    stages = static_cast<int>(std::min<size_t>(3, (227 * 1024 - kSweepRing - slabs) / L::kStage));
-    shared = kSweepRing + stages * L::kStage + slabs;
+  using L = DeltaLayout<T, DK, PS, PO>;
+  static constexpr size_t kHeld = kSweepRing + sizeof(SweepShared<T, DK, PS, PO, VB, BACK>);
+  static constexpr size_t kRoom = kHeld < 227 * 1024 ? (227 * 1024 - kHeld) / L::kStage : 0;
+  static constexpr int kStages = kRoom < 3 ? kRoom : 3;
+  static constexpr size_t kShared = kHeld + kStages * L::kStage;
+  static long long grid(const DeltaParams& p) {
+    return static_cast<long long>(p.sequences) * p.hv * ((p.dv + VB - 1) / VB);
   }
 };
 
+// Value features of a sweep's block.  A block's time is the latency of its
+// chunks' chain whatever it holds, so the fewest features that still put every
+// block on an SM of its own; many sequences or heads fill the SMs anyway, and
+// more features share one copy of a chunk's tiles, as long as shared memory
+// holds the next chunk's beside it.  f(features)
+template <typename T, int DK, int PS, int PO, bool BACK, typename F>
+int with_columns(const DeltaParams& p, int sms, F&& f) {
+  constexpr int kMost = SweepShape<T, DK, PS, PO, 64, BACK>::kStages >= 2 ? 64 : 32;
+  static_assert(SweepShape<T, DK, PS, PO, kMost, BACK>::kStages >= 1, "no room for a chunk's tiles");
+  const long long heads = static_cast<long long>(p.sequences) * p.hv;
+  if (p.dv <= 16 || heads * ((p.dv + 15) / 16) <= sms) return f(Int<16>{});
+  if (p.dv <= 32 || heads * ((p.dv + 31) / 32) <= sms) return f(Int<32>{});
+  return f(Int<kMost>{});
+}
+
 template <typename T, int DK, int PS, int PO, bool KEEP>
 int launch_sweep(const DeltaParams& p, int sms, cudaStream_t stream) {
-  const SweepShape<T, DeltaLayout<T, DK, PS, PO>> at(p, sms);
-  if (at.grid > kMaxGrid) return PLA_ERR_TOO_LARGE;
-  if (!at.grid) return PLA_OK;
-  const int st = allow_shared<delta_sweep<T, DK, PS, PO, KEEP>>(at.shared);
-  if (st != PLA_OK) return st;
-  delta_sweep<T, DK, PS, PO, KEEP><<<static_cast<int>(at.grid), at.warps * 32, at.shared, stream>>>(p, at.stages);
-  return launched("delta_sweep");
+  return with_columns<T, DK, PS, PO, false>(p, sms, [&](auto vb) {
+    constexpr int VB = decltype(vb)::value;
+    using S = SweepShape<T, DK, PS, PO, VB, false>;
+    const long long grid = S::grid(p);
+    if (grid > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
+    const int st = allow_shared<delta_sweep<T, DK, PS, PO, VB, KEEP>>(S::kShared);
+    if (st != PLA_OK) return st;
+    delta_sweep<T, DK, PS, PO, VB, KEEP><<<static_cast<int>(grid), VB * 8, S::kShared, stream>>>(p, S::kStages);
+    return launched("delta_sweep");
+  });
 }
 
 template <typename T, int DK, int PS, int PO>
 int launch_gradient(const DeltaParams& p, int sms, cudaStream_t stream) {
-  const SweepShape<T, DeltaLayout<T, DK, PS, PO>> at(p, sms);
-  int st = allow_shared<delta_sweep_back<T, DK, PS, PO>>(at.shared);
+  int st = with_columns<T, DK, PS, PO, true>(p, sms, [&](auto vb) {
+    constexpr int VB = decltype(vb)::value;
+    using S = SweepShape<T, DK, PS, PO, VB, true>;
+    const int st = allow_shared<delta_sweep_back<T, DK, PS, PO, VB>>(S::kShared);
+    if (st != PLA_OK) return st;
+    delta_sweep_back<T, DK, PS, PO, VB><<<static_cast<int>(S::grid(p)), VB * 8, S::kShared, stream>>>(p, S::kStages);
+    return launched("delta_sweep_back");
+  });
   if (st != PLA_OK) return st;
-  delta_sweep_back<T, DK, PS, PO><<<static_cast<int>(at.grid), at.warps * 32, at.shared, stream>>>(p, at.stages);
-  if ((st = launched("delta_sweep_back")) != PLA_OK) return st;
   if (p.cu) {
     delta_clear_rows<T><<<std::min(p.tokens + 1, 4 * sms), 256, 0, stream>>>(p);
     if ((st = launched("delta_clear_rows")) != PLA_OK) return st;
@@ -741,7 +751,7 @@ int pla_gated_delta_rule_backward(const pla_delta* a, const pla_delta_gradient* 
     p.dstate_in = g->dstate_in;
     p.dq = g->dq, p.dk_out = g->dk, p.dv_out = g->dv, p.dg = g->dg, p.dbeta = g->dbeta;
     const int whole = static_cast<int>(16 / es);
-    p.vec_do = aligned_to(g->d_o, 16) && !((g->do_batch | g->do_token | g->do_head) % whole);
+    p.vec_do = a->dv % whole == 0 && aligned_to(g->d_o, 16) && !((g->do_batch | g->do_token | g->do_head) % whole);
     p.vec_o = aligned_to(g->dv, 16) && a->dv % whole == 0;
     p.state_out = nullptr;
     int st = launch_prepare<T, DK, PS, PO>(p, as_stream(stream));
