@@ -8,9 +8,8 @@
 //     N = Gamma . dP           B = beta Gamma . dA          Gamma_ij = e^{G_i - G_j}
 //     dq = e^G (do' S0^T) + N K
 //     dk = -beta e^G (dX S0^T) + e^{G_C - G} (U D^T) + N^T Q + (B + B^T) K
-//     dbeta = -e^G k . (dX S0^T) + dX . v + rowsum(Gamma . dA . K K^T)
-//     dG = beta part of the same + q . dq_state + rowsum(Z) - colsum(Z) - H,
-//          Z = N . (Q K^T) + B . (K K^T),  H = e^{G_C - G} k . (U D^T),
+//     dbeta = k . (Y - e^G dX S0^T) + dX . v,    Y = (Gamma . dA) K
+//     dG = beta k . (Y - e^G dX S0^T) + q . dq - k . (N^T Q + B^T K) - H,    H = e^{G_C - G} k . (U D^T)
 //     dG_C += e^{G_C} <S0, D> + sum H,      dg = sums of dG from each token to the chunk's end.
 // S0 and U come from the forward's sweep run again: the forward keeps only its
 // inputs.  Every sum has a fixed order.
@@ -55,14 +54,14 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int st
 
   for (int turn = 0; turn < a.chunks; ++turn) {
     const int c = a.chunks - 1 - turn, len = min(kChunk, a.len - c * kChunk);
-    const long long slab_at = (static_cast<long long>(a.first + c) * p.hv + a.vh) * p.slabs + a.column / 16 + wm;
-    const bool kept = m0 < a.width;
-    if (kept) fragments_store(p.dstates + slab_at * 16 * DK, p.largest + (slab_at * 4 + wn) * 4 + 1, wn * QN, lane, d);
+    const long long head_at = static_cast<long long>(a.first + c) * p.hv + a.vh;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     const char* stage = ring.wait(turn);
     __syncthreads();  // planes of D and this chunk's do are there; the other slab is free
     if (c > 0)
       slab_fetch<T, VB>(m.slab[~turn & 1], d_o + (c - 1) * kChunk * p.do_token, p.do_token, kChunk, a.width, p.vec_do);
+    keep_tile<PS, VB, DK>(m.s, m.scale[0], p.dstates + kept_at<PS, DK>(p, head_at), p.scales + (head_at * 16 + 4) * p.rows,
+                          p.rows, a.column);
     const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
     const char* coef = stage + L::kTiles + L::kT + L::kP;
     float2 w[2];
@@ -122,7 +121,7 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int st
       product<PS, PS, true>(bx[0], bx[1], hi, lo, tt + ts + kk * 16 * kChunk * 2, L::kSquare);
       add_scaled(x, bx, &m.scale[1][kk][m0], lane);
     }
-    if (kept) fragments_store(p.dxs + slab_at * 16 * kChunk, p.largest + (slab_at * 4 + wn) * 4 + 3, wn * 2, lane, x);
+    tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, x, &m.scale[3][wn][m0]);  // PO = PS; do' is done with
     {
       float out[2][4], minus[2][4];
       float2 b[2];
@@ -140,6 +139,8 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int st
                      p.vec_o);
     }
     __syncthreads();
+    keep_tile<PO, VB, kChunk>(m.c, m.scale[3], p.dxs + kept_at<PO, kChunk>(p, head_at), p.scales + (head_at * 16 + 12) * p.rows,
+                              p.rows, a.column);
     // D = e^{G_C} D + (e^G do')^T Q - (beta e^G dX)^T K
     const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
 #pragma unroll
@@ -171,7 +172,14 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int st
 }
 
 // ---- what is left, in parallel over chunks ---------------------------------
-constexpr int kGradThreads = 256;
+// One (chunk, key head) a block, its value heads one after another, 64 value
+// features at a time; 16 warps, each 16 tokens of a quarter of Dk (and of the
+// 64 x 64 matrices).  S0, D, U and dX come as the planes that the sweeps had as
+// operands; their row scales are brought to one by exact powers of two on the
+// way to shared memory, because here the value features are summed over.  The
+// row and column sums over N . (Q K^T) and B . (K K^T) are taken as q . (N K),
+// k . (N^T Q) and so on, so neither Q K^T nor K K^T is needed.
+constexpr int kGradThreads = 512;
 constexpr int kGradBlock = 64;  // value features at a time
 
 template <typename T, int DK, int PS>
@@ -184,365 +192,414 @@ struct GradShared {
       __half u[PS][kGradBlock * kChunk], x[PS][kGradBlock * kChunk];                    // U^T, dX^T
       __half o[PS][kChunk * kGradBlock];                                                // do
     } in;
-    alignas(128) __half square[4][PS][kChunk * kChunk];  // N f_k, N f_q (rows), B f_k, B f_k (rows)
+    alignas(128) __half square[4][PS][kChunk * kChunk];  // N f_k, N f_q (rows), Gamma dA f_k, B f_k (rows)
   };
-  float kk[kChunk][kChunk + 2], qk[kChunk][kChunk + 2];
-  float krow[kChunk], qrow[kChunk], orow[kChunk], oscale[kChunk];
+  float krow[kChunk], qrow[kChunk], orow[kChunk];
   float beta[kChunk], hi[kChunk], lo[kChunk], down[kChunk], tail[kChunk];  // down: e^G, tail: e^{G_C - G}
-  float dots[2][3][kChunk];    // column halves: k.r1, q.dq, k.r3
-  float rows[2][2][kChunk];    // column halves: row sums of Z, of Gamma dA K K^T
-  float cols[4][kChunk];       // row blocks: column sums of Z
-  float warp_sum[8];
-  unsigned int most[4];
-  float xv[kChunk];            // dX . v
+  float ratio[4][4][128];      // a row's scale over the common one: S, dS, U, dX; quarters of the columns
+  float dots[4][4][kChunk];    // quarters of Dk: k.r1, q.dq, k.(r3 + ..), k.Y
+  float xv[8][kChunk];         // dX . v, groups of value features
+  float warp_sum[16];
+  unsigned int common[4], most[4];
 };
-
-// Fragments [slab][tile n][lane][4] of a [feature][W] matrix as planes in shared memory.
-template <int PS, int W>
-__device__ __forceinline__ void tile_from_fragments(const float4& f, float scale, char* tile, uint32_t plane, int slab, int n, int lane) {
-  const int row = slab * 16 + (lane >> 2);
-  uint32_t hi, lo;
-  uint32_t at = tile_at<W>(row, n) + (lane & 3) * 4;
-  split<PS>(f.x * scale, f.y * scale, &hi, &lo);
-  *reinterpret_cast<uint32_t*>(tile + at) = hi;
-  if (PS > 1) *reinterpret_cast<uint32_t*>(tile + plane + at) = lo;
-  at = tile_at<W>(row + 8, n) + (lane & 3) * 4;
-  split<PS>(f.z * scale, f.w * scale, &hi, &lo);
-  *reinterpret_cast<uint32_t*>(tile + at) = hi;
-  if (PS > 1) *reinterpret_cast<uint32_t*>(tile + plane + at) = lo;
-}
-
-// acc[2 n], acc[2 n + 1] += A B over PA x PB planes, lo x lo left out.
-template <int PA, int PB, bool A_T, bool B_T>
-__device__ __forceinline__ void tile_product(float (&d0)[4], float (&d1)[4], uint32_t a_at, uint32_t a_plane, uint32_t b_at,
-                                             uint32_t b_plane) {
-#pragma unroll
-  for (int i = 0; i < PA; ++i) {
-    uint32_t a[4];
-    if (A_T) ldsm_t(a, a_at + i * a_plane); else ldsm(a, a_at + i * a_plane);
-#pragma unroll
-    for (int j = 0; i + j < (PA > PB ? PA : PB) && j < PB; ++j) {
-      uint32_t b[4];
-      if (B_T) ldsm_t(b, b_at + j * b_plane); else ldsm(b, b_at + j * b_plane);
-      mma(d0, a, b[0], b[1]);
-      mma(d1, a, b[2], b[3]);
-    }
-  }
-}
 
 __device__ __forceinline__ float quad_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-template <typename G>
-__device__ __forceinline__ void store_pair(G* to, float a, float b, int n) {
-  if (n > 0) to[0] = down<G>(a);
-  if (n > 1) to[1] = down<G>(b);
+// d0, d1 += A B over planes, lo x lo left out.
+template <int PA, int PB>
+__device__ __forceinline__ void planes_product(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[PA][4], const uint32_t (&b)[PB][4]) {
+#pragma unroll
+  for (int i = 0; i < PA; ++i)
+#pragma unroll
+    for (int j = 0; j < PB; ++j) {
+      if (i + j >= (PA > PB ? PA : PB)) continue;
+      mma(d0, a[i], b[j][0], b[j][1]);
+      mma(d1, a[i], b[j][2], b[j][3]);
+    }
+}
+template <int PLANES, bool TRANS>
+__device__ __forceinline__ void planes_load(uint32_t (&f)[PLANES][4], uint32_t at, uint32_t plane) {
+#pragma unroll
+  for (int i = 0; i < PLANES; ++i)
+    if (TRANS) ldsm_t(f[i], at + i * plane); else ldsm(f[i], at + i * plane);
+}
+
+// Rows [row0, row0 + 64) of kept planes into a tile, times their rows' ratios.
+// Gives the sum over the values of the product with what the last call's did
+// (DOT), to be scaled by the caller: <S, D>.
+template <int PS, int W>
+__device__ __forceinline__ void load_kept(const char* from, int rows, int row0, int used, const float (*ratio)[128], char* tile, int tid) {
+  constexpr int UNITS = kGradBlock * W / 8;
+#pragma unroll
+  for (int i = 0; i < UNITS / kGradThreads; ++i) {
+    const int at = i * kGradThreads + tid, row = at / (W / 8), unit = (at % (W / 8)) ^ (row & 7);
+    const __half2 f = __float2half2_rn(row0 + row < used ? ratio[unit / (W / 32)][row0 + row] : 0.f);
+#pragma unroll
+    for (int n = 0; n < PS; ++n) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row0 + row < used)
+        v = reinterpret_cast<const uint4*>(from + (static_cast<long long>(n) * rows + row0) * W * 2)[at];
+      __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = __hmul2(h[e], f);
+      reinterpret_cast<uint4*>(tile + n * kGradBlock * W * 2)[at] = v;
+    }
+  }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* to, const float (&f)[N], int count, bool whole) {
+  if (whole) {
+    store<T, N>(to, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < count) to[i] = down<T>(f[i]);
+  }
 }
 
 template <typename T, int DK, int PS, int PO>
-__global__ void __launch_bounds__(kGradThreads) delta_gradient(DeltaParams p) {
+__global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p) {
   using L = DeltaLayout<T, DK, PS, PO>;
-  constexpr int IN = L::kIn;
+  constexpr int IN = L::kIn, NT = DK / 32;  // column tiles of a warp
   constexpr uint32_t kWide = kGradBlock * DK * 2, kNarrow = kGradBlock * kChunk * 2, kSq = kChunk * kChunk * 2;
-  constexpr int NT = DK / 16;  // column tiles of a warp's half of the DK columns
   extern __shared__ __align__(128) char shared_bytes[];
   GradShared<T, DK, PS>& s = *reinterpret_cast<GradShared<T, DK, PS>*>(shared_bytes);
   const int chunk = blockIdx.x / p.hk, kh = blockIdx.x % p.hk;
   ChunkAt c;
   if (!chunk_at(p, chunk, &c)) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rb = warp & 3, half = warp >> 2;  // 16 tokens, half of the columns
+  const int rb = warp & 3, cg = warp >> 2;  // 16 tokens; a quarter of the columns
   const int r0 = rb * 16 + (lane >> 2);
   const uint32_t kt = shared_u32(s.tile[0][0]), qt = shared_u32(s.tile[1][0]);
+  const int group = p.hv / p.hk, used = p.slabs * 16;
   {
     const uint4* from = reinterpret_cast<const uint4*>(p.tiles + (static_cast<long long>(chunk) * p.hk + kh) * L::kTiles);
-    for (int i = tid; i < static_cast<int>(L::kTiles / 16); i += kGradThreads) reinterpret_cast<uint4*>(s.tile)[i] = from[i];
-    const float* coef = reinterpret_cast<const float*>(
-        p.heads + (static_cast<long long>(chunk) * p.hv + kh * (p.hv / p.hk)) * L::kHead + L::kT + L::kP);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(L::kTiles / 16 / kGradThreads); ++i)
+      reinterpret_cast<uint4*>(s.tile)[i * kGradThreads + tid] = from[i * kGradThreads + tid];
+    const float* coef = reinterpret_cast<const float*>(p.heads + (static_cast<long long>(chunk) * p.hv + kh * group) * L::kHead +
+                                                       L::kT + L::kP);
     if (tid < kChunk) {
       s.krow[tid] = coef[kKRow * kChunk + tid];
       s.qrow[tid] = coef[kQRow * kChunk + tid];
     }
   }
-  __syncthreads();
-  {  // k_i . k_j and q_i . k_j: 16 rows, 32 columns a warp
-    float a[4][4] = {}, b[4][4] = {};
-#pragma unroll
-    for (int kk = 0; kk < DK / 16; ++kk)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint32_t am = at_mk<DK>(lane, rb * 16, kk * 16), bm = kt + at_nk<DK>(lane, half * 32 + n * 16, kk * 16);
-        tile_product<IN, IN, false, false>(a[2 * n], a[2 * n + 1], kt + am, L::kTile, bm, L::kTile);
-        tile_product<IN, IN, false, false>(b[2 * n], b[2 * n + 1], qt + am, L::kTile, bm, L::kTile);
-      }
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = r0 + (e >> 1) * 8, j = half * 32 + n * 8 + (lane & 3) * 2 + (e & 1);
-        s.kk[i][j] = a[n][e] * s.krow[i] * s.krow[j];
-        s.qk[i][j] = b[n][e] * s.qrow[i] * s.krow[j];
-      }
-  }
   float dq[NT][4] = {}, dk[NT][4] = {};
-  const int group = p.hv / p.hk;
   for (int sub = 0; sub < group; ++sub) {
     const int vh = kh * group + sub;
     const long long head_at = static_cast<long long>(chunk) * p.hv + vh;
     const float* coef = reinterpret_cast<const float*>(p.heads + head_at * L::kHead + L::kT + L::kP);
     __syncthreads();
+    if (tid < 4) s.common[tid] = s.most[tid] = 0;
     if (tid < kChunk) {
+      const float hi = coef[kSumHi * kChunk + tid], lo = coef[kSumLo * kChunk + tid];
       s.beta[tid] = coef[kBeta * kChunk + tid];
-      s.hi[tid] = coef[kSumHi * kChunk + tid];
-      s.lo[tid] = coef[kSumLo * kChunk + tid];
-      s.down[tid] = exp_sum(s.hi[tid], s.lo[tid]);
-      s.tail[tid] = expf((coef[kSumHi * kChunk + kChunk - 1] - s.hi[tid]) + (coef[kSumLo * kChunk + kChunk - 1] - s.lo[tid]));
+      s.hi[tid] = hi;
+      s.lo[tid] = lo;
+      s.down[tid] = exp_sum(hi, lo);
+      s.tail[tid] = expf((coef[kSumHi * kChunk + kChunk - 1] - hi) + (coef[kSumLo * kChunk + kChunk - 1] - lo));
     }
-    if (tid < 4) s.most[tid] = 0;
     const float decay = coef[kDecay * kChunk];
-    float most[4] = {};
-    for (int i = 0; i < p.slabs * 4; ++i) {
-      const float4 m = *reinterpret_cast<const float4*>(p.largest + (head_at * p.slabs * 4 + i) * 4);
-      most[0] = fmaxf(most[0], m.x);
-      most[1] = fmaxf(most[1], m.y);
-      most[2] = fmaxf(most[2], m.z);
-      most[3] = fmaxf(most[3], m.w);
-    }
-    const Pow2 fs = pow2_for(most[0]), fd = pow2_for(most[1]), fu = pow2_for(most[2]), fx = pow2_for(most[3]);
-
-    const T* d_o = static_cast<const T*>(p.d_o) + c.batch * p.do_batch + c.token * p.do_token + vh * p.do_head;
-    for (int row = warp; row < kChunk; row += 8) {  // one scale for each row of do
+    // do: 8 threads a row, 8 features each of both blocks; one scale a row
+    const int o_row = tid >> 3, o_col = (tid & 7) * 8;
+    float o[2][8] = {};
+    {
+      const T* from = static_cast<const T*>(p.d_o) + c.batch * p.do_batch + (c.token + o_row) * p.do_token + vh * p.do_head;
+      if (o_row < c.len)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int col = b * kGradBlock + o_col;
+          constexpr int V = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;
+          if (p.vec_do) {
+#pragma unroll
+            for (int e = 0; e < 8; e += V)
+              if (col + e < p.dv) load<T, V>(from + col + e, *reinterpret_cast<float(*)[V]>(&o[b][e]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (col + e < p.dv) o[b][e] = up(from[col + e]);
+          }
+        }
       float m = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (row < c.len && lane + 32 * e < p.dv) m = fmaxf(m, fabsf(up(d_o[row * p.do_token + lane + 32 * e])));
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaxf(fabsf(o[0][e]), fabsf(o[1][e])));
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const Pow2 fo = pow2_for(m);
-      if (lane == 0) {
-        s.oscale[row] = fo.f;
-        s.orow[row] = fo.inverse;
-      }
+      for (int w = 4; w >= 1; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+      const Pow2 f = pow2_for(m);
+      if ((tid & 7) == 0) s.orow[o_row] = f.inverse;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[0][e] *= f.f, o[1][e] *= f.f;
+    }
+    // scales of the kept planes: the largest of each kind is the common one
+    float row_scale[4];
+#pragma unroll
+    for (int kind = 0; kind < 4; ++kind) {
+      const int quarter = tid >> 7, row = tid & 127;
+      row_scale[kind] = row < used ? p.scales[((head_at * 4 + kind) * 4 + quarter) * p.rows + row] : 0.f;
+      const unsigned int m = __reduce_max_sync(0xffffffffu, __float_as_uint(row_scale[kind]));
+      // non-negative floats order as integers: the maximum does not depend on the order
+      if (kind == 0) __syncthreads();  // common is cleared
+      if (lane == 0) atomicMax(&s.common[kind], m);
+    }
+    __syncthreads();
+    float common[4];
+#pragma unroll
+    for (int kind = 0; kind < 4; ++kind) {
+      common[kind] = __uint_as_float(s.common[kind]);
+      s.ratio[kind][tid >> 7][tid & 127] = row_scale[kind] / common[kind];
     }
 
-    float a_q[NT][4] = {}, a_x[NT][4] = {}, a_u[NT][4] = {}, a_p[4][4] = {}, a_a[4][4] = {};
-    float sd_sum = 0.f, xv[2] = {};
-    for (int block = 0; block * kGradBlock < p.slabs * 16; ++block) {
+    float a_q[NT][4] = {}, a_x[NT][4] = {}, a_u[NT][4] = {}, a_p[2][4] = {}, a_a[2][4] = {};
+    float sd = 0.f, xv = 0.f;
+#pragma unroll 1
+    for (int block = 0; block * kGradBlock < used; ++block) {
       __syncthreads();
-      // S^T, D^T (64 features), U^T, dX^T as planes; <S, D>
-      for (int i = warp; i < 4 * (DK / 8); i += 8) {
-        const int slab = i / (DK / 8), n = i % (DK / 8), at = block * 4 + slab;
-        float4 f = make_float4(0, 0, 0, 0), g = f;
-        if (at < p.slabs) {
-          const long long where = (head_at * p.slabs + at) * 16 * DK + (n * 32 + lane) * 4;
-          f = *reinterpret_cast<const float4*>(p.states + where);
-          g = *reinterpret_cast<const float4*>(p.dstates + where);
-        }
-        sd_sum += (f.x * g.x + f.y * g.y) + (f.z * g.z + f.w * g.w);
-        tile_from_fragments<PS, DK>(f, fs.f, reinterpret_cast<char*>(s.in.s), kWide, slab, n, lane);
-        tile_from_fragments<PS, DK>(g, fd.f, reinterpret_cast<char*>(s.in.d), kWide, slab, n, lane);
+      const int v0 = block * kGradBlock;
+      load_kept<PS, DK>(p.states + kept_at<PS, DK>(p, head_at), p.rows, v0, used, s.ratio[0], reinterpret_cast<char*>(s.in.s), tid);
+      load_kept<PS, DK>(p.dstates + kept_at<PS, DK>(p, head_at), p.rows, v0, used, s.ratio[1], reinterpret_cast<char*>(s.in.d), tid);
+      load_kept<PS, kChunk>(p.us + kept_at<PS, kChunk>(p, head_at), p.rows, v0, used, s.ratio[2], reinterpret_cast<char*>(s.in.u), tid);
+      load_kept<PS, kChunk>(p.dxs + kept_at<PS, kChunk>(p, head_at), p.rows, v0, used, s.ratio[3], reinterpret_cast<char*>(s.in.x), tid);
+      {
+        Vec<uint32_t, 4> plane[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          split<PS>(block ? o[1][2 * e] : o[0][2 * e], block ? o[1][2 * e + 1] : o[0][2 * e + 1], &plane[0].e[e], &plane[1].e[e]);
+#pragma unroll
+        for (int n = 0; n < PS; ++n)
+          *reinterpret_cast<Vec<uint32_t, 4>*>(reinterpret_cast<char*>(s.in.o) + n * kNarrow + tile_at<kGradBlock>(o_row, tid & 7)) = plane[n];
       }
-      for (int i = warp; i < 4 * 8; i += 8) {
-        const int slab = i / 8, n = i % 8, at = block * 4 + slab;
-        float4 f = make_float4(0, 0, 0, 0), g = f;
-        if (at < p.slabs) {
-          const long long where = (head_at * p.slabs + at) * 16 * kChunk + (n * 32 + lane) * 4;
-          f = *reinterpret_cast<const float4*>(p.us + where);
-          g = *reinterpret_cast<const float4*>(p.dxs + where);
+      float v[8] = {};  // of token tid & 63, eight features
+      {
+        const int t = tid & 63, col = v0 + (tid >> 6) * 8;
+        const T* from = static_cast<const T*>(p.v) + c.batch * p.v_batch + (c.token + t) * p.v_token + vh * p.v_head;
+        constexpr int V = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;
+        if (t < c.len) {
+          if (p.vec_v) {
+#pragma unroll
+            for (int e = 0; e < 8; e += V)
+              if (col + e < p.dv) load<T, V>(from + col + e, *reinterpret_cast<float(*)[V]>(&v[e]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (col + e < p.dv) v[e] = up(from[col + e]);
+          }
         }
-        tile_from_fragments<PS, kChunk>(f, fu.f, reinterpret_cast<char*>(s.in.u), kNarrow, slab, n, lane);
-        tile_from_fragments<PS, kChunk>(g, fx.f, reinterpret_cast<char*>(s.in.x), kNarrow, slab, n, lane);
-        // dX . v of the tokens: this lane's features
-        const T* v = static_cast<const T*>(p.v) + c.batch * p.v_batch + vh * p.v_head;
-        float two[2] = {};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = n * 8 + (lane & 3) * 2 + (e & 1), col = at * 16 + (lane >> 2) + (e >> 1) * 8;
-          const float x = e == 0 ? g.x : e == 1 ? g.y : e == 2 ? g.z : g.w;
-          if (t < c.len && col < p.dv) two[e & 1] = fmaf(x, up(v[(c.token + t) * p.v_token + col]), two[e & 1]);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) two[e] += __shfl_xor_sync(0xffffffffu, two[e], o);
-        }
-        // a warp meets token tile n = warp once a slab, in slab order
-        xv[0] += two[0];
-        xv[1] += two[1];
-      }
-      // do, this block's features
-      for (int row = warp; row < kChunk; row += 8) {
-        float f[2] = {};
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (row < c.len && block * kGradBlock + lane * 2 + e < p.dv)
-            f[e] = up(d_o[row * p.do_token + block * kGradBlock + lane * 2 + e]) * s.oscale[row];
-        uint32_t hi, lo;
-        split<PS>(f[0], f[1], &hi, &lo);
-        const uint32_t at = tile_at<kGradBlock>(row, lane / 4) + (lane % 4) * 4;
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(s.in.o) + at) = hi;
-        if (PS > 1) *reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(s.in.o) + kNarrow + at) = lo;
       }
       __syncthreads();
       const uint32_t st = shared_u32(s.in.s), dt = shared_u32(s.in.d), ut = shared_u32(s.in.u), xt = shared_u32(s.in.x),
                      ot = shared_u32(s.in.o);
+      {  // dX . v and <S, D>
+        const int t = tid & 63, row = (tid >> 6) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t at = tile_at<kChunk>(row + e, t >> 3) + (t & 7) * 2;
+          float x = 0.f;
+#pragma unroll
+          for (int n = 0; n < PS; ++n) x += __half2float(*reinterpret_cast<const __half*>(reinterpret_cast<const char*>(s.in.x) + n * kNarrow + at));
+          xv = fmaf(x, v[e], xv);
+        }
+#pragma unroll
+        for (int i = 0; i < kGradBlock * DK / 8 / kGradThreads; ++i) {
+          float f[8] = {}, g[8] = {};
+#pragma unroll
+          for (int n = 0; n < PS; ++n) {
+            const uint4 a = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s.in.s) + n * kWide)[i * kGradThreads + tid];
+            const uint4 b = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s.in.d) + n * kWide)[i * kGradThreads + tid];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 x = __half22float2(reinterpret_cast<const __half2*>(&a)[e]), y = __half22float2(reinterpret_cast<const __half2*>(&b)[e]);
+              f[2 * e] += x.x, f[2 * e + 1] += x.y, g[2 * e] += y.x, g[2 * e + 1] += y.y;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sd = fmaf(f[e], g[e], sd);
+        }
+      }
 #pragma unroll
       for (int kk = 0; kk < kGradBlock / 16; ++kk) {
-        const uint32_t o_at = ot + at_mk<kGradBlock>(lane, rb * 16, kk * 16);
-        const uint32_t u_at = ut + at_km<kChunk>(lane, rb * 16, kk * 16), x_at = xt + at_km<kChunk>(lane, rb * 16, kk * 16);
+        uint32_t fo[PS][4], fu[PS][4], fx[PS][4], b[PS][4];
+        planes_load<PS, false>(fo, ot + at_mk<kGradBlock>(lane, rb * 16, kk * 16), kNarrow);
+        planes_load<PS, true>(fu, ut + at_km<kChunk>(lane, rb * 16, kk * 16), kNarrow);
+        planes_load<PS, true>(fx, xt + at_km<kChunk>(lane, rb * 16, kk * 16), kNarrow);
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) {
-          const uint32_t b = at_kn<DK>(lane, half * (DK / 2) + n * 16, kk * 16);
-          tile_product<PS, PS, false, true>(a_q[2 * n], a_q[2 * n + 1], o_at, kNarrow, st + b, kWide);
-          tile_product<PS, PS, true, true>(a_x[2 * n], a_x[2 * n + 1], x_at, kNarrow, st + b, kWide);
-          tile_product<PS, PS, true, true>(a_u[2 * n], a_u[2 * n + 1], u_at, kNarrow, dt + b, kWide);
+          const uint32_t at = at_kn<DK>(lane, cg * (DK / 4) + n * 16, kk * 16);
+          planes_load<PS, true>(b, st + at, kWide);
+          planes_product<PS, PS>(a_q[2 * n], a_q[2 * n + 1], fo, b);
+          planes_product<PS, PS>(a_x[2 * n], a_x[2 * n + 1], fx, b);
+          planes_load<PS, true>(b, dt + at, kWide);
+          planes_product<PS, PS>(a_u[2 * n], a_u[2 * n + 1], fu, b);
         }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint32_t b = ut + at_kn<kChunk>(lane, half * 32 + n * 16, kk * 16);
-          tile_product<PS, PS, false, true>(a_p[2 * n], a_p[2 * n + 1], o_at, kNarrow, b, kNarrow);
-          tile_product<PS, PS, true, true>(a_a[2 * n], a_a[2 * n + 1], x_at, kNarrow, b, kNarrow);
-        }
+        planes_load<PS, true>(b, ut + at_kn<kChunk>(lane, cg * 16, kk * 16), kNarrow);
+        planes_product<PS, PS>(a_p[0], a_p[1], fo, b);
+        planes_product<PS, PS>(a_a[0], a_a[1], fx, b);
       }
     }
-    // <S, D> of the block; dX . v of this warp's token tile
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) sd_sum += __shfl_xor_sync(0xffffffffu, sd_sum, o);
-    if (lane == 0) s.warp_sum[warp] = sd_sum;
-    if (lane < 4) {
-      s.xv[warp * 8 + lane * 2] = xv[0];
-      s.xv[warp * 8 + lane * 2 + 1] = xv[1];
-    }
+    for (int w = 16; w >= 1; w >>= 1) sd += __shfl_xor_sync(0xffffffffu, sd, w);
+    if (lane == 0) s.warp_sum[warp] = sd;
+    s.xv[tid >> 6][tid & 63] = xv;
 
     // parts of dq and dk that see the states, and their products with q and k
-    {
-      float dot[3][2] = {};
+    float dot[4][2] = {};
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = r0 + (e >> 1) * 8, col = half * (DK / 2) + n * 8 + (lane & 3) * 2 + (e & 1);
-          const uint32_t at = tile_at<DK>(i, col >> 3) + (col & 7) * 2;
-          float kv = 0.f, qv = 0.f;
-#pragma unroll
-          for (int plane = 0; plane < IN; ++plane) {
-            kv += __half2float(*reinterpret_cast<const __half*>(reinterpret_cast<const char*>(s.tile[0][plane]) + at));
-            qv += __half2float(*reinterpret_cast<const __half*>(reinterpret_cast<const char*>(s.tile[1][plane]) + at));
-          }
-          kv *= s.krow[i];
-          qv *= s.qrow[i];
-          const float one = -s.down[i] * (a_x[n][e] * (fx.inverse * fs.inverse));
-          const float two = p.scale * s.down[i] * (a_q[n][e] * s.orow[i] * fs.inverse);
-          const float three = s.tail[i] * (a_u[n][e] * (fu.inverse * fd.inverse));
-          dot[0][e >> 1] = fmaf(kv, one, dot[0][e >> 1]);
-          dot[1][e >> 1] = fmaf(qv, two, dot[1][e >> 1]);
-          dot[2][e >> 1] = fmaf(kv, three, dot[2][e >> 1]);
-          dq[n][e] += two;
-          dk[n][e] += fmaf(s.beta[i], one, three);
-        }
-#pragma unroll
-      for (int w = 0; w < 3; ++w)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float v = quad_sum(dot[w][h]);
-          if ((lane & 3) == 0) s.dots[half][w][r0 + h * 8] = v;
-        }
-    }
-    // N, B, their row and column sums with Q K^T and K K^T
-    float n_k[4][4], n_q[4][4], b_k[4][4], b_r[4][4], top[4] = {};
-    {
-      float row_z[2] = {}, row_a[2] = {}, col_z[4][2];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        col_z[n][0] = col_z[n][1] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = r0 + (e >> 1) * 8, j = half * 32 + n * 8 + (lane & 3) * 2 + (e & 1);
-          const float gamma = j <= i ? expf((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j])) : 0.f;
-          const float nn = j <= i ? gamma * (p.scale * (a_p[n][e] * s.orow[i] * fu.inverse)) : 0.f;
-          const float ga = j < i ? -gamma * (a_a[n][e] * (fx.inverse * fu.inverse)) : 0.f;
-          const float with = j < i ? ga * s.kk[i][j] : 0.f;
-          const float z = (j <= i ? nn * s.qk[i][j] : 0.f) + s.beta[i] * with;
-          row_z[e >> 1] += z;
-          row_a[e >> 1] += with;
-          col_z[n][e & 1] += z;
-          n_k[n][e] = nn * s.krow[j];
-          n_q[n][e] = nn * s.qrow[i];
-          b_k[n][e] = s.beta[i] * ga * s.krow[j];
-          b_r[n][e] = s.beta[i] * ga * s.krow[i];
-          top[0] = fmaxf(top[0], fabsf(n_k[n][e]));
-          top[1] = fmaxf(top[1], fabsf(n_q[n][e]));
-          top[2] = fmaxf(top[2], fabsf(b_k[n][e]));
-          top[3] = fmaxf(top[3], fabsf(b_r[n][e]));
-        }
-      }
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float z = quad_sum(row_z[h]), v = quad_sum(row_a[h]);
-        if ((lane & 3) == 0) {
-          s.rows[half][0][r0 + h * 8] = z;
-          s.rows[half][1][r0 + h * 8] = v;
-        }
-      }
+        const int i = r0 + h * 8;
+        const uint32_t at = tile_at<DK>(i, cg * (DK / 32) + n) + (lane & 3) * 4;
+        float kv[2] = {}, qv[2] = {};
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+        for (int plane = 0; plane < IN; ++plane) {
+          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(s.tile[0][plane]) + at));
+          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(s.tile[1][plane]) + at));
+          kv[0] += a.x, kv[1] += a.y, qv[0] += b.x, qv[1] += b.y;
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float z = col_z[n][e];
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-          if (lane < 4) s.cols[rb][half * 32 + n * 8 + lane * 2 + e] = z;
+          const int at_e = 2 * h + e;
+          const float one = -s.down[i] * (a_x[n][at_e] * (common[3] * common[0]));
+          const float two = p.scale * s.down[i] * (a_q[n][at_e] * (s.orow[i] * common[0]));
+          const float three = s.tail[i] * (a_u[n][at_e] * (common[2] * common[1]));
+          dot[0][h] = fmaf(kv[e], one, dot[0][h]);
+          dot[1][h] = fmaf(qv[e], two, dot[1][h]);
+          dot[2][h] = fmaf(kv[e], three, dot[2][h]);
+          dq[n][at_e] += two;
+          dk[n][at_e] += fmaf(s.beta[i], one, three);
         }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float m = quad_max(top[w]);
-        m = warp_max(m);
-        // non-negative floats order as integers: the maximum does not depend on the order
-        if (lane == 0) atomicMax(&s.most[w], __float_as_uint(m));
       }
+    // sum of H = e^{G_C - G} k . (U D^T) over the chunk, before the rest joins that dot
+    float h_part = quad_sum(dot[2][0]) * s.krow[r0] + quad_sum(dot[2][1]) * s.krow[r0 + 8];
+
+    // N, Gamma dA and B with the row factors of what they meet
+    float sq[4][2][4], top[4] = {};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = r0 + (e >> 1) * 8, j = cg * 16 + n * 8 + (lane & 3) * 2 + (e & 1);
+        const float gamma = j <= i ? expf((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j])) : 0.f;
+        const float nn = j <= i ? gamma * (p.scale * (a_p[n][e] * (s.orow[i] * common[2]))) : 0.f;
+        const float ga = j < i ? -gamma * (a_a[n][e] * (common[3] * common[2])) : 0.f;
+        sq[0][n][e] = nn * s.krow[j];
+        sq[1][n][e] = nn * s.qrow[i];
+        sq[2][n][e] = ga * s.krow[j];
+        sq[3][n][e] = s.beta[i] * ga * s.krow[i];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top[w] = fmaxf(top[w], fabsf(sq[w][n][e]));
+      }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const unsigned int m = __reduce_max_sync(0xffffffffu, __float_as_uint(top[w]));
+      if (lane == 0) atomicMax(&s.most[w], m);
     }
     __syncthreads();
-    const Pow2 f[4] = {pow2_for(__uint_as_float(s.most[0])), pow2_for(__uint_as_float(s.most[1])),
-                       pow2_for(__uint_as_float(s.most[2])), pow2_for(__uint_as_float(s.most[3]))};
+    Pow2 f[4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int w = 0; w < 4; ++w) f[w] = pow2_for(__uint_as_float(s.most[w]));
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t at = tile_at<kChunk>(r0 + h * 8, half * 4 + n) + (lane & 3) * 4;
+        const uint32_t at = tile_at<kChunk>(r0 + h * 8, cg * 2 + n) + (lane & 3) * 4;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const float(&m)[4] = w == 0 ? n_k[n] : w == 1 ? n_q[n] : w == 2 ? b_k[n] : b_r[n];
           uint32_t hi, lo;
-          split<PS>(m[2 * h] * f[w].f, m[2 * h + 1] * f[w].f, &hi, &lo);
+          split<PS>(sq[w][n][2 * h] * f[w].f, sq[w][n][2 * h + 1] * f[w].f, &hi, &lo);
           char* to = reinterpret_cast<char*>(s.square[w]);
           *reinterpret_cast<uint32_t*>(to + at) = hi;
           if (PS > 1) *reinterpret_cast<uint32_t*>(to + kSq + at) = lo;
         }
       }
-    // the gates' gradients
-    if (warp == 0) {
-      float h[2], dg[2];
-      float sum_h = 0.f;
+    __syncthreads();
+    // dq += N K; dk += N^T Q + beta Y + B^T K, Y = (Gamma dA) K; all lower triangular
+    {
+      float b_q[NT][4] = {}, b_n[NT][4] = {}, b_y[NT][4] = {}, b_t[NT][4] = {};
+      const uint32_t base = shared_u32(s.square);
+      constexpr uint32_t one = PS * kSq;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int t = 2 * lane + e;
-        h[e] = s.dots[0][2][t] + s.dots[1][2][t];
-        sum_h += h[e];
+      for (int kk = 0; kk < 4; ++kk) {
+        const uint32_t mk = at_mk<kChunk>(lane, rb * 16, kk * 16), km = at_km<kChunk>(lane, rb * 16, kk * 16);
+        uint32_t a[PS][4], g[PS][4], b[IN][4];
+        if (kk <= rb) {
+          planes_load<PS, false>(a, base + mk, kSq);
+          planes_load<PS, false>(g, base + 2 * one + mk, kSq);
+#pragma unroll
+          for (int n = 0; n < NT / 2; ++n) {
+            planes_load<IN, true>(b, kt + at_kn<DK>(lane, cg * (DK / 4) + n * 16, kk * 16), L::kTile);
+            planes_product<PS, IN>(b_q[2 * n], b_q[2 * n + 1], a, b);
+            planes_product<PS, IN>(b_y[2 * n], b_y[2 * n + 1], g, b);
+          }
+        }
+        if (kk >= rb) {
+          planes_load<PS, true>(a, base + one + km, kSq);
+          planes_load<PS, true>(g, base + 3 * one + km, kSq);
+#pragma unroll
+          for (int n = 0; n < NT / 2; ++n) {
+            const uint32_t at = at_kn<DK>(lane, cg * (DK / 4) + n * 16, kk * 16);
+            planes_load<IN, true>(b, qt + at, L::kTile);
+            planes_product<PS, IN>(b_n[2 * n], b_n[2 * n + 1], a, b);
+            planes_load<IN, true>(b, kt + at, L::kTile);
+            planes_product<PS, IN>(b_t[2 * n], b_t[2 * n + 1], g, b);
+          }
+        }
       }
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) sum_h += __shfl_xor_sync(0xffffffffu, sum_h, o);
-      float total = 0.f;
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int w = 0; w < 8; ++w) total += s.warp_sum[w];
+        for (int h = 0; h < 2; ++h) {
+          const int i = r0 + h * 8;
+          const uint32_t at = tile_at<DK>(i, cg * (DK / 32) + n) + (lane & 3) * 4;
+          float kv[2] = {}, qv[2] = {};
+#pragma unroll
+          for (int plane = 0; plane < IN; ++plane) {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(s.tile[0][plane]) + at));
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(s.tile[1][plane]) + at));
+            kv[0] += x.x, kv[1] += x.y, qv[0] += y.x, qv[1] += y.y;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int at_e = 2 * h + e;
+            const float two = b_q[n][at_e] * f[0].inverse, y = b_y[n][at_e] * f[2].inverse;
+            const float three = fmaf(b_n[n][at_e], f[1].inverse, b_t[n][at_e] * f[3].inverse);
+            dot[1][h] = fmaf(qv[e], two, dot[1][h]);
+            dot[2][h] = fmaf(kv[e], three, dot[2][h]);
+            dot[3][h] = fmaf(kv[e], y, dot[3][h]);
+            dq[n][at_e] += two;
+            dk[n][at_e] += fmaf(s.beta[i], y, three);
+          }
+        }
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = r0 + h * 8;
+        const float v = quad_sum(dot[w][h]) * (w == 1 ? s.qrow[i] : s.krow[i]);
+        if ((lane & 3) == 0) s.dots[cg][w][i] = v;
+      }
+    // H summed over this warp's rows (a lane of each quad)
+#pragma unroll
+    for (int w = 4; w < 32; w <<= 1) h_part += __shfl_xor_sync(0xffffffffu, h_part, w);
+    if (lane == 0) s.warp_sum[warp] = fmaf(decay * (common[0] * common[1]), s.warp_sum[warp], h_part);
+    __syncthreads();
+    if (warp == 0) {  // the gates' gradients
+      float dg[2], total = 0.f;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) total += s.warp_sum[w];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int t = 2 * lane + e;
-        const float k1 = s.dots[0][0][t] + s.dots[1][0][t], q1 = s.dots[0][1][t] + s.dots[1][1][t];
-        const float z = (s.rows[0][0][t] + s.rows[1][0][t]) - ((s.cols[0][t] + s.cols[1][t]) + (s.cols[2][t] + s.cols[3][t]));
-        dg[e] = s.beta[t] * k1 + q1 + z - h[e];
-        const float db = k1 + s.xv[t] + (s.rows[0][1][t] + s.rows[1][1][t]);
+        float v[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v[w] = (s.dots[0][w][t] + s.dots[1][w][t]) + (s.dots[2][w][t] + s.dots[3][w][t]);
+        const float with_v = ((s.xv[0][t] + s.xv[1][t]) + (s.xv[2][t] + s.xv[3][t])) + ((s.xv[4][t] + s.xv[5][t]) + (s.xv[6][t] + s.xv[7][t]));
+        dg[e] = s.beta[t] * (v[0] + v[3]) + v[1] - v[2];
+        const float db = (v[0] + v[3]) + common[3] * with_v;
         if (t < c.len) {
           const long long at = (static_cast<long long>(c.batch) * p.tokens + c.token + t) * p.hv + vh;
           if (p.gates32)
@@ -551,13 +608,13 @@ __global__ void __launch_bounds__(kGradThreads) delta_gradient(DeltaParams p) {
             static_cast<T*>(p.dbeta)[at] = down<T>(db);
         }
       }
-      if (lane == 31) dg[1] += decay * total + sum_h;
+      if (lane == 31) dg[1] += total;
       dg[0] += dg[1];
       float after = dg[0];  // sums from this pair to the end
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float v = __shfl_down_sync(0xffffffffu, after, o);
-        if (lane + o < 32) after += v;
+      for (int w = 1; w < 32; w <<= 1) {
+        const float v = __shfl_down_sync(0xffffffffu, after, w);
+        if (lane + w < 32) after += v;
       }
       const float rest = after - dg[0];
 #pragma unroll
@@ -572,47 +629,18 @@ __global__ void __launch_bounds__(kGradThreads) delta_gradient(DeltaParams p) {
         }
       }
     }
-    __syncthreads();
-    // dq += N K; dk += N^T Q + B K + B^T K, the matrices lower triangular
-    {
-      float b_q[NT][4] = {}, b_n[NT][4] = {}, b_b[NT][4] = {}, b_t[NT][4] = {};
-      const uint32_t sq = shared_u32(s.square);
-      constexpr uint32_t one = PS * kSq;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const uint32_t mk = at_mk<kChunk>(lane, rb * 16, kk * 16), km = at_km<kChunk>(lane, rb * 16, kk * 16);
-#pragma unroll
-        for (int n = 0; n < NT / 2; ++n) {
-          const uint32_t b = at_kn<DK>(lane, half * (DK / 2) + n * 16, kk * 16);
-          if (kk <= rb) {
-            tile_product<PS, IN, false, true>(b_q[2 * n], b_q[2 * n + 1], sq + mk, kSq, kt + b, L::kTile);
-            tile_product<PS, IN, false, true>(b_b[2 * n], b_b[2 * n + 1], sq + 2 * one + mk, kSq, kt + b, L::kTile);
-          }
-          if (kk >= rb) {
-            tile_product<PS, IN, true, true>(b_n[2 * n], b_n[2 * n + 1], sq + one + km, kSq, qt + b, L::kTile);
-            tile_product<PS, IN, true, true>(b_t[2 * n], b_t[2 * n + 1], sq + 3 * one + km, kSq, kt + b, L::kTile);
-          }
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          dq[n][e] = fmaf(b_q[n][e], f[0].inverse, dq[n][e]);
-          dk[n][e] += fmaf(b_n[n][e], f[1].inverse, fmaf(b_b[n][e], f[2].inverse, b_t[n][e] * f[3].inverse));
-        }
-    }
   }
   // dq, dk: dense [batch, tokens, key heads, Dk]
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int t = r0 + h * 8, col = half * (DK / 2) + n * 8 + (lane & 3) * 2;
-      if (t >= c.len) continue;
+      const int t = r0 + h * 8, col = cg * (DK / 4) + n * 8 + (lane & 3) * 2;
+      if (t >= c.len || col >= p.dk) continue;
       const long long at = ((static_cast<long long>(c.batch) * p.tokens + c.token + t) * p.hk + kh) * p.dk + col;
-      store_pair(static_cast<T*>(p.dq) + at, dq[n][2 * h], dq[n][2 * h + 1], p.dk - col);
-      store_pair(static_cast<T*>(p.dk_out) + at, dk[n][2 * h], dk[n][2 * h + 1], p.dk - col);
+      const float q2[2] = {dq[n][2 * h], dq[n][2 * h + 1]}, k2[2] = {dk[n][2 * h], dk[n][2 * h + 1]};
+      store_row(static_cast<T*>(p.dq) + at, q2, p.dk - col, p.dk % 2 == 0);
+      store_row(static_cast<T*>(p.dk_out) + at, k2, p.dk - col, p.dk % 2 == 0);
     }
 }
 

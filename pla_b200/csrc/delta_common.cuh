@@ -57,18 +57,19 @@ struct DeltaParams {
   int row_chunks;    // dense: chunks of a batch row
   int chunk_bound;   // chunks the workspace has room for
   int* plan;         // ragged: lo [N], len [N], first chunk [N + 1]
+  int4* table;       // ragged: sequence (-1: none), first token, tokens of every chunk
   char* tiles;       // K, Q planes of every (chunk, key head)
   char* heads;       // T, P planes and coefficients of every (chunk, value head)
-  float* states;     // backward: S at every chunk's start, fragment order
-  float* us;         // backward: U
   // backward
   const void* d_o;
   long long do_batch, do_token, do_head;
   const float* dstate_out;
   float* dstate_in;
-  float* dstates;    // dS at every chunk's end, fragment order
-  float* dxs;        // dX
-  float* largest;    // magnitudes of S, dS, U, dX: [chunk, value head, slab, warp, 4]
+  // planes of S and U (kept by the forward sweep), of dS at the chunks' ends and of
+  // dX: [chunk, value head][plane][rows][Dk or 64], tiles of delta_common's order
+  char *states, *us, *dstates, *dxs;
+  float* scales;     // the inverses of their scales: [chunk, value head][S, dS, U, dX][4][rows]
+  int rows;          // dv rounded up to 64
   void *dq, *dk_out, *dv_out, *dg, *dbeta;
   int slabs;         // ceil(dv / 16)
   int vec_qk, vec_v, vec_o, vec_do;
@@ -85,21 +86,19 @@ __device__ __forceinline__ bool chunk_at(const DeltaParams& p, int chunk, ChunkA
     c->len = min(kChunk, p.tokens - c->token);
     return true;
   }
-  const int n = p.sequences;
-  const int s = find_sequence(p.plan + 2 * n, n, chunk);
-  if (s < 0) return false;
-  const int at = (chunk - p.plan[2 * n + s]) * kChunk;
-  c->sequence = s;
+  const int4 t = p.table[chunk];
+  if (t.x < 0) return false;
+  c->sequence = t.x;
   c->batch = 0;
-  c->token = p.plan[s] + at;
-  c->len = min(kChunk, p.plan[n + s] - at);
+  c->token = t.y;
+  c->len = t.z;
   return true;
 }
 
 // Ragged batches: first token, length and first chunk of every sequence.  A
 // running maximum over the clamped entries keeps sequences in order and apart
 // whatever cu_seqlens holds, so their chunks never exceed tokens / 64 + N.
-__global__ void __launch_bounds__(1024) delta_plan(const int* cu, int tokens, int n, int* plan) {
+__global__ void __launch_bounds__(1024) delta_plan(const int* cu, int tokens, int n, int* plan, int4* table, int chunks) {
   __shared__ int scan[1024];
   __shared__ int carry_max, carry_sum;
   const int i = threadIdx.x;
@@ -141,6 +140,15 @@ __global__ void __launch_bounds__(1024) delta_plan(const int* cu, int tokens, in
       carry_sum += scan[i];
     }
     __syncthreads();
+  }
+  for (int chunk = i; chunk < chunks; chunk += 1024) {
+    const int at = find_sequence(plan + 2 * n, n, chunk);
+    int4 t = make_int4(-1, 0, 0, 0);
+    if (at >= 0) {
+      const int from = (chunk - plan[2 * n + at]) * kChunk;
+      t = make_int4(at, plan[at] + from, min(kChunk, plan[n + at] - from), 0);
+    }
+    table[chunk] = t;
   }
 }
 

@@ -2,6 +2,15 @@
 // one (chunk, key head) a block and the value heads that share the key head:
 // the fp16 planes of K and Q, T = (1 + diag(beta) M)^-1 and P as planes, and
 // the per-token coefficients (delta_common.cuh).
+//
+// K K^T and Q K^T are one pass of tensor-core products for all value heads of
+// the key head; then 128 threads a value head, two heads at a time.  The unit
+// lower triangular 64 x 64 matrix is inverted in blocks, in fp32: four 16 x 16
+// diagonal blocks by substitution (a thread a column, in registers), then
+//     [A 0; B C]^-1 = [A^-1 0; -C^-1 B A^-1 C^-1]
+// from 16 to 32 to 64.  Substitution over all 64 rows took 25 us a block's
+// head, nearly all of it latency; in blocks it is some 700 multiply-adds a
+// thread.
 #pragma once
 
 #include "delta_common.cuh"
@@ -9,148 +18,229 @@
 namespace pla {
 namespace seq {
 
-constexpr int kPrepThreads = 128;
+constexpr int kPrepPitch = 68;  // floats of a row: rows 4 banks apart
 
-template <typename T, int DK>
-struct PrepShared {
-  alignas(16) __half tile[2][DeltaType<T>::kIn][kChunk * DK];  // K, Q planes
-  float kk[kChunk][kChunk + 1], qk[kChunk][kChunk + 1];
-  alignas(16) float a[kChunk][kChunk + 4];  // diag(beta) M, then T
-  float row[2][kChunk];      // what K / Q rows are to be multiplied by
-  float hi[kChunk], lo[kChunk], beta[kChunk];
+struct PrepHead {
+  // diag(beta) M below the diagonal, turned into T in place; the blocks above
+  // the diagonal hold the products on the way
+  alignas(16) float t[kChunk][kPrepPitch];
 };
 
-// Rows of q or k as planes, in shared memory and in the workspace.
-template <typename T, int DK>
-__device__ __forceinline__ void prepare_rows(const DeltaParams& p, const T* x, long long step, int vec, int len, int tid,
-                                             __half* tile, float* factor, char* out) {
-  constexpr int IN = DeltaType<T>::kIn, E = DK / 32;
-  const int lane = tid & 31, warp = tid >> 5;
-#pragma unroll 4
-  for (int i = 0; i < kChunk / 4; ++i) {
-    const int row = warp * (kChunk / 4) + i;
-    float f[E] = {};
-    if (row < len) {
-      const T* r = x + row * step;
-      if (vec) {
-        if (lane * E < p.dk) load<T, E>(r + lane * E, f);
-      } else {
+template <typename T, int DK, int HEADS>
+struct PrepShared {
+  union {
+    alignas(16) __half tile[2][DeltaType<T>::kIn][kChunk * DK];  // K, Q planes, until their products are done
+    PrepHead head[HEADS];
+  };
+  alignas(16) float kk[kChunk][kPrepPitch], qk[kChunk][kPrepPitch];
+  float row[2][kChunk];               // what K / Q rows are to be multiplied by
+  alignas(16) float most[2][kChunk];  // largest magnitude of the rows
+  float hi[HEADS][kChunk], lo[HEADS][kChunk], beta[HEADS][kChunk];
+  float rise[HEADS];                  // the largest e^{G_i - G_j}, i >= j
+};
+
+// Rows of q and k as planes, in shared memory and in the workspace; eight
+// rows of both are in flight at a time.
+template <typename T, int DK, int HEADS, typename S>
+__device__ __forceinline__ void prepare_rows(const DeltaParams& p, const T* k, const T* q, int len, int lane, int warp, S& s,
+                                             char* out) {
+  constexpr int IN = DeltaType<T>::kIn, E = DK / 32, ROWS = kChunk / (4 * HEADS), U = 8;
+#pragma unroll 1
+  for (int base = 0; base < ROWS; base += U) {
+    float f[2][U][E] = {};
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (lane * E + e < p.dk) f[e] = up(r[lane * E + e]);
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int row = warp * ROWS + base + i;
+        if (row < len) {
+          const T* r = side ? q + row * p.q_token : k + row * p.k_token;
+          if (p.vec_qk) {
+            if (lane * E < p.dk) load<T, E>(r + lane * E, f[side][i]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (lane * E + e < p.dk) f[side][i][e] = up(r[lane * E + e]);
+          }
+        }
+      }
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int row = warp * ROWS + base + i;
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fmaxf(m, fabsf(f[side][i][e]));
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const Pow2 scale = pow2_for(m);
+        if (lane == 0) {
+          s.row[side][row] = scale.inverse;
+          s.most[side][row] = m;
+        }
+        Vec<uint32_t, E / 2> plane[2];
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e)
+          split<IN>(f[side][i][2 * e] * scale.f, f[side][i][2 * e + 1] * scale.f, &plane[0].e[e], &plane[1].e[e]);
+        const uint32_t at = tile_at<DK>(row, lane * E / 8) + (lane * E % 8) * 2;
+#pragma unroll
+        for (int n = 0; n < IN; ++n) {
+          *reinterpret_cast<Vec<uint32_t, E / 2>*>(reinterpret_cast<char*>(s.tile[side][n]) + at) = plane[n];
+          *reinterpret_cast<Vec<uint32_t, E / 2>*>(out + (side * IN + n) * kChunk * DK * 2 + at) = plane[n];
+        }
+      }
+  }
+}
+
+// Eight columns of a row as planes.
+template <int PLANES>
+__device__ __forceinline__ void store_unit(char* out, int row, int unit, const float (&f)[8], float scale) {
+  Vec<uint32_t, 4> plane[2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) split<PLANES>(f[2 * e] * scale, f[2 * e + 1] * scale, &plane[0].e[e], &plane[1].e[e]);
+#pragma unroll
+  for (int n = 0; n < PLANES; ++n)
+    *reinterpret_cast<Vec<uint32_t, 4>*>(out + n * kChunk * kChunk * 2 + tile_at<kChunk>(row, unit)) = plane[n];
+}
+
+// The four units of a row that thread id of a pair takes: the pair 16 banks
+// apart and four rows 4 banks each keep eight 16-byte accesses conflict free.
+__device__ __forceinline__ int unit_of(int i, int id) { return (i & 1) + 4 * (i >> 1) + 2 * (id & 1); }
+
+__device__ __forceinline__ void head_sync(int head) { asm volatile("bar.sync %0, 128;" ::"r"(head + 1) : "memory"); }
+
+// e^x by the hardware's 2^x: off by 2^-22 |x| relative, that is below 2^-23 of 1.
+__device__ __forceinline__ float exp_fast(float x) { return exp2f(x * 1.4426950408889634f); }
+
+// c = sign a b, N x N each inside the 64 x 64 matrix; a thread computes R rows
+// of 4 columns.  LOWER_B / LOWER_A: that operand is lower triangular in blocks
+// of 16 and holds other values above.
+template <int N, int R, bool LOWER_B = false, bool LOWER_A = false>
+__device__ __forceinline__ void block_product(const float* a, const float* b, float* c, float sign, int id) {
+  constexpr int ACROSS = N / 4, P = kPrepPitch;
+  const int col = id % ACROSS * 4, row = id / ACROSS * R;
+  float4 sum[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) sum[r] = make_float4(0, 0, 0, 0);
+#pragma unroll
+  for (int k = 0; k < N; k += 4) {
+    if (LOWER_B && k < (col & ~15)) continue;
+    if (LOWER_A && k >= (row & ~15) + 16) continue;
+    float4 bv[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bv[i] = *reinterpret_cast<const float4*>(b + (k + i) * P + col);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float4 av = *reinterpret_cast<const float4*>(a + (row + r) * P + k);
+      const float v[4] = {av.x, av.y, av.z, av.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum[r].x = fmaf(v[i], bv[i].x, sum[r].x);
+        sum[r].y = fmaf(v[i], bv[i].y, sum[r].y);
+        sum[r].z = fmaf(v[i], bv[i].z, sum[r].z);
+        sum[r].w = fmaf(v[i], bv[i].w, sum[r].w);
       }
     }
-    float m = 0.f;
+  }
 #pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, fabsf(f[e]));
+  for (int r = 0; r < R; ++r)
+    *reinterpret_cast<float4*>(c + (row + r) * P + col) =
+        make_float4(sign * sum[r].x, sign * sum[r].y, sign * sum[r].z, sign * sum[r].w);
+}
+
+// g and beta of two tokens a lane; 0 past the chunk's end.
+template <typename T>
+__device__ __forceinline__ void load_gates(const DeltaParams& p, const ChunkAt& c, int vh, int lane, float (&g)[2], float (&b)[2]) {
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const Pow2 s = pow2_for(m);
-    if (lane == 0) factor[row] = s.inverse;
-    uint32_t hi[E / 2], lo[E / 2];
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) split<IN>(f[2 * e] * s.f, f[2 * e + 1] * s.f, &hi[e], &lo[e]);
-    const uint32_t at = tile_at<DK>(row, lane * E / 8) + (lane * E % 8) * 2;
-#pragma unroll
-    for (int plane = 0; plane < IN; ++plane) {
-      const uint32_t* w = plane ? lo : hi;
-      char* s_to = reinterpret_cast<char*>(tile) + plane * kChunk * DK * 2 + at;
-      char* g_to = out + plane * kChunk * DK * 2 + at;
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        reinterpret_cast<uint32_t*>(s_to)[e] = w[e];
-        reinterpret_cast<uint32_t*>(g_to)[e] = w[e];
-      }
+  for (int e = 0; e < 2; ++e) {
+    const int t = 2 * lane + e;
+    g[e] = b[e] = 0.f;
+    if (t < c.len) {
+      const long long gi = c.batch * p.g_batch + (c.token + t) * p.g_token + vh * p.g_head;
+      const long long bi = c.batch * p.beta_batch + (c.token + t) * p.beta_token + vh * p.beta_head;
+      g[e] = p.gates32 ? static_cast<const float*>(p.g)[gi] : up(static_cast<const T*>(p.g)[gi]);
+      b[e] = p.gates32 ? static_cast<const float*>(p.beta)[bi] : up(static_cast<const T*>(p.beta)[bi]);
     }
   }
 }
 
-// One row of a 64 x 64 matrix as planes: a lane holds columns 2 lane, 2 lane + 1.
-template <int PLANES>
-__device__ __forceinline__ float store_square_row(char* out, int row, int lane, float a, float b) {
-  float m = fmaxf(fabsf(a), fabsf(b));
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const Pow2 s = pow2_for(m);
-  uint32_t hi, lo;
-  split<PLANES>(a * s.f, b * s.f, &hi, &lo);
-  const uint32_t at = tile_at<kChunk>(row, lane / 4) + (lane % 4) * 4;
-  *reinterpret_cast<uint32_t*>(out + at) = hi;
-  if (PLANES > 1) *reinterpret_cast<uint32_t*>(out + kChunk * kChunk * 2 + at) = lo;
-  return s.inverse;
-}
-
-template <typename T, int DK, int PS, int PO>
-__global__ void __launch_bounds__(kPrepThreads) delta_prepare(DeltaParams p) {
+template <typename T, int DK, int PS, int PO, int HEADS>
+__global__ void __launch_bounds__(128 * HEADS) delta_prepare(DeltaParams p) {
   using L = DeltaLayout<T, DK, PS, PO>;
-  extern __shared__ char shared_bytes[];
-  PrepShared<T, DK>& s = *reinterpret_cast<PrepShared<T, DK>*>(shared_bytes);
+  extern __shared__ __align__(16) char shared_bytes[];
+  PrepShared<T, DK, HEADS>& s = *reinterpret_cast<PrepShared<T, DK, HEADS>*>(shared_bytes);
   const int chunk = blockIdx.x / p.hk, kh = blockIdx.x % p.hk;
   ChunkAt c;
   if (!chunk_at(p, chunk, &c)) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int id = threadIdx.x & 127, which = threadIdx.x >> 7;  // thread of a head, head of the block
+  float(*t)[kPrepPitch] = s.head[which].t;
+  float *hi = s.hi[which], *lo = s.lo[which], *beta = s.beta[which];
+  const int group = p.hv / p.hk;
   char* tiles = p.tiles + (static_cast<long long>(chunk) * p.hk + kh) * L::kTiles;
-  const T* k = static_cast<const T*>(p.k) + c.batch * p.k_batch + c.token * p.k_token + kh * p.k_head;
-  const T* q = static_cast<const T*>(p.q) + c.batch * p.q_batch + c.token * p.q_token + kh * p.q_head;
-  prepare_rows<T, DK>(p, k, p.k_token, p.vec_qk, c.len, tid, s.tile[0][0], s.row[0], tiles);
-  prepare_rows<T, DK>(p, q, p.q_token, p.vec_qk, c.len, tid, s.tile[1][0], s.row[1], tiles + L::kIn * L::kTile);
+  float gate[2], bias[2];
+  if (id < 32 && which < group) load_gates<T>(p, c, kh * group + which, lane, gate, bias);
+  {
+    const T* k = static_cast<const T*>(p.k) + c.batch * p.k_batch + c.token * p.k_token + kh * p.k_head;
+    const T* q = static_cast<const T*>(p.q) + c.batch * p.q_batch + c.token * p.q_token + kh * p.q_head;
+    prepare_rows<T, DK, HEADS>(p, k, q, c.len, lane, warp, s, tiles);
+  }
   __syncthreads();
 
-  // k_i . k_j and q_i . k_j for the 16 rows of this warp, columns up to them
-  const uint32_t kt = shared_u32(s.tile[0][0]), qt = shared_u32(s.tile[1][0]);
+  // k_i . k_j and q_i . k_j, 16 rows a warp, columns up to them
   {
-    float dk[8][4] = {}, dq[8][4] = {};
+    const int rb = warp & 3;
+    const uint32_t kt = shared_u32(s.tile[0][0]), qt = shared_u32(s.tile[1][0]);
 #pragma unroll
-    for (int kk = 0; kk < DK / 16; ++kk)
+    for (int side = 0; side < 2; ++side) {
+      if (HEADS == 2 && side != which) continue;
+      float d[8][4] = {};
 #pragma unroll
-      for (int pa = 0; pa < L::kIn; ++pa) {
-        uint32_t ak[4], aq[4];
-        ldsm(ak, kt + pa * L::kTile + at_mk<DK>(lane, warp * 16, kk * 16));
-        ldsm(aq, qt + pa * L::kTile + at_mk<DK>(lane, warp * 16, kk * 16));
+      for (int kk = 0; kk < DK / 16; ++kk)
 #pragma unroll
-        for (int pb = 0; pb + pa < L::kIn; ++pb)
+        for (int pa = 0; pa < L::kIn; ++pa) {
+          uint32_t a[4];
+          ldsm(a, (side ? qt : kt) + pa * L::kTile + at_mk<DK>(lane, rb * 16, kk * 16));
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            if (n > warp) break;
-            uint32_t b[4];
-            ldsm(b, kt + pb * L::kTile + at_nk<DK>(lane, n * 16, kk * 16));
-            mma(dk[2 * n], ak, b[0], b[1]);
-            mma(dk[2 * n + 1], ak, b[2], b[3]);
-            mma(dq[2 * n], aq, b[0], b[1]);
-            mma(dq[2 * n + 1], aq, b[2], b[3]);
-          }
-      }
+          for (int pb = 0; pb + pa < L::kIn; ++pb)
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
+            for (int n = 0; n < 4; ++n) {
+              if (n > rb) break;
+              uint32_t b[4];
+              ldsm(b, kt + pb * L::kTile + at_nk<DK>(lane, n * 16, kk * 16));
+              mma(d[2 * n], a, b[0], b[1]);
+              mma(d[2 * n + 1], a, b[2], b[3]);
+            }
+        }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = warp * 16 + (lane >> 2) + (e >> 1) * 8, j = n * 8 + (lane & 3) * 2 + (e & 1);
-        s.kk[i][j] = dk[n][e] * s.row[0][j] * s.row[0][i];
-        s.qk[i][j] = dq[n][e] * s.row[0][j] * s.row[1][i];
-      }
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = rb * 16 + (lane >> 2) + e * 8, j = n * 8 + (lane & 3) * 2;
+          const float f = s.row[side][i];
+          *reinterpret_cast<float2*>(&(side ? s.qk : s.kk)[i][j]) =
+              make_float2(d[n][2 * e] * s.row[0][j] * f, d[n][2 * e + 1] * s.row[0][j + 1] * f);
+        }
+    }
   }
+  float k_most = 0.f;
+#pragma unroll
+  for (int j = 0; j < kChunk; ++j) k_most = fmaxf(k_most, s.most[0][j]);
 
-  const int group = p.hv / p.hk;
-  for (int sub = 0; sub < group; ++sub) {
+  __syncthreads();
+  for (int sub = which; sub < group; sub += HEADS) {  // from here on the 128 threads of a head meet among themselves
     const int vh = kh * group + sub;
     char* head = p.heads + (static_cast<long long>(chunk) * p.hv + vh) * L::kHead;
     float* coef = reinterpret_cast<float*>(head + L::kT + L::kP);
-    __syncthreads();
-    if (warp == 0) {  // running sum of g in 64 bits, kept as two floats
+    if (id < 32) {  // running sum of g in 64 bits, kept as two floats
+      if (sub != which) load_gates<T>(p, c, vh, lane, gate, bias);
       double sum[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int t = 2 * lane + e;
-        float g = 0.f, b = 0.f;
-        if (t < c.len) {
-          const long long gi = c.batch * p.g_batch + (c.token + t) * p.g_token + vh * p.g_head;
-          const long long bi = c.batch * p.beta_batch + (c.token + t) * p.beta_token + vh * p.beta_head;
-          g = p.gates32 ? static_cast<const float*>(p.g)[gi] : up(static_cast<const T*>(p.g)[gi]);
-          b = p.gates32 ? static_cast<const float*>(p.beta)[bi] : up(static_cast<const T*>(p.beta)[bi]);
-        }
         // e^-200 is 0 in fp32 already: a smaller g, -inf among them, is the same reset
-        sum[e] = g < -200.f ? -200.f : g;
-        s.beta[t] = b;
+        sum[e] = gate[e] < -200.f ? -200.f : gate[e];
+        beta[2 * lane + e] = bias[e];
       }
       sum[1] += sum[0];
       double total = sum[1];
@@ -160,71 +250,128 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prepare(DeltaParams p) {
         if (lane >= o) total += v;
       }
       const double before = total - sum[1];
+      float gf[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const double v = before + sum[e];
-        s.hi[2 * lane + e] = static_cast<float>(v);
-        s.lo[2 * lane + e] = static_cast<float>(v - static_cast<double>(static_cast<float>(v)));
+        gf[e] = static_cast<float>(v);
+        hi[2 * lane + e] = gf[e];
+        lo[2 * lane + e] = static_cast<float>(v - static_cast<double>(gf[e]));
+      }
+      float low = fminf(gf[0], gf[1]);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float v = __shfl_up_sync(0xffffffffu, low, o);
+        if (lane >= o) low = fminf(low, v);
+      }
+      float earlier = __shfl_up_sync(0xffffffffu, low, 1);
+      if (lane == 0) earlier = gf[0];
+      float rise = fmaxf(gf[1] - low, gf[0] - fminf(earlier, gf[0]));
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) rise = fmaxf(rise, __shfl_xor_sync(0xffffffffu, rise, o));
+      if (lane == 0) s.rise[which] = expf(fminf(rise, 80.f));
+    }
+    head_sync(which);
+    // diag(beta) M below the diagonal, and P as planes at a scale from a bound:
+    // |q_i . k_j| <= Dk max|q_i| max|k|
+    {
+      const int row = id >> 1;
+      const float g_hi = hi[row], g_lo = lo[row], b = beta[row];
+      const Pow2 f = pow2_for(DK * s.most[1][row] * k_most * s.rise[which]);
+      if (!(id & 1)) coef[kOutP * kChunk + row] = p.scale * f.inverse;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int unit = unit_of(i, id);
+        float pv[8], av[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pv[e] = av[e] = 0.f;
+        if (unit * 8 <= row) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int j = unit * 8 + e;
+            const float decay = exp_fast((g_hi - hi[j]) + (g_lo - lo[j]));
+            pv[e] = j <= row ? decay * s.qk[row][j] : 0.f;
+            av[e] = j < row ? b * (decay * s.kk[row][j]) : 0.f;
+          }
+        }
+        store_unit<PO>(head + L::kT, row, unit, pv, f.f);
+        *reinterpret_cast<float4*>(&t[row][unit * 8]) = make_float4(av[0], av[1], av[2], av[3]);
+        *reinterpret_cast<float4*>(&t[row][unit * 8 + 4]) = make_float4(av[4], av[5], av[6], av[7]);
       }
     }
-    __syncthreads();
-    // diag(beta) M below the diagonal; P as planes
-    char* to_p = head + L::kT;
-    for (int i = 0; i < kChunk / 4; ++i) {
-      const int row = warp * (kChunk / 4) + i;
-      float pv[2];
+    head_sync(which);
+    float x[16];
+    if (id < kChunk) {  // a column of a diagonal block's inverse
+      const int base = id & ~15, col = id & 15;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int j = 2 * lane + e;
-        const float decay = j <= row ? expf((s.hi[row] - s.hi[j]) + (s.lo[row] - s.lo[j])) : 0.f;
-        pv[e] = j <= row ? decay * s.qk[row][j] : 0.f;
-        s.a[row][j] = j < row ? s.beta[row] * (decay * s.kk[row][j]) : 0.f;
-      }
-      const float back = store_square_row<PO>(to_p, row, lane, pv[0], pv[1]);
-      if (lane == 0) coef[kOutP * kChunk + row] = p.scale * back;
-    }
-    __syncthreads();
-    // column j of T by forward substitution, in registers
-    float x[kChunk];
-    if (tid < kChunk) {
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i) {
+      for (int i = 0; i < 16; ++i) {
         float sum[4] = {};
 #pragma unroll
-        for (int l = 0; l + 4 <= i + 3; l += 4) {
-          const float4 a = *reinterpret_cast<const float4*>(&s.a[i][l]);
-          sum[0] = fmaf(a.x, l < i ? x[l] : 0.f, sum[0]);
+        for (int l = 0; l < i; l += 4) {
+          const float4 a = *reinterpret_cast<const float4*>(&t[base + i][base + l]);
+          sum[0] = fmaf(a.x, x[l], sum[0]);
           if (l + 1 < i) sum[1] = fmaf(a.y, x[l + 1], sum[1]);
           if (l + 2 < i) sum[2] = fmaf(a.z, x[l + 2], sum[2]);
           if (l + 3 < i) sum[3] = fmaf(a.w, x[l + 3], sum[3]);
         }
-        x[i] = (i == tid ? 1.f : 0.f) - ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        x[i] = (i == col ? 1.f : 0.f) - ((sum[0] + sum[1]) + (sum[2] + sum[3]));
       }
     }
-    __syncthreads();
-    if (tid < kChunk)
+    head_sync(which);
+    if (id < kChunk)
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) s.a[i][tid] = x[i];
-    __syncthreads();
-    for (int i = 0; i < kChunk / 4; ++i) {
-      const int row = warp * (kChunk / 4) + i;
-      const float2 v = *reinterpret_cast<const float2*>(&s.a[row][2 * lane]);
-      const float back = store_square_row<PS>(head, row, lane, v.x, v.y);
-      if (lane == 0) coef[kTRow * kChunk + row] = back;
+      for (int i = 0; i < 16; ++i) t[(id & ~15) + i][id] = x[i];
+    head_sync(which);
+    {  // 16 -> 32, two blocks side by side
+      const int b = (id >> 6) * 32, i = id & 63;
+      block_product<16, 1>(&t[b + 16][b], &t[b][b], &t[b][b + 16], 1.f, i);
+      head_sync(which);
+      block_product<16, 1>(&t[b + 16][b + 16], &t[b][b + 16], &t[b + 16][b], -1.f, i);
+      head_sync(which);
     }
-    if (tid < kChunk) {
-      const float gamma = exp_sum(s.hi[tid], s.lo[tid]), b = s.beta[tid];
-      const float tail = expf((s.hi[kChunk - 1] - s.hi[tid]) + (s.lo[kChunk - 1] - s.lo[tid]));
-      coef[kBeta * kChunk + tid] = b;
-      coef[kDown * kChunk + tid] = b * gamma * s.row[0][tid];
-      coef[kTail * kChunk + tid] = tail * s.row[0][tid];
-      coef[kOutQ * kChunk + tid] = p.scale * gamma * s.row[1][tid];
-      coef[kSumHi * kChunk + tid] = s.hi[tid];
-      coef[kSumLo * kChunk + tid] = s.lo[tid];
-      coef[kKRow * kChunk + tid] = s.row[0][tid];
-      coef[kQRow * kChunk + tid] = s.row[1][tid];
-      coef[kDecay * kChunk + tid] = exp_sum(s.hi[kChunk - 1], s.lo[kChunk - 1]);
+    // 32 -> 64; what lies above the diagonal blocks of 32 is not T and is masked
+    block_product<32, 2, true>(&t[32][0], &t[0][0], &t[0][32], 1.f, id);
+    head_sync(which);
+    block_product<32, 2, false, true>(&t[32][32], &t[0][32], &t[32][0], -1.f, id);
+    head_sync(which);
+    // T as planes, the coefficients
+    {
+      const int row = id >> 1;
+      float v[4][8], m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int unit = unit_of(i, id);
+        const float4 a = *reinterpret_cast<const float4*>(&t[row][unit * 8]), b = *reinterpret_cast<const float4*>(&t[row][unit * 8 + 4]);
+        v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
+        v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z, v[i][7] = b.w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (unit * 8 + e > row) v[i][e] = 0.f;
+          m = fmaxf(m, fabsf(v[i][e]));
+        }
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      const Pow2 f = pow2_for(m);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) store_unit<PS>(head, row, unit_of(i, id), v[i], f.f);
+      if (!(id & 1)) coef[kTRow * kChunk + row] = f.inverse;
     }
+    if (id < kChunk) {
+      const float gamma = exp_sum(hi[id], lo[id]), b = beta[id];
+      const float tail = expf((hi[kChunk - 1] - hi[id]) + (lo[kChunk - 1] - lo[id]));
+      coef[kBeta * kChunk + id] = b;
+      coef[kDown * kChunk + id] = b * gamma * s.row[0][id];
+      coef[kTail * kChunk + id] = tail * s.row[0][id];
+      coef[kOutQ * kChunk + id] = p.scale * gamma * s.row[1][id];
+    } else {
+      const int at = id - kChunk;
+      coef[kSumHi * kChunk + at] = hi[at];
+      coef[kSumLo * kChunk + at] = lo[at];
+      coef[kKRow * kChunk + at] = s.row[0][at];
+      coef[kQRow * kChunk + at] = s.row[1][at];
+      coef[kDecay * kChunk + at] = exp_sum(hi[kChunk - 1], lo[kChunk - 1]);
+    }
+    head_sync(which);
   }
 }
 

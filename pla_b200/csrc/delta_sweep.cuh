@@ -188,13 +188,6 @@ __device__ __forceinline__ void row_max(const float (&f)[N][4], float (&m)[2]) {
   m[1] = quad_max(m[1]);
 }
 
-// Over the quads of a warp, of what row_max gives.
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-
 // Accumulators of 16 rows x 8 N columns as planes of a tile of W columns, at
 // one scale for each row; the inverses go to `inverse` (16 of them).
 template <int PLANES, int W, int N>
@@ -365,17 +358,26 @@ __device__ __forceinline__ void state_store(float* to, const DeltaParams& p, con
         to[((static_cast<long long>(a.sequence) * p.hv + a.vh) * p.dk + dk) * p.dv + a.column + dv] = s[n][e];
     }
 }
-// Accumulators in fragment order [.., column tile, lane, 4], and the warp's
-// largest magnitude.
-template <int N>
-__device__ __forceinline__ void fragments_store(float* to, float* largest, int tile, int lane, const float (&f)[N][4]) {
+// A block's planes of a tile and the inverses of their scales to the
+// workspace: VB rows of W columns of plane after plane.
+template <int PLANES, int VB, int W>
+__device__ __forceinline__ void keep_tile(const char* tile, const float (*scale)[VB], char* to, float* scales, int rows, int column) {
+  constexpr int UNITS = VB * W * 2 / 16;
+  char* at = to + static_cast<long long>(column) * W * 2;
 #pragma unroll
-  for (int n = 0; n < N; ++n)
-    *reinterpret_cast<float4*>(to + ((tile + n) * 32 + lane) * 4) = make_float4(f[n][0], f[n][1], f[n][2], f[n][3]);
-  float m[2];
-  row_max(f, m);
-  const float most = warp_max(fmaxf(m[0], m[1]));
-  if (lane == 0) *largest = most;
+  for (int n = 0; n < PLANES; ++n)
+#pragma unroll
+    for (int i = 0; i < UNITS / (VB * 8); ++i) {
+      const int u = i * VB * 8 + threadIdx.x;
+      reinterpret_cast<uint4*>(at + static_cast<long long>(n) * rows * W * 2)[u] =
+          reinterpret_cast<const uint4*>(tile + n * VB * W * 2)[u];
+    }
+  if (threadIdx.x < 4 * VB) scales[threadIdx.x / VB * rows + column + threadIdx.x % VB] = (&scale[0][0])[threadIdx.x];
+}
+// Where a (chunk, value head) keeps what: bytes of the planes, floats of the scales.
+template <int PLANES, int W>
+__device__ __forceinline__ long long kept_at(const DeltaParams& p, long long head) {
+  return head * PLANES * p.rows * W * 2;
 }
 
 template <int N>
@@ -444,16 +446,16 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p, int stages)
 
   for (int c = 0; c < a.chunks; ++c) {
     const int len = min(kChunk, a.len - c * kChunk);
-    const long long slab_at = (static_cast<long long>(a.first + c) * p.hv + a.vh) * p.slabs + a.column / 16 + wm;
-    const bool kept = m0 < a.width;
-    if (KEEP && kept)
-      fragments_store(p.states + slab_at * 16 * DK, p.largest + (slab_at * 4 + wn) * 4, wn * QN, lane, s);
+    const long long head_at = static_cast<long long>(a.first + c) * p.hv + a.vh;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     const char* stage = ring.wait(c);
     __syncthreads();  // planes of S and this chunk's v are there; the other slab is free
     if (c + 1 < a.chunks)
       slab_fetch<T, VB>(m.slab[~c & 1], v + (c + 1) * kChunk * p.v_token, p.v_token, min(kChunk, a.len - (c + 1) * kChunk),
                         a.width, p.vec_v);
+    if (KEEP)
+      keep_tile<PS, VB, DK>(m.s, m.scale[0], p.states + kept_at<PS, DK>(p, head_at), p.scales + head_at * 16 * p.rows, p.rows,
+                            a.column);
     const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
     const char* coef = stage + L::kTiles + L::kT + L::kP;
     float x[2][4] = {}, q[2][4] = {};
@@ -500,15 +502,14 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p, int stages)
     }
     coef_read(coef, kTRow, wn * 2, lane, w);
     scale_columns(u, w);
-    if (KEEP) {
-      if (kept) fragments_store(p.us + slab_at * 16 * kChunk, p.largest + (slab_at * 4 + wn) * 4 + 2, wn * 2, lane, u);
-    } else {
-      tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, u, &m.scale[3][wn][m0]);
-    }
+    tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, u, &m.scale[3][wn][m0]);
     coef_read(coef, kTail, wn * 2, lane, w);
     scale_columns(u, w);
     tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, u, &m.scale[2][wn][m0]);
     __syncthreads();
+    if (KEEP)  // here PO = PS
+      keep_tile<PO, VB, kChunk>(m.c, m.scale[3], p.us + kept_at<PO, kChunk>(p, head_at),
+                                p.scales + (head_at * 16 + 8) * p.rows, p.rows, a.column);
     // S^T = e^{G_C} S^T + (e^{G_C - G} U)^T K
     const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
 #pragma unroll

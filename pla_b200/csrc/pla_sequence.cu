@@ -273,7 +273,7 @@ int check_delta(const pla_delta* a) {
 
 struct DeltaSizes {
   long long chunks = 0;
-  size_t plan = 0, tiles = 0, heads = 0, states = 0, us = 0, largest = 0, total = 0;
+  size_t plan = 0, tiles = 0, heads = 0, states = 0, us = 0, scales = 0, total = 0;
 };
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -283,16 +283,16 @@ DeltaSizes delta_sizes_of(const pla_delta* a, bool backward) {
   DeltaSizes s;
   s.chunks = a->cu_seqlens ? a->tokens / kChunk + static_cast<long long>(a->sequences)
                            : static_cast<long long>(a->batch) * ((a->tokens + kChunk - 1) / kChunk);
-  s.plan = a->cu_seqlens ? up256((3ull * a->sequences + 1) * sizeof(int)) : 0;
+  s.plan = a->cu_seqlens ? up256(s.chunks * sizeof(int4)) + up256((3ull * a->sequences + 1) * sizeof(int)) : 0;
   s.tiles = up256(static_cast<size_t>(s.chunks) * a->hk * L::kTiles);
   s.heads = up256(static_cast<size_t>(s.chunks) * a->hv * L::kHead);
   if (backward) {
-    const size_t columns = static_cast<size_t>(s.chunks) * a->hv * ((a->dv + 15) / 16) * 16;
-    s.states = up256(columns * DK * sizeof(float));
-    s.us = up256(columns * kChunk * sizeof(float));
-    s.largest = up256(columns * sizeof(float));
+    const size_t rows = static_cast<size_t>(s.chunks) * a->hv * ((a->dv + 63) / 64) * 64;
+    s.states = up256(rows * PS * DK * 2);
+    s.us = up256(rows * PS * kChunk * 2);
+    s.scales = up256(rows * 16 * sizeof(float));
   }
-  s.total = s.plan + s.tiles + s.heads + 2 * s.states + 2 * s.us + s.largest;
+  s.total = s.plan + s.tiles + s.heads + 2 * s.states + 2 * s.us + s.scales;
   return s;
 }
 
@@ -348,21 +348,23 @@ DeltaParams delta_params(const pla_delta* a, const DeltaSizes& s) {
   p.chunk_bound = static_cast<int>(s.chunks);
   p.slabs = (a->dv + 15) / 16;
   char* w = static_cast<char*>(a->workspace);
-  p.plan = reinterpret_cast<int*>(w);
+  p.table = reinterpret_cast<int4*>(w);
+  p.plan = reinterpret_cast<int*>(w + up256(s.chunks * sizeof(int4)));
   w += s.plan;
   p.tiles = w;
   w += s.tiles;
   p.heads = w;
   w += s.heads;
-  p.states = reinterpret_cast<float*>(w);
+  p.states = w;
   w += s.states;
-  p.dstates = reinterpret_cast<float*>(w);
+  p.dstates = w;
   w += s.states;
-  p.us = reinterpret_cast<float*>(w);
+  p.us = w;
   w += s.us;
-  p.dxs = reinterpret_cast<float*>(w);
+  p.dxs = w;
   w += s.us;
-  p.largest = reinterpret_cast<float*>(w);
+  p.scales = reinterpret_cast<float*>(w);
+  p.rows = (a->dv + 63) / 64 * 64;
   const size_t es = type_size(a->dtype);
   const int whole = static_cast<int>(16 / es);
   p.vec_qk = a->dk % 4 == 0 && aligned_to(a->q, 4 * es) && aligned_to(a->k, 4 * es) &&
@@ -375,17 +377,21 @@ DeltaParams delta_params(const pla_delta* a, const DeltaSizes& s) {
 template <typename T, int DK, int PS, int PO>
 int launch_prepare(const DeltaParams& p, cudaStream_t stream) {
   if (p.cu) {
-    delta_plan<<<1, 1024, 0, stream>>>(p.cu, p.tokens, p.sequences, p.plan);
+    delta_plan<<<1, 1024, 0, stream>>>(p.cu, p.tokens, p.sequences, p.plan, p.table, p.chunk_bound);
     const int st = launched("delta_plan");
     if (st != PLA_OK) return st;
   }
   if (static_cast<long long>(p.chunk_bound) * p.hk > kMaxGrid) return PLA_ERR_TOO_LARGE;
   if (!p.chunk_bound) return PLA_OK;
-  const size_t shared = sizeof(PrepShared<T, DK>);
-  const int st = allow_shared<delta_prepare<T, DK, PS, PO>>(shared);
-  if (st != PLA_OK) return st;
-  delta_prepare<T, DK, PS, PO><<<p.chunk_bound * p.hk, kPrepThreads, shared, stream>>>(p);
-  return launched("delta_prepare");
+  const auto go = [&](auto heads) {
+    constexpr int HEADS = decltype(heads)::value;
+    const size_t shared = sizeof(PrepShared<T, DK, HEADS>);
+    const int st = allow_shared<delta_prepare<T, DK, PS, PO, HEADS>>(shared);
+    if (st != PLA_OK) return st;
+    delta_prepare<T, DK, PS, PO, HEADS><<<p.chunk_bound * p.hk, 128 * HEADS, shared, stream>>>(p);
+    return launched("delta_prepare");
+  };
+  return p.hv > p.hk ? go(Int<2>{}) : go(Int<1>{});  // two value heads of a key head side by side
 }
 
 // Stages of the ring and shared memory of a sweep.
