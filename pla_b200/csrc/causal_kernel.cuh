@@ -5,11 +5,14 @@
 // (oldest first) or zero.
 //
 // Bound by HBM: x is read and y written once, 2 K flops an element.  A thread
-// owns V neighbouring channels (16 bytes a load) of a strip of tokens and
-// walks it with the last K - 1 inputs in registers, so an input is fetched
-// once plus (K - 1) / strip of overlap that neighbouring strips leave in L2;
-// loads of four tokens are issued together to keep bytes in flight.  The
-// products are summed in fp32 in tap order, rounded once.
+// owns four neighbouring channels of a strip of tokens and walks it with the
+// last K - 1 inputs in registers, so an input is fetched once plus
+// (K - 1) / strip of overlap that neighbouring strips leave in L2; the loads of
+// four tokens are issued while the four before them are worked on.  Four
+// channels (8 bytes a 16-bit load) and not eight: eight took 148 registers a
+// thread, which left 8 warps an SM and too few bytes in flight (140 us for
+// 8191 x 8192 bf16, against CAUSALFWD).  The products are summed in fp32 in tap
+// order, two channels an instruction, and rounded once.
 //
 // Backward, with dp[t] = dy[t] act'(p[t]) recomputed from x:
 //     dx[t] = sum_j w[j] dp[t + K - 1 - j],  dw[j] = sum_t dp[t] x[t - K + 1 + j],  db = sum_t dp[t].
@@ -91,13 +94,17 @@ __device__ __forceinline__ void input_before(const CausalParams& p, const T* x, 
 
 template <typename T, int V, int K>
 __device__ __forceinline__ void load_filter(const CausalParams& p, int c, float (&w)[K][V], float (&b)[V]) {
-  const T* wt = static_cast<const T*>(p.w) + static_cast<long long>(c) * K;
+  const T* wt = static_cast<const T*>(p.w) + static_cast<long long>(c) * K;  // V filters of K taps
+  float flat[V * K];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int i = 0; i < K; ++i) load<T, V>(wt + i * V, *reinterpret_cast<float(*)[V]>(&flat[i * V]));
 #pragma unroll
-    for (int j = 0; j < K; ++j) w[j][i] = up(wt[i * K + j]);
-    b[i] = p.b ? up(static_cast<const T*>(p.b)[c + i]) : 0.f;
-  }
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < K; ++j) w[j][i] = flat[i * K + j];
+#pragma unroll
+  for (int i = 0; i < V; ++i) b[i] = 0.f;
+  if (p.b) load<T, V>(static_cast<const T*>(p.b) + c, b);
 }
 
 // The K - 1 inputs behind a sequence's last token: rows len .. len + K - 2 of [state; x].
@@ -123,7 +130,7 @@ __device__ __forceinline__ void copy_state(const CausalParams& p, long long item
 constexpr int kCausalThreads = 256;
 
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kCausalThreads) causal_forward(CausalParams p, int main_blocks) {
+__global__ void __launch_bounds__(kCausalThreads, 3) causal_forward(CausalParams p, int main_blocks) {
   if (static_cast<int>(blockIdx.x) >= main_blocks) {
     copy_state<T, V, K>(p, static_cast<long long>(blockIdx.x - main_blocks) * kCausalThreads + threadIdx.x);
     return;
@@ -137,44 +144,84 @@ __global__ void __launch_bounds__(kCausalThreads) causal_forward(CausalParams p,
   const int t0 = static_cast<int>(strip % p.strips) * p.strip;
   const int t1 = min(t0 + p.strip, p.tokens);
   const T* x = static_cast<const T*>(p.x) + batch * p.x_batch;
-  T* y = static_cast<T*>(p.y) + static_cast<long long>(batch) * p.tokens * p.channels + c;
+  T* y = static_cast<T*>(p.y) + (static_cast<long long>(batch) * p.tokens + t0) * p.channels + c;
 
-  float w[K][V], b[V], seen[K - 1][V];
-  load_filter<T, V, K>(p, c, w, b);
+  constexpr int U = 4, H = (V + 1) / 2;
+  using Row = Vec<T, V>;
+  const T* from = x + t0 * p.x_token + c;
+  Row next[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i)
+    if (t0 + i < t1) next[i] = *reinterpret_cast<const Row*>(from + i * p.x_token);
+  Pair w[K][H], b[H], seen[K - 1][H];
   SequenceWalk s;
   s.begin(p, batch, t0);
+  {
+    float wf[K][V], bf[V];
+    load_filter<T, V, K>(p, c, wf, bf);
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j) input_before<T, V, K>(p, x, s, t0, K - 1 - j, c, seen[j]);
-
-  constexpr int U = 4;
+    for (int v = 0; v < H; ++v) {
+#pragma unroll
+      for (int j = 0; j < K; ++j) w[j][v] = pair(wf[j][2 * v], 2 * v + 1 < V ? wf[j][(2 * v + 1) % V] : 0.f);
+      b[v] = pair(bf[2 * v], 2 * v + 1 < V ? bf[(2 * v + 1) % V] : 0.f);
+    }
+  }
+  const auto refill = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+      float f[V];
+      input_before<T, V, K>(p, x, s, t, K - 1 - j, c, f);
+#pragma unroll
+      for (int v = 0; v < H; ++v) seen[j][v] = pair(f[2 * v], 2 * v + 1 < V ? f[(2 * v + 1) % V] : 0.f);
+    }
+  };
+  refill(t0);
   for (int t = t0; t < t1; t += U) {
-    Vec<T, V> in[U];
+    Row in[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) in[i] = next[i];
+    from += U * p.x_token;
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (t + i < t1) in[i] = *reinterpret_cast<const Vec<T, V>*>(x + (t + i) * p.x_token + c);
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (t + i >= t1) break;
-      if (t + i >= s.end) {
-        s.next(p, batch, t + i);
-#pragma unroll
-        for (int j = 0; j < K - 1; ++j) input_before<T, V, K>(p, x, s, t + i, K - 1 - j, c, seen[j]);
-      }
+      if (t + U + i < t1) next[i] = *reinterpret_cast<const Row*>(from + i * p.x_token);
+    const auto one = [&](const Row& row) {
       float out[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float now = up(in[i].e[v]);
-        float a = b[v];
+      for (int v = 0; v < H; ++v) {
+        const Pair now = pair(up(row.e[2 * v]), 2 * v + 1 < V ? up(row.e[(2 * v + 1) % V]) : 0.f);
+        Pair a = b[v];
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) a = fmaf(w[j][v], seen[j][v], a);
-        a = fmaf(w[K - 1][v], now, a);
-        if (p.silu) a *= sigmoid<T>(a);
-        out[v] = s.index >= 0 ? a : 0.f;
+        for (int j = 0; j < K - 1; ++j) a = fma2(w[j][v], seen[j][v], a);
+        a = fma2(w[K - 1][v], now, a);
+        const float2 f = both(a);
+        out[2 * v] = f.x;
+        if (2 * v + 1 < V) out[(2 * v + 1) % V] = f.y;
 #pragma unroll
         for (int j = 0; j + 1 < K - 1; ++j) seen[j][v] = seen[j + 1][v];
         seen[K - 2][v] = now;
       }
-      store<T, V>(y + static_cast<long long>(t + i) * p.channels, out);
+      if (p.silu)
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[v] *= sigmoid<T>(out[v]);
+      if (s.index < 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[v] = 0.f;
+      store<T, V>(y, out);
+      y += p.channels;
+    };
+    if (t + U <= t1 && t + U <= s.end) {  // four tokens of one sequence
+#pragma unroll
+      for (int i = 0; i < U; ++i) one(in[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (t + i >= t1) break;
+        if (t + i >= s.end) {
+          s.next(p, batch, t + i);
+          refill(t + i);
+        }
+        one(in[i]);
+      }
     }
   }
 }
@@ -189,8 +236,10 @@ __device__ __forceinline__ float act_slope(float a) {
 constexpr int kCausalRows = 8;  // strips of a block in the backward pass
 
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kCausalThreads) causal_backward(CausalParams p) {
+__global__ void __launch_bounds__(kCausalThreads, V > 1 ? 2 : 3) causal_backward(CausalParams p) {
   __shared__ float part[kCausalRows / 2][K + 1][32 * V];
+  constexpr int H = (V + 1) / 2, U = 4;
+  using Row = Vec<T, V>;
   const int nvec = p.channels / V;
   const int across = (nvec + 31) / 32;
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
@@ -203,71 +252,141 @@ __global__ void __launch_bounds__(kCausalThreads) causal_backward(CausalParams p
   if (cv < nvec && batch < p.batch) {
     const int t0 = static_cast<int>(strip % p.strips) * p.strip;
     const int t1 = min(t0 + p.strip, p.tokens);
+    const int last = t1 + K - 1, there = min(last, p.tokens);  // tokens past the strip only finish its last dx
     const T* x = static_cast<const T*>(p.x) + batch * p.x_batch;
-    const T* dy = static_cast<const T*>(p.dy) + batch * p.dy_batch;
-    T* dx = static_cast<T*>(p.dx) + static_cast<long long>(batch) * p.tokens * p.channels + c;
-    float w[K][V], b[V], seen[K][V], ahead[K][V] = {};  // ahead[j]: dx of token t - K + 1 + j so far
-    load_filter<T, V, K>(p, c, w, b);
+    const T* x_at = x + t0 * p.x_token + c;
+    const T* dy_at = static_cast<const T*>(p.dy) + batch * p.dy_batch + t0 * p.dy_token + c;
+    T* dx = static_cast<T*>(p.dx) + (static_cast<long long>(batch) * p.tokens + t0) * p.channels + c;
+    Row x_next[U], dy_next[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (t0 + i < there) {
+        x_next[i] = *reinterpret_cast<const Row*>(x_at + i * p.x_token);
+        dy_next[i] = *reinterpret_cast<const Row*>(dy_at + i * p.dy_token);
+      }
+    const auto two = [](const float (&f)[V], int v) { return pair(f[2 * v], 2 * v + 1 < V ? f[(2 * v + 1) % V] : 0.f); };
+    Pair w[K][H], b[H], seen[K][H], ahead[K][H], gw[K][H], gb[H];  // ahead[j]: dx of token t - K + 1 + j so far
+    {
+      float wf[K][V], bf[V];
+      load_filter<T, V, K>(p, c, wf, bf);
+#pragma unroll
+      for (int v = 0; v < H; ++v) {
+        b[v] = two(bf, v);
+        gb[v] = pair(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+          w[j][v] = two(wf[j], v);
+          ahead[j][v] = gw[j][v] = pair(0.f, 0.f);
+        }
+      }
+    }
     SequenceWalk s;
     s.begin(p, batch, t0);
+    const auto refill = [&](int t) {
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) input_before<T, V, K>(p, x, s, t0, K - 1 - j, c, seen[j + 1]);
-    constexpr int U = 2;
-    const int last = t1 + K - 1;  // tokens past the strip only finish its last dx
+      for (int j = 0; j < K - 1; ++j) {
+        float f[V];
+        input_before<T, V, K>(p, x, s, t, K - 1 - j, c, f);
+#pragma unroll
+        for (int v = 0; v < H; ++v) seen[j + 1][v] = two(f, v);
+      }
+    };
+    refill(t0);
     for (int t = t0; t < last; t += U) {
-      Vec<T, V> in[U], up_in[U];
+      Row in[U], give_in[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) in[i] = x_next[i], give_in[i] = dy_next[i];
+      x_at += U * p.x_token;
+      dy_at += U * p.dy_token;
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        if (t + i < last && t + i < p.tokens) {
-          in[i] = *reinterpret_cast<const Vec<T, V>*>(x + (t + i) * p.x_token + c);
-          up_in[i] = *reinterpret_cast<const Vec<T, V>*>(dy + (t + i) * p.dy_token + c);
+        if (t + U + i < there) {
+          x_next[i] = *reinterpret_cast<const Row*>(x_at + i * p.x_token);
+          dy_next[i] = *reinterpret_cast<const Row*>(dy_at + i * p.dy_token);
         }
+      // gradient of one token that is in a sequence, without what the state after it gives
+      const auto one = [&](const Row& row, const Row& grad, bool own, int reach) {
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int now = t + i;
-        if (now >= last) break;
-        if (now < p.tokens && now >= s.end) {
-          s.next(p, batch, now);
+        for (int v = 0; v < H; ++v) {
+          seen[K - 1][v] = pair(up(row.e[2 * v]), 2 * v + 1 < V ? up(row.e[(2 * v + 1) % V]) : 0.f);
+          Pair g = pair(up(grad.e[2 * v]), 2 * v + 1 < V ? up(grad.e[(2 * v + 1) % V]) : 0.f);
+          if (p.silu) {
+            Pair a = b[v];
 #pragma unroll
-          for (int j = 0; j < K - 1; ++j) input_before<T, V, K>(p, x, s, now, K - 1 - j, c, seen[j + 1]);
-        }
-        const bool live = now < p.tokens && s.index >= 0;
-        float give[V] = {};
-        if (live && p.dstate_out) {  // the state after the sequence holds this token's input
-          const int r = K - 1 + now - min(s.end, p.tokens);
-          if (r >= 0)
-            load<T, V>(static_cast<const T*>(p.dstate_out) +
-                           (static_cast<long long>(s.index) * (K - 1) + r) * p.channels + c, give);
-        }
+            for (int j = 0; j < K; ++j) a = fma2(w[j][v], seen[j][v], a);
+            const float2 f = both(a);
+            float2 gf = both(g);
+            gf.x *= act_slope<T>(f.x);
+            if (2 * v + 1 < V) gf.y *= act_slope<T>(f.y);
+            g = pair(gf.x, gf.y);
+          }
+          if (own) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-#pragma unroll
-          for (int j = 0; j < K - 1; ++j) seen[j][v] = seen[j + 1][v];
-          float g = 0.f;
-          if (live) {
-            seen[K - 1][v] = up(in[i].e[v]);
-            g = up(up_in[i].e[v]);
-            if (p.silu) {
-              float a = b[v];
-#pragma unroll
-              for (int j = 0; j < K; ++j) a = fmaf(w[j][v], seen[j][v], a);
-              g *= act_slope<T>(a);
-            }
-            if (now < t1) {
-#pragma unroll
-              for (int j = 0; j < K; ++j) dw[j][v] = fmaf(g, seen[j][v], dw[j][v]);
-              db[v] += g;
-            }
+            for (int j = 0; j < K; ++j) gw[j][v] = fma2(g, seen[j][v], gw[j][v]);
+            gb[v] = fma2(g, pair(1.f, 1.f), gb[v]);
           }
 #pragma unroll
-          for (int j = 0; j < K - 1; ++j) ahead[j][v] = ahead[j + 1][v];
-          ahead[K - 1][v] = give[v];
-#pragma unroll
           for (int j = 0; j < K; ++j)
-            if (live && now - (K - 1 - j) >= s.start) ahead[j][v] = fmaf(w[j][v], g, ahead[j][v]);
+            if (K - 1 - j <= reach) ahead[j][v] = fma2(w[j][v], g, ahead[j][v]);
         }
-        const int done = now - (K - 1);
-        if (done >= t0 && done < t1) store<T, V>(dx + static_cast<long long>(done) * p.channels, ahead[0]);
+      };
+      const auto shift = [&](const float (&give)[V]) {
+#pragma unroll
+        for (int v = 0; v < H; ++v) {
+#pragma unroll
+          for (int j = 0; j < K - 1; ++j) seen[j][v] = seen[j + 1][v], ahead[j][v] = ahead[j + 1][v];
+          ahead[K - 1][v] = two(give, v);
+        }
+      };
+      const auto emit = [&]() {
+        float out[V];
+#pragma unroll
+        for (int v = 0; v < H; ++v) {
+          const float2 f = both(ahead[0][v]);
+          out[2 * v] = f.x;
+          if (2 * v + 1 < V) out[(2 * v + 1) % V] = f.y;
+        }
+        store<T, V>(dx, out);
+        dx += p.channels;
+      };
+      const float none[V] = {};
+      if (s.index >= 0 && t >= t0 + K - 1 && t >= s.start + K - 1 && t + U <= t1 && t + U + K - 1 <= s.end) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {  // four tokens well inside a sequence and the strip
+          shift(none);
+          one(in[i], give_in[i], true, K - 1);
+          emit();
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int now = t + i;
+          if (now >= last) break;
+          if (now < p.tokens && now >= s.end) {
+            s.next(p, batch, now);
+            refill(now);
+          }
+          const bool live = now < p.tokens && s.index >= 0;
+          float give[V] = {};
+          if (live && p.dstate_out) {  // the state after the sequence holds this token's input
+            const int r = K - 1 + now - min(s.end, p.tokens);
+            if (r >= 0)
+              load<T, V>(static_cast<const T*>(p.dstate_out) +
+                             (static_cast<long long>(s.index) * (K - 1) + r) * p.channels + c, give);
+          }
+          shift(give);
+          if (live) one(in[i], give_in[i], now < t1, now - s.start);
+          if (now - (K - 1) >= t0) emit();
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < H; ++v) {
+#pragma unroll
+      for (int j = 0; j <= K; ++j) {
+        const float2 f = both(j < K ? gw[j % K][v] : gb[v]);
+        (j < K ? dw[j % K] : db)[2 * v] = f.x;
+        if (2 * v + 1 < V) (j < K ? dw[j % K] : db)[(2 * v + 1) % V] = f.y;
       }
     }
   }

@@ -20,8 +20,8 @@
 namespace pla {
 namespace seq {
 
-template <typename T, int DK, int PS, int PO, int VB>
-__global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int stages) {
+template <typename T, int DK, int PS, int PO, int VB, int STAGES>
+__global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p) {
   using L = DeltaLayout<T, DK, PS, PO>;
   using M = SweepShared<T, DK, PS, PO, VB, true>;
   constexpr int IN = L::kIn, QN = DK / 32;
@@ -29,16 +29,16 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int st
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int wm = warp % (VB / 16), wn = warp / (VB / 16), m0 = wm * 16;
   const SweepAt a = sweep_at(p, VB);
-  Ring<L> ring;
-  ring.begin(shared_bytes, stages, VB / 4);
-  M& m = *reinterpret_cast<M*>(shared_bytes + kSweepRing + stages * L::kStage);
+  Ring<L, STAGES> ring;
+  ring.begin(shared_bytes, VB / 4);
+  M& m = *reinterpret_cast<M*>(shared_bytes + kSweepRing + STAGES * L::kStage);
   const uint32_t dt = shared_u32(m.s), yt = shared_u32(m.a), xt = shared_u32(m.b), wt = shared_u32(m.c), ft = shared_u32(m.d);
   const T* d_o = static_cast<const T*>(p.d_o) + a.batch * p.do_batch + a.lo * p.do_token + a.vh * p.do_head + a.column;
   const long long dv_step = static_cast<long long>(p.hv) * p.dv;
   T* dv = static_cast<T*>(p.dv_out) + (static_cast<long long>(a.batch) * p.tokens + a.lo) * dv_step +
           static_cast<long long>(a.vh) * p.dv + a.column;
   if (threadIdx.x == 0)
-    for (int i = 0; i < stages && i < a.chunks; ++i) ring.fill(p, i, a.first + a.chunks - 1 - i, a.kh, a.vh);
+    for (int i = 0; i < STAGES && i < a.chunks; ++i) ring.fill(p, i, a.first + a.chunks - 1 - i, a.kh, a.vh);
   if (a.chunks)
     slab_fetch<T, VB>(m.slab[0], d_o + (a.chunks - 1) * kChunk * p.do_token, p.do_token, a.len - (a.chunks - 1) * kChunk,
                       a.width, p.vec_do);
@@ -48,25 +48,42 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int st
   uint32_t ks[QN / 2];                                                              // in K and Q, for the state's update
 #pragma unroll
   for (int n = 0; n < QN / 2; ++n) ks[n] = at_kn<DK>(lane, wn * (DK / 4) + n * 16, 0);
-  float d[QN][4];
+  float d[QN][4], top[2];
+  Pow2 fd[2];
   state_load(p.dstate_out, p, a, m0, wn * (DK / 4), lane, d);
-  tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, &m.scale[0][wn][m0]);
+  {
+    row_max(d, top);
+    share(m.most_s, wn, m0, lane, top[0], top[1]);
+    __syncthreads();
+    float4 all[2];
+    shared_of(m.most_s, m0, lane, all);
+    fd[0] = scale_below(most_of(all[0]));
+    fd[1] = scale_below(most_of(all[1]));
+    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, fd);
+  }
 
   for (int turn = 0; turn < a.chunks; ++turn) {
     const int c = a.chunks - 1 - turn, len = min(kChunk, a.len - c * kChunk);
     const long long head_at = static_cast<long long>(a.first + c) * p.hv + a.vh;
+    if (wn == 0 && (lane & 3) == 0) {
+      m.keep_s[m0 + (lane >> 2)] = fd[0].inverse;
+      m.keep_s[m0 + (lane >> 2) + 8] = fd[1].inverse;
+    }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    const char* stage = ring.wait(turn);
+    const char* stage = ring.wait();
     __syncthreads();  // planes of D and this chunk's do are there; the other slab is free
     if (c > 0)
       slab_fetch<T, VB>(m.slab[~turn & 1], d_o + (c - 1) * kChunk * p.do_token, p.do_token, kChunk, a.width, p.vec_do);
-    keep_tile<PS, VB, DK>(m.s, m.scale[0], p.dstates + kept_at<PS, DK>(p, head_at), p.scales + (head_at * 16 + 4) * p.rows,
-                          p.rows, a.column);
+    keep_tile<PS, VB, DK>(m.s, m.keep_s, p.dstates + kept_at<PS, DK>(p, head_at), p.scales + (head_at * 4 + 1) * p.rows, p.rows,
+                          a.column);
     const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
     const char* coef = stage + L::kTiles + L::kT + L::kP;
+    const float4 bounds = *reinterpret_cast<const float4*>(coef + kBounds * kChunk * 4);
+    const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
     float2 w[2];
-    {  // do' with the weights of P's rows and with e^G
-      float f[2][4], g[2][4];
+    float g[2][4];  // e^G do'
+    {
+      float f[2][4];
       slab_read<T, VB>(m.slab[turn & 1], wn * 16, m0, lane, f);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -74,56 +91,84 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int st
         for (int e = 0; e < 4; ++e) g[n][e] = f[n][e];
       coef_read(coef, kOutP, wn * 2, lane, w);
       scale_columns(f, w);
-      tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, f, &m.scale[3][wn][m0]);
+      row_max(f, top);
+      const Pow2 fw[2] = {pow2_for(top[0]), pow2_for(top[1])};
+      share(m.scale_c, wn, m0, lane, fw[0].inverse, fw[1].inverse);
+      tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, f, fw);
       coef_read(coef, kOutQ, wn * 2, lane, w);
       scale_columns(g, w);
-      tile_write<PS, kChunk>(m.d, M::kNarrow, m0, wn * 16, lane, g, &m.scale[4][wn][m0]);
+      row_max(g, top);
+      share(m.most_d, wn, m0, lane, top[0], top[1]);
     }
     // (K D)^T
-    float du[2][4] = {};
+    float du[2][4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      float bx[2][4] = {};
-#pragma unroll
-      for (int k = 0; k < DK / 64; ++k) {
-        const int kk = b * (DK / 64) + k;
-        uint32_t hi[4], lo[4];
-        tile_operand<PS>(dw[kk], M::kWide, hi, lo);
-        product<PS, IN, false>(bx[0], bx[1], hi, lo, kt + kw[kk], L::kTile);
-      }
-      add_scaled(du, bx, &m.scale[0][b][m0], lane);
+    for (int kk = 0; kk < DK / 16; ++kk) {
+      uint32_t hi[4], lo[4];
+      tile_operand<PS>(dw[kk], M::kWide, hi, lo);
+      product<PS, IN, false>(du[0], du[1], hi, lo, kt + kw[kk], L::kTile, kk == 0);
     }
+    float4 most[2];
+    shared_of(m.most_s, m0, lane, most);
     coef_read(coef, kTail, wn * 2, lane, w);
-    scale_columns(du, w);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) du[n][e] *= (e & 1 ? w[n].y : w[n].x) * fd[e >> 1].inverse;
     __syncthreads();
     // dU = P^T do' + e^{G_C - G} (K D): tokens j take from i >= j
+    float4 back[2], most_g[2];
+    shared_of(m.scale_c, m0, lane, back);
+    shared_of(m.most_d, m0, lane, most_g);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       if (VB == 64 && kk < wn) continue;  // the other blocks are zero
       uint32_t hi[4], lo[4];
-      float bx[2][4] = {};
+      float bx[2][4];
       tile_operand<PO>(yw[kk] + (wt - yt), M::kNarrow, hi, lo);
-      product<PO, PO, true>(bx[0], bx[1], hi, lo, pt + ts + kk * 16 * kChunk * 2, L::kSquare);
-      add_scaled(du, bx, &m.scale[3][kk][m0], lane);
+      product<PO, PO, true>(bx[0], bx[1], hi, lo, pt + ts + kk * 16 * kChunk * 2, L::kSquare, true);
+      add_scaled(du, bx, element(back[0], kk), element(back[1], kk));
     }
     coef_read(coef, kTRow, wn * 2, lane, w);
     scale_columns(du, w);
-    tile_write<PS, kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, du, &m.scale[1][wn][m0]);
+    {
+      row_max(du, top);
+      const Pow2 fy[2] = {pow2_for(top[0]), pow2_for(top[1])};
+      share(m.scale_a, wn, m0, lane, fy[0].inverse, fy[1].inverse);
+      tile_write<PS, kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, du, fy);
+    }
     __syncthreads();
     // dX^T = (T^T dU)^T
     float x[2][4] = {};
+    shared_of(m.scale_a, m0, lane, back);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       if (VB == 64 && kk < wn) continue;  // the other blocks are zero
       uint32_t hi[4], lo[4];
-      float bx[2][4] = {};
+      float bx[2][4];
       tile_operand<PS>(yw[kk], M::kNarrow, hi, lo);
-      product<PS, PS, true>(bx[0], bx[1], hi, lo, tt + ts + kk * 16 * kChunk * 2, L::kSquare);
-      add_scaled(x, bx, &m.scale[1][kk][m0], lane);
+      product<PS, PS, true>(bx[0], bx[1], hi, lo, tt + ts + kk * 16 * kChunk * 2, L::kSquare, true);
+      add_scaled(x, bx, element(back[0], kk), element(back[1], kk));
     }
-    tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, x, &m.scale[3][wn][m0]);  // PO = PS; do' is done with
+    const float bound_x[2] = {kSumTop * kPlaneTop * most_of(back[0]), kSumTop * kPlaneTop * most_of(back[1])};
+    // dX is kept, at a scale from its bound; do' is done with, and PO = PS
+    const Pow2 fk[2] = {scale_below(bound_x[0]), scale_below(bound_x[1])};
+    tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, x, fk);
+    if (wn == 0 && (lane & 3) == 0) {
+      m.keep_c[m0 + (lane >> 2)] = fk[0].inverse;
+      m.keep_c[m0 + (lane >> 2) + 8] = fk[1].inverse;
+    }
+    // e^G do' and -beta e^G dX at one scale
+    float bound_f[2];
+    Pow2 ff[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bound_f[h] = fmaxf(most_of(most_g[h]), bounds.z * bound_x[h]);
+      ff[h] = scale_below(bound_f[h]);
+    }
+    tile_write<PS, kChunk>(m.d, M::kNarrow, m0, wn * 16, lane, g, ff);
     {
-      float out[2][4], minus[2][4];
+      float out[2][4];
       float2 b[2];
       coef_read(coef, kBeta, wn * 2, lane, b);
       coef_read(coef, kDown, wn * 2, lane, w);
@@ -132,41 +177,39 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p, int st
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           out[n][e] = (e & 1 ? b[n].y : b[n].x) * x[n][e];
-          minus[n][e] = (e & 1 ? -w[n].y : -w[n].x) * x[n][e];
+          x[n][e] *= e & 1 ? -w[n].y : -w[n].x;
         }
-      tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, minus, &m.scale[2][wn][m0]);
+      tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, x, ff);
       strip_store<T>(m.strip[warp], lane, out, dv + (c * kChunk + wn * 16) * dv_step + m0, dv_step, len - wn * 16, a.width - m0,
                      p.vec_o);
     }
     __syncthreads();
-    keep_tile<PO, VB, kChunk>(m.c, m.scale[3], p.dxs + kept_at<PO, kChunk>(p, head_at), p.scales + (head_at * 16 + 12) * p.rows,
+    keep_tile<PO, VB, kChunk>(m.c, m.keep_c, p.dxs + kept_at<PO, kChunk>(p, head_at), p.scales + (head_at * 4 + 3) * p.rows,
                               p.rows, a.column);
     // D = e^{G_C} D + (e^G do')^T Q - (beta e^G dX)^T K
-    const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
-#pragma unroll
-    for (int n = 0; n < QN; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) d[n][e] *= decay;
+    float bs[QN][4];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       uint32_t hi[4], lo[4];
-      float bs[QN][4] = {}, bt[QN][4] = {};
       tile_operand<PS>(yw[kk] + (ft - yt), M::kNarrow, hi, lo);
 #pragma unroll
       for (int n = 0; n < QN / 2; ++n)
-        product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, qt + ks[n] + kk * 16 * DK * 2, L::kTile);
-      add_scaled(d, bs, &m.scale[4][kk][m0], lane);
+        product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, qt + ks[n] + kk * 16 * DK * 2, L::kTile, kk == 0);
       tile_operand<PS>(yw[kk] + (xt - yt), M::kNarrow, hi, lo);
 #pragma unroll
       for (int n = 0; n < QN / 2; ++n)
-        product<PS, IN, true>(bt[2 * n], bt[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile);
-      add_scaled(d, bt, &m.scale[2][kk][m0], lane);
+        product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile, false);
     }
-    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, &m.scale[0][wn][m0]);
-    ring.done(turn, lane);
-    if (threadIdx.x == 0 && turn + stages < a.chunks)
-      ring.fill(p, turn + stages, a.first + a.chunks - 1 - turn - stages, a.kh, a.vh);
-    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < QN; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[n][e] = fmaf(bs[n][e], ff[e >> 1].inverse, decay * d[n][e]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) fd[h] = scale_below(fmaf(decay, most_of(most[h]), 2 * kSumTop * bound_f[h]));
+    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, fd);
+    row_max(d, top);
+    share(m.most_s, wn, m0, lane, top[0], top[1]);
+    ring.next(p, turn + STAGES < a.chunks ? a.first + a.chunks - 1 - turn - STAGES : -1, a.kh, a.vh);
   }
   if (p.dstate_in) state_store(p.dstate_in, p, a, m0, wn * (DK / 4), lane, d);
 }
@@ -196,7 +239,7 @@ struct GradShared {
   };
   float krow[kChunk], qrow[kChunk], orow[kChunk];
   float beta[kChunk], hi[kChunk], lo[kChunk], down[kChunk], tail[kChunk];  // down: e^G, tail: e^{G_C - G}
-  float ratio[4][4][128];      // a row's scale over the common one: S, dS, U, dX; quarters of the columns
+  float ratio[4][128];         // a row's scale over the common one: S, dS, U, dX
   float dots[4][4][kChunk];    // quarters of Dk: k.r1, q.dq, k.(r3 + ..), k.Y
   float xv[8][kChunk];         // dX . v, groups of value features
   float warp_sum[16];
@@ -228,15 +271,13 @@ __device__ __forceinline__ void planes_load(uint32_t (&f)[PLANES][4], uint32_t a
 }
 
 // Rows [row0, row0 + 64) of kept planes into a tile, times their rows' ratios.
-// Gives the sum over the values of the product with what the last call's did
-// (DOT), to be scaled by the caller: <S, D>.
 template <int PS, int W>
-__device__ __forceinline__ void load_kept(const char* from, int rows, int row0, int used, const float (*ratio)[128], char* tile, int tid) {
+__device__ __forceinline__ void load_kept(const char* from, int rows, int row0, int used, const float* ratio, char* tile, int tid) {
   constexpr int UNITS = kGradBlock * W / 8;
 #pragma unroll
   for (int i = 0; i < UNITS / kGradThreads; ++i) {
-    const int at = i * kGradThreads + tid, row = at / (W / 8), unit = (at % (W / 8)) ^ (row & 7);
-    const __half2 f = __float2half2_rn(row0 + row < used ? ratio[unit / (W / 32)][row0 + row] : 0.f);
+    const int at = i * kGradThreads + tid, row = at / (W / 8);
+    const __half2 f = __float2half2_rn(row0 + row < used ? ratio[row0 + row] : 0.f);
 #pragma unroll
     for (int n = 0; n < PS; ++n) {
       uint4 v = make_uint4(0, 0, 0, 0);
@@ -335,23 +376,19 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
       for (int e = 0; e < 8; ++e) o[0][e] *= f.f, o[1][e] *= f.f;
     }
     // scales of the kept planes: the largest of each kind is the common one
-    float row_scale[4];
-#pragma unroll
-    for (int kind = 0; kind < 4; ++kind) {
-      const int quarter = tid >> 7, row = tid & 127;
-      row_scale[kind] = row < used ? p.scales[((head_at * 4 + kind) * 4 + quarter) * p.rows + row] : 0.f;
-      const unsigned int m = __reduce_max_sync(0xffffffffu, __float_as_uint(row_scale[kind]));
+    const int kind = tid >> 7, scale_row = tid & 127;
+    const float row_scale = scale_row < used ? p.scales[(head_at * 4 + kind) * p.rows + scale_row] : 0.f;
+    {
+      const unsigned int m = __reduce_max_sync(0xffffffffu, __float_as_uint(row_scale));
       // non-negative floats order as integers: the maximum does not depend on the order
-      if (kind == 0) __syncthreads();  // common is cleared
+      __syncthreads();  // common is cleared
       if (lane == 0) atomicMax(&s.common[kind], m);
     }
     __syncthreads();
     float common[4];
 #pragma unroll
-    for (int kind = 0; kind < 4; ++kind) {
-      common[kind] = __uint_as_float(s.common[kind]);
-      s.ratio[kind][tid >> 7][tid & 127] = row_scale[kind] / common[kind];
-    }
+    for (int i = 0; i < 4; ++i) common[i] = __uint_as_float(s.common[i]);
+    s.ratio[kind][scale_row] = row_scale / __uint_as_float(s.common[kind]);
 
     float a_q[NT][4] = {}, a_x[NT][4] = {}, a_u[NT][4] = {}, a_p[2][4] = {}, a_a[2][4] = {};
     float sd = 0.f, xv = 0.f;

@@ -41,7 +41,8 @@ enum DeltaCoef {
   kKRow = 8,   // f_k, f_q: what a row of the K / Q planes is to be multiplied by
   kQRow = 9,
   kDecay = 10, // e^{G_C} in every place
-  kCoefs = 11
+  kBounds = 11,  // largest sum of |T| over a row; of the same times kTail; of |kDown|
+  kCoefs = 12
 };
 
 struct DeltaParams {
@@ -68,7 +69,7 @@ struct DeltaParams {
   // planes of S and U (kept by the forward sweep), of dS at the chunks' ends and of
   // dX: [chunk, value head][plane][rows][Dk or 64], tiles of delta_common's order
   char *states, *us, *dstates, *dxs;
-  float* scales;     // the inverses of their scales: [chunk, value head][S, dS, U, dX][4][rows]
+  float* scales;     // the inverses of their scales: [chunk, value head][S, dS, U, dX][rows]
   int rows;          // dv rounded up to 64
   void *dq, *dk_out, *dv_out, *dg, *dbeta;
   int slabs;         // ceil(dv / 16)
@@ -189,6 +190,13 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same from zero.
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"

@@ -37,6 +37,7 @@ struct PrepShared {
   alignas(16) float most[2][kChunk];  // largest magnitude of the rows
   float hi[HEADS][kChunk], lo[HEADS][kChunk], beta[HEADS][kChunk];
   float rise[HEADS];                  // the largest e^{G_i - G_j}, i >= j
+  unsigned int bound[HEADS][4];       // kBounds
 };
 
 // Rows of q and k as planes, in shared memory and in the workspace; eight
@@ -166,7 +167,7 @@ __device__ __forceinline__ void load_gates(const DeltaParams& p, const ChunkAt& 
 }
 
 template <typename T, int DK, int PS, int PO, int HEADS>
-__global__ void __launch_bounds__(128 * HEADS) delta_prepare(DeltaParams p) {
+__global__ void __launch_bounds__(128 * HEADS, HEADS == 2 ? 3 : 5) delta_prepare(DeltaParams p) {
   using L = DeltaLayout<T, DK, PS, PO>;
   extern __shared__ __align__(16) char shared_bytes[];
   PrepShared<T, DK, HEADS>& s = *reinterpret_cast<PrepShared<T, DK, HEADS>*>(shared_bytes);
@@ -299,6 +300,7 @@ __global__ void __launch_bounds__(128 * HEADS) delta_prepare(DeltaParams p) {
         *reinterpret_cast<float4*>(&t[row][unit * 8 + 4]) = make_float4(av[4], av[5], av[6], av[7]);
       }
     }
+    if (id < 4) s.bound[which][id] = 0;
     head_sync(which);
     float x[16];
     if (id < kChunk) {  // a column of a diagonal block's inverse
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(128 * HEADS) delta_prepare(DeltaParams p) {
     // T as planes, the coefficients
     {
       const int row = id >> 1;
-      float v[4][8], m = 0.f;
+      float v[4][8], m = 0.f, sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int unit = unit_of(i, id);
@@ -348,20 +350,32 @@ __global__ void __launch_bounds__(128 * HEADS) delta_prepare(DeltaParams p) {
         for (int e = 0; e < 8; ++e) {
           if (unit * 8 + e > row) v[i][e] = 0.f;
           m = fmaxf(m, fabsf(v[i][e]));
+          sum += fabsf(v[i][e]);
         }
       }
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       const Pow2 f = pow2_for(m);
+      const float tail = expf((hi[kChunk - 1] - hi[row]) + (lo[kChunk - 1] - lo[row])) * s.row[0][row];
+      const float down = fabsf(beta[row]) * exp_sum(hi[row], lo[row]) * s.row[0][row];
+      // non-negative floats order as integers: the maximum does not depend on the order
+      const unsigned int b0 = __reduce_max_sync(0xffffffffu, __float_as_uint(sum));
+      const unsigned int b1 = __reduce_max_sync(0xffffffffu, __float_as_uint(sum * tail));
+      const unsigned int b2 = __reduce_max_sync(0xffffffffu, __float_as_uint(down));
+      if (lane == 0) {
+        atomicMax(&s.bound[which][0], b0);
+        atomicMax(&s.bound[which][1], b1);
+        atomicMax(&s.bound[which][2], b2);
+      }
+      if (!(id & 1)) coef[kTail * kChunk + row] = tail;
 #pragma unroll
       for (int i = 0; i < 4; ++i) store_unit<PS>(head, row, unit_of(i, id), v[i], f.f);
       if (!(id & 1)) coef[kTRow * kChunk + row] = f.inverse;
     }
     if (id < kChunk) {
       const float gamma = exp_sum(hi[id], lo[id]), b = beta[id];
-      const float tail = expf((hi[kChunk - 1] - hi[id]) + (lo[kChunk - 1] - lo[id]));
       coef[kBeta * kChunk + id] = b;
       coef[kDown * kChunk + id] = b * gamma * s.row[0][id];
-      coef[kTail * kChunk + id] = tail * s.row[0][id];
       coef[kOutQ * kChunk + id] = p.scale * gamma * s.row[1][id];
     } else {
       const int at = id - kChunk;
@@ -372,6 +386,7 @@ __global__ void __launch_bounds__(128 * HEADS) delta_prepare(DeltaParams p) {
       coef[kDecay * kChunk + at] = exp_sum(hi[kChunk - 1], lo[kChunk - 1]);
     }
     head_sync(which);
+    if (id < 4) coef[kBounds * kChunk + id] = __uint_as_float(s.bound[which][id]);
   }
 }
 

@@ -16,9 +16,12 @@
 // registers instead needed no barrier, but its 400 products and 1500 other
 // instructions a chunk took 8.6 us where this takes KSWEEP us (bf16, Dk = 128).
 //
-// Planes are scaled per row and per 16 tokens (or per quarter of Dk), as each
-// warp knows them; the products of such a block are scaled back and added in
-// fp32 registers, which also keeps the tensor cores' accumulations short.
+// A row's planes take one scale wherever a bound gives it before the warps
+// have met: |U| <= max_i sum_j |T_ij| max|X| (delta_prepare has the sums), and
+// |S| <= e^{G_C} max|S0| + 64 max|e^{G_C - G} U| max|K|, the maxima being those
+// of the last step, exact.  A bound a thousand times too large costs ten of
+// the 26 bits that two planes have below 2^15.  X is scaled per 16 tokens, as
+// each warp finds it, and its products are scaled back one by one.
 #pragma once
 
 #include "delta_common.cuh"
@@ -188,28 +191,37 @@ __device__ __forceinline__ void row_max(const float (&f)[N][4], float (&m)[2]) {
   m[1] = quad_max(m[1]);
 }
 
-// Accumulators of 16 rows x 8 N columns as planes of a tile of W columns, at
-// one scale for each row; the inverses go to `inverse` (16 of them).
+// Accumulators of 16 rows x 8 N columns, times a scale for each row, as planes
+// of a tile of W columns.
 template <int PLANES, int W, int N>
 __device__ __forceinline__ void tile_write(char* tile, uint32_t plane, int row0, int col0, int lane, const float (&f)[N][4],
-                                           float* inverse) {
-  float m[2];
-  row_max(f, m);
+                                           const Pow2 (&s)[2]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const Pow2 s = pow2_for(m[h]);
     const int row = row0 + (lane >> 2) + h * 8;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       uint32_t hi, lo;
-      split<PLANES>(f[n][2 * h] * s.f, f[n][2 * h + 1] * s.f, &hi, &lo);
+      split<PLANES>(f[n][2 * h] * s[h].f, f[n][2 * h + 1] * s[h].f, &hi, &lo);
       const uint32_t at = tile_at<W>(row, (col0 >> 3) + n) + (lane & 3) * 4;
       *reinterpret_cast<uint32_t*>(tile + at) = hi;
       if (PLANES > 1) *reinterpret_cast<uint32_t*>(tile + plane + at) = lo;
     }
-    if ((lane & 3) == 0) inverse[(lane >> 2) + h * 8] = s.inverse;
   }
 }
+// Of each row, what the four warps that share it have: [row][warp].
+__device__ __forceinline__ void share(float* to, int warp, int row0, int lane, float a, float b) {
+  if ((lane & 3) == 0) {
+    to[(row0 + (lane >> 2)) * 4 + warp] = a;
+    to[(row0 + (lane >> 2) + 8) * 4 + warp] = b;
+  }
+}
+__device__ __forceinline__ void shared_of(const float* from, int row0, int lane, float4 (&v)[2]) {
+  v[0] = *reinterpret_cast<const float4*>(from + (row0 + (lane >> 2)) * 4);
+  v[1] = *reinterpret_cast<const float4*>(from + (row0 + (lane >> 2) + 8) * 4);
+}
+__device__ __forceinline__ float most_of(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+__device__ __forceinline__ float element(const float4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // Left operand: 16 x 16 of a tile's planes.
 template <int PLANES>
@@ -218,10 +230,9 @@ __device__ __forceinline__ void tile_operand(uint32_t at, uint32_t plane, uint32
   if (PLANES > 1) ldsm(lo, at + plane);
 }
 
-// f += g, row by row times the inverse of a block's scale.
+// f += g, row by row times a factor.
 template <int N>
-__device__ __forceinline__ void add_scaled(float (&f)[N][4], const float (&g)[N][4], const float* inverse, int lane) {
-  const float a = inverse[lane >> 2], b = inverse[(lane >> 2) + 8];
+__device__ __forceinline__ void add_scaled(float (&f)[N][4], const float (&g)[N][4], float a, float b) {
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     f[n][0] = fmaf(g[n][0], a, f[n][0]);
@@ -243,15 +254,20 @@ __device__ __forceinline__ void scale_columns(float (&f)[N][4], const float2 (&w
   }
 }
 
-// d0, d1 += A B for two column tiles: A in PA planes (hi, lo), B in PB planes
+// d0, d1 (+)= A B for two column tiles: A in PA planes (hi, lo), B in PB planes
 // `apart` bytes apart at `at`; the product of two lo planes is left out.
 template <int PA, int PB, bool TRANS>
 __device__ __forceinline__ void product(float (&d0)[4], float (&d1)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
-                                        uint32_t at, uint32_t apart) {
+                                        uint32_t at, uint32_t apart, bool first) {
   uint32_t b[4];
   if (TRANS) ldsm_t(b, at); else ldsm(b, at);
-  mma(d0, hi, b[0], b[1]);
-  mma(d1, hi, b[2], b[3]);
+  if (first) {
+    mma_first(d0, hi, b[0], b[1]);
+    mma_first(d1, hi, b[2], b[3]);
+  } else {
+    mma(d0, hi, b[0], b[1]);
+    mma(d1, hi, b[2], b[3]);
+  }
   if (PA > 1) {
     mma(d0, lo, b[0], b[1]);
     mma(d1, lo, b[2], b[3]);
@@ -265,18 +281,18 @@ __device__ __forceinline__ void product(float (&d0)[4], float (&d1)[4], const ui
 
 // Copies of the chunks' tiles into a ring of stages.  Thread 0 issues them; a
 // stage is refilled when every warp has arrived at its `empty` barrier.
-template <typename L>
+template <typename L, int STAGES>
 struct Ring {
   char* stages;
   uint64_t *full, *empty;
-  int count;
-  __device__ __forceinline__ void begin(char* bytes, int n, int warps) {
+  int at, filled;             // stage and fills of it so far, of the chunk that is worked on
+  __device__ __forceinline__ void begin(char* bytes, int warps) {
     full = reinterpret_cast<uint64_t*>(bytes);
     empty = full + 8;
     stages = bytes + 128;
-    count = n;
+    at = filled = 0;
     if (threadIdx.x == 0) {
-      for (int i = 0; i < n; ++i) {
+      for (int i = 0; i < STAGES; ++i) {
         barrier_init(full + i, 1);
         barrier_init(empty + i, warps);
       }
@@ -284,21 +300,29 @@ struct Ring {
     }
     __syncthreads();
   }
-  __device__ __forceinline__ void fill(const DeltaParams& p, int turn, int chunk, int kh, int vh) {
-    const int s = turn % count;
-    if (turn >= count) barrier_wait(empty + s, (turn / count - 1) & 1);
-    char* to = stages + s * L::kStage;
-    barrier_expect(full + s, L::kStage);
-    bulk_copy(to, p.tiles + (static_cast<long long>(chunk) * p.hk + kh) * L::kTiles, L::kTiles, full + s);
-    bulk_copy(to + L::kTiles, p.heads + (static_cast<long long>(chunk) * p.hv + vh) * L::kHead, L::kHead, full + s);
+  __device__ __forceinline__ void fill(const DeltaParams& p, int stage, int chunk, int kh, int vh) {
+    char* to = stages + stage * L::kStage;
+    barrier_expect(full + stage, L::kStage);
+    bulk_copy(to, p.tiles + (static_cast<long long>(chunk) * p.hk + kh) * L::kTiles, L::kTiles, full + stage);
+    bulk_copy(to + L::kTiles, p.heads + (static_cast<long long>(chunk) * p.hv + vh) * L::kHead, L::kHead, full + stage);
   }
-  __device__ __forceinline__ const char* wait(int turn) {
-    barrier_wait(full + turn % count, (turn / count) & 1);
-    return stages + (turn % count) * L::kStage;
+  __device__ __forceinline__ const char* wait() {
+    barrier_wait(full + at, filled & 1);
+    return stages + at * L::kStage;
   }
-  __device__ __forceinline__ void done(int turn, int lane) {
+  // This chunk's stage is done with; chunk `refill` (if >= 0) takes its place.
+  __device__ __forceinline__ void next(const DeltaParams& p, int refill, int kh, int vh) {
     __syncwarp();
-    if (lane == 0) barrier_arrive(empty + turn % count);
+    if ((threadIdx.x & 31) == 0) barrier_arrive(empty + at);
+    if (threadIdx.x == 0 && refill >= 0) {
+      barrier_wait(empty + at, filled & 1);
+      fill(p, at, refill, kh, vh);
+    }
+    __syncwarp();
+    if (++at == STAGES) {
+      at = 0;
+      ++filled;
+    }
   }
 };
 
@@ -358,10 +382,10 @@ __device__ __forceinline__ void state_store(float* to, const DeltaParams& p, con
         to[((static_cast<long long>(a.sequence) * p.hv + a.vh) * p.dk + dk) * p.dv + a.column + dv] = s[n][e];
     }
 }
-// A block's planes of a tile and the inverses of their scales to the
+// A block's planes of a tile and the inverses of their rows' scales to the
 // workspace: VB rows of W columns of plane after plane.
 template <int PLANES, int VB, int W>
-__device__ __forceinline__ void keep_tile(const char* tile, const float (*scale)[VB], char* to, float* scales, int rows, int column) {
+__device__ __forceinline__ void keep_tile(const char* tile, const float* scale, char* to, float* scales, int rows, int column) {
   constexpr int UNITS = VB * W * 2 / 16;
   char* at = to + static_cast<long long>(column) * W * 2;
 #pragma unroll
@@ -372,7 +396,7 @@ __device__ __forceinline__ void keep_tile(const char* tile, const float (*scale)
       reinterpret_cast<uint4*>(at + static_cast<long long>(n) * rows * W * 2)[u] =
           reinterpret_cast<const uint4*>(tile + n * VB * W * 2)[u];
     }
-  if (threadIdx.x < 4 * VB) scales[threadIdx.x / VB * rows + column + threadIdx.x % VB] = (&scale[0][0])[threadIdx.x];
+  if (threadIdx.x < VB) scales[column + threadIdx.x] = scale[threadIdx.x];
 }
 // Where a (chunk, value head) keeps what: bytes of the planes, floats of the scales.
 template <int PLANES, int W>
@@ -390,23 +414,35 @@ __device__ __forceinline__ void coef_read(const char* coef, int which, int tile,
 constexpr int kSweepRing = 128;  // bytes of the ring's barriers
 
 // Shared memory of a sweep behind the ring: planes of S, X, U and what else
-// the steps hand on, with the inverses of their scales.
+// the steps hand on.
 template <typename T, int DK, int PS, int PO, int VB, bool BACK>
 struct SweepShared {
   static constexpr uint32_t kWide = VB * DK * 2, kNarrow = VB * kChunk * 2;
   alignas(128) char s[PS * kWide];
   char a[PS * kNarrow];  // X; back: Y
   char b[PS * kNarrow];  // e^{G_C - G} U; back: beta e^G dX
-  char c[PO * kNarrow];  // U; back: do' with P's weights
+  char c[PO * kNarrow];  // U; back: do' with P's weights, then dX
   char d[BACK ? PS * kNarrow : 128];  // back: e^G do'
-  float scale[BACK ? 5 : 4][4][VB];
+  alignas(16) float most_s[VB * 4];   // largest of S's rows, by warp
+  alignas(16) float scale_a[VB * 4];  // inverses of the scales of X (Y), by warp
+  alignas(16) float scale_c[VB * 4];  // back: of do'
+  alignas(16) float most_d[VB * 4];   // back: largest of e^G do', by warp
+  float keep_s[VB], keep_c[VB];       // inverses of the scales of S and U (dX), for what is kept
   alignas(16) char slab[2][Slab<T, VB>::kBytes];
   char strip[VB / 4][Strip<T>::kBytes];
 };
 
+// |A B| over 64 tokens with one operand's planes below 2^13.
+constexpr float kPlaneTop = 8192.f, kSumTop = 64.f * kPlaneTop;
+// Scale for what lies below `bound`: brings it below 2^15.
+__device__ __forceinline__ Pow2 scale_below(float bound) {
+  const Pow2 s = pow2_for(bound);
+  return {s.f * 4.f, s.inverse * 0.25f};
+}
+
 // KEEP: store S at every chunk's start and U for the backward pass instead of O.
-template <typename T, int DK, int PS, int PO, int VB, bool KEEP>
-__global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p, int stages) {
+template <typename T, int DK, int PS, int PO, int VB, int STAGES, bool KEEP>
+__global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p) {
   using L = DeltaLayout<T, DK, PS, PO>;
   using M = SweepShared<T, DK, PS, PO, VB, false>;
   constexpr int IN = L::kIn, QN = DK / 32;  // column tiles of a quarter of Dk
@@ -414,9 +450,9 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p, int stages)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int wm = warp % (VB / 16), wn = warp / (VB / 16), m0 = wm * 16;
   const SweepAt a = sweep_at(p, VB);
-  Ring<L> ring;
-  ring.begin(shared_bytes, stages, VB / 4);
-  M& m = *reinterpret_cast<M*>(shared_bytes + kSweepRing + stages * L::kStage);
+  Ring<L, STAGES> ring;
+  ring.begin(shared_bytes, VB / 4);
+  M& m = *reinterpret_cast<M*>(shared_bytes + kSweepRing + STAGES * L::kStage);
   const uint32_t st = shared_u32(m.s), xt = shared_u32(m.a), ut = shared_u32(m.b), vt = shared_u32(m.c);
 
   const T* v = static_cast<const T*>(p.v) + a.batch * p.v_batch + a.lo * p.v_token + a.vh * p.v_head + a.column;
@@ -433,48 +469,59 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p, int stages)
         if (at % VB < a.width) o[(a.len + at / VB) * o_step + at % VB] = down<T>(0.f);
   }
   if (threadIdx.x == 0)
-    for (int i = 0; i < stages && i < a.chunks; ++i) ring.fill(p, i, a.first + i, a.kh, a.vh);
+    for (int i = 0; i < STAGES && i < a.chunks; ++i) ring.fill(p, i, a.first + i, a.kh, a.vh);
   if (a.chunks) slab_fetch<T, VB>(m.slab[0], v, p.v_token, min(a.len, kChunk), a.width, p.vec_v);
   const Walk sw(st + at_mk<DK>(lane, m0, 0)), xw(xt + at_mk<kChunk>(lane, m0, 0));  // planes of S and X; U's follow X's
   const Walk kw(at_nk<DK>(lane, wn * 16, 0)), tw(at_nk<kChunk>(lane, wn * 16, 0));  // in K and Q; in T and P
   uint32_t ks[QN / 2];  // in K, for the state's update
 #pragma unroll
   for (int n = 0; n < QN / 2; ++n) ks[n] = at_kn<DK>(lane, wn * (DK / 4) + n * 16, 0);
-  float s[QN][4];
+  float s[QN][4], top[2];
+  Pow2 fs[2];
   state_load(p.state_in, p, a, m0, wn * (DK / 4), lane, s);
-  tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, &m.scale[0][wn][m0]);
+  {  // S's planes, after the four warps have met once over their rows' largest
+    row_max(s, top);
+    share(m.most_s, wn, m0, lane, top[0], top[1]);
+    __syncthreads();
+    float4 all[2];
+    shared_of(m.most_s, m0, lane, all);
+    fs[0] = scale_below(most_of(all[0]));
+    fs[1] = scale_below(most_of(all[1]));
+    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, fs);
+  }
 
   for (int c = 0; c < a.chunks; ++c) {
     const int len = min(kChunk, a.len - c * kChunk);
     const long long head_at = static_cast<long long>(a.first + c) * p.hv + a.vh;
+    if (KEEP && wn == 0 && (lane & 3) == 0) {
+      m.keep_s[m0 + (lane >> 2)] = fs[0].inverse;
+      m.keep_s[m0 + (lane >> 2) + 8] = fs[1].inverse;
+    }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    const char* stage = ring.wait(c);
+    const char* stage = ring.wait();
     __syncthreads();  // planes of S and this chunk's v are there; the other slab is free
     if (c + 1 < a.chunks)
       slab_fetch<T, VB>(m.slab[~c & 1], v + (c + 1) * kChunk * p.v_token, p.v_token, min(kChunk, a.len - (c + 1) * kChunk),
                         a.width, p.vec_v);
     if (KEEP)
-      keep_tile<PS, VB, DK>(m.s, m.scale[0], p.states + kept_at<PS, DK>(p, head_at), p.scales + head_at * 16 * p.rows, p.rows,
+      keep_tile<PS, VB, DK>(m.s, m.keep_s, p.states + kept_at<PS, DK>(p, head_at), p.scales + head_at * 4 * p.rows, p.rows,
                             a.column);
     const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
     const char* coef = stage + L::kTiles + L::kT + L::kP;
-    float x[2][4] = {}, q[2][4] = {};
+    const float4 bounds = *reinterpret_cast<const float4*>(coef + kBounds * kChunk * 4);
+    const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
+    float x[2][4], q[2][4];
     float2 w[2];
     // (K S)^T and (Q S)^T
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      float bx[2][4] = {}, bq[2][4] = {};
-#pragma unroll
-      for (int k = 0; k < DK / 64; ++k) {
-        const int kk = b * (DK / 64) + k;
-        uint32_t hi[4], lo[4];
-        tile_operand<PS>(sw[kk], M::kWide, hi, lo);
-        product<PS, IN, false>(bx[0], bx[1], hi, lo, kt + kw[kk], L::kTile);
-        if (!KEEP) product<PO, IN, false>(bq[0], bq[1], hi, lo, qt + kw[kk], L::kTile);
-      }
-      add_scaled(x, bx, &m.scale[0][b][m0], lane);
-      if (!KEEP) add_scaled(q, bq, &m.scale[0][b][m0], lane);
+    for (int kk = 0; kk < DK / 16; ++kk) {
+      uint32_t hi[4], lo[4];
+      tile_operand<PS>(sw[kk], M::kWide, hi, lo);
+      product<PS, IN, false>(x[0], x[1], hi, lo, kt + kw[kk], L::kTile, kk == 0);
+      if (!KEEP) product<PO, IN, false>(q[0], q[1], hi, lo, qt + kw[kk], L::kTile, kk == 0);
     }
+    float4 most[2];
+    shared_of(m.most_s, m0, lane, most);
     {  // X = beta v - beta e^G K S
       float vv[2][4];
       slab_read<T, VB>(m.slab[c & 1], wn * 16, m0, lane, vv);
@@ -485,73 +532,90 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p, int stages)
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          x[n][e] = (e & 1 ? b[n].y : b[n].x) * vv[n][e] - (e & 1 ? w[n].y : w[n].x) * x[n][e];
+          x[n][e] = (e & 1 ? b[n].y : b[n].x) * vv[n][e] - ((e & 1 ? w[n].y : w[n].x) * fs[e >> 1].inverse) * x[n][e];
     }
-    tile_write<PS, kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, x, &m.scale[1][wn][m0]);
+    {
+      row_max(x, top);
+      const Pow2 fx[2] = {pow2_for(top[0]), pow2_for(top[1])};
+      share(m.scale_a, wn, m0, lane, fx[0].inverse, fx[1].inverse);
+      tile_write<PS, kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, x, fx);
+    }
     __syncthreads();
     // U^T = X^T T^T, T lower triangular
     float u[2][4] = {};
+    float4 back[2];
+    shared_of(m.scale_a, m0, lane, back);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       if (VB == 64 && kk > wn) break;  // T's other blocks are zero
       uint32_t hi[4], lo[4];
-      float bu[2][4] = {};
+      float bu[2][4];
       tile_operand<PS>(xw[kk], M::kNarrow, hi, lo);
-      product<PS, PS, false>(bu[0], bu[1], hi, lo, tt + tw[kk], L::kSquare);
-      add_scaled(u, bu, &m.scale[1][kk][m0], lane);
+      product<PS, PS, false>(bu[0], bu[1], hi, lo, tt + tw[kk], L::kSquare, true);
+      add_scaled(u, bu, element(back[0], kk), element(back[1], kk));
     }
     coef_read(coef, kTRow, wn * 2, lane, w);
     scale_columns(u, w);
-    tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, u, &m.scale[3][wn][m0]);
+    const float bound_x[2] = {most_of(back[0]) * kPlaneTop, most_of(back[1]) * kPlaneTop};
+    const Pow2 fu[2] = {scale_below(bounds.x * bound_x[0]), scale_below(bounds.x * bound_x[1])};
+    tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, u, fu);
+    if (KEEP && wn == 0 && (lane & 3) == 0) {
+      m.keep_c[m0 + (lane >> 2)] = fu[0].inverse;
+      m.keep_c[m0 + (lane >> 2) + 8] = fu[1].inverse;
+    }
     coef_read(coef, kTail, wn * 2, lane, w);
     scale_columns(u, w);
-    tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, u, &m.scale[2][wn][m0]);
+    const float bound_u[2] = {bounds.y * bound_x[0], bounds.y * bound_x[1]};
+    const Pow2 ft[2] = {scale_below(bound_u[0]), scale_below(bound_u[1])};
+    tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, u, ft);
     __syncthreads();
     if (KEEP)  // here PO = PS
-      keep_tile<PO, VB, kChunk>(m.c, m.scale[3], p.us + kept_at<PO, kChunk>(p, head_at),
-                                p.scales + (head_at * 16 + 8) * p.rows, p.rows, a.column);
+      keep_tile<PO, VB, kChunk>(m.c, m.keep_c, p.us + kept_at<PO, kChunk>(p, head_at), p.scales + (head_at * 4 + 2) * p.rows,
+                                p.rows, a.column);
     // S^T = e^{G_C} S^T + (e^{G_C - G} U)^T K
-    const float decay = reinterpret_cast<const float*>(coef)[kDecay * kChunk];
-#pragma unroll
-    for (int n = 0; n < QN; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] *= decay;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint32_t hi[4], lo[4];
-      float bs[QN][4] = {};
-      tile_operand<PS>(xw[kk] + (ut - xt), M::kNarrow, hi, lo);
-#pragma unroll
-      for (int n = 0; n < QN / 2; ++n)
-        product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile);
-      add_scaled(s, bs, &m.scale[2][kk][m0], lane);
-    }
-    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, &m.scale[0][wn][m0]);
-    if (!KEEP) {  // O^T = (Q S)^T + U^T P^T, each with its weights
-      float pu[2][4] = {};
+    {
+      float bs[QN][4];
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
-        if (VB == 64 && kk > wn) break;
         uint32_t hi[4], lo[4];
-        float bu[2][4] = {};
-        tile_operand<PO>(xw[kk] + (vt - xt), M::kNarrow, hi, lo);
-        product<PO, PO, false>(bu[0], bu[1], hi, lo, pt + tw[kk], L::kSquare);
-        add_scaled(pu, bu, &m.scale[3][kk][m0], lane);
+        tile_operand<PS>(xw[kk] + (ut - xt), M::kNarrow, hi, lo);
+#pragma unroll
+        for (int n = 0; n < QN / 2; ++n)
+          product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile, kk == 0);
       }
-      float2 wq[2];
-      coef_read(coef, kOutQ, wn * 2, lane, wq);
-      coef_read(coef, kOutP, wn * 2, lane, w);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < QN; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          q[n][e] = (e & 1 ? wq[n].y : wq[n].x) * q[n][e] + (e & 1 ? w[n].y : w[n].x) * pu[n][e];
-      strip_store<T>(m.strip[warp], lane, q, o + (c * kChunk + wn * 16) * o_step + m0, o_step, len - wn * 16, a.width - m0,
-                     p.vec_o);
+        for (int e = 0; e < 4; ++e) s[n][e] = fmaf(bs[n][e], ft[e >> 1].inverse, decay * s[n][e]);
+      const Pow2 old[2] = {fs[0], fs[1]};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) fs[h] = scale_below(fmaf(decay, most_of(most[h]), kSumTop * bound_u[h]));
+      tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, fs);
+      row_max(s, top);
+      share(m.most_s, wn, m0, lane, top[0], top[1]);
+      if (!KEEP) {  // O^T = (Q S)^T + U^T P^T, each with its weights
+        float pu[2][4];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if (VB == 64 && kk > wn) break;
+          uint32_t hi[4], lo[4];
+          tile_operand<PO>(xw[kk] + (vt - xt), M::kNarrow, hi, lo);
+          product<PO, PO, false>(pu[0], pu[1], hi, lo, pt + tw[kk], L::kSquare, kk == 0);
+        }
+        float2 wq[2];
+        coef_read(coef, kOutQ, wn * 2, lane, wq);
+        coef_read(coef, kOutP, wn * 2, lane, w);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            q[n][e] = (e & 1 ? wq[n].y : wq[n].x) * (q[n][e] * old[e >> 1].inverse) +
+                      (e & 1 ? w[n].y : w[n].x) * (pu[n][e] * fu[e >> 1].inverse);
+        strip_store<T>(m.strip[warp], lane, q, o + (c * kChunk + wn * 16) * o_step + m0, o_step, len - wn * 16, a.width - m0,
+                       p.vec_o);
+      }
     }
-    ring.done(c, lane);
-    if (threadIdx.x == 0 && c + stages < a.chunks) ring.fill(p, c + stages, a.first + c + stages, a.kh, a.vh);
-    __syncwarp();
+    ring.next(p, c + STAGES < a.chunks ? a.first + c + STAGES : -1, a.kh, a.vh);
   }
   if (p.state_out) state_store(p.state_out, p, a, m0, wn * (DK / 4), lane, s);
 }

@@ -5,6 +5,7 @@
 #include <atomic>
 #include <cmath>
 #include <mutex>
+#include <numeric>
 #include <type_traits>
 
 #include "../../include/pla_b200.h"
@@ -35,6 +36,7 @@ using namespace seq;
   } while (0)
 
 constexpr long long kMaxGrid = 0x7fffffff;
+constexpr long long kMaxTokens = 1 << 30;  // 32-bit token numbers, with room for a stride past the end
 
 size_t type_size(int dtype) { return dtype == PLA_F32 ? 4 : dtype == PLA_F16 || dtype == PLA_BF16 ? 2 : 0; }
 bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -102,6 +104,7 @@ struct Int {
 int check_causal(const pla_causal* a) {
   if (!a) return PLA_ERR_INVALID_ARGUMENT;
   if (a->batch < 0 || a->tokens < 0 || a->channels < 0 || a->sequences < 0) return PLA_ERR_INVALID_ARGUMENT;
+  if (a->tokens > kMaxTokens) return PLA_ERR_TOO_LARGE;
   if (!type_size(a->dtype)) return PLA_ERR_UNSUPPORTED;
   if (a->taps < 2 || a->taps > 4) return PLA_ERR_UNSUPPORTED;
   if (a->cu_seqlens ? a->batch != 1 : a->sequences != a->batch) return PLA_ERR_INVALID_ARGUMENT;
@@ -129,8 +132,8 @@ CausalParams causal_params(const pla_causal* a) {
   return p;
 }
 
-// Strips of 32 tokens re-read the least; shorter ones while a device's threads
-// would stay idle (a strip's thread keeps four loads in flight).
+// Long strips re-read the least; shorter ones while the device's threads would
+// stay idle.
 void cut_strips(CausalParams* p, int vec, long long threads, int longest) {
   const long long across = p->channels / vec;
   p->strip = longest;
@@ -143,15 +146,14 @@ bool causal_vector(const pla_causal* a, int vec, std::initializer_list<const voi
   if (a->channels % vec || a->x_batch % vec || a->x_token % vec) return false;
   for (const void* p : more)
     if (!aligned_to(p, unit)) return false;
-  return aligned_to(a->x, unit) && aligned_to(a->state_in, unit);
+  return aligned_to(a->x, unit) && aligned_to(a->state_in, unit) && aligned_to(a->w, unit) && aligned_to(a->b, unit);
 }
 
-// f(element type, V, K)
+// f(element type, V, K): 8 bytes of channels a thread (backward, which holds
+// five times as much: two channels), or single ones.
 template <typename F>
 int with_causal(int dtype, int taps, bool wide, bool backward, F&& f) {
   return with_type(dtype, [&](auto zero) {
-    using T = decltype(zero);
-    constexpr int W = 16 / sizeof(T);
     auto with_taps = [&](auto v) {
       switch (taps) {
         case 2: return f(zero, v, Int<2>{});
@@ -159,8 +161,9 @@ int with_causal(int dtype, int taps, bool wide, bool backward, F&& f) {
         default: return f(zero, v, Int<4>{});
       }
     };
+    constexpr int W = 8 / sizeof(decltype(zero));
     if (!wide) return with_taps(Int<1>{});
-    return backward ? with_taps(Int<4>{}) : with_taps(Int<W>{});
+    return backward ? with_taps(Int<2>{}) : with_taps(Int<W>{});
   });
 }
 
@@ -170,6 +173,7 @@ int check_norm(const pla_qk_norm* a, bool backward) {
   if (a->batch < 0 || a->tokens < 0 || a->dim < 0 || a->rot < 0 || a->q.heads < 0 || a->k.heads < 0 || a->table_rows < 0 ||
       a->rot > a->dim || a->rot % 2 || !(a->eps >= 0.f))
     return PLA_ERR_INVALID_ARGUMENT;
+  if (a->tokens > kMaxTokens) return PLA_ERR_TOO_LARGE;
   if (!type_size(a->dtype)) return PLA_ERR_UNSUPPORTED;
   if (a->dim > 256) return PLA_ERR_UNSUPPORTED;
   if (a->rot && (!a->cos_table || !a->sin_table)) return PLA_ERR_INVALID_ARGUMENT;
@@ -249,12 +253,16 @@ int with_norm(const pla_qk_norm* a, bool wide, F&& f) {
   });
 }
 
-// Blocks of one side in the backward pass: enough turns each that a block's
-// partial sum is small beside what it reads, never more than eight an SM.
+// Blocks of one side in the backward pass: a number of groups that is a
+// multiple of the heads (a group keeps its head), a few turns each so that a
+// block's partial sum is small beside what it reads, no more than the device
+// holds at a time.
 int norm_side_blocks(const pla_qk_norm* a, int heads, int lanes) {
   const long long rows = static_cast<long long>(a->batch) * a->tokens * heads;
-  const long long groups = kNormThreads / lanes;
-  return static_cast<int>(std::min<long long>((rows + groups * 4 - 1) / (groups * 4), 148 * 4));
+  if (!rows) return 0;
+  const int groups = kNormThreads / lanes, step = heads / std::gcd(heads, groups);
+  const long long want = std::min<long long>((rows + groups * 4 - 1) / (groups * 4), 148 * 4);
+  return static_cast<int>(std::max<long long>(1, (want + step - 1) / step) * step);
 }
 
 // ---- gated delta rule ------------------------------------------------------
@@ -262,6 +270,7 @@ int check_delta(const pla_delta* a) {
   if (!a) return PLA_ERR_INVALID_ARGUMENT;
   if (a->batch < 0 || a->tokens < 0 || a->sequences < 0 || a->hk < 0 || a->hv < 0 || a->dk < 0 || a->dv < 0)
     return PLA_ERR_INVALID_ARGUMENT;
+  if (a->tokens > kMaxTokens) return PLA_ERR_TOO_LARGE;
   if (!type_size(a->dtype)) return PLA_ERR_UNSUPPORTED;
   if (a->cu_seqlens ? a->batch != 1 : a->sequences != a->batch) return PLA_ERR_INVALID_ARGUMENT;
   if (a->hv && (a->hk < 1 || a->hv % a->hk)) return PLA_ERR_INVALID_ARGUMENT;
@@ -290,7 +299,7 @@ DeltaSizes delta_sizes_of(const pla_delta* a, bool backward) {
     const size_t rows = static_cast<size_t>(s.chunks) * a->hv * ((a->dv + 63) / 64) * 64;
     s.states = up256(rows * PS * DK * 2);
     s.us = up256(rows * PS * kChunk * 2);
-    s.scales = up256(rows * 16 * sizeof(float));
+    s.scales = up256(rows * 4 * sizeof(float));
   }
   s.total = s.plan + s.tiles + s.heads + 2 * s.states + 2 * s.us + s.scales;
   return s;
@@ -429,9 +438,9 @@ int launch_sweep(const DeltaParams& p, int sms, cudaStream_t stream) {
     using S = SweepShape<T, DK, PS, PO, VB, false>;
     const long long grid = S::grid(p);
     if (grid > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
-    const int st = allow_shared<delta_sweep<T, DK, PS, PO, VB, KEEP>>(S::kShared);
+    const int st = allow_shared<delta_sweep<T, DK, PS, PO, VB, S::kStages, KEEP>>(S::kShared);
     if (st != PLA_OK) return st;
-    delta_sweep<T, DK, PS, PO, VB, KEEP><<<static_cast<int>(grid), VB * 8, S::kShared, stream>>>(p, S::kStages);
+    delta_sweep<T, DK, PS, PO, VB, S::kStages, KEEP><<<static_cast<int>(grid), VB * 8, S::kShared, stream>>>(p);
     return launched("delta_sweep");
   });
 }
@@ -441,9 +450,9 @@ int launch_gradient(const DeltaParams& p, int sms, cudaStream_t stream) {
   int st = with_columns<T, DK, PS, PO, true>(p, sms, [&](auto vb) {
     constexpr int VB = decltype(vb)::value;
     using S = SweepShape<T, DK, PS, PO, VB, true>;
-    const int st = allow_shared<delta_sweep_back<T, DK, PS, PO, VB>>(S::kShared);
+    const int st = allow_shared<delta_sweep_back<T, DK, PS, PO, VB, S::kStages>>(S::kShared);
     if (st != PLA_OK) return st;
-    delta_sweep_back<T, DK, PS, PO, VB><<<static_cast<int>(S::grid(p)), VB * 8, S::kShared, stream>>>(p, S::kStages);
+    delta_sweep_back<T, DK, PS, PO, VB, S::kStages><<<static_cast<int>(S::grid(p)), VB * 8, S::kShared, stream>>>(p);
     return launched("delta_sweep_back");
   });
   if (st != PLA_OK) return st;
@@ -479,12 +488,12 @@ int pla_causal_depthwise_forward(const pla_causal* a, pla_stream_t stream) {
   if (!a->channels || (!work && !(a->state_out && a->sequences))) return PLA_OK;
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
-  const bool wide = causal_vector(a, static_cast<int>(16 / es), {a->y, a->state_out});
+  const bool wide = causal_vector(a, static_cast<int>(8 / es), {a->y, a->state_out});
   return with_causal(a->dtype, a->taps, wide, false, [&](auto zero, auto v, auto k) {
     using T = decltype(zero);
     constexpr int V = decltype(v)::value, K = decltype(k)::value;
     CausalParams p = causal_params(a);
-    cut_strips(&p, V, sms * 1024ll, 32);
+    cut_strips(&p, V, sms * 768ll, 32);
     const long long items = work ? static_cast<long long>(p.batch) * p.strips * (p.channels / V) : 0;
     const long long states = p.state_out ? held / V : 0;
     const long long main_blocks = (items + kCausalThreads - 1) / kCausalThreads;
@@ -500,7 +509,7 @@ namespace {
 // Blocks of strips in the backward pass (what the workspace is sized by).
 CausalParams causal_backward_params(const pla_causal* a, bool wide, long long* block_rows) {
   CausalParams p = causal_params(a);
-  cut_strips(&p, wide ? 4 : 1, 148 * 512, 64);
+  cut_strips(&p, wide ? 2 : 1, 148 * 768, 64);
   *block_rows = (static_cast<long long>(p.batch) * p.strips + kCausalRows - 1) / kCausalRows;
   return p;
 }
@@ -509,7 +518,7 @@ CausalParams causal_backward_params(const pla_causal* a, bool wide, long long* b
 size_t pla_causal_depthwise_workspace(const pla_causal* a) {
   if (check_causal(a) != PLA_OK || !a->batch || !a->tokens || !a->channels) return 0;
   long long wide_rows, rows;
-  causal_backward_params(a, a->channels % 4 == 0, &wide_rows);
+  causal_backward_params(a, a->channels % 2 == 0, &wide_rows);
   causal_backward_params(a, false, &rows);
   return static_cast<size_t>(std::max(rows, wide_rows)) * (a->taps + 1) * a->channels * sizeof(float);
 }
@@ -531,7 +540,7 @@ int pla_causal_depthwise_backward(const pla_causal* a, const pla_causal_gradient
   if (!a->channels) return PLA_OK;
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
-  const bool wide = causal_vector(a, 4, {g->dy, g->dx, g->dstate_out}) && g->dy_batch % 4 == 0 && g->dy_token % 4 == 0;
+  const bool wide = causal_vector(a, 2, {g->dy, g->dx, g->dstate_out}) && g->dy_batch % 2 == 0 && g->dy_token % 2 == 0;
   return with_causal(a->dtype, a->taps, wide, true, [&](auto zero, auto v, auto k) {
     using T = decltype(zero);
     constexpr int V = decltype(v)::value, K = decltype(k)::value;
@@ -582,9 +591,9 @@ int pla_causal_depthwise_step(const void* x, int64_t x_row, void* state, int64_t
   if (meets(ys, xs) || meets(ys, ss) || meets(xs, ss)) return PLA_ERR_INVALID_ARGUMENT;
   int sms, st;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
-  const int vec = static_cast<int>(16 / es);
-  const bool wide = channels % vec == 0 && x_row % vec == 0 && state_row % vec == 0 && aligned_to(x, 16) &&
-                    aligned_to(state, 16) && aligned_to(y, 16);
+  const int vec = static_cast<int>(8 / es);
+  const bool wide = channels % vec == 0 && x_row % vec == 0 && state_row % vec == 0 && aligned_to(x, 8) &&
+                    aligned_to(state, 8) && aligned_to(y, 8) && aligned_to(w, 8) && aligned_to(b, 8);
   return with_causal(dtype, taps, wide, false, [&](auto zero, auto v, auto k) {
     using T = decltype(zero);
     constexpr int V = decltype(v)::value, K = decltype(k)::value;
@@ -616,22 +625,31 @@ int pla_qk_norm_rotate_forward(const pla_qk_norm* a, pla_stream_t stream) {
     NormParams p = norm_params(a);
     // four heads a group once that still leaves every SM a thousand threads
     const bool many = tokens * (a->q.heads + a->k.heads) / 4 * LANES >= sms * 1024ll;
-    const int hb = many ? 4 : 1;
+    const int hb = many ? 4 : 1, groups = kNormThreads / LANES;
     p.units[0] = (a->q.heads + hb - 1) / hb;
     p.units[1] = (a->k.heads + hb - 1) / hb;
-    const long long blocks = (tokens * (p.units[0] + p.units[1]) * LANES + kNormThreads - 1) / kNormThreads;
-    if (blocks > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
+    const int units = p.units[0] + p.units[1];
+    // as many blocks as the device holds at a time, each group walking tokens
+    const long long whole = (static_cast<long long>(a->tokens) * units + groups - 1) / groups;
+    const long long share = std::max<long long>(1, sms * 6ll / std::max(1, a->batch));
+    // a number of groups that is a multiple of the units, so that a group keeps its unit
+    const int step = units / std::gcd(units, groups);
+    const long long blocks = whole <= share ? whole : (share + step - 1) / step * step;
+    if (a->batch > 65535) return static_cast<int>(PLA_ERR_TOO_LARGE);
+    p.stride = whole <= share ? a->tokens : static_cast<int>(blocks * groups / units);
+    const dim3 grid(static_cast<int>(blocks), a->batch);
     if (many)
-      qk_norm_forward<T, CH, NC, LANES, 4><<<static_cast<int>(blocks), kNormThreads, 0, as_stream(stream)>>>(p);
+      qk_norm_forward<T, CH, NC, LANES, 4><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
     else
-      qk_norm_forward<T, CH, NC, LANES, 1><<<static_cast<int>(blocks), kNormThreads, 0, as_stream(stream)>>>(p);
+      qk_norm_forward<T, CH, NC, LANES, 1><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
     return launched("qk_norm_forward");
   });
 }
 
 size_t pla_qk_norm_rotate_workspace(const pla_qk_norm* a) {
   if (!a || a->dim < 0 || a->batch < 0 || a->tokens < 0 || a->q.heads < 0 || a->k.heads < 0) return 0;
-  const int most = norm_side_blocks(a, a->q.heads, 32) + norm_side_blocks(a, a->k.heads, 32);
+  int most = 0;
+  for (int lanes : {8, 16, 32}) most = std::max(most, norm_side_blocks(a, a->q.heads, lanes) + norm_side_blocks(a, a->k.heads, lanes));
   return static_cast<size_t>(most) * a->dim * sizeof(float);
 }
 
@@ -645,6 +663,8 @@ int pla_qk_norm_rotate_backward(const pla_qk_norm* a, void* workspace, size_t wo
        !aligned_to(workspace, 16)))
     return PLA_ERR_INVALID_ARGUMENT;
   if (!a->dim) return PLA_OK;
+  const long long tokens = static_cast<long long>(a->batch) * a->tokens;
+  if (tokens * std::max(a->q.heads, a->k.heads) > kMaxTokens) return PLA_ERR_TOO_LARGE;
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
   const bool wide = norm_vector(a, true);
@@ -653,8 +673,11 @@ int pla_qk_norm_rotate_backward(const pla_qk_norm* a, void* workspace, size_t wo
     constexpr int CH = decltype(ch)::value, NC = decltype(nc)::value, LANES = decltype(lanes)::value;
     NormParams p = norm_params(a);
     p.partial = sums ? static_cast<float*>(workspace) : nullptr;
-    p.side_blocks[0] = norm_side_blocks(a, a->q.heads, LANES);
-    p.side_blocks[1] = norm_side_blocks(a, a->k.heads, LANES);
+    for (int i = 0; i < 2; ++i) {
+      const int heads = i ? a->k.heads : a->q.heads, groups = kNormThreads / LANES;
+      p.side_blocks[i] = norm_side_blocks(a, heads, LANES);
+      p.side_stride[i] = heads ? p.side_blocks[i] * groups / heads : 1;
+    }
     int st = PLA_OK;
     if (p.side_blocks[0] + p.side_blocks[1] > 0) {
       qk_norm_backward<T, CH, NC, LANES>
@@ -798,22 +821,30 @@ int pla_gated_delta_rule_step(const pla_delta_step* a, pla_stream_t stream) {
   p.n = a->n, p.hk = a->hk, p.hv = a->hv, p.dk = a->dk, p.dv = a->dv;
   p.gates32 = a->gates32 != 0;
   p.scale = a->scale;
-  const bool wide = a->dv % 4 == 0 && a->state_row % 4 == 0 && aligned_to(a->state, 16) && aligned_to(a->o, 4 * es);
+  // whole states by bulk copies: rows a warp can share out evenly, 16-byte addresses
+  const bool whole = (a->dv == 32 || a->dv == 64 || a->dv == 128) && a->dk <= 128 && head % 4 == 0 && a->state_row % 4 == 0 &&
+                     aligned_to(a->state, 16);
   return with_type(a->dtype, [&](auto zero) {
     using T = decltype(zero);
-    auto go = [&](auto rows, auto v) {
-      constexpr int ROWS = decltype(rows)::value, V = decltype(v)::value;
-      const long long blocks = static_cast<long long>(p.n) * p.hv * ((p.dv + 32 * V - 1) / (32 * V));
+    if (whole) {
+      const long long blocks = static_cast<long long>(p.n) * p.hv;
       if (blocks > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
-      delta_step<T, ROWS, V><<<static_cast<int>(blocks), kStepWarps * 32, 0, as_stream(stream)>>>(p);
+      const size_t shared = static_cast<size_t>(head) * 4;
+      const int st = allow_shared<delta_step<T>>(128 * 128 * 4);
+      if (st != PLA_OK) return st;
+      delta_step<T><<<static_cast<int>(blocks), kStepWarps * 32, shared, as_stream(stream)>>>(p);
       return launched("delta_step");
+    }
+    const auto go = [&](auto rows) {
+      constexpr int ROWS = decltype(rows)::value;
+      const long long blocks = static_cast<long long>(p.n) * p.hv * ((p.dv + 31) / 32);
+      if (blocks > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
+      delta_step_any<T, ROWS><<<static_cast<int>(blocks), kStepAnyWarps * 32, 0, as_stream(stream)>>>(p);
+      return launched("delta_step_any");
     };
-    auto rows = [&](auto v) {
-      if (p.dk <= 64) return go(Int<8>{}, v);
-      if (p.dk <= 128) return go(Int<16>{}, v);
-      return go(Int<32>{}, v);
-    };
-    return wide ? rows(Int<4>{}) : rows(Int<1>{});
+    if (p.dk <= 64) return go(Int<4>{});
+    if (p.dk <= 128) return go(Int<8>{});
+    return go(Int<16>{});
   });
 }
 

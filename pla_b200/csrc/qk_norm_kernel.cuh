@@ -13,9 +13,12 @@
 // twice, written once), about 8 flops an element.  A group of 8, 16 or 32
 // lanes owns a head; a lane holds pairs in the layout the rotation needs, so
 // the partner is in the same lane and the sum of squares is the only exchange
-// (shuffles).  A group takes several heads of one token at a time: their loads
-// are in flight together and share the token's cosines and sines.  All
-// arithmetic is fp32 with one rounding at the end.
+// (shuffles).  A group keeps one set of heads (four in large calls) and walks
+// tokens with their weights in registers: the set's loads are in flight
+// together and share the token's cosines and sines, and a token costs no
+// division and no set-up (with a set-up per token the kernel was bound by
+// instructions, 68 us for 8192 tokens of 40 heads of 128 in bf16, against
+// NORMFWD).  All arithmetic is fp32 with one rounding at the end.
 #pragma once
 
 #include "seq_common.cuh"
@@ -44,8 +47,9 @@ struct NormParams {
   int batch, tokens, dim, rot, interleaved, l2;
   float eps;
   int units[2];            // groups of heads of a token, per side
+  int stride;              // tokens from one of a group to its next
   float* partial;          // backward: [blocks of a side][D] twice, or nullptr
-  int side_blocks[2];
+  int side_blocks[2], side_stride[2];
 };
 
 // A lane's NC chunks of CH pairs of a head's features.  CH = 4 needs rot / 2
@@ -64,7 +68,7 @@ struct PairMap {
       adjacent[n] = turned[n] && interleaved;
       angle[n] = p;
       const int q = p - half;
-      single[n] = CH == 1 && !turned[n] && q == rest_half && (rest & 1);
+      single[n] = CH == 1 && !turned[n] && q == rest_half && (rest & 1);  // CH = 4: never
       there[n] = turned[n] || q < rest_half || single[n];
       first[n] = turned[n] ? (interleaved ? 2 * p : p) : (single[n] ? D - 1 : rot + q);
       second[n] = turned[n] ? (interleaved ? 2 * p + CH : p + half) : rot + rest_half + q;
@@ -144,36 +148,9 @@ __device__ __forceinline__ void load_angles(const NormParams& p, const PairMap<C
 
 constexpr int kNormThreads = 256;
 
-template <typename T, int CH, int NC, int LANES, int HB>
-__global__ void __launch_bounds__(kNormThreads) qk_norm_forward(NormParams p) {
-  const int lane = threadIdx.x % LANES;
-  const long long group = (static_cast<long long>(blockIdx.x) * kNormThreads + threadIdx.x) / LANES;
-  const int units = p.units[0] + p.units[1];
-  const long long token = group / units;
-  int unit = static_cast<int>(group % units);
-  const bool live = token < static_cast<long long>(p.batch) * p.tokens;  // whole groups: every lane still shuffles
-  const int b = live ? static_cast<int>(token / p.tokens) : 0, t = live ? static_cast<int>(token % p.tokens) : 0;
-  const int which = unit >= p.units[0];
-  if (which) unit -= p.units[0];
-  const NormSide& side = p.side[which];
-  const PairMap<CH, NC> map(lane, LANES, p.dim, p.rot, p.interleaved);
-  const T* x = static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token;
-  T* y = static_cast<T*>(side.y) + (static_cast<long long>(b) * p.tokens + t) * side.heads * p.dim;
-  const int h0 = unit * HB;
-
-  float xa[HB][NC][CH], xb[HB][NC][CH];
-#pragma unroll
-  for (int h = 0; h < HB; ++h)
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-#pragma unroll
-      for (int i = 0; i < CH; ++i) xa[h][n][i] = xb[h][n][i] = 0.f;
-      if (live && h0 + h < side.heads && map.there[n])
-        load_pairs<T, CH>(x + (h0 + h) * side.x_head, map.first[n], map.second[n], map.adjacent[n], map.single[n],
-                          xa[h][n], xb[h][n]);
-    }
-  float c[NC][CH], s[NC][CH], wa[NC][CH], wb[NC][CH];
-  if (live) load_angles<CH, NC>(p, map, b, t, c, s);
+// A lane's parts of a weight; ones without.
+template <typename T, int CH, int NC>
+__device__ __forceinline__ void load_weight(const NormSide& side, const PairMap<CH, NC>& map, float (&wa)[NC][CH], float (&wb)[NC][CH]) {
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
 #pragma unroll
@@ -182,35 +159,71 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_forward(NormParams p) {
       load_pairs<T, CH>(static_cast<const T*>(side.w), map.first[n], map.second[n], map.adjacent[n], map.single[n], wa[n],
                         wb[n]);
   }
+}
+
+// blockIdx.y: batch row.  The groups of the grid's row are numbered; group g
+// takes unit g % units of tokens g / units, g / units + stride, ...
+template <typename T, int CH, int NC, int LANES, int HB>
+__global__ void __launch_bounds__(kNormThreads) qk_norm_forward(NormParams p) {
+  const int lane = threadIdx.x % LANES;
+  const int group = (blockIdx.x * kNormThreads + threadIdx.x) / LANES;
+  const int units = p.units[0] + p.units[1], b = blockIdx.y;
+  int t = group / units, unit = group - t * units;
+  const int which = unit >= p.units[0];
+  if (which) unit -= p.units[0];
+  const NormSide& side = p.side[which];
+  const PairMap<CH, NC> map(lane, LANES, p.dim, p.rot, p.interleaved);
+  const int h0 = unit * HB, heads = min(HB, side.heads - h0);
+  const T* x = static_cast<const T*>(side.x) + b * side.x_batch + h0 * side.x_head;
+  T* y = static_cast<T*>(side.y) + (static_cast<long long>(b) * p.tokens * side.heads + h0) * p.dim;
+  float wa[NC][CH], wb[NC][CH];
+  load_weight<T, CH, NC>(side, map, wa, wb);
   const float per = p.l2 ? 1.f : 1.f / p.dim;
+  // a warp's groups make the same number of turns: all lanes shuffle
+  for (int turn = __reduce_min_sync(0xffffffffu, t); turn < p.tokens; turn += p.stride, t += p.stride) {
+    const bool live = t < p.tokens;
+    float xa[HB][NC][CH], xb[HB][NC][CH];
 #pragma unroll
-  for (int h = 0; h < HB; ++h) {
-    float sum = 0.f;
+    for (int h = 0; h < HB; ++h)
 #pragma unroll
-    for (int n = 0; n < NC; ++n)
+      for (int n = 0; n < NC; ++n) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) sum = fmaf(xa[h][n][i], xa[h][n][i], fmaf(xb[h][n][i], xb[h][n][i], sum));
-    const float r = 1.f / sqrtf(fmaf(group_sum<LANES>(sum), per, p.eps));
-    if (!live || h0 + h >= side.heads) continue;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      if (!map.there[n]) continue;
-      float oa[CH], ob[CH];
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const float na = xa[h][n][i] * r * wa[n][i], nb = xb[h][n][i] * r * wb[n][i];
-        oa[i] = map.turned[n] ? fmaf(na, c[n][i], -nb * s[n][i]) : na;
-        ob[i] = map.turned[n] ? fmaf(nb, c[n][i], na * s[n][i]) : nb;
+        for (int i = 0; i < CH; ++i) xa[h][n][i] = xb[h][n][i] = 0.f;
+        if (live && h < heads && map.there[n])
+          load_pairs<T, CH>(x + t * side.x_token + h * side.x_head, map.first[n], map.second[n], map.adjacent[n], map.single[n],
+                            xa[h][n], xb[h][n]);
       }
-      store_pairs<T, CH>(y + (h0 + h) * static_cast<long long>(p.dim), map.first[n], map.second[n], map.adjacent[n],
-                         map.single[n], oa, ob);
+    float c[NC][CH], s[NC][CH];
+    if (live) load_angles<CH, NC>(p, map, b, t, c, s);
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int i = 0; i < CH; ++i) sum = fmaf(xa[h][n][i], xa[h][n][i], fmaf(xb[h][n][i], xb[h][n][i], sum));
+      const float r = 1.f / sqrtf(fmaf(group_sum<LANES>(sum), per, p.eps));
+      if (!live || h >= heads) continue;
+      T* to = y + (static_cast<long long>(t) * side.heads + h) * p.dim;
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        if (!map.there[n]) continue;
+        float oa[CH], ob[CH];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {  // features that are not rotated have cos 1, sin 0
+          const float na = xa[h][n][i] * r * wa[n][i], nb = xb[h][n][i] * r * wb[n][i];
+          oa[i] = fmaf(na, c[n][i], -nb * s[n][i]);
+          ob[i] = fmaf(nb, c[n][i], na * s[n][i]);
+        }
+        store_pairs<T, CH>(to, map.first[n], map.second[n], map.adjacent[n], map.single[n], oa, ob);
+      }
     }
   }
 }
 
-// dx, and the block's sums for dw: a group walks tokens of one side with dw
-// in registers, the groups of a block are added in shared memory, the blocks
-// in qk_norm_reduce, all in a fixed order.
+// dx, and the block's sums for dw.  A block works on one side: its groups walk
+// tokens with one head each and dw in registers, and are added in shared
+// memory, the blocks in qk_norm_reduce, all in a fixed order.
 template <typename T, int CH, int NC, int LANES>
 __global__ void __launch_bounds__(kNormThreads) qk_norm_backward(NormParams p) {
   constexpr int GROUPS = kNormThreads / LANES;
@@ -221,28 +234,21 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_backward(NormParams p) {
   const int block = which ? blockIdx.x - p.side_blocks[0] : blockIdx.x;
   const PairMap<CH, NC> map(lane, LANES, p.dim, p.rot, p.interleaved);
   float wa[NC][CH], wb[NC][CH], ga[NC][CH] = {}, gb[NC][CH] = {};
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) wa[n][i] = wb[n][i] = 1.f;
-    if (side.w && map.there[n])
-      load_pairs<T, CH>(static_cast<const T*>(side.w), map.first[n], map.second[n], map.adjacent[n], map.single[n], wa[n],
-                        wb[n]);
-  }
+  load_weight<T, CH, NC>(side, map, wa, wb);
   const float per = p.l2 ? 1.f : 1.f / p.dim;
-  const long long rows = static_cast<long long>(p.batch) * p.tokens * side.heads;
-  const long long step = static_cast<long long>(p.side_blocks[which]) * GROUPS;
-  // every group of the block makes the same number of turns: all lanes shuffle
-  for (long long base = static_cast<long long>(block) * GROUPS; base < rows; base += step) {
-    const long long row = base + in_block;
-    const bool live = row < rows;
-    const long long token = live ? row / side.heads : 0;
-    const int h = live ? static_cast<int>(row % side.heads) : 0;
-    const int b = static_cast<int>(token / p.tokens), t = static_cast<int>(token % p.tokens);
-    const T* x = static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token + h * side.x_head;
-    const T* dy = static_cast<const T*>(side.dy) + b * side.dy_batch + t * side.dy_token + h * side.dy_head;
-    float xa[NC][CH] = {}, xb[NC][CH] = {}, da[NC][CH] = {}, db[NC][CH] = {}, c[NC][CH], s[NC][CH];
+  const int rows = p.batch * p.tokens;  // below 2^31
+  const int group = block * GROUPS + in_block;
+  int row = group / side.heads;  // batch row and token as one number
+  const int h = group - row * side.heads;
+  int b = row / p.tokens, t = row - b * p.tokens;
+  // stride[which] tokens on for every turn; a warp's groups make the same number of turns
+  for (int turn = __reduce_min_sync(0xffffffffu, row); turn < rows; turn += p.side_stride[which], row += p.side_stride[which]) {
+    const bool live = row < rows && h < side.heads;
+    float xa[NC][CH] = {}, xb[NC][CH] = {}, da[NC][CH] = {}, db[NC][CH] = {}, c[NC][CH] = {}, s[NC][CH] = {};
     if (live) {
+      while (t >= p.tokens) t -= p.tokens, ++b;
+      const T* x = static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token + h * side.x_head;
+      const T* dy = static_cast<const T*>(side.dy) + b * side.dy_batch + t * side.dy_token + h * side.dy_head;
 #pragma unroll
       for (int n = 0; n < NC; ++n)
         if (map.there[n]) {
@@ -251,16 +257,15 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_backward(NormParams p) {
         }
       load_angles<CH, NC>(p, map, b, t, c, s);
     }
+    t += p.side_stride[which];
     float square = 0.f, dot = 0.f;
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        if (live && map.turned[n]) {  // rotate back
-          const float ya = da[n][i], yb = db[n][i];
-          da[n][i] = fmaf(ya, c[n][i], yb * s[n][i]);
-          db[n][i] = fmaf(yb, c[n][i], -ya * s[n][i]);
-        }
+        const float ya = da[n][i], yb = db[n][i];  // rotated back; cos 1, sin 0 where there is no rotation
+        da[n][i] = fmaf(ya, c[n][i], yb * s[n][i]);
+        db[n][i] = fmaf(yb, c[n][i], -ya * s[n][i]);
         square = fmaf(xa[n][i], xa[n][i], fmaf(xb[n][i], xb[n][i], square));
         dot = fmaf(da[n][i] * wa[n][i], xa[n][i], fmaf(db[n][i] * wb[n][i], xb[n][i], dot));
       }
@@ -269,7 +274,7 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_backward(NormParams p) {
     if (!live) continue;
     const float r = 1.f / sqrtf(fmaf(square, per, p.eps));
     const float back = dot * r * r * per;  // sum(h xhat) r / count
-    T* dx = static_cast<T*>(side.y) + row * p.dim;
+    T* dx = static_cast<T*>(side.y) + (static_cast<long long>(row) * side.heads + h) * p.dim;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       if (!map.there[n]) continue;
@@ -298,14 +303,14 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_backward(NormParams p) {
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     if (!map.there[n]) continue;
-    float a[CH] = {}, b[CH] = {};
+    float a[CH] = {}, b2[CH] = {};
     for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         a[i] += part[g][2 * (n * CH + i)][lane];
-        b[i] += part[g][2 * (n * CH + i) + 1][lane];
+        b2[i] += part[g][2 * (n * CH + i) + 1][lane];
       }
-    store_pairs<float, CH>(out, map.first[n], map.second[n], map.adjacent[n], map.single[n], a, b);
+    store_pairs<float, CH>(out, map.first[n], map.second[n], map.adjacent[n], map.single[n], a, b2);
   }
 }
 

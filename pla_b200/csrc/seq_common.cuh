@@ -44,9 +44,36 @@ __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
   *reinterpret_cast<Vec<T, V>*>(p) = v;
 }
 
-// 1 / (1 + e^-p).  16-bit results take the hardware exponential and divide
-// (relative error below 2^-20, their own rounding is 2^-12 at best).
-template <typename T> __device__ __forceinline__ float sigmoid(float p) { return __fdividef(1.f, 1.f + __expf(-p)); }
+// Two fp32 values in one register pair, and their fused multiply-add in one
+// instruction (sm_100), each rounded once.
+struct Pair {
+  unsigned long long v;
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ float2 both(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+  return f;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+
+// 1 / (1 + e^-p).  16-bit results take the hardware's 2^x and reciprocal (2^-22
+// relative each, their own rounding is 2^-12 at best; subnormal values of
+// either count as 0, that is |p| above 87).
+template <typename T> __device__ __forceinline__ float sigmoid(float p) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(p * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
 template <> __device__ __forceinline__ float sigmoid<float>(float p) { return 1.f / (1.f + expf(-p)); }
 
 __device__ __forceinline__ int clamp_token(int v, int tokens) { return v < 0 ? 0 : (v > tokens ? tokens : v); }
