@@ -7,11 +7,11 @@
 // Bound by HBM: x is read and y written once, 2 K flops an element.  A thread
 // owns four neighbouring channels of a strip of tokens and walks it with the
 // last K - 1 inputs in registers, so an input is fetched once plus
-// (K - 1) / strip of overlap that neighbouring strips leave in L2; the loads of
-// four tokens are issued while the four before them are worked on.  Four
-// channels (8 bytes a 16-bit load) and not eight: eight took 148 registers a
-// thread, which left 8 warps an SM and too few bytes in flight (140 us for
-// 8191 x 8192 bf16, against CAUSALFWD).  The products are summed in fp32 in tap
+// (K - 1) / strip of overlap that neighbouring strips leave in L2; a ring of
+// eight rows is in flight, each refilled as soon as it is used.  Four channels
+// (8 bytes a 16-bit load) and not eight: eight took 148 registers a thread,
+// which left 8 warps an SM and too few bytes in flight (140 us for 8191 x 8192
+// bf16, against CAUSALFWD).  The products are summed in fp32 in tap
 // order, two channels an instruction, and rounded once.
 //
 // Backward, with dp[t] = dy[t] act'(p[t]) recomputed from x:
@@ -146,13 +146,14 @@ __global__ void __launch_bounds__(kCausalThreads, 3) causal_forward(CausalParams
   const T* x = static_cast<const T*>(p.x) + batch * p.x_batch;
   T* y = static_cast<T*>(p.y) + (static_cast<long long>(batch) * p.tokens + t0) * p.channels + c;
 
-  constexpr int U = 4, H = (V + 1) / 2;
+  constexpr int U = 8, H = (V + 1) / 2;
   using Row = Vec<T, V>;
   const T* from = x + t0 * p.x_token + c;
-  Row next[U];
+  Row ring[U];
 #pragma unroll
   for (int i = 0; i < U; ++i)
-    if (t0 + i < t1) next[i] = *reinterpret_cast<const Row*>(from + i * p.x_token);
+    if (t0 + i < t1) ring[i] = *reinterpret_cast<const Row*>(from + i * p.x_token);
+  from += U * p.x_token;
   Pair w[K][H], b[H], seen[K - 1][H];
   SequenceWalk s;
   s.begin(p, batch, t0);
@@ -160,58 +161,48 @@ __global__ void __launch_bounds__(kCausalThreads, 3) causal_forward(CausalParams
     float wf[K][V], bf[V];
     load_filter<T, V, K>(p, c, wf, bf);
 #pragma unroll
-    for (int v = 0; v < H; ++v) {
-#pragma unroll
-      for (int j = 0; j < K; ++j) w[j][v] = pair(wf[j][2 * v], 2 * v + 1 < V ? wf[j][(2 * v + 1) % V] : 0.f);
-      b[v] = pair(bf[2 * v], 2 * v + 1 < V ? bf[(2 * v + 1) % V] : 0.f);
-    }
+    for (int j = 0; j < K; ++j) as_pair_array(wf[j], w[j]);
+    as_pair_array(bf, b);
   }
   const auto refill = [&](int t) {
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
       float f[V];
       input_before<T, V, K>(p, x, s, t, K - 1 - j, c, f);
-#pragma unroll
-      for (int v = 0; v < H; ++v) seen[j][v] = pair(f[2 * v], 2 * v + 1 < V ? f[(2 * v + 1) % V] : 0.f);
+      as_pair_array(f, seen[j]);
     }
+  };
+  const auto one = [&](const Row& row) {
+    float in[V], out[V];
+    unpack(row, in);
+    Pair now[H], a[H];
+    as_pair_array(in, now);
+#pragma unroll
+    for (int v = 0; v < H; ++v) {
+      a[v] = b[v];
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) a[v] = fma2(w[j][v], seen[j][v], a[v]);
+      a[v] = fma2(w[K - 1][v], now[v], a[v]);
+#pragma unroll
+      for (int j = 0; j + 1 < K - 1; ++j) seen[j][v] = seen[j + 1][v];
+      seen[K - 2][v] = now[v];
+    }
+    as_float_array(a, out);
+    if (p.silu)
+#pragma unroll
+      for (int v = 0; v < V; ++v) out[v] *= sigmoid<T>(out[v]);
+    store<T, V>(y, out);
+    y += p.channels;
   };
   refill(t0);
   for (int t = t0; t < t1; t += U) {
-    Row in[U];
+    if (t + 2 * U <= t1 && t + U <= s.end && s.index >= 0) {  // eight tokens of one sequence, and eight more to fetch
 #pragma unroll
-    for (int i = 0; i < U; ++i) in[i] = next[i];
-    from += U * p.x_token;
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (t + U + i < t1) next[i] = *reinterpret_cast<const Row*>(from + i * p.x_token);
-    const auto one = [&](const Row& row) {
-      float out[V];
-#pragma unroll
-      for (int v = 0; v < H; ++v) {
-        const Pair now = pair(up(row.e[2 * v]), 2 * v + 1 < V ? up(row.e[(2 * v + 1) % V]) : 0.f);
-        Pair a = b[v];
-#pragma unroll
-        for (int j = 0; j < K - 1; ++j) a = fma2(w[j][v], seen[j][v], a);
-        a = fma2(w[K - 1][v], now, a);
-        const float2 f = both(a);
-        out[2 * v] = f.x;
-        if (2 * v + 1 < V) out[(2 * v + 1) % V] = f.y;
-#pragma unroll
-        for (int j = 0; j + 1 < K - 1; ++j) seen[j][v] = seen[j + 1][v];
-        seen[K - 2][v] = now;
+      for (int i = 0; i < U; ++i) {
+        one(ring[i]);
+        ring[i] = *reinterpret_cast<const Row*>(from);
+        from += p.x_token;
       }
-      if (p.silu)
-#pragma unroll
-        for (int v = 0; v < V; ++v) out[v] *= sigmoid<T>(out[v]);
-      if (s.index < 0)
-#pragma unroll
-        for (int v = 0; v < V; ++v) out[v] = 0.f;
-      store<T, V>(y, out);
-      y += p.channels;
-    };
-    if (t + U <= t1 && t + U <= s.end) {  // four tokens of one sequence
-#pragma unroll
-      for (int i = 0; i < U; ++i) one(in[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < U; ++i) {
@@ -220,7 +211,15 @@ __global__ void __launch_bounds__(kCausalThreads, 3) causal_forward(CausalParams
           s.next(p, batch, t + i);
           refill(t + i);
         }
-        one(in[i]);
+        if (s.index >= 0) {
+          one(ring[i]);
+        } else {
+          const float none[V] = {};
+          store<T, V>(y, none);
+          y += p.channels;
+        }
+        if (t + U + i < t1) ring[i] = *reinterpret_cast<const Row*>(from);
+        from += p.x_token;
       }
     }
   }
@@ -238,7 +237,7 @@ constexpr int kCausalRows = 8;  // strips of a block in the backward pass
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(kCausalThreads, V > 1 ? 2 : 3) causal_backward(CausalParams p) {
   __shared__ float part[kCausalRows / 2][K + 1][32 * V];
-  constexpr int H = (V + 1) / 2, U = 4;
+  constexpr int H = (V + 1) / 2, U = 8;
   using Row = Vec<T, V>;
   const int nvec = p.channels / V;
   const int across = (nvec + 31) / 32;
@@ -257,27 +256,29 @@ __global__ void __launch_bounds__(kCausalThreads, V > 1 ? 2 : 3) causal_backward
     const T* x_at = x + t0 * p.x_token + c;
     const T* dy_at = static_cast<const T*>(p.dy) + batch * p.dy_batch + t0 * p.dy_token + c;
     T* dx = static_cast<T*>(p.dx) + (static_cast<long long>(batch) * p.tokens + t0) * p.channels + c;
-    Row x_next[U], dy_next[U];
+    Row ring[U], dy_ring[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i)
+    for (int i = 0; i < U; ++i) {
       if (t0 + i < there) {
-        x_next[i] = *reinterpret_cast<const Row*>(x_at + i * p.x_token);
-        dy_next[i] = *reinterpret_cast<const Row*>(dy_at + i * p.dy_token);
+        ring[i] = *reinterpret_cast<const Row*>(x_at);
+        dy_ring[i] = *reinterpret_cast<const Row*>(dy_at);
       }
-    const auto two = [](const float (&f)[V], int v) { return pair(f[2 * v], 2 * v + 1 < V ? f[(2 * v + 1) % V] : 0.f); };
+      x_at += p.x_token;
+      dy_at += p.dy_token;
+    }
     Pair w[K][H], b[H], seen[K][H], ahead[K][H], gw[K][H], gb[H];  // ahead[j]: dx of token t - K + 1 + j so far
+    const Pair zero = pair(0.f, 0.f), ones = pair(1.f, 1.f);
     {
       float wf[K][V], bf[V];
       load_filter<T, V, K>(p, c, wf, bf);
+      as_pair_array(bf, b);
+#pragma unroll
+      for (int j = 0; j < K; ++j) as_pair_array(wf[j], w[j]);
 #pragma unroll
       for (int v = 0; v < H; ++v) {
-        b[v] = two(bf, v);
-        gb[v] = pair(0.f, 0.f);
+        gb[v] = zero;
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-          w[j][v] = two(wf[j], v);
-          ahead[j][v] = gw[j][v] = pair(0.f, 0.f);
-        }
+        for (int j = 0; j < K; ++j) seen[j][v] = ahead[j][v] = gw[j][v] = zero;
       }
     }
     SequenceWalk s;
@@ -287,75 +288,68 @@ __global__ void __launch_bounds__(kCausalThreads, V > 1 ? 2 : 3) causal_backward
       for (int j = 0; j < K - 1; ++j) {
         float f[V];
         input_before<T, V, K>(p, x, s, t, K - 1 - j, c, f);
-#pragma unroll
-        for (int v = 0; v < H; ++v) seen[j + 1][v] = two(f, v);
+        as_pair_array(f, seen[j + 1]);
       }
     };
+    // gradient of one token that is in a sequence, without what the state after it gives
+    const auto one = [&](const Row& row, const Row& grad, bool own, int reach) {
+      float in[V], up_in[V];
+      unpack(row, in);
+      unpack(grad, up_in);
+      as_pair_array(in, seen[K - 1]);
+      if (p.silu) {
+        Pair a[H];
+        float f[V];
+#pragma unroll
+        for (int v = 0; v < H; ++v) {
+          a[v] = b[v];
+#pragma unroll
+          for (int j = 0; j < K; ++j) a[v] = fma2(w[j][v], seen[j][v], a[v]);
+        }
+        as_float_array(a, f);
+#pragma unroll
+        for (int v = 0; v < V; ++v) up_in[v] *= act_slope<T>(f[v]);
+      }
+      Pair g[H];
+      as_pair_array(up_in, g);
+#pragma unroll
+      for (int v = 0; v < H; ++v) {
+        if (own) {
+#pragma unroll
+          for (int j = 0; j < K; ++j) gw[j][v] = fma2(g[v], seen[j][v], gw[j][v]);
+          gb[v] = fma2(g[v], ones, gb[v]);
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+          if (K - 1 - j <= reach) ahead[j][v] = fma2(w[j][v], g[v], ahead[j][v]);
+      }
+    };
+    const auto shift = [&](const float (&give)[V]) {
+#pragma unroll
+      for (int v = 0; v < H; ++v)
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) seen[j][v] = seen[j + 1][v], ahead[j][v] = ahead[j + 1][v];
+      as_pair_array(give, ahead[K - 1]);
+    };
+    const auto emit = [&]() {
+      float out[V];
+      as_float_array(ahead[0], out);
+      store<T, V>(dx, out);
+      dx += p.channels;
+    };
+    const float none[V] = {};
     refill(t0);
     for (int t = t0; t < last; t += U) {
-      Row in[U], give_in[U];
+      if (s.index >= 0 && t >= t0 + K - 1 && t >= s.start + K - 1 && t + U <= t1 && t + U + K - 1 <= s.end && t + 2 * U <= there) {
 #pragma unroll
-      for (int i = 0; i < U; ++i) in[i] = x_next[i], give_in[i] = dy_next[i];
-      x_at += U * p.x_token;
-      dy_at += U * p.dy_token;
-#pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (t + U + i < there) {
-          x_next[i] = *reinterpret_cast<const Row*>(x_at + i * p.x_token);
-          dy_next[i] = *reinterpret_cast<const Row*>(dy_at + i * p.dy_token);
-        }
-      // gradient of one token that is in a sequence, without what the state after it gives
-      const auto one = [&](const Row& row, const Row& grad, bool own, int reach) {
-#pragma unroll
-        for (int v = 0; v < H; ++v) {
-          seen[K - 1][v] = pair(up(row.e[2 * v]), 2 * v + 1 < V ? up(row.e[(2 * v + 1) % V]) : 0.f);
-          Pair g = pair(up(grad.e[2 * v]), 2 * v + 1 < V ? up(grad.e[(2 * v + 1) % V]) : 0.f);
-          if (p.silu) {
-            Pair a = b[v];
-#pragma unroll
-            for (int j = 0; j < K; ++j) a = fma2(w[j][v], seen[j][v], a);
-            const float2 f = both(a);
-            float2 gf = both(g);
-            gf.x *= act_slope<T>(f.x);
-            if (2 * v + 1 < V) gf.y *= act_slope<T>(f.y);
-            g = pair(gf.x, gf.y);
-          }
-          if (own) {
-#pragma unroll
-            for (int j = 0; j < K; ++j) gw[j][v] = fma2(g, seen[j][v], gw[j][v]);
-            gb[v] = fma2(g, pair(1.f, 1.f), gb[v]);
-          }
-#pragma unroll
-          for (int j = 0; j < K; ++j)
-            if (K - 1 - j <= reach) ahead[j][v] = fma2(w[j][v], g, ahead[j][v]);
-        }
-      };
-      const auto shift = [&](const float (&give)[V]) {
-#pragma unroll
-        for (int v = 0; v < H; ++v) {
-#pragma unroll
-          for (int j = 0; j < K - 1; ++j) seen[j][v] = seen[j + 1][v], ahead[j][v] = ahead[j + 1][v];
-          ahead[K - 1][v] = two(give, v);
-        }
-      };
-      const auto emit = [&]() {
-        float out[V];
-#pragma unroll
-        for (int v = 0; v < H; ++v) {
-          const float2 f = both(ahead[0][v]);
-          out[2 * v] = f.x;
-          if (2 * v + 1 < V) out[(2 * v + 1) % V] = f.y;
-        }
-        store<T, V>(dx, out);
-        dx += p.channels;
-      };
-      const float none[V] = {};
-      if (s.index >= 0 && t >= t0 + K - 1 && t >= s.start + K - 1 && t + U <= t1 && t + U + K - 1 <= s.end) {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {  // four tokens well inside a sequence and the strip
+        for (int i = 0; i < U; ++i) {  // eight tokens well inside a sequence and the strip, and eight more to fetch
           shift(none);
-          one(in[i], give_in[i], true, K - 1);
+          one(ring[i], dy_ring[i], true, K - 1);
           emit();
+          ring[i] = *reinterpret_cast<const Row*>(x_at);
+          dy_ring[i] = *reinterpret_cast<const Row*>(dy_at);
+          x_at += p.x_token;
+          dy_at += p.dy_token;
         }
       } else {
 #pragma unroll
@@ -375,20 +369,20 @@ __global__ void __launch_bounds__(kCausalThreads, V > 1 ? 2 : 3) causal_backward
                              (static_cast<long long>(s.index) * (K - 1) + r) * p.channels + c, give);
           }
           shift(give);
-          if (live) one(in[i], give_in[i], now < t1, now - s.start);
+          if (live) one(ring[i], dy_ring[i], now < t1, now - s.start);
           if (now - (K - 1) >= t0) emit();
+          if (now + U < there) {
+            ring[i] = *reinterpret_cast<const Row*>(x_at);
+            dy_ring[i] = *reinterpret_cast<const Row*>(dy_at);
+          }
+          x_at += p.x_token;
+          dy_at += p.dy_token;
         }
       }
     }
 #pragma unroll
-    for (int v = 0; v < H; ++v) {
-#pragma unroll
-      for (int j = 0; j <= K; ++j) {
-        const float2 f = both(j < K ? gw[j % K][v] : gb[v]);
-        (j < K ? dw[j % K] : db)[2 * v] = f.x;
-        if (2 * v + 1 < V) (j < K ? dw[j % K] : db)[(2 * v + 1) % V] = f.y;
-      }
-    }
+    for (int j = 0; j < K; ++j) as_float_array(gw[j], dw[j]);
+    as_float_array(gb, db);
   }
   if (!p.partial) return;
   // the block's eight strips, added pairwise in a fixed order

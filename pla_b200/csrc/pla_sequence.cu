@@ -623,9 +623,10 @@ int pla_qk_norm_rotate_forward(const pla_qk_norm* a, pla_stream_t stream) {
     using T = decltype(zero);
     constexpr int CH = decltype(ch)::value, NC = decltype(nc)::value, LANES = decltype(lanes)::value;
     NormParams p = norm_params(a);
-    // four heads a group once that still leaves every SM a thousand threads
-    const bool many = tokens * (a->q.heads + a->k.heads) / 4 * LANES >= sms * 1024ll;
-    const int hb = many ? 4 : 1, groups = kNormThreads / LANES;
+    // several heads a group (64 bytes a lane in flight) once that still leaves every SM a thousand threads
+    constexpr int HB = CH == 1 ? 1 : sizeof(T) == 4 ? 2 : 4;
+    const bool many = HB > 1 && tokens * (a->q.heads + a->k.heads) / HB * LANES >= sms * 1024ll;
+    const int hb = many ? HB : 1, groups = kNormThreads / LANES;
     p.units[0] = (a->q.heads + hb - 1) / hb;
     p.units[1] = (a->k.heads + hb - 1) / hb;
     const int units = p.units[0] + p.units[1];
@@ -639,7 +640,7 @@ int pla_qk_norm_rotate_forward(const pla_qk_norm* a, pla_stream_t stream) {
     p.stride = whole <= share ? a->tokens : static_cast<int>(blocks * groups / units);
     const dim3 grid(static_cast<int>(blocks), a->batch);
     if (many)
-      qk_norm_forward<T, CH, NC, LANES, 4><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
+      qk_norm_forward<T, CH, NC, LANES, HB><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
     else
       qk_norm_forward<T, CH, NC, LANES, 1><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
     return launched("qk_norm_forward");

@@ -76,22 +76,35 @@ struct PairMap {
   }
 };
 
+// The two chunks of a lane as they lie in memory, and as pairs.
+template <typename T, int CH>
+struct RawPairs {
+  Vec<T, CH> first, second;
+};
+template <typename T, int CH>
+__device__ __forceinline__ RawPairs<T, CH> raw_pairs(const T* x, int first, int second, bool there, bool single) {
+  RawPairs<T, CH> r;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) r.first.e[i] = r.second.e[i] = down<T>(0.f);
+  if (there) r.first = *reinterpret_cast<const Vec<T, CH>*>(x + first);
+  if (there && !single) r.second = *reinterpret_cast<const Vec<T, CH>*>(x + second);
+  return r;
+}
+template <typename T, int CH>
+__device__ __forceinline__ void as_pairs(const RawPairs<T, CH>& r, bool adjacent, float (&a)[CH], float (&b)[CH]) {
+  float f[CH], s[CH];
+  unpack(r.first, f);
+  unpack(r.second, s);
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {  // adjacent: 2 CH neighbours, even ones are a, odd ones b
+    a[i] = CH > 1 && adjacent ? (2 * i < CH ? f[(2 * i) % CH] : s[(2 * i) % CH]) : f[i];
+    b[i] = CH > 1 && adjacent ? (2 * i < CH ? f[(2 * i + 1) % CH] : s[(2 * i + 1) % CH]) : s[i];
+  }
+}
 template <typename T, int CH>
 __device__ __forceinline__ void load_pairs(const T* x, int first, int second, bool adjacent, bool single, float (&a)[CH],
                                            float (&b)[CH]) {
-  float f[CH], s[CH] = {};
-  load<T, CH>(x + first, f);
-  if (!single) load<T, CH>(x + (CH == 1 && adjacent ? first + 1 : second), s);
-  if (CH > 1 && adjacent) {  // 2 CH neighbours: even ones are a, odd ones b
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      a[i] = 2 * i < CH ? f[(2 * i) % CH] : s[(2 * i) % CH];
-      b[i] = 2 * i < CH ? f[(2 * i + 1) % CH] : s[(2 * i + 1) % CH];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) a[i] = f[i], b[i] = s[i];
-  }
+  as_pairs(raw_pairs<T, CH>(x, first, second, true, single), adjacent, a, b);
 }
 
 template <typename T, int CH>
@@ -109,7 +122,7 @@ __device__ __forceinline__ void store_pairs(T* y, int first, int second, bool ad
     }
   }
   store<T, CH>(y + first, f);
-  if (!single) store<T, CH>(y + (CH == 1 && adjacent ? first + 1 : second), s);
+  if (!single) store<T, CH>(y + second, s);
 }
 
 template <int LANES>
@@ -122,6 +135,7 @@ __device__ __forceinline__ float group_sum(float v) {
 // Row of the tables for a token; -1 if the position is outside them.
 __device__ __forceinline__ long long table_row(const NormParams& p, int b, int t) {
   long long m = t;
+  if (!p.cos) return 0;
   if (p.positions) {
     const long long at = b * p.position_batch + t;
     m = p.position_bytes == 8 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
@@ -129,11 +143,11 @@ __device__ __forceinline__ long long table_row(const NormParams& p, int b, int t
   return m >= 0 && m < p.table_rows ? m : -1;
 }
 
-// A position outside the tables reads nothing: its rotated features are NaN.
+// A position outside the tables (m < 0) reads nothing: its rotated features
+// are NaN.  Features that are not rotated have cosine 1 and sine 0.
 template <int CH, int NC>
-__device__ __forceinline__ void load_angles(const NormParams& p, const PairMap<CH, NC>& map, int b, int t, float (&c)[NC][CH],
+__device__ __forceinline__ void load_angles(const NormParams& p, const PairMap<CH, NC>& map, long long m, float (&c)[NC][CH],
                                             float (&s)[NC][CH]) {
-  const long long m = p.cos ? table_row(p, b, t) : 0;
   const float nan = __int_as_float(0x7fc00000);
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
@@ -165,6 +179,7 @@ __device__ __forceinline__ void load_weight(const NormSide& side, const PairMap<
 // takes unit g % units of tokens g / units, g / units + stride, ...
 template <typename T, int CH, int NC, int LANES, int HB>
 __global__ void __launch_bounds__(kNormThreads) qk_norm_forward(NormParams p) {
+  constexpr int H = (CH + 1) / 2;
   const int lane = threadIdx.x % LANES;
   const int group = (blockIdx.x * kNormThreads + threadIdx.x) / LANES;
   const int units = p.units[0] + p.units[1], b = blockIdx.y;
@@ -179,44 +194,92 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_forward(NormParams p) {
   float wa[NC][CH], wb[NC][CH];
   load_weight<T, CH, NC>(side, map, wa, wb);
   const float per = p.l2 ? 1.f : 1.f / p.dim;
+  using Raw = RawPairs<T, CH>;
+  // heads and angles of the next token are fetched while this one's are worked on
+  Raw next[HB][NC];
+  float c_next[NC][CH], s_next[NC][CH];
+  const auto fetch = [&](int at, long long m) {
+    const T* from = x + at * side.x_token;
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        next[h][n] = raw_pairs<T, CH>(from, map.first[n], map.second[n], at < p.tokens && h < heads && map.there[n],
+                                      map.single[n]);
+      from += side.x_head;
+    }
+    load_angles<CH, NC>(p, map, m, c_next, s_next);
+  };
+  const auto position = [&](int at) { return at < p.tokens ? table_row(p, b, at) : -1ll; };
+  fetch(t, position(t));
+  long long m_next = position(t + p.stride);
   // a warp's groups make the same number of turns: all lanes shuffle
   for (int turn = __reduce_min_sync(0xffffffffu, t); turn < p.tokens; turn += p.stride, t += p.stride) {
     const bool live = t < p.tokens;
-    float xa[HB][NC][CH], xb[HB][NC][CH];
-#pragma unroll
-    for (int h = 0; h < HB; ++h)
-#pragma unroll
-      for (int n = 0; n < NC; ++n) {
-#pragma unroll
-        for (int i = 0; i < CH; ++i) xa[h][n][i] = xb[h][n][i] = 0.f;
-        if (live && h < heads && map.there[n])
-          load_pairs<T, CH>(x + t * side.x_token + h * side.x_head, map.first[n], map.second[n], map.adjacent[n], map.single[n],
-                            xa[h][n], xb[h][n]);
-      }
+    Raw raw[HB][NC];
     float c[NC][CH], s[NC][CH];
-    if (live) load_angles<CH, NC>(p, map, b, t, c, s);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int h = 0; h < HB; ++h) raw[h][n] = next[h][n];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) c[n][i] = c_next[n][i], s[n][i] = s_next[n][i];
+    }
+    if (turn + p.stride < p.tokens) {
+      fetch(t + p.stride, m_next);
+      m_next = position(t + 2 * p.stride);
+    }
+    // weights and angles together: a' = r (xa (wa cos) - xb (wb sin)), b' = r (xb (wb cos) + xa (wa sin))
+    Pair ac[NC][H], bs[NC][H], bc[NC][H], as[NC][H];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      float f[4][CH];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        f[0][i] = wa[n][i] * c[n][i];
+        f[1][i] = -wb[n][i] * s[n][i];
+        f[2][i] = wb[n][i] * c[n][i];
+        f[3][i] = wa[n][i] * s[n][i];
+      }
+      as_pair_array(f[0], ac[n]);
+      as_pair_array(f[1], bs[n]);
+      as_pair_array(f[2], bc[n]);
+      as_pair_array(f[3], as[n]);
+    }
+    T* to = y + static_cast<long long>(t) * side.heads * p.dim;
 #pragma unroll
     for (int h = 0; h < HB; ++h) {
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < NC; ++n)
-#pragma unroll
-        for (int i = 0; i < CH; ++i) sum = fmaf(xa[h][n][i], xa[h][n][i], fmaf(xb[h][n][i], xb[h][n][i], sum));
-      const float r = 1.f / sqrtf(fmaf(group_sum<LANES>(sum), per, p.eps));
-      if (!live || h >= heads) continue;
-      T* to = y + (static_cast<long long>(t) * side.heads + h) * p.dim;
+      Pair xa[NC][H], xb[NC][H], sums = pair(0.f, 0.f);
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
-        if (!map.there[n]) continue;
-        float oa[CH], ob[CH];
+        float fa[CH], fb[CH];
+        as_pairs(raw[h][n], map.adjacent[n], fa, fb);
+        as_pair_array(fa, xa[n]);
+        as_pair_array(fb, xb[n]);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {  // features that are not rotated have cos 1, sin 0
-          const float na = xa[h][n][i] * r * wa[n][i], nb = xb[h][n][i] * r * wb[n][i];
-          oa[i] = fmaf(na, c[n][i], -nb * s[n][i]);
-          ob[i] = fmaf(nb, c[n][i], na * s[n][i]);
-        }
-        store_pairs<T, CH>(to, map.first[n], map.second[n], map.adjacent[n], map.single[n], oa, ob);
+        for (int i = 0; i < H; ++i) sums = fma2(xa[n][i], xa[n][i], fma2(xb[n][i], xb[n][i], sums));
       }
+      const float2 sum = both(sums);
+      const float r = 1.f / sqrtf(fmaf(group_sum<LANES>(sum.x + sum.y), per, p.eps));
+      if (live && h < heads) {
+        const Pair rr = pair(r, r);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          if (!map.there[n]) continue;
+          Pair oa[H], ob[H];
+          float fa[CH], fb[CH];
+#pragma unroll
+          for (int i = 0; i < H; ++i) {
+            const Pair na = mul2(xa[n][i], rr), nb = mul2(xb[n][i], rr);
+            oa[i] = fma2(na, ac[n][i], mul2(nb, bs[n][i]));
+            ob[i] = fma2(nb, bc[n][i], mul2(na, as[n][i]));
+          }
+          as_float_array(oa, fa);
+          as_float_array(ob, fb);
+          store_pairs<T, CH>(to, map.first[n], map.second[n], map.adjacent[n], map.single[n], fa, fb);
+        }
+      }
+      to += p.dim;
     }
   }
 }
@@ -241,23 +304,37 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_backward(NormParams p) {
   int row = group / side.heads;  // batch row and token as one number
   const int h = group - row * side.heads;
   int b = row / p.tokens, t = row - b * p.tokens;
-  // stride[which] tokens on for every turn; a warp's groups make the same number of turns
-  for (int turn = __reduce_min_sync(0xffffffffu, row); turn < rows; turn += p.side_stride[which], row += p.side_stride[which]) {
-    const bool live = row < rows && h < side.heads;
-    float xa[NC][CH] = {}, xb[NC][CH] = {}, da[NC][CH] = {}, db[NC][CH] = {}, c[NC][CH] = {}, s[NC][CH] = {};
-    if (live) {
-      while (t >= p.tokens) t -= p.tokens, ++b;
-      const T* x = static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token + h * side.x_head;
-      const T* dy = static_cast<const T*>(side.dy) + b * side.dy_batch + t * side.dy_token + h * side.dy_head;
+  using Raw = RawPairs<T, CH>;
+  // the next token's head and angles are fetched while this one's are worked on
+  Raw x_next[NC], dy_next[NC];
+  float c_next[NC][CH], s_next[NC][CH];
+  const int stride = p.side_stride[which];
+  const auto fetch = [&](int at_row) {
+    while (t >= p.tokens) t -= p.tokens, ++b;
+    const bool in = at_row < rows;
+    const T* x = static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token + h * side.x_head;
+    const T* dy = static_cast<const T*>(side.dy) + b * side.dy_batch + t * side.dy_token + h * side.dy_head;
 #pragma unroll
-      for (int n = 0; n < NC; ++n)
-        if (map.there[n]) {
-          load_pairs<T, CH>(x, map.first[n], map.second[n], map.adjacent[n], map.single[n], xa[n], xb[n]);
-          load_pairs<T, CH>(dy, map.first[n], map.second[n], map.adjacent[n], map.single[n], da[n], db[n]);
-        }
-      load_angles<CH, NC>(p, map, b, t, c, s);
+    for (int n = 0; n < NC; ++n) {
+      x_next[n] = raw_pairs<T, CH>(x, map.first[n], map.second[n], in && map.there[n], map.single[n]);
+      dy_next[n] = raw_pairs<T, CH>(dy, map.first[n], map.second[n], in && map.there[n], map.single[n]);
     }
-    t += p.side_stride[which];
+    load_angles<CH, NC>(p, map, in ? table_row(p, b, t) : -1, c_next, s_next);
+    t += stride;
+  };
+  fetch(row);
+  // `stride` tokens on for every turn; a warp's groups make the same number of turns
+  for (int turn = __reduce_min_sync(0xffffffffu, row); turn < rows; turn += stride, row += stride) {
+    const bool live = row < rows;
+    float xa[NC][CH], xb[NC][CH], da[NC][CH], db[NC][CH], c[NC][CH], s[NC][CH];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      as_pairs(x_next[n], map.adjacent[n], xa[n], xb[n]);
+      as_pairs(dy_next[n], map.adjacent[n], da[n], db[n]);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) c[n][i] = c_next[n][i], s[n][i] = s_next[n][i];
+    }
+    if (turn + stride < rows) fetch(row + stride);
     float square = 0.f, dot = 0.f;
 #pragma unroll
     for (int n = 0; n < NC; ++n)

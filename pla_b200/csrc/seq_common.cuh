@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace pla {
 namespace seq {
 
@@ -31,16 +33,44 @@ struct alignas(sizeof(T) * V) Vec {
   T e[V];
 };
 template <typename T, int V>
-__device__ __forceinline__ void load(const T* p, float (&f)[V]) {
-  const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(p);
+__device__ __forceinline__ void unpack(const Vec<T, V>& v, float (&f)[V]) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {  // two at a time, from whole registers
 #pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = up(v.e[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      const uint32_t r = reinterpret_cast<const uint32_t*>(v.e)[i];
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f[2 * i] = __uint_as_float(r << 16);
+        f[2 * i + 1] = __uint_as_float(r & 0xffff0000u);
+      } else {
+        const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        f[2 * i] = g.x;
+        f[2 * i + 1] = g.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = up(v.e[i]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void load(const T* p, float (&f)[V]) {
+  unpack(*reinterpret_cast<const Vec<T, V>*>(p), f);
 }
 template <typename T, int V>
 __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
   Vec<T, V> v;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) v.e[i] = down<T>(f[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        reinterpret_cast<__nv_bfloat162*>(v.e)[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      else
+        reinterpret_cast<__half2*>(v.e)[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v.e[i] = down<T>(f[i]);
+  }
   *reinterpret_cast<Vec<T, V>*>(p) = v;
 }
 
@@ -63,6 +93,32 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   Pair d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return d;
+}
+
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+// V values as (V + 1) / 2 pairs (a zero behind an odd one) and back.
+template <int V>
+__device__ __forceinline__ void as_pair_array(const float (&f)[V], Pair (&p)[(V + 1) / 2]) {
+#pragma unroll
+  for (int i = 0; i < (V + 1) / 2; ++i) p[i] = pair(f[2 * i], 2 * i + 1 < V ? f[(2 * i + 1) % V] : 0.f);
+}
+template <int V>
+__device__ __forceinline__ void as_float_array(const Pair (&p)[(V + 1) / 2], float (&f)[V]) {
+#pragma unroll
+  for (int i = 0; i < (V + 1) / 2; ++i) {
+    const float2 g = both(p[i]);
+    f[2 * i] = g.x;
+    if (2 * i + 1 < V) f[(2 * i + 1) % V] = g.y;
+  }
 }
 
 // 1 / (1 + e^-p).  16-bit results take the hardware's 2^x and reciprocal (2^-22
