@@ -241,17 +241,20 @@ bool norm_vector(const pla_qk_norm* a, bool backward) {
   return true;
 }
 
-// f(element type, CH, NC, LANES): 4 pairs a lane where rows allow it, else
-// single pairs, the group as small as holds a head.
+// f(element type, lanes of a head, pairs adjacent): the group as small as holds
+// a head at 4 pairs a lane.
 template <typename F>
-int with_norm(const pla_qk_norm* a, bool wide, F&& f) {
+int with_norm4(const pla_qk_norm* a, F&& f) {
   return with_type(a->dtype, [&](auto zero) {
-    if (!wide) return f(zero, Int<1>{}, Int<4>{}, Int<32>{});
-    if (a->dim <= 64) return f(zero, Int<4>{}, Int<1>{}, Int<8>{});
-    if (a->dim <= 128) return f(zero, Int<4>{}, Int<1>{}, Int<16>{});
-    return f(zero, Int<4>{}, Int<1>{}, Int<32>{});
+    const auto lanes = [&](auto inter) {
+      if (a->dim <= 64) return f(zero, Int<8>{}, inter);
+      if (a->dim <= 128) return f(zero, Int<16>{}, inter);
+      return f(zero, Int<32>{}, inter);
+    };
+    return a->interleaved && a->rot ? lanes(std::true_type{}) : lanes(std::false_type{});
   });
 }
+int norm_lanes(const pla_qk_norm* a, bool wide) { return !wide || a->dim > 128 ? 32 : a->dim > 64 ? 16 : 8; }
 
 // Blocks of one side in the backward pass: a number of groups that is a
 // multiple of the heads (a group keeps its head), a few turns each so that a
@@ -617,33 +620,40 @@ int pla_qk_norm_rotate_forward(const pla_qk_norm* a, pla_stream_t stream) {
   if (st != PLA_OK) return st;
   const long long tokens = static_cast<long long>(a->batch) * a->tokens;
   if (!tokens || !a->dim || !(a->q.heads + a->k.heads)) return PLA_OK;
+  if (a->batch > 65535) return PLA_ERR_TOO_LARGE;
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
-  return with_norm(a, norm_vector(a, false), [&](auto zero, auto ch, auto nc, auto lanes) {
+  const bool wide = norm_vector(a, false);
+  const int lanes = norm_lanes(a, wide), groups = kNormThreads / lanes;
+  // several heads a group (64 bytes a lane in flight) once that still leaves every SM a thousand threads
+  const int most = !wide ? 1 : a->dtype == PLA_F32 ? 2 : 4;
+  const int hb = most > 1 && tokens * (a->q.heads + a->k.heads) / most * lanes >= sms * 1024ll ? most : 1;
+  NormParams p = norm_params(a);
+  p.units[0] = (a->q.heads + hb - 1) / hb;
+  p.units[1] = (a->k.heads + hb - 1) / hb;
+  const int units = p.units[0] + p.units[1];
+  // a few times the blocks that the device holds at a time, each group walking tokens
+  const long long whole = (static_cast<long long>(a->tokens) * units + groups - 1) / groups;
+  const long long share = std::max<long long>(1, sms * 8ll / a->batch);
+  // a number of groups that is a multiple of the units, so that a group keeps its unit
+  const int step = units / std::gcd(units, groups);
+  const long long blocks = whole <= share ? whole : (share + step - 1) / step * step;
+  p.stride = whole <= share ? a->tokens : static_cast<int>(blocks * groups / units);
+  const dim3 grid(static_cast<int>(blocks), a->batch);
+  if (!wide)
+    return with_type(a->dtype, [&](auto zero) {
+      qk_norm_forward1<decltype(zero)><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
+      return launched("qk_norm_forward1");
+    });
+  return with_norm4(a, [&](auto zero, auto l, auto inter) {
     using T = decltype(zero);
-    constexpr int CH = decltype(ch)::value, NC = decltype(nc)::value, LANES = decltype(lanes)::value;
-    NormParams p = norm_params(a);
-    // several heads a group (64 bytes a lane in flight) once that still leaves every SM a thousand threads
-    constexpr int HB = CH == 1 ? 1 : sizeof(T) == 4 ? 2 : 4;
-    const bool many = HB > 1 && tokens * (a->q.heads + a->k.heads) / HB * LANES >= sms * 1024ll;
-    const int hb = many ? HB : 1, groups = kNormThreads / LANES;
-    p.units[0] = (a->q.heads + hb - 1) / hb;
-    p.units[1] = (a->k.heads + hb - 1) / hb;
-    const int units = p.units[0] + p.units[1];
-    // as many blocks as the device holds at a time, each group walking tokens
-    const long long whole = (static_cast<long long>(a->tokens) * units + groups - 1) / groups;
-    const long long share = std::max<long long>(1, sms * 6ll / std::max(1, a->batch));
-    // a number of groups that is a multiple of the units, so that a group keeps its unit
-    const int step = units / std::gcd(units, groups);
-    const long long blocks = whole <= share ? whole : (share + step - 1) / step * step;
-    if (a->batch > 65535) return static_cast<int>(PLA_ERR_TOO_LARGE);
-    p.stride = whole <= share ? a->tokens : static_cast<int>(blocks * groups / units);
-    const dim3 grid(static_cast<int>(blocks), a->batch);
-    if (many)
-      qk_norm_forward<T, CH, NC, LANES, HB><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
+    constexpr int LANES = decltype(l)::value, HB = sizeof(T) == 4 ? 2 : 4;
+    constexpr bool INTER = decltype(inter)::value;
+    if (hb > 1)
+      qk_norm_forward4<T, LANES, HB, INTER><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
     else
-      qk_norm_forward<T, CH, NC, LANES, 1><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
-    return launched("qk_norm_forward");
+      qk_norm_forward4<T, LANES, 1, INTER><<<grid, kNormThreads, 0, as_stream(stream)>>>(p);
+    return launched("qk_norm_forward4");
   });
 }
 
@@ -669,29 +679,35 @@ int pla_qk_norm_rotate_backward(const pla_qk_norm* a, void* workspace, size_t wo
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
   const bool wide = norm_vector(a, true);
-  return with_norm(a, wide, [&](auto zero, auto ch, auto nc, auto lanes) {
-    using T = decltype(zero);
-    constexpr int CH = decltype(ch)::value, NC = decltype(nc)::value, LANES = decltype(lanes)::value;
-    NormParams p = norm_params(a);
-    p.partial = sums ? static_cast<float*>(workspace) : nullptr;
-    for (int i = 0; i < 2; ++i) {
-      const int heads = i ? a->k.heads : a->q.heads, groups = kNormThreads / LANES;
-      p.side_blocks[i] = norm_side_blocks(a, heads, LANES);
-      p.side_stride[i] = heads ? p.side_blocks[i] * groups / heads : 1;
-    }
-    int st = PLA_OK;
-    if (p.side_blocks[0] + p.side_blocks[1] > 0) {
-      qk_norm_backward<T, CH, NC, LANES>
-          <<<p.side_blocks[0] + p.side_blocks[1], kNormThreads, 0, as_stream(stream)>>>(p);
-      if ((st = launched("qk_norm_backward")) != PLA_OK) return st;
-    }
-    if (sums) {
-      qk_norm_reduce<T><<<dim3((a->dim + 31) / 32, 2), 256, 0, as_stream(stream)>>>(
+  const int lanes = norm_lanes(a, wide);
+  NormParams p = norm_params(a);
+  p.partial = sums ? static_cast<float*>(workspace) : nullptr;
+  for (int i = 0; i < 2; ++i) {
+    const int heads = i ? a->k.heads : a->q.heads;
+    p.side_blocks[i] = norm_side_blocks(a, heads, lanes);
+    p.side_stride[i] = heads ? p.side_blocks[i] * (kNormThreads / lanes) / heads : 1;
+  }
+  const int blocks = p.side_blocks[0] + p.side_blocks[1];
+  if (blocks > 0) {
+    st = !wide ? with_type(a->dtype, [&](auto zero) {
+      qk_norm_backward1<decltype(zero)><<<blocks, kNormThreads, 0, as_stream(stream)>>>(p);
+      return launched("qk_norm_backward1");
+    })
+               : with_norm4(a, [&](auto zero, auto l, auto inter) {
+      qk_norm_backward4<decltype(zero), decltype(l)::value, decltype(inter)::value>
+          <<<blocks, kNormThreads, 0, as_stream(stream)>>>(p);
+      return launched("qk_norm_backward4");
+    });
+    if (st != PLA_OK) return st;
+  }
+  if (sums)
+    st = with_type(a->dtype, [&](auto zero) {
+      using T = decltype(zero);
+      qk_norm_reduce<T><<<dim3((a->dim + 31) / 32, 2), 1024, 0, as_stream(stream)>>>(
           p.partial, p.side_blocks[0], p.side_blocks[1], a->dim, static_cast<T*>(a->q.dw), static_cast<T*>(a->k.dw));
-      st = launched("qk_norm_reduce");
-    }
-    return st;
-  });
+      return launched("qk_norm_reduce");
+    });
+  return st;
 }
 
 size_t pla_gated_delta_rule_workspace(const pla_delta* a, int backward) {

@@ -52,77 +52,93 @@ struct NormParams {
   int side_blocks[2], side_stride[2];
 };
 
-// A lane's NC chunks of CH pairs of a head's features.  CH = 4 needs rot / 2
-// and (D - rot) / 2 to be multiples of 4 and 16-byte rows; CH = 1 takes any D.
-template <int CH, int NC>
-struct PairMap {
-  int first[NC], second[NC];  // first feature of each chunk's a and b parts
-  bool turned[NC], there[NC], adjacent[NC], single[NC];
-  int angle[NC];
-  __device__ __forceinline__ PairMap(int lane, int lanes, int D, int rot, int interleaved) {
-    const int half = rot >> 1, rest = D - rot, rest_half = rest >> 1;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      const int p = (n * lanes + lane) * CH;  // pair number
-      turned[n] = p < half;
-      adjacent[n] = turned[n] && interleaved;
-      angle[n] = p;
-      const int q = p - half;
-      single[n] = CH == 1 && !turned[n] && q == rest_half && (rest & 1);  // CH = 4: never
-      there[n] = turned[n] || q < rest_half || single[n];
-      first[n] = turned[n] ? (interleaved ? 2 * p : p) : (single[n] ? D - 1 : rot + q);
-      second[n] = turned[n] ? (interleaved ? 2 * p + CH : p + half) : rot + rest_half + q;
-    }
+// Rows whose parts are multiples of 4 pairs, at addresses that allow it: a
+// lane holds 4 pairs, that is two groups of 4 features, `first` and `second`
+// (2 x 4 neighbours if their pairs are adjacent).  Lanes without pairs (heads
+// that do not fill the group) read what lane 0 reads and count it as 0.
+struct Lane4 {
+  int first, second, angle;
+  bool turned, there, adjacent;
+  __device__ __forceinline__ Lane4(int lane, int D, int rot, bool interleaved) {
+    const int half = rot >> 1, rest_half = (D - rot) >> 1;
+    there = lane * 4 < D / 2;
+    const int p = there ? lane * 4 : 0, q = p - half;
+    turned = p < half;
+    adjacent = turned && interleaved;
+    angle = p;
+    first = turned ? (interleaved ? 2 * p : p) : rot + q;
+    second = turned ? (interleaved ? 2 * p + 4 : p + half) : rot + rest_half + q;
   }
 };
-
-// The two chunks of a lane as they lie in memory, and as pairs.
-template <typename T, int CH>
-struct RawPairs {
-  Vec<T, CH> first, second;
+template <typename T>
+struct Raw4 {
+  Vec<T, 4> first, second;
 };
-template <typename T, int CH>
-__device__ __forceinline__ RawPairs<T, CH> raw_pairs(const T* x, int first, int second, bool there, bool single) {
-  RawPairs<T, CH> r;
-#pragma unroll
-  for (int i = 0; i < CH; ++i) r.first.e[i] = r.second.e[i] = down<T>(0.f);
-  if (there) r.first = *reinterpret_cast<const Vec<T, CH>*>(x + first);
-  if (there && !single) r.second = *reinterpret_cast<const Vec<T, CH>*>(x + second);
-  return r;
+template <typename T>
+__device__ __forceinline__ Raw4<T> raw4(const T* x, const Lane4& l) {
+  return {*reinterpret_cast<const Vec<T, 4>*>(x + l.first), *reinterpret_cast<const Vec<T, 4>*>(x + l.second)};
 }
-template <typename T, int CH>
-__device__ __forceinline__ void as_pairs(const RawPairs<T, CH>& r, bool adjacent, float (&a)[CH], float (&b)[CH]) {
-  float f[CH], s[CH];
+// Pairs (a, b) as two packed values each.  INTER: some lanes' pairs are adjacent.
+template <bool INTER>
+__device__ __forceinline__ void pairs_of(const float (&f)[4], const float (&s)[4], bool adjacent, Pair (&a)[2], Pair (&b)[2]) {
+  a[0] = pair(f[0], INTER && adjacent ? f[2] : f[1]);
+  a[1] = pair(INTER && adjacent ? s[0] : f[2], INTER && adjacent ? s[2] : f[3]);
+  b[0] = pair(INTER && adjacent ? f[1] : s[0], INTER && adjacent ? f[3] : s[1]);
+  b[1] = pair(INTER && adjacent ? s[1] : s[2], s[3]);
+}
+template <typename T, bool INTER>
+__device__ __forceinline__ void unpack4(const Raw4<T>& r, const Lane4& l, Pair (&a)[2], Pair (&b)[2]) {
+  float f[4], s[4];
   unpack(r.first, f);
   unpack(r.second, s);
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {  // adjacent: 2 CH neighbours, even ones are a, odd ones b
-    a[i] = CH > 1 && adjacent ? (2 * i < CH ? f[(2 * i) % CH] : s[(2 * i) % CH]) : f[i];
-    b[i] = CH > 1 && adjacent ? (2 * i < CH ? f[(2 * i + 1) % CH] : s[(2 * i + 1) % CH]) : s[i];
-  }
+  pairs_of<INTER>(f, s, l.adjacent, a, b);
 }
-template <typename T, int CH>
-__device__ __forceinline__ void load_pairs(const T* x, int first, int second, bool adjacent, bool single, float (&a)[CH],
-                                           float (&b)[CH]) {
-  as_pairs(raw_pairs<T, CH>(x, first, second, true, single), adjacent, a, b);
+template <typename T, bool INTER>
+__device__ __forceinline__ void store4(T* y, const Lane4& l, const Pair (&a)[2], const Pair (&b)[2]) {
+  float fa[4], fb[4], f[4], s[4];
+  as_float_array(a, fa);
+  as_float_array(b, fb);
+  const bool adjacent = INTER && l.adjacent;
+  f[0] = fa[0], f[1] = adjacent ? fb[0] : fa[1], f[2] = adjacent ? fa[1] : fa[2], f[3] = adjacent ? fb[1] : fa[3];
+  s[0] = adjacent ? fa[2] : fb[0], s[1] = adjacent ? fb[2] : fb[1], s[2] = adjacent ? fa[3] : fb[2], s[3] = fb[3];
+  store<T, 4>(y + l.first, f);
+  store<T, 4>(y + l.second, s);
 }
 
-template <typename T, int CH>
-__device__ __forceinline__ void store_pairs(T* y, int first, int second, bool adjacent, bool single, const float (&a)[CH],
-                                            const float (&b)[CH]) {
-  float f[CH], s[CH];
+// Any other row: a lane of 32 holds every 32nd pair, and an odd last feature
+// as the first of a pair.
+struct Lane1 {
+  int first[4], second[4], angle[4];
+  bool turned[4], there[4], single[4];
+  __device__ __forceinline__ Lane1(int lane, int D, int rot, bool interleaved) {
+    const int half = rot >> 1, rest = D - rot, rest_half = rest >> 1;
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    if (CH > 1 && adjacent) {
-      f[i] = i % 2 == 0 ? a[i / 2] : b[i / 2];
-      s[i] = i % 2 == 0 ? a[(CH + i) / 2] : b[(CH + i) / 2];
-    } else {
-      f[i] = a[i];
-      s[i] = b[i];
+    for (int n = 0; n < 4; ++n) {
+      const int p = n * 32 + lane, q = p - half;
+      turned[n] = p < half;
+      angle[n] = p;
+      single[n] = !turned[n] && q == rest_half && (rest & 1);
+      there[n] = turned[n] || q < rest_half || single[n];
+      first[n] = turned[n] ? (interleaved ? 2 * p : p) : (single[n] ? D - 1 : rot + q);
+      second[n] = turned[n] ? (interleaved ? 2 * p + 1 : p + half) : rot + rest_half + q;
     }
   }
-  store<T, CH>(y + first, f);
-  if (!single) store<T, CH>(y + second, s);
+};
+template <typename T>
+__device__ __forceinline__ void load1(const T* x, const Lane1& l, float (&a)[4], float (&b)[4]) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    a[n] = l.there[n] ? up(x[l.first[n]]) : 0.f;
+    b[n] = l.there[n] && !l.single[n] ? up(x[l.second[n]]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store1(T* y, const Lane1& l, const float (&a)[4], const float (&b)[4]) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    if (l.there[n]) y[l.first[n]] = down<T>(a[n]);
+    if (l.there[n] && !l.single[n]) y[l.second[n]] = down<T>(b[n]);
+  }
 }
 
 template <int LANES>
@@ -130,6 +146,16 @@ __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
   for (int o = LANES / 2; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// 1 / sqrt(v): the hardware's approximation (2^-22) and one Newton step, which
+// leaves a few units of the last place.  No branch, so that the heads of a
+// group overlap (1.f / sqrtf(v) has two; with them 8192 tokens of 40 heads of
+// 128 in bf16 took 56 us, against NORMFWD).
+__device__ __forceinline__ float inverse_root(float v) {
+  const float r = rsqrtf(v);
+  const float better = r * fmaf(-0.5f * v * r, r, 1.5f);
+  return v > 0.f && v < __int_as_float(0x7f800000) ? better : r;
 }
 
 // Row of the tables for a token; -1 if the position is outside them.
@@ -145,256 +171,311 @@ __device__ __forceinline__ long long table_row(const NormParams& p, int b, int t
 
 // A position outside the tables (m < 0) reads nothing: its rotated features
 // are NaN.  Features that are not rotated have cosine 1 and sine 0.
-template <int CH, int NC>
-__device__ __forceinline__ void load_angles(const NormParams& p, const PairMap<CH, NC>& map, long long m, float (&c)[NC][CH],
-                                            float (&s)[NC][CH]) {
+__device__ __forceinline__ void angles4(const NormParams& p, const Lane4& l, long long m, float (&c)[4], float (&s)[4]) {
   const float nan = __int_as_float(0x7fc00000);
+  if (l.turned && m >= 0) {
+    load<float, 4>(p.cos + m * (p.rot >> 1) + l.angle, c);
+    load<float, 4>(p.sin + m * (p.rot >> 1) + l.angle, s);
+  } else {
 #pragma unroll
-  for (int n = 0; n < NC; ++n) {
+    for (int i = 0; i < 4; ++i) c[i] = l.turned ? nan : 1.f, s[i] = l.turned ? nan : 0.f;
+  }
+}
+__device__ __forceinline__ void angles1(const NormParams& p, const Lane1& l, long long m, float (&c)[4], float (&s)[4]) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) c[n][i] = map.turned[n] ? nan : 1.f, s[n][i] = map.turned[n] ? nan : 0.f;
-    if (map.turned[n] && m >= 0) {
-      load<float, CH>(p.cos + m * (p.rot >> 1) + map.angle[n], c[n]);
-      load<float, CH>(p.sin + m * (p.rot >> 1) + map.angle[n], s[n]);
+  for (int n = 0; n < 4; ++n) {
+    c[n] = 1.f, s[n] = 0.f;
+    if (l.turned[n]) c[n] = s[n] = __int_as_float(0x7fc00000);
+    if (l.turned[n] && m >= 0) {
+      c[n] = p.cos[m * (p.rot >> 1) + l.angle[n]];
+      s[n] = p.sin[m * (p.rot >> 1) + l.angle[n]];
     }
   }
 }
 
 constexpr int kNormThreads = 256;
 
-// A lane's parts of a weight; ones without.
-template <typename T, int CH, int NC>
-__device__ __forceinline__ void load_weight(const NormSide& side, const PairMap<CH, NC>& map, float (&wa)[NC][CH], float (&wb)[NC][CH]) {
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) wa[n][i] = wb[n][i] = 1.f;
-    if (side.w && map.there[n])
-      load_pairs<T, CH>(static_cast<const T*>(side.w), map.first[n], map.second[n], map.adjacent[n], map.single[n], wa[n],
-                        wb[n]);
-  }
-}
-
 // blockIdx.y: batch row.  The groups of the grid's row are numbered; group g
-// takes unit g % units of tokens g / units, g / units + stride, ...
-template <typename T, int CH, int NC, int LANES, int HB>
-__global__ void __launch_bounds__(kNormThreads) qk_norm_forward(NormParams p) {
-  constexpr int H = (CH + 1) / 2;
-  const int lane = threadIdx.x % LANES;
+// takes unit g % units (HB heads of one side) of tokens g / units,
+// g / units + stride, ...  The next token's heads and angles are fetched while
+// this one's are worked on.
+template <typename T, int LANES, int HB, bool INTER>
+__global__ void __launch_bounds__(kNormThreads) qk_norm_forward4(NormParams p) {
   const int group = (blockIdx.x * kNormThreads + threadIdx.x) / LANES;
   const int units = p.units[0] + p.units[1], b = blockIdx.y;
   int t = group / units, unit = group - t * units;
   const int which = unit >= p.units[0];
   if (which) unit -= p.units[0];
   const NormSide& side = p.side[which];
-  const PairMap<CH, NC> map(lane, LANES, p.dim, p.rot, p.interleaved);
-  const int h0 = unit * HB, heads = min(HB, side.heads - h0);
+  const Lane4 lane(threadIdx.x % LANES, p.dim, p.rot, INTER);
+  const int h0 = unit * HB, heads = min(HB, side.heads - h0), end = p.tokens, stride = p.stride;
   const T* x = static_cast<const T*>(side.x) + b * side.x_batch + h0 * side.x_head;
-  T* y = static_cast<T*>(side.y) + (static_cast<long long>(b) * p.tokens * side.heads + h0) * p.dim;
-  float wa[NC][CH], wb[NC][CH];
-  load_weight<T, CH, NC>(side, map, wa, wb);
-  const float per = p.l2 ? 1.f : 1.f / p.dim;
-  using Raw = RawPairs<T, CH>;
-  // heads and angles of the next token are fetched while this one's are worked on
-  Raw next[HB][NC];
-  float c_next[NC][CH], s_next[NC][CH];
+  const long long x_token = side.x_token, y_token = static_cast<long long>(side.heads) * p.dim;
+  T* y = static_cast<T*>(side.y) + b * (p.tokens * y_token) + static_cast<long long>(h0) * p.dim;
+  Pair wa[2], wb[2];
+  {
+    float f[4] = {1.f, 1.f, 1.f, 1.f}, g[4] = {1.f, 1.f, 1.f, 1.f};
+    if (side.w) {
+      load<T, 4>(static_cast<const T*>(side.w) + lane.first, f);
+      load<T, 4>(static_cast<const T*>(side.w) + lane.second, g);
+    }
+    pairs_of<INTER>(f, g, lane.adjacent, wa, wb);
+  }
+  const float per = p.l2 ? 1.f : 1.f / p.dim, counted = lane.there ? 1.f : 0.f;
+  Raw4<T> next[HB];
+  float c_next[4], s_next[4];
+  // past the end the last token, and past the heads the last head, are fetched again
   const auto fetch = [&](int at, long long m) {
-    const T* from = x + at * side.x_token;
+    const T* from = x + min(at, end - 1) * x_token;
 #pragma unroll
-    for (int h = 0; h < HB; ++h) {
-#pragma unroll
-      for (int n = 0; n < NC; ++n)
-        next[h][n] = raw_pairs<T, CH>(from, map.first[n], map.second[n], at < p.tokens && h < heads && map.there[n],
-                                      map.single[n]);
-      from += side.x_head;
-    }
-    load_angles<CH, NC>(p, map, m, c_next, s_next);
+    for (int h = 0; h < HB; ++h) next[h] = raw4(from + min(h, heads - 1) * side.x_head, lane);
+    angles4(p, lane, m, c_next, s_next);
   };
-  const auto position = [&](int at) { return at < p.tokens ? table_row(p, b, at) : -1ll; };
-  fetch(t, position(t));
-  long long m_next = position(t + p.stride);
+  fetch(t, table_row(p, b, min(t, end - 1)));
+  long long m_next = table_row(p, b, min(t + stride, end - 1));
   // a warp's groups make the same number of turns: all lanes shuffle
-  for (int turn = __reduce_min_sync(0xffffffffu, t); turn < p.tokens; turn += p.stride, t += p.stride) {
-    const bool live = t < p.tokens;
-    Raw raw[HB][NC];
-    float c[NC][CH], s[NC][CH];
+  for (int turn = __reduce_min_sync(0xffffffffu, t); turn < end; turn += stride, t += stride) {
+    Pair ac[2], bs[2], bc[2], as[2];  // a' = r (xa (wa cos) - xb (wb sin)), b' = r (xb (wb cos) + xa (wa sin))
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-#pragma unroll
-      for (int h = 0; h < HB; ++h) raw[h][n] = next[h][n];
-#pragma unroll
-      for (int i = 0; i < CH; ++i) c[n][i] = c_next[n][i], s[n][i] = s_next[n][i];
+    for (int i = 0; i < 2; ++i) {
+      const Pair c = pair(c_next[2 * i], c_next[2 * i + 1]), s = pair(s_next[2 * i], s_next[2 * i + 1]);
+      ac[i] = mul2(wa[i], c), bc[i] = mul2(wb[i], c), as[i] = mul2(wa[i], s);
+      bs[i] = mul2(mul2(wb[i], s), pair(-1.f, -1.f));
     }
-    if (turn + p.stride < p.tokens) {
-      fetch(t + p.stride, m_next);
-      m_next = position(t + 2 * p.stride);
-    }
-    // weights and angles together: a' = r (xa (wa cos) - xb (wb sin)), b' = r (xb (wb cos) + xa (wa sin))
-    Pair ac[NC][H], bs[NC][H], bc[NC][H], as[NC][H];
+    Raw4<T> raw[HB];
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      float f[4][CH];
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        f[0][i] = wa[n][i] * c[n][i];
-        f[1][i] = -wb[n][i] * s[n][i];
-        f[2][i] = wb[n][i] * c[n][i];
-        f[3][i] = wa[n][i] * s[n][i];
-      }
-      as_pair_array(f[0], ac[n]);
-      as_pair_array(f[1], bs[n]);
-      as_pair_array(f[2], bc[n]);
-      as_pair_array(f[3], as[n]);
+    for (int h = 0; h < HB; ++h) raw[h] = next[h];
+    if (turn + stride < end) {
+      fetch(t + stride, m_next);
+      m_next = table_row(p, b, min(t + 2 * stride, end - 1));
     }
-    T* to = y + static_cast<long long>(t) * side.heads * p.dim;
+    Pair xa[HB][2], xb[HB][2];
+    float sum[HB];
 #pragma unroll
     for (int h = 0; h < HB; ++h) {
-      Pair xa[NC][H], xb[NC][H], sums = pair(0.f, 0.f);
+      unpack4<T, INTER>(raw[h], lane, xa[h], xb[h]);
+      const float2 f = both(fma2(xa[h][0], xa[h][0], fma2(xb[h][0], xb[h][0], fma2(xa[h][1], xa[h][1], mul2(xb[h][1], xb[h][1])))));
+      sum[h] = (f.x + f.y) * counted;
+    }
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        float fa[CH], fb[CH];
-        as_pairs(raw[h][n], map.adjacent[n], fa, fb);
-        as_pair_array(fa, xa[n]);
-        as_pair_array(fb, xb[n]);
+    for (int o = LANES / 2; o >= 1; o >>= 1)
 #pragma unroll
-        for (int i = 0; i < H; ++i) sums = fma2(xa[n][i], xa[n][i], fma2(xb[n][i], xb[n][i], sums));
+      for (int h = 0; h < HB; ++h) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
+    T* to = y + t * y_token;
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+      const float r = inverse_root(fmaf(sum[h], per, p.eps));
+      const Pair rr = pair(r, r);
+      Pair oa[2], ob[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Pair na = mul2(xa[h][i], rr), nb = mul2(xb[h][i], rr);
+        oa[i] = fma2(na, ac[i], mul2(nb, bs[i]));
+        ob[i] = fma2(nb, bc[i], mul2(na, as[i]));
       }
-      const float2 sum = both(sums);
-      const float r = 1.f / sqrtf(fmaf(group_sum<LANES>(sum.x + sum.y), per, p.eps));
-      if (live && h < heads) {
-        const Pair rr = pair(r, r);
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-          if (!map.there[n]) continue;
-          Pair oa[H], ob[H];
-          float fa[CH], fb[CH];
-#pragma unroll
-          for (int i = 0; i < H; ++i) {
-            const Pair na = mul2(xa[n][i], rr), nb = mul2(xb[n][i], rr);
-            oa[i] = fma2(na, ac[n][i], mul2(nb, bs[n][i]));
-            ob[i] = fma2(nb, bc[n][i], mul2(na, as[n][i]));
-          }
-          as_float_array(oa, fa);
-          as_float_array(ob, fb);
-          store_pairs<T, CH>(to, map.first[n], map.second[n], map.adjacent[n], map.single[n], fa, fb);
-        }
-      }
+      if (t < end && h < heads && lane.there) store4<T, INTER>(to, lane, oa, ob);
       to += p.dim;
     }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads) qk_norm_forward1(NormParams p) {
+  const int group = (blockIdx.x * kNormThreads + threadIdx.x) / 32;
+  const int units = p.units[0] + p.units[1], b = blockIdx.y;
+  int t = group / units, unit = group - t * units;
+  const int which = unit >= p.units[0];
+  if (which) unit -= p.units[0];
+  const NormSide& side = p.side[which];
+  const Lane1 lane(threadIdx.x & 31, p.dim, p.rot, p.interleaved);
+  float wa[4] = {1.f, 1.f, 1.f, 1.f}, wb[4] = {1.f, 1.f, 1.f, 1.f};
+  if (side.w) load1(static_cast<const T*>(side.w), lane, wa, wb);
+  const float per = p.l2 ? 1.f : 1.f / p.dim;
+  for (; t < p.tokens; t += p.stride) {
+    float a[4], c4[4], b4[4], s4[4];
+    load1(static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token + unit * side.x_head, lane, a, b4);
+    angles1(p, lane, table_row(p, b, t), c4, s4);
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) sum = fmaf(a[n], a[n], fmaf(b4[n], b4[n], sum));
+    const float r = inverse_root(fmaf(group_sum<32>(sum), per, p.eps));
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const float na = a[n] * r * wa[n], nb = b4[n] * r * wb[n];
+      a[n] = lane.turned[n] ? fmaf(na, c4[n], -nb * s4[n]) : na;
+      b4[n] = lane.turned[n] ? fmaf(nb, c4[n], na * s4[n]) : nb;
+    }
+    store1(static_cast<T*>(side.y) + ((static_cast<long long>(b) * p.tokens + t) * side.heads + unit) * p.dim, lane, a, b4);
   }
 }
 
 // dx, and the block's sums for dw.  A block works on one side: its groups walk
 // tokens with one head each and dw in registers, and are added in shared
 // memory, the blocks in qk_norm_reduce, all in a fixed order.
-template <typename T, int CH, int NC, int LANES>
-__global__ void __launch_bounds__(kNormThreads) qk_norm_backward(NormParams p) {
-  constexpr int GROUPS = kNormThreads / LANES;
-  __shared__ float part[GROUPS][2 * CH * NC][LANES + 1];
+template <int GROUPS, int LANES>
+__device__ __forceinline__ void block_weight_sums(const NormParams& p, float (&ga)[4], float (&gb)[4], float (*part)[8][LANES + 1],
+                                                  float (&a)[4], float (&b)[4]) {
   const int lane = threadIdx.x % LANES, in_block = threadIdx.x / LANES;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    part[in_block][2 * i][lane] = ga[i];
+    part[in_block][2 * i + 1][lane] = gb[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = b[i] = 0.f;
+  if (in_block) return;
+  for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] += part[g][2 * i][lane];
+      b[i] += part[g][2 * i + 1][lane];
+    }
+}
+
+template <typename T, int LANES, bool INTER>
+__global__ void __launch_bounds__(kNormThreads) qk_norm_backward4(NormParams p) {
+  constexpr int GROUPS = kNormThreads / LANES;
+  __shared__ float part[GROUPS][8][LANES + 1];
+  const int in_block = threadIdx.x / LANES;
   const int which = static_cast<int>(blockIdx.x) >= p.side_blocks[0];
   const NormSide& side = p.side[which];
   const int block = which ? blockIdx.x - p.side_blocks[0] : blockIdx.x;
-  const PairMap<CH, NC> map(lane, LANES, p.dim, p.rot, p.interleaved);
-  float wa[NC][CH], wb[NC][CH], ga[NC][CH] = {}, gb[NC][CH] = {};
-  load_weight<T, CH, NC>(side, map, wa, wb);
-  const float per = p.l2 ? 1.f : 1.f / p.dim;
-  const int rows = p.batch * p.tokens;  // below 2^31
+  const Lane4 lane(threadIdx.x % LANES, p.dim, p.rot, INTER);
+  Pair wa[2], wb[2], ga[2], gb[2];
+  ga[0] = ga[1] = gb[0] = gb[1] = pair(0.f, 0.f);
+  {
+    float f[4] = {1.f, 1.f, 1.f, 1.f}, g[4] = {1.f, 1.f, 1.f, 1.f};
+    if (side.w) {
+      load<T, 4>(static_cast<const T*>(side.w) + lane.first, f);
+      load<T, 4>(static_cast<const T*>(side.w) + lane.second, g);
+    }
+    pairs_of<INTER>(f, g, lane.adjacent, wa, wb);
+  }
+  const float per = p.l2 ? 1.f : 1.f / p.dim, counted = lane.there ? 1.f : 0.f;
+  const int rows = p.batch * p.tokens, stride = p.side_stride[which];  // rows below 2^30
   const int group = block * GROUPS + in_block;
   int row = group / side.heads;  // batch row and token as one number
   const int h = group - row * side.heads;
   int b = row / p.tokens, t = row - b * p.tokens;
-  using Raw = RawPairs<T, CH>;
-  // the next token's head and angles are fetched while this one's are worked on
-  Raw x_next[NC], dy_next[NC];
-  float c_next[NC][CH], s_next[NC][CH];
-  const int stride = p.side_stride[which];
+  const T* x = static_cast<const T*>(side.x) + h * side.x_head;
+  const T* dy = static_cast<const T*>(side.dy) + h * side.dy_head;
+  // the next token's head and angles are fetched while this one's are worked on; past the end, the first's
+  Raw4<T> x_next, dy_next;
+  float c_next[4], s_next[4];
   const auto fetch = [&](int at_row) {
     while (t >= p.tokens) t -= p.tokens, ++b;
-    const bool in = at_row < rows;
-    const T* x = static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token + h * side.x_head;
-    const T* dy = static_cast<const T*>(side.dy) + b * side.dy_batch + t * side.dy_token + h * side.dy_head;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      x_next[n] = raw_pairs<T, CH>(x, map.first[n], map.second[n], in && map.there[n], map.single[n]);
-      dy_next[n] = raw_pairs<T, CH>(dy, map.first[n], map.second[n], in && map.there[n], map.single[n]);
-    }
-    load_angles<CH, NC>(p, map, in ? table_row(p, b, t) : -1, c_next, s_next);
+    const int bb = at_row < rows ? b : 0, tt = at_row < rows ? t : 0;
+    x_next = raw4(x + bb * side.x_batch + tt * side.x_token, lane);
+    dy_next = raw4(dy + bb * side.dy_batch + tt * side.dy_token, lane);
+    angles4(p, lane, table_row(p, bb, tt), c_next, s_next);
     t += stride;
   };
   fetch(row);
   // `stride` tokens on for every turn; a warp's groups make the same number of turns
   for (int turn = __reduce_min_sync(0xffffffffu, row); turn < rows; turn += stride, row += stride) {
-    const bool live = row < rows;
-    float xa[NC][CH], xb[NC][CH], da[NC][CH], db[NC][CH], c[NC][CH], s[NC][CH];
+    Pair xa[2], xb[2], ya[2], yb[2], da[2], db[2], c[2], s[2], n[2];
+    unpack4<T, INTER>(x_next, lane, xa, xb);
+    unpack4<T, INTER>(dy_next, lane, ya, yb);
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      as_pairs(x_next[n], map.adjacent[n], xa[n], xb[n]);
-      as_pairs(dy_next[n], map.adjacent[n], da[n], db[n]);
-#pragma unroll
-      for (int i = 0; i < CH; ++i) c[n][i] = c_next[n][i], s[n][i] = s_next[n][i];
+    for (int i = 0; i < 2; ++i) {
+      c[i] = pair(c_next[2 * i], c_next[2 * i + 1]), s[i] = pair(s_next[2 * i], s_next[2 * i + 1]);
+      n[i] = pair(-s_next[2 * i], -s_next[2 * i + 1]);
     }
     if (turn + stride < rows) fetch(row + stride);
-    float square = 0.f, dot = 0.f;
+    Pair squares = pair(0.f, 0.f), dots = pair(0.f, 0.f);
 #pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const float ya = da[n][i], yb = db[n][i];  // rotated back; cos 1, sin 0 where there is no rotation
-        da[n][i] = fmaf(ya, c[n][i], yb * s[n][i]);
-        db[n][i] = fmaf(yb, c[n][i], -ya * s[n][i]);
-        square = fmaf(xa[n][i], xa[n][i], fmaf(xb[n][i], xb[n][i], square));
-        dot = fmaf(da[n][i] * wa[n][i], xa[n][i], fmaf(db[n][i] * wb[n][i], xb[n][i], dot));
-      }
-    square = group_sum<LANES>(square);
-    dot = group_sum<LANES>(dot);
-    if (!live) continue;
-    const float r = 1.f / sqrtf(fmaf(square, per, p.eps));
-    const float back = dot * r * r * per;  // sum(h xhat) r / count
-    T* dx = static_cast<T*>(side.y) + (static_cast<long long>(row) * side.heads + h) * p.dim;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      if (!map.there[n]) continue;
-      float oa[CH], ob[CH];
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        oa[i] = r * fmaf(-back, xa[n][i], da[n][i] * wa[n][i]);
-        ob[i] = r * fmaf(-back, xb[n][i], db[n][i] * wb[n][i]);
-        ga[n][i] = fmaf(da[n][i], xa[n][i] * r, ga[n][i]);
-        gb[n][i] = fmaf(db[n][i], xb[n][i] * r, gb[n][i]);
-      }
-      store_pairs<T, CH>(dx, map.first[n], map.second[n], map.adjacent[n], map.single[n], oa, ob);
+    for (int i = 0; i < 2; ++i) {  // rotated back; cos 1, sin 0 where there is no rotation
+      da[i] = fma2(ya[i], c[i], mul2(yb[i], s[i]));
+      db[i] = fma2(yb[i], c[i], mul2(ya[i], n[i]));
+      squares = fma2(xa[i], xa[i], fma2(xb[i], xb[i], squares));
+      dots = fma2(mul2(da[i], wa[i]), xa[i], fma2(mul2(db[i], wb[i]), xb[i], dots));
     }
+    const float2 q = both(squares), d = both(dots);
+    const float square = group_sum<LANES>((q.x + q.y) * counted);
+    const float dot = group_sum<LANES>(lane.there ? d.x + d.y : 0.f);
+    if (row >= rows) continue;
+    const float r = inverse_root(fmaf(square, per, p.eps));
+    const Pair back = pair(-dot * r * r * per, -dot * r * r * per), rr = pair(r, r);  // - sum(h xhat) r / count
+    Pair oa[2], ob[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      oa[i] = mul2(rr, fma2(back, xa[i], mul2(da[i], wa[i])));
+      ob[i] = mul2(rr, fma2(back, xb[i], mul2(db[i], wb[i])));
+      ga[i] = fma2(da[i], mul2(xa[i], rr), ga[i]);
+      gb[i] = fma2(db[i], mul2(xb[i], rr), gb[i]);
+    }
+    if (lane.there)
+      store4<T, INTER>(static_cast<T*>(side.y) + (static_cast<long long>(row) * side.heads + h) * p.dim, lane, oa, ob);
   }
   if (!p.partial || !side.w) return;
-#pragma unroll
-  for (int n = 0; n < NC; ++n)
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      part[in_block][2 * (n * CH + i)][lane] = ga[n][i];
-      part[in_block][2 * (n * CH + i) + 1][lane] = gb[n][i];
-    }
-  __syncthreads();
-  if (in_block) return;
-  float* out = p.partial + static_cast<long long>(blockIdx.x) * p.dim;
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    if (!map.there[n]) continue;
-    float a[CH] = {}, b2[CH] = {};
-    for (int g = 0; g < GROUPS; ++g)
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        a[i] += part[g][2 * (n * CH + i)][lane];
-        b2[i] += part[g][2 * (n * CH + i) + 1][lane];
-      }
-    store_pairs<float, CH>(out, map.first[n], map.second[n], map.adjacent[n], map.single[n], a, b2);
-  }
+  float fa[4], fb[4], a[4], b2[4];
+  as_float_array(ga, fa);
+  as_float_array(gb, fb);
+  block_weight_sums<GROUPS, LANES>(p, fa, fb, part, a, b2);
+  if (in_block || !lane.there) return;
+  Pair pa[2], pb[2];
+  as_pair_array(a, pa);
+  as_pair_array(b2, pb);
+  store4<float, INTER>(p.partial + static_cast<long long>(blockIdx.x) * p.dim, lane, pa, pb);
 }
 
-// dw of one side: blocks' sums in eight interleaved parts, the parts pairwise.
 template <typename T>
-__global__ void __launch_bounds__(256) qk_norm_reduce(const float* partial, int blocks_q, int blocks_k, int dim, T* dwq, T* dwk) {
-  __shared__ float part[8][33];
+__global__ void __launch_bounds__(kNormThreads) qk_norm_backward1(NormParams p) {
+  constexpr int GROUPS = kNormThreads / 32;
+  __shared__ float part[GROUPS][8][33];
+  const int in_block = threadIdx.x / 32;
+  const int which = static_cast<int>(blockIdx.x) >= p.side_blocks[0];
+  const NormSide& side = p.side[which];
+  const int block = which ? blockIdx.x - p.side_blocks[0] : blockIdx.x;
+  const Lane1 lane(threadIdx.x & 31, p.dim, p.rot, p.interleaved);
+  float wa[4] = {1.f, 1.f, 1.f, 1.f}, wb[4] = {1.f, 1.f, 1.f, 1.f}, ga[4] = {}, gb[4] = {};
+  if (side.w) load1(static_cast<const T*>(side.w), lane, wa, wb);
+  const float per = p.l2 ? 1.f : 1.f / p.dim;
+  const int rows = p.batch * p.tokens, stride = p.side_stride[which];
+  const int group = block * GROUPS + in_block;
+  int row = group / side.heads;
+  const int h = group - row * side.heads;
+  for (; row < rows; row += stride) {
+    const int b = row / p.tokens, t = row - b * p.tokens;
+    float xa[4], xb[4], da[4], db[4], c[4], s[4];
+    load1(static_cast<const T*>(side.x) + b * side.x_batch + t * side.x_token + h * side.x_head, lane, xa, xb);
+    load1(static_cast<const T*>(side.dy) + b * side.dy_batch + t * side.dy_token + h * side.dy_head, lane, da, db);
+    angles1(p, lane, table_row(p, b, t), c, s);
+    float square = 0.f, dot = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if (lane.turned[n]) {
+        const float ya = da[n], yb = db[n];
+        da[n] = fmaf(ya, c[n], yb * s[n]);
+        db[n] = fmaf(yb, c[n], -ya * s[n]);
+      }
+      square = fmaf(xa[n], xa[n], fmaf(xb[n], xb[n], square));
+      dot = fmaf(da[n] * wa[n], xa[n], fmaf(db[n] * wb[n], xb[n], dot));
+    }
+    square = group_sum<32>(square);
+    dot = group_sum<32>(dot);
+    const float r = inverse_root(fmaf(square, per, p.eps));
+    const float back = dot * r * r * per;  // sum(h xhat) r / count
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      ga[n] = fmaf(da[n], xa[n] * r, ga[n]);
+      gb[n] = fmaf(db[n], xb[n] * r, gb[n]);
+      da[n] = r * fmaf(-back, xa[n], da[n] * wa[n]);
+      db[n] = r * fmaf(-back, xb[n], db[n] * wb[n]);
+    }
+    store1(static_cast<T*>(side.y) + (static_cast<long long>(row) * side.heads + h) * p.dim, lane, da, db);
+  }
+  if (!p.partial || !side.w) return;
+  float a[4], b2[4];
+  block_weight_sums<GROUPS, 32>(p, ga, gb, part, a, b2);
+  if (!in_block) store1(p.partial + static_cast<long long>(blockIdx.x) * p.dim, lane, a, b2);
+}
+
+// dw of one side: blocks' sums in 32 interleaved parts, the parts in order.
+template <typename T>
+__global__ void __launch_bounds__(1024) qk_norm_reduce(const float* partial, int blocks_q, int blocks_k, int dim, T* dwq, T* dwk) {
+  __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
   const int d = blockIdx.x * 32 + lane;
   const int blocks = blockIdx.y ? blocks_k : blocks_q;
@@ -403,12 +484,14 @@ __global__ void __launch_bounds__(256) qk_norm_reduce(const float* partial, int 
   if (!to) return;
   float sum = 0.f;
   if (d < dim)
-    for (int i = row; i < blocks; i += 8) sum += from[static_cast<long long>(i) * dim + d];
+#pragma unroll 8
+    for (int i = row; i < blocks; i += 32) sum += from[static_cast<long long>(i) * dim + d];
   part[row][lane] = sum;
   __syncthreads();
   if (row || d >= dim) return;
-  sum = ((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane])) +
-        ((part[4][lane] + part[5][lane]) + (part[6][lane] + part[7][lane]));
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) sum += part[i][lane];
   to[d] = down<T>(sum);
 }
 
