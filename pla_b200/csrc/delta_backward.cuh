@@ -20,11 +20,11 @@
 namespace pla {
 namespace seq {
 
-template <typename T, int DK, int PS, int PO, int VB, int STAGES>
-__global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p) {
+template <typename T, int DK, int PS, int PO, int VB, int STAGES, int PER_SM>
+__global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p) {
   using L = DeltaLayout<T, DK, PS, PO>;
   using M = SweepShared<T, DK, PS, PO, VB, true>;
-  constexpr int IN = L::kIn, QN = DK / 32;
+  constexpr int IN = L::kIn, QN = DK / 32, kPitch = Slab<T, VB>::kPitch;
   extern __shared__ __align__(128) char shared_bytes[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int wm = warp % (VB / 16), wn = warp / (VB / 16), m0 = wm * 16;
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep_back(DeltaParams p) {
           x[n][e] *= e & 1 ? -w[n].y : -w[n].x;
         }
       tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, x, ff);
-      strip_store<T>(m.strip[warp], lane, out, dv + (c * kChunk + wn * 16) * dv_step + m0, dv_step, len - wn * 16, a.width - m0,
+      strip_store<T, kPitch>(m.slab[turn & 1] + wn * 16 * kPitch + m0 * sizeof(T), lane, out, dv + (c * kChunk + wn * 16) * dv_step + m0, dv_step, len - wn * 16, a.width - m0,
                      p.vec_o);
     }
     __syncthreads();

@@ -57,7 +57,7 @@ struct DeltaParams {
   float scale;
   int row_chunks;    // dense: chunks of a batch row
   int chunk_bound;   // chunks the workspace has room for
-  int* plan;         // ragged: lo [N], len [N], first chunk [N + 1]
+  int* plan;         // ragged: lo [N], len [N], first chunk [N + 1], sequences by length [N]
   int4* table;       // ragged: sequence (-1: none), first token, tokens of every chunk
   char* tiles;       // K, Q planes of every (chunk, key head)
   char* heads;       // T, P planes and coefficients of every (chunk, value head)
@@ -141,6 +141,17 @@ __global__ void __launch_bounds__(1024) delta_plan(const int* cu, int tokens, in
       carry_sum += scan[i];
     }
     __syncthreads();
+  }
+  // the longest sequences first, so that the last blocks to start are short; a
+  // comparison of all with all, left out for very many
+  for (int s = i; s < n; s += 1024) {
+    int rank = s;
+    if (n <= 2048) {
+      const int len = plan[n + s];
+      rank = 0;
+      for (int j = 0; j < n; ++j) rank += plan[n + j] > len || (plan[n + j] == len && j < s);
+    }
+    plan[3 * n + 1 + rank] = s;
   }
   for (int chunk = i; chunk < chunks; chunk += 1024) {
     const int at = find_sequence(plan + 2 * n, n, chunk);

@@ -128,17 +128,11 @@ __device__ __forceinline__ void slab_read(const char* from, int t0, int f0, int 
   }
 }
 
-// Accumulators of [16 features x 16 tokens] to rows of a tensor, through 16
-// rows of the warp's own shared memory.
-template <typename T>
-struct Strip {
-  static constexpr int kPitch = 16 * sizeof(T) + 16;
-  static constexpr int kBytes = 16 * kPitch;
-};
-template <typename T>
+// Accumulators of [16 features x 16 tokens] to rows of a tensor, through the
+// warp's own 16 x 16 part of a slab that has been read.
+template <typename T, int PITCH>
 __device__ __forceinline__ void strip_store(char* buffer, int lane, const float (&f)[2][4], T* to, long long step, int len,
                                             int width, int vec) {
-  constexpr int PITCH = Strip<T>::kPitch;
   __syncwarp();
   if constexpr (sizeof(T) == 2) {
     const int m = lane >> 3;
@@ -338,6 +332,7 @@ __device__ __forceinline__ SweepAt sweep_at(const DeltaParams& p, int vb) {
   b /= parts;
   a.vh = b % p.hv;
   a.sequence = b / p.hv;
+  if (p.cu) a.sequence = p.plan[3 * p.sequences + 1 + a.sequence];  // the longest first
   a.kh = a.vh / (p.hv / p.hk);
   if (p.cu) {
     a.batch = 0;
@@ -429,7 +424,6 @@ struct SweepShared {
   alignas(16) float most_d[VB * 4];   // back: largest of e^G do', by warp
   float keep_s[VB], keep_c[VB];       // inverses of the scales of S and U (dX), for what is kept
   alignas(16) char slab[2][Slab<T, VB>::kBytes];
-  char strip[VB / 4][Strip<T>::kBytes];
 };
 
 // |A B| over 64 tokens with one operand's planes below 2^13.
@@ -441,11 +435,12 @@ __device__ __forceinline__ Pow2 scale_below(float bound) {
 }
 
 // KEEP: store S at every chunk's start and U for the backward pass instead of O.
-template <typename T, int DK, int PS, int PO, int VB, int STAGES, bool KEEP>
-__global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p) {
+template <typename T, int DK, int PS, int PO, int VB, int STAGES, int PER_SM, bool KEEP>
+__global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
   using L = DeltaLayout<T, DK, PS, PO>;
   using M = SweepShared<T, DK, PS, PO, VB, false>;
   constexpr int IN = L::kIn, QN = DK / 32;  // column tiles of a quarter of Dk
+  constexpr int kPitch = Slab<T, VB>::kPitch;
   extern __shared__ __align__(128) char shared_bytes[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int wm = warp % (VB / 16), wn = warp / (VB / 16), m0 = wm * 16;
@@ -611,7 +606,7 @@ __global__ void __launch_bounds__(VB * 8) delta_sweep(DeltaParams p) {
           for (int e = 0; e < 4; ++e)
             q[n][e] = (e & 1 ? wq[n].y : wq[n].x) * (q[n][e] * old[e >> 1].inverse) +
                       (e & 1 ? w[n].y : w[n].x) * (pu[n][e] * fu[e >> 1].inverse);
-        strip_store<T>(m.strip[warp], lane, q, o + (c * kChunk + wn * 16) * o_step + m0, o_step, len - wn * 16, a.width - m0,
+        strip_store<T, kPitch>(m.slab[c & 1] + wn * 16 * kPitch + m0 * sizeof(T), lane, q, o + (c * kChunk + wn * 16) * o_step + m0, o_step, len - wn * 16, a.width - m0,
                        p.vec_o);
       }
     }

@@ -295,7 +295,7 @@ DeltaSizes delta_sizes_of(const pla_delta* a, bool backward) {
   DeltaSizes s;
   s.chunks = a->cu_seqlens ? a->tokens / kChunk + static_cast<long long>(a->sequences)
                            : static_cast<long long>(a->batch) * ((a->tokens + kChunk - 1) / kChunk);
-  s.plan = a->cu_seqlens ? up256(s.chunks * sizeof(int4)) + up256((3ull * a->sequences + 1) * sizeof(int)) : 0;
+  s.plan = a->cu_seqlens ? up256(s.chunks * sizeof(int4)) + up256((4ull * a->sequences + 1) * sizeof(int)) : 0;
   s.tiles = up256(static_cast<size_t>(s.chunks) * a->hk * L::kTiles);
   s.heads = up256(static_cast<size_t>(s.chunks) * a->hv * L::kHead);
   if (backward) {
@@ -406,56 +406,67 @@ int launch_prepare(const DeltaParams& p, cudaStream_t stream) {
   return p.hv > p.hk ? go(Int<2>{}) : go(Int<1>{});  // two value heads of a key head side by side
 }
 
-// Stages of the ring and shared memory of a sweep.
-template <typename T, int DK, int PS, int PO, int VB, bool BACK>
+// Stages of the ring and shared memory of a sweep; PER_SM blocks fit an SM.
+template <typename T, int DK, int PS, int PO, int VB, int PER_SM, bool BACK>
 struct SweepShape {
   using L = DeltaLayout<T, DK, PS, PO>;
   static constexpr size_t kHeld = kSweepRing + sizeof(SweepShared<T, DK, PS, PO, VB, BACK>);
-  static constexpr size_t kRoom = kHeld < 227 * 1024 ? (227 * 1024 - kHeld) / L::kStage : 0;
+  static constexpr size_t kMost = 227 * 1024 / PER_SM - (PER_SM > 1 ? 1024 : 0);  // 1 KB of a block is the system's
+  static constexpr size_t kRoom = kHeld < kMost ? (kMost - kHeld) / L::kStage : 0;
   static constexpr int kStages = kRoom < 3 ? kRoom : 3;
   static constexpr size_t kShared = kHeld + kStages * L::kStage;
+  static constexpr int kColumns = VB, kPerSm = PER_SM;
   static long long grid(const DeltaParams& p) {
     return static_cast<long long>(p.sequences) * p.hv * ((p.dv + VB - 1) / VB);
   }
 };
 
 // Value features of a sweep's block.  A block's time is the latency of its
-// chunks' chain whatever it holds, so the fewest features that still put every
-// block on an SM of its own; many sequences or heads fill the SMs anyway, and
-// more features share one copy of a chunk's tiles, as long as shared memory
-// holds the next chunk's beside it.  f(features)
+// chunks' chain whatever it holds, so while every block has an SM of its own:
+// the fewest features that still leave it so.  With more blocks than SMs two
+// of 32 features side by side fill each other's waits, if their shared memory
+// fits; else 64 features share one copy of a chunk's tiles.
+//   8192 tokens x 32 heads of 128, bf16: SWEEPRULE
+// f(shape)
 template <typename T, int DK, int PS, int PO, bool BACK, typename F>
 int with_columns(const DeltaParams& p, int sms, F&& f) {
-  constexpr int kMost = SweepShape<T, DK, PS, PO, 64, BACK>::kStages >= 2 ? 64 : 32;
-  static_assert(SweepShape<T, DK, PS, PO, kMost, BACK>::kStages >= 1, "no room for a chunk's tiles");
+  using Two = SweepShape<T, DK, PS, PO, 32, 2, BACK>;
+  using Wide = SweepShape<T, DK, PS, PO, 64, 1, BACK>;
   const long long heads = static_cast<long long>(p.sequences) * p.hv;
-  if (p.dv <= 16 || heads * ((p.dv + 15) / 16) <= sms) return f(Int<16>{});
-  if (p.dv <= 32 || heads * ((p.dv + 31) / 32) <= sms) return f(Int<32>{});
-  return f(Int<kMost>{});
+  if (p.dv <= 16 || heads * ((p.dv + 15) / 16) <= sms) return f(SweepShape<T, DK, PS, PO, 16, 1, BACK>{});
+  if (p.dv <= 32 || heads * ((p.dv + 31) / 32) <= sms) return f(SweepShape<T, DK, PS, PO, 32, 1, BACK>{});
+  if constexpr (Two::kStages >= 1)
+    return f(Two{});
+  else if constexpr (Wide::kStages >= 2)
+    return f(Wide{});
+  else
+    return f(SweepShape<T, DK, PS, PO, 32, 1, BACK>{});
 }
 
 template <typename T, int DK, int PS, int PO, bool KEEP>
 int launch_sweep(const DeltaParams& p, int sms, cudaStream_t stream) {
-  return with_columns<T, DK, PS, PO, false>(p, sms, [&](auto vb) {
-    constexpr int VB = decltype(vb)::value;
-    using S = SweepShape<T, DK, PS, PO, VB, false>;
+  return with_columns<T, DK, PS, PO, false>(p, sms, [&](auto shape) {
+    using S = decltype(shape);
+    constexpr int VB = S::kColumns;
+    static_assert(S::kStages >= 1, "no room for a chunk's tiles");
     const long long grid = S::grid(p);
     if (grid > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
-    const int st = allow_shared<delta_sweep<T, DK, PS, PO, VB, S::kStages, KEEP>>(S::kShared);
+    const int st = allow_shared<delta_sweep<T, DK, PS, PO, VB, S::kStages, S::kPerSm, KEEP>>(S::kShared);
     if (st != PLA_OK) return st;
-    delta_sweep<T, DK, PS, PO, VB, S::kStages, KEEP><<<static_cast<int>(grid), VB * 8, S::kShared, stream>>>(p);
+    delta_sweep<T, DK, PS, PO, VB, S::kStages, S::kPerSm, KEEP><<<static_cast<int>(grid), VB * 8, S::kShared, stream>>>(p);
     return launched("delta_sweep");
   });
 }
 
 template <typename T, int DK, int PS, int PO>
 int launch_gradient(const DeltaParams& p, int sms, cudaStream_t stream) {
-  int st = with_columns<T, DK, PS, PO, true>(p, sms, [&](auto vb) {
-    constexpr int VB = decltype(vb)::value;
-    using S = SweepShape<T, DK, PS, PO, VB, true>;
-    const int st = allow_shared<delta_sweep_back<T, DK, PS, PO, VB, S::kStages>>(S::kShared);
+  int st = with_columns<T, DK, PS, PO, true>(p, sms, [&](auto shape) {
+    using S = decltype(shape);
+    constexpr int VB = S::kColumns;
+    static_assert(S::kStages >= 1, "no room for a chunk's tiles");
+    const int st = allow_shared<delta_sweep_back<T, DK, PS, PO, VB, S::kStages, S::kPerSm>>(S::kShared);
     if (st != PLA_OK) return st;
-    delta_sweep_back<T, DK, PS, PO, VB, S::kStages><<<static_cast<int>(S::grid(p)), VB * 8, S::kShared, stream>>>(p);
+    delta_sweep_back<T, DK, PS, PO, VB, S::kStages, S::kPerSm><<<static_cast<int>(S::grid(p)), VB * 8, S::kShared, stream>>>(p);
     return launched("delta_sweep_back");
   });
   if (st != PLA_OK) return st;
