@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -526,9 +527,11 @@ Tensor delta_step_meta(const Tensor&, const Tensor&, const Tensor& v, const Tens
 }
 
 // ---- autograd --------------------------------------------------------------
+// One typed handle per signature (each is used for one op).
 template <typename Sig>
-auto op_of(const char* name) {
-  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
+const c10::TypedOperatorHandle<Sig>& op_of(const char* name) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
+  return op;
 }
 template <typename... Ts>
 bool wants_gradient(const Ts&... ts) {
@@ -544,7 +547,7 @@ Tensor grad_if(const Tensor& g, const Tensor& input) { return input.defined() ? 
 
 std::tuple<Tensor, Tensor> causal_below(const Tensor& x, const Tensor& w, const optional<Tensor>& b, bool silu,
                                         const optional<Tensor>& cu, const optional<Tensor>& state, bool return_state) {
-  static const auto op = op_of<decltype(causal_cuda)>("pla_b200::causal_depthwise");
+  const auto& op = op_of<decltype(causal_cuda)>("pla_b200::causal_depthwise");
   at::AutoDispatchBelowADInplaceOrView guard;
   return op.call(x, w, b, silu, cu, state, return_state);
 }
@@ -560,7 +563,7 @@ struct CausalFunction : torch::autograd::Function<CausalFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    static const auto op = op_of<decltype(causal_backward_cuda)>("pla_b200::causal_depthwise_backward");
+    const auto& op = op_of<decltype(causal_backward_cuda)>("pla_b200::causal_depthwise_backward");
     const Tensor dy = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
     auto [dx, dw, db, dstate] = op.call(dy, as_optional(grads[1]), s[0], s[1], as_optional(s[2]),
                                         ctx->saved_data["silu"].toBool(), as_optional(s[3]), as_optional(s[4]));
@@ -577,7 +580,7 @@ std::tuple<Tensor, Tensor> causal_autograd(const Tensor& x, const Tensor& w, con
 std::tuple<Tensor, Tensor> norm_below(const Tensor& q, const Tensor& k, const optional<Tensor>& wq, const optional<Tensor>& wk,
                                       const optional<Tensor>& cos, const optional<Tensor>& sin, const optional<Tensor>& pos,
                                       bool l2, double eps, bool interleaved) {
-  static const auto op = op_of<decltype(norm_cuda)>("pla_b200::qk_norm_rotate");
+  const auto& op = op_of<decltype(norm_cuda)>("pla_b200::qk_norm_rotate");
   at::AutoDispatchBelowADInplaceOrView guard;
   return op.call(q, k, wq, wk, cos, sin, pos, l2, eps, interleaved);
 }
@@ -594,7 +597,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    static const auto op = op_of<decltype(norm_backward_cuda)>("pla_b200::qk_norm_rotate_backward");
+    const auto& op = op_of<decltype(norm_backward_cuda)>("pla_b200::qk_norm_rotate_backward");
     auto [dq, dk, dwq, dwk] =
         op.call(grads[0], grads[1], s[0], s[1], as_optional(s[2]), as_optional(s[3]), as_optional(s[4]), as_optional(s[5]),
                 as_optional(s[6]), ctx->saved_data["l2"].toBool(), ctx->saved_data["eps"].toDouble(),
@@ -614,7 +617,7 @@ std::tuple<Tensor, Tensor> norm_autograd(const Tensor& q, const Tensor& k, const
 std::tuple<Tensor, Tensor> delta_below(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
                                        double scale, const optional<Tensor>& cu, const optional<Tensor>& state,
                                        bool return_state) {
-  static const auto op = op_of<decltype(delta_cuda)>("pla_b200::gated_delta_rule");
+  const auto& op = op_of<decltype(delta_cuda)>("pla_b200::gated_delta_rule");
   at::AutoDispatchBelowADInplaceOrView guard;
   return op.call(q, k, v, g, beta, scale, cu, state, return_state);
 }
@@ -631,7 +634,7 @@ struct DeltaFunction : torch::autograd::Function<DeltaFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    static const auto op = op_of<decltype(delta_backward_cuda)>("pla_b200::gated_delta_rule_backward");
+    const auto& op = op_of<decltype(delta_backward_cuda)>("pla_b200::gated_delta_rule_backward");
     const Tensor d_o = grads[0].defined() ? grads[0] : at::zeros_like(s[2]);
     auto [dq, dk, dv, dg, dbeta, dstate] = op.call(d_o, as_optional(grads[1]), s[0], s[1], s[2], s[3], s[4],
                                                    ctx->saved_data["scale"].toDouble(), as_optional(s[5]), as_optional(s[6]));
@@ -644,6 +647,42 @@ std::tuple<Tensor, Tensor> delta_autograd(const Tensor& q, const Tensor& k, cons
   if (!wants_gradient(q, k, v, g, beta, state)) return delta_below(q, k, v, g, beta, scale, cu, state, return_state);
   auto r = DeltaFunction::apply(q, k, v, g, beta, scale, cu, state, return_state);
   return {r[0], r[1]};
+}
+
+// The single-token forms have no gradient: the call goes through where none is
+// asked for, and a result of inputs that ask for one raises when a backward
+// pass reaches it.  (An unboxed kernel: the general fallback costs a decoding
+// step 1.5 us.)  `state` changes in place, so its version does.
+template <typename Sig, typename... Args>
+Tensor step_below(const char* name, const Tensor& state, const Args&... args) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  Tensor out = op_of<Sig>(name).call(args...);
+  if (!state.is_inference()) torch::autograd::impl::bump_version(state);
+  return out;
+}
+struct NoGradient : torch::autograd::Function<NoGradient> {
+  // what the result depends on
+  static Tensor forward(AutogradContext*, const Tensor& result, const Tensor&, const Tensor&, const optional<Tensor>&,
+                        const optional<Tensor>&, const optional<Tensor>&) {
+    return result;
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "pla_b200: the single-token operators have no gradient");
+    return {};
+  }
+};
+Tensor causal_step_autograd(const Tensor& x, const Tensor& state, const Tensor& w, const optional<Tensor>& b, bool silu) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && state.requires_grad()),
+              "causal_depthwise_step: state is updated in place and must not require grad");
+  Tensor y = step_below<decltype(causal_step_cuda)>("pla_b200::causal_depthwise_step", state, x, state, w, b, silu);
+  return wants_gradient(x, w, b) ? NoGradient::apply(y, x, w, b, optional<Tensor>(), optional<Tensor>()) : y;
+}
+Tensor delta_step_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
+                           const Tensor& state, double scale) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && state.requires_grad()),
+              "gated_delta_rule_step: state is updated in place and must not require grad");
+  Tensor o = step_below<decltype(delta_step_cuda)>("pla_b200::gated_delta_rule_step", state, q, k, v, g, beta, state, scale);
+  return wants_gradient(q, k, v, g, beta) ? NoGradient::apply(o, q, k, optional<Tensor>(v), optional<Tensor>(g), optional<Tensor>(beta)) : o;
 }
 
 }  // namespace
@@ -700,7 +739,8 @@ TORCH_LIBRARY_IMPL(pla_b200, Autograd, m) {
   m.impl("causal_depthwise", &causal_autograd);
   m.impl("qk_norm_rotate", &norm_autograd);
   m.impl("gated_delta_rule", &delta_autograd);
-  for (const char* op : {"causal_depthwise_backward", "causal_depthwise_step", "qk_norm_rotate_backward",
-                         "gated_delta_rule_backward", "gated_delta_rule_step"})
+  m.impl("causal_depthwise_step", &causal_step_autograd);
+  m.impl("gated_delta_rule_step", &delta_step_autograd);
+  for (const char* op : {"causal_depthwise_backward", "qk_norm_rotate_backward", "gated_delta_rule_backward"})
     m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }

@@ -32,10 +32,15 @@ import torch
 from . import _lib
 
 
-def _cuda(t, op: str):
+_ops: dict = {}
+
+
+def _op(name: str, t):
     if not isinstance(t, torch.Tensor) or not (t.is_cuda or t.is_meta):
-        raise ValueError(f"{op} requires CUDA inputs")
-    return _lib.ops()
+        raise ValueError(f"{name} requires CUDA inputs")
+    if name not in _ops:
+        _ops[name] = getattr(_lib.ops(), name).default
+    return _ops[name]
 
 
 def causal_depthwise(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, silu: bool = False,
@@ -48,14 +53,14 @@ def causal_depthwise(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
     if None).  Returns y, or (y, state after the sequences).  Differentiable
     in x, weight, bias and state.
     """
-    y, last = _cuda(x, "causal_depthwise").causal_depthwise.default(x, weight, bias, silu, cu_seqlens, state, return_state)
+    y, last = _op("causal_depthwise", x)(x, weight, bias, silu, cu_seqlens, state, return_state)
     return (y, last) if return_state else y
 
 
 def causal_depthwise_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
                           silu: bool = False) -> torch.Tensor:
     """One token of ``causal_depthwise`` for x [N, C]; ``state`` [N, K - 1, C] moves up by one row in place."""
-    return _cuda(x, "causal_depthwise_step").causal_depthwise_step.default(x, state, weight, bias, silu)
+    return _op("causal_depthwise_step", x)(x, state, weight, bias, silu)
 
 
 def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None = None,
@@ -74,8 +79,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     """
     if norm not in ("rms", "l2"):
         raise ValueError('norm must be "rms" or "l2"')
-    return _cuda(q, "qk_norm_rotate").qk_norm_rotate.default(q, k, q_weight, k_weight, cos, sin, positions, norm == "l2",
-                                                             eps, interleaved)
+    return _op("qk_norm_rotate", q)(q, k, q_weight, k_weight, cos, sin, positions, norm == "l2", eps, interleaved)
 
 
 def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -93,9 +97,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     Differentiable in q, k, v, g, beta and state; the backward pass computes
     the states again and keeps only the inputs.
     """
-    ops = _cuda(q, "gated_delta_rule")
+    op = _op("gated_delta_rule", q)
     scale = q.shape[-1] ** -0.5 if scale is None else scale
-    o, last = ops.gated_delta_rule.default(q, k, v, g, beta, scale, cu_seqlens, state, return_state)
+    o, last = op(q, k, v, g, beta, scale, cu_seqlens, state, return_state)
     return (o, last) if return_state else o
 
 
@@ -106,5 +110,5 @@ def gated_delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: 
     ``state``, float32 [N, Hv, Dk, Dv], is updated in place.  Dk is at most
     256.  Returns o [N, Hv, Dv].
     """
-    ops = _cuda(q, "gated_delta_rule_step")
-    return ops.gated_delta_rule_step.default(q, k, v, g, beta, state, q.shape[-1] ** -0.5 if scale is None else scale)
+    op = _op("gated_delta_rule_step", q)
+    return op(q, k, v, g, beta, state, q.shape[-1] ** -0.5 if scale is None else scale)

@@ -520,3 +520,21 @@ def test_second_derivatives_raise():
     (dx,) = torch.autograd.grad(P.causal_depthwise(x, w).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+def test_steps_have_no_gradient_and_count_as_changes_of_the_state():
+    x, w = torch.randn(2, 16, device=DEV), torch.randn(16, 4, device=DEV, requires_grad=True)
+    s = torch.zeros(2, 3, 16, device=DEV)
+    before = s._version
+    y = P.causal_depthwise_step(x, s, w)
+    assert y.requires_grad and s._version > before
+    with pytest.raises(RuntimeError, match="no gradient"):
+        y.sum().backward()
+    with pytest.raises(RuntimeError, match="in place"):
+        P.causal_depthwise_step(x, s.clone().requires_grad_(), w)
+    q, v, g = torch.randn(2, 1, 32, device=DEV, requires_grad=True), torch.randn(2, 1, 32, device=DEV), torch.zeros(2, 1, device=DEV)
+    o = P.gated_delta_rule_step(q, q, v, g, g + 1, torch.zeros(2, 1, 32, 32, device=DEV))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        o.sum().backward()
+    with torch.inference_mode():
+        assert not P.causal_depthwise_step(x, torch.zeros(2, 3, 16, device=DEV), w).requires_grad
