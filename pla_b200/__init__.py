@@ -9,7 +9,7 @@ replace ``data/depthwise_conv_7x7.py`` and ``data/stencil_7x7.py``.
   ``depthwise7x7_layernorm()`` / ``DepthwiseLayerNorm`` (depthwise + channel LayerNorm, NHWC, fused)
 * ``pla_b200.sequence``  — the layers of a sequence block: ``causal_depthwise()``, ``qk_norm_rotate()``,
   ``gated_delta_rule()`` with their gradients, and the single-token forms ``causal_depthwise_step()``,
-  ``gated_delta_rule_step()``
+  ``gated_delta_rule_step()``; ``DeltaMixer`` chains them
 * ``pla_b200.iterate``   — ``stencil7x7_iterate()``, ``BandedStencil`` (multi-GPU)
 
 All compute goes through the C ABI in ``include/pla_b200.h``
@@ -28,10 +28,10 @@ except ImportError:  # not built yet (e.g. while pla_b200.build runs): the ops r
 
 from .depthwise import DepthwiseLayerNorm, depthwise7x7, depthwise7x7_layernorm, depthwise7x7_many, depthwise_kxk
 from .iterate import BandedStencil, band_rows, stencil7x7_iterate
-from .sequence import (causal_depthwise, causal_depthwise_step, gated_delta_rule, gated_delta_rule_step,
+from .sequence import (DeltaMixer, causal_depthwise, causal_depthwise_step, gated_delta_rule, gated_delta_rule_step,
                        qk_norm_rotate)
 from .stencil import stencil7x7
 
 __all__ = ["stencil7x7", "depthwise7x7", "depthwise7x7_many", "depthwise_kxk", "depthwise7x7_layernorm", "DepthwiseLayerNorm",
            "stencil7x7_iterate", "BandedStencil", "band_rows", "causal_depthwise", "causal_depthwise_step",
-           "qk_norm_rotate", "gated_delta_rule", "gated_delta_rule_step"]
+           "qk_norm_rotate", "gated_delta_rule", "gated_delta_rule_step", "DeltaMixer"]

@@ -112,3 +112,68 @@ def gated_delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: 
     """
     op = _op("gated_delta_rule_step", q)
     return op(q, k, v, g, beta, state, q.shape[-1] ** -0.5 if scale is None else scale)
+
+
+class DeltaMixer(torch.nn.Module):
+    """A delta-rule sequence block: projection, short convolution, norms, gated delta rule, output projection.
+
+    ``in_proj`` gives queries and keys (``num_heads`` of ``head_dim``) and
+    values (``value_heads`` of ``value_dim``); ``conv`` is the causal
+    depthwise convolution with SiLU over all of them; queries and keys are L2
+    normalised per head; ``gate_proj`` gives each value head's decay
+    ``g = -exp(A_log) softplus(a + dt_bias)`` and ``beta = sigmoid(b)``, in
+    fp32; ``out_proj`` maps the heads back.  ``forward`` takes [B, T, dim] (or
+    a ragged [1, T, dim] with ``cu_seqlens``); ``step`` takes [N, dim] and a
+    state from ``new_state`` or ``forward(..., return_state=True)``, which it
+    updates in place.
+    """
+
+    def __init__(self, dim: int, num_heads: int, head_dim: int = 128, value_heads: int | None = None,
+                 value_dim: int | None = None, taps: int = 4):
+        super().__init__()
+        self.num_heads, self.head_dim = num_heads, head_dim
+        self.value_heads = num_heads if value_heads is None else value_heads
+        self.value_dim = head_dim if value_dim is None else value_dim
+        if self.value_heads % num_heads:
+            raise ValueError("value_heads must be a multiple of num_heads")
+        self.widths = [num_heads * head_dim, num_heads * head_dim, self.value_heads * self.value_dim]
+        channels = sum(self.widths)
+        self.in_proj = torch.nn.Linear(dim, channels, bias=False)
+        self.gate_proj = torch.nn.Linear(dim, 2 * self.value_heads, bias=False)
+        self.conv = torch.nn.Conv1d(channels, channels, taps, groups=channels)
+        self.A_log = torch.nn.Parameter(torch.empty(self.value_heads).uniform_(1, 8).log())
+        self.dt_bias = torch.nn.Parameter(torch.full((self.value_heads,), -2.0))
+        self.out_proj = torch.nn.Linear(self.value_heads * self.value_dim, dim, bias=False)
+
+    def new_state(self, n: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Zero states of n sequences: the convolution's inputs and the delta rule's fp32 state."""
+        w = self.in_proj.weight
+        return (torch.zeros(n, self.conv.weight.shape[-1] - 1, sum(self.widths), device=w.device, dtype=w.dtype),
+                torch.zeros(n, self.value_heads, self.head_dim, self.value_dim, device=w.device))
+
+    def _gates(self, x):
+        a, b = self.gate_proj(x).float().chunk(2, -1)
+        g = -self.A_log.float().exp() * torch.nn.functional.softplus(a + self.dt_bias.float())
+        return g, torch.sigmoid(b)
+
+    def _heads(self, h):
+        q, k, v = h.split(self.widths, -1)
+        heads = (self.num_heads, self.head_dim)
+        return q.unflatten(-1, heads), k.unflatten(-1, heads), v.unflatten(-1, (self.value_heads, self.value_dim))
+
+    def forward(self, x: torch.Tensor, cu_seqlens: torch.Tensor | None = None, state=None, return_state: bool = False):
+        before = (None, None) if state is None else state
+        h, conv_state = causal_depthwise(self.in_proj(x), self.conv.weight, self.conv.bias, silu=True,
+                                         cu_seqlens=cu_seqlens, state=before[0], return_state=True)
+        q, k, v = self._heads(h)
+        q, k = qk_norm_rotate(q, k, norm="l2")
+        o = gated_delta_rule(q, k, v, *self._gates(x), cu_seqlens=cu_seqlens, state=before[1], return_state=return_state)
+        if return_state:
+            return self.out_proj(o[0].flatten(-2)), (conv_state, o[1])
+        return self.out_proj(o.flatten(-2))
+
+    def step(self, x: torch.Tensor, state: tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
+        h = causal_depthwise_step(self.in_proj(x), state[0], self.conv.weight, self.conv.bias, silu=True)
+        q, k, v = self._heads(h)
+        q, k = (t[:, 0] for t in qk_norm_rotate(q[:, None], k[:, None], norm="l2"))
+        return self.out_proj(gated_delta_rule_step(q, k, v, *self._gates(x), state[1]).flatten(-2))

@@ -538,3 +538,136 @@ def test_steps_have_no_gradient_and_count_as_changes_of_the_state():
         o.sum().backward()
     with torch.inference_mode():
         assert not P.causal_depthwise_step(x, torch.zeros(2, 3, 16, device=DEV), w).requires_grad
+
+
+# ---- the block that chains them --------------------------------------------
+def mixer_reference(m, x, cu):
+    p = {n: t.detach().double().cpu().requires_grad_() for n, t in m.named_parameters()}
+    h, conv = R.causal_depthwise(x @ p["in_proj.weight"].T, p["conv.weight"][:, 0], p["conv.bias"], True, cu)
+    q, k, v = h.split(m.widths, -1)
+    q, k = (R.norm_rotate(t.unflatten(-1, (m.num_heads, m.head_dim)), l2=True) for t in (q, k))
+    a, b = (x @ p["gate_proj.weight"].T).chunk(2, -1)
+    g = -p["A_log"].exp() * torch.nn.functional.softplus(a + p["dt_bias"])
+    o, s = R.gated_delta_rule(q, k, v.unflatten(-1, (m.value_heads, m.value_dim)), g, torch.sigmoid(b), cu=cu)
+    return o.flatten(-2) @ p["out_proj.weight"].T, conv, s, p
+
+
+def make_mixer(dtype=F32):
+    torch.manual_seed(71)
+    return P.DeltaMixer(48, 2, head_dim=32, value_heads=4, value_dim=16, taps=4).to(DEV, dtype)
+
+
+@pytest.mark.parametrize("cu", [None, [0, 5, 70, 131]])
+def test_mixer_runs_and_its_gradients(cu):
+    """fp32 throughout: the operators' tolerances (2.4e-5 forward, 4.8e-5
+    backward) and matrix products of 48 to 128 terms (128 * 2^-24 = 2^-17) on
+    either side of them: below 1e-4, twice that for gradients, of each
+    tensor's norm."""
+    m = make_mixer()
+    g = torch.Generator().manual_seed(72)
+    x = rand(g, 1 if cu else 2, 131, 48)
+    dy = rand(g, *x.shape)
+    cu = None if cu is None else torch.tensor(cu, dtype=torch.int32)
+    x64 = f64(x, True)
+    want, conv, s, p = mixer_reference(m, x64, cu)
+    xd = gpu(x).requires_grad_()
+    y, state = m(xd, cu_seqlens=gpu(cu), return_state=True)
+    for a, b in ((y, want), (state[0], conv), (state[1], s)):
+        assert float((a.detach().cpu().double() - b.detach()).norm() / b.detach().norm()) <= 1e-4
+    want = torch.autograd.grad(want, [x64, *p.values()], f64(dy))
+    got = torch.autograd.grad(y, [xd, *m.parameters()], gpu(dy))
+    for a, b, name in zip(got, want, ["x", *p]):
+        assert float((a.cpu().double() - b).norm() / b.norm()) <= 2e-4, name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_mixer_decodes_from_its_prompts_states(dtype):
+    m = make_mixer(dtype)
+    x = gpu(rand(torch.Generator().manual_seed(73), 3, 40, 48, dtype=dtype))
+    with torch.no_grad():
+        whole, end = m(x, return_state=True)
+        _, state = m(x[:, :30], return_state=True)
+        out = torch.stack([m.step(x[:, t], state) for t in range(30, 40)], 1)
+        fresh = m.new_state(3)
+        first = m.step(x[:, 0], fresh)
+    # the same sums in another order, the inputs of each layer rounded to dtype: a few roundings through two products
+    tol = 2e-4 if dtype == F32 else 16 * half(BF16)
+    assert float((out - whole[:, 30:]).norm() / whole[:, 30:].norm()) <= tol
+    assert float((first - whole[:, 0]).norm() / whole[:, 0].norm()) <= tol
+    assert float((state[1] - end[1]).norm() / end[1].norm()) <= tol
+
+
+# ---- refusals and edges ----------------------------------------------------
+def test_refusals_name_the_argument():
+    x, w = torch.zeros(1, 8, 16, device=DEV), torch.zeros(16, 4, device=DEV)
+    bad = [
+        lambda: P.causal_depthwise(x[0], w), lambda: P.causal_depthwise(x, w[:, :1]),
+        lambda: P.causal_depthwise(x, torch.zeros(16, 5, device=DEV)), lambda: P.causal_depthwise(x, w.half()),
+        lambda: P.causal_depthwise(x.double(), w.double()), lambda: P.causal_depthwise(x, w.cpu()),
+        lambda: P.causal_depthwise(x, w, state=torch.zeros(2, 3, 16, device=DEV)),
+        lambda: P.causal_depthwise(x, w, cu_seqlens=torch.zeros(1, dtype=torch.int32, device=DEV)),
+        lambda: P.causal_depthwise(x, w, cu_seqlens=torch.zeros(3, dtype=torch.int64, device=DEV)),
+        lambda: P.causal_depthwise(x.expand(2, 8, 16), w, cu_seqlens=torch.zeros(3, dtype=torch.int32, device=DEV)),
+        lambda: P.causal_depthwise_step(x[:, 0], torch.zeros(1, 16, 3, device=DEV).mT, w),
+        lambda: P.causal_depthwise_step(x[0], torch.zeros(1, 3, 16, device=DEV).expand(8, 3, 16), w),
+    ]
+    q = torch.zeros(1, 8, 2, 32, device=DEV)
+    t = torch.zeros(8, 8, device=DEV)
+    bad += [
+        lambda: P.qk_norm_rotate(q, q[..., :16]), lambda: P.qk_norm_rotate(q, q, cos=t), lambda: P.qk_norm_rotate(q, q, cos=t.half(), sin=t),
+        lambda: P.qk_norm_rotate(q, q, torch.zeros(31, device=DEV)), lambda: P.qk_norm_rotate(q, q, positions=torch.zeros(8, device=DEV)),
+        lambda: P.qk_norm_rotate(q, q, cos=torch.zeros(8, 17, device=DEV), sin=torch.zeros(8, 17, device=DEV)),
+        lambda: P.qk_norm_rotate(q, q, cos=t, sin=t, positions=torch.zeros(3, dtype=torch.long, device=DEV)),
+        lambda: P.qk_norm_rotate(torch.zeros(1, 1, 1, 258, device=DEV), torch.zeros(1, 1, 1, 258, device=DEV)),
+        lambda: P.qk_norm_rotate(q, q, eps=-1.0), lambda: P.qk_norm_rotate(q, q, cos=t.clone().requires_grad_(), sin=t),
+    ]
+    g = torch.zeros(1, 8, 2, device=DEV)
+    big = torch.zeros(1, 8, 2, 160, device=DEV)
+    bad += [
+        lambda: P.gated_delta_rule(q, q, q, g, g[:, :4]), lambda: P.gated_delta_rule(q, q, q, g, g.half()),
+        lambda: P.gated_delta_rule(q, q, q[:, :, :1].expand(1, 8, 3, 32), torch.zeros(1, 8, 3, device=DEV), torch.zeros(1, 8, 3, device=DEV)),
+        lambda: P.gated_delta_rule(big, big, q, g, g), lambda: P.gated_delta_rule(q, q, big, g, g),
+        lambda: P.gated_delta_rule(q, q, q, g, g, state=torch.zeros(1, 2, 32, 32, device=DEV, dtype=BF16)),
+        lambda: P.gated_delta_rule_step(q[0], q[0], q[0], g[0], g[0], torch.zeros(8, 2, 32, 32, device=DEV).transpose(2, 3)),
+        lambda: P.gated_delta_rule_step(q[0], q[0], q[0], g[0], g[0], torch.zeros(1, 2, 32, 32, device=DEV).expand(8, 2, 32, 32)),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    with pytest.raises(ValueError):
+        P.qk_norm_rotate(q, q, norm="batch")
+
+
+def test_empty_calls():
+    w = torch.zeros(16, 4, device=DEV)
+    s = torch.randn(2, 3, 16, device=DEV)
+    y, last = P.causal_depthwise(torch.zeros(2, 0, 16, device=DEV), w, state=s, return_state=True)
+    assert y.shape == (2, 0, 16) and torch.equal(last, s)
+    a, b = P.qk_norm_rotate(torch.zeros(0, 3, 2, 32, device=DEV), torch.zeros(0, 3, 1, 32, device=DEV))
+    assert a.shape == (0, 3, 2, 32) and b.shape == (0, 3, 1, 32)
+    q, g, s = torch.zeros(2, 0, 1, 32, device=DEV), torch.zeros(2, 0, 1, device=DEV), torch.randn(2, 1, 32, 32, device=DEV)
+    o, last = P.gated_delta_rule(q, q, q, g, g, state=s, return_state=True)
+    assert o.shape == q.shape and torch.equal(last, s)
+    x = torch.zeros(0, 16, device=DEV)
+    assert P.causal_depthwise_step(x, torch.zeros(0, 3, 16, device=DEV), w).shape == (0, 16)
+    wq = torch.ones(32, device=DEV, requires_grad=True)
+    q = torch.zeros(1, 0, 1, 32, device=DEV, requires_grad=True)
+    yq, yk = P.qk_norm_rotate(q, q, wq, wq)
+    assert not torch.autograd.grad((yq, yk), wq, (yq.detach(), yk.detach()))[0].any()
+    xg = torch.zeros(1, 0, 16, device=DEV, requires_grad=True)
+    wg = w.clone().requires_grad_()
+    y = P.causal_depthwise(xg, wg)
+    assert not torch.autograd.grad(y, wg, y.detach())[0].any()
+
+
+def test_compiled_and_fake_tensors_trace():
+    q, k, v, g, beta, _, _ = (gpu(t) for t in delta_inputs((1, 70, 1, 1, 32, 32, False, None, None), BF16, seed=91))
+    f = lambda *a: P.gated_delta_rule(*P.qk_norm_rotate(a[0], a[1], norm="l2"), *a[2:]) * 2  # noqa: E731
+    compiled = torch.compile(f, fullgraph=True, backend="aot_eager")
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, g, beta)]
+    again = [t.clone().requires_grad_() for t in (q, k, v, g, beta)]
+    a, b = f(*leaves), compiled(*again)
+    assert torch.equal(a, b)
+    for x, y in zip(torch.autograd.grad(a, leaves, v), torch.autograd.grad(b, again, v)):
+        assert torch.equal(x, y)
