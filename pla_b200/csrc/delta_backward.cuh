@@ -237,7 +237,8 @@ struct GradShared {
     } in;
     alignas(128) __half square[4][PS][kChunk * kChunk];  // N f_k, N f_q (rows), Gamma dA f_k, B f_k (rows)
   };
-  float krow[kChunk], qrow[kChunk], orow[kChunk];
+  alignas(16) float krow[kChunk];
+  float qrow[kChunk], orow[kChunk];
   float beta[kChunk], hi[kChunk], lo[kChunk], down[kChunk], tail[kChunk];  // down: e^G, tail: e^{G_C - G}
   float ratio[4][128];         // a row's scale over the common one: S, dS, U, dX
   float dots[4][4][kChunk];    // quarters of Dk: k.r1, q.dq, k.(r3 + ..), k.Y
@@ -251,17 +252,30 @@ __device__ __forceinline__ float quad_sum(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-// d0, d1 += A B over planes, lo x lo left out.
-template <int PA, int PB>
+// d0, d1 += A B over planes, lo x lo left out.  The tensor cores cut a sum's
+// last bits at every step, towards zero, so with two planes the small products
+// are summed first (LOW) over all steps and the large ones after them: a third
+// of the cuts happen at full size.
+template <int PA, int PB, bool LOW>
 __device__ __forceinline__ void planes_product(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[PA][4], const uint32_t (&b)[PB][4]) {
 #pragma unroll
   for (int i = 0; i < PA; ++i)
 #pragma unroll
     for (int j = 0; j < PB; ++j) {
-      if (i + j >= (PA > PB ? PA : PB)) continue;
+      if (i + j >= (PA > PB ? PA : PB) || LOW != (i + j > 0)) continue;
       mma(d0, a[i], b[j][0], b[j][1]);
       mma(d1, a[i], b[j][2], b[j][3]);
     }
+}
+// Two neighbours of a tile as the sum of its planes.
+template <int PLANES>
+__device__ __forceinline__ void tile_pair(const __half* tile, uint32_t plane, uint32_t at, float (&f)[2]) {
+#pragma unroll
+  for (int i = 0; i < PLANES; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(tile) + i * plane + at));
+    f[0] = i ? f[0] + v.x : v.x;
+    f[1] = i ? f[1] + v.y : v.y;
+  }
 }
 template <int PLANES, bool TRANS>
 __device__ __forceinline__ void planes_load(uint32_t (&f)[PLANES][4], uint32_t at, uint32_t plane) {
@@ -282,12 +296,29 @@ __device__ __forceinline__ void load_kept(const char* from, int rows, int row0, 
     for (int n = 0; n < PS; ++n) {
       uint4 v = make_uint4(0, 0, 0, 0);
       if (row0 + row < used)
-        v = reinterpret_cast<const uint4*>(from + (static_cast<long long>(n) * rows + row0) * W * 2)[at];
+        v = __ldg(reinterpret_cast<const uint4*>(from + (static_cast<long long>(n) * rows + row0) * W * 2) + at);
       __half2* h = reinterpret_cast<__half2*>(&v);
 #pragma unroll
       for (int e = 0; e < 4; ++e) h[e] = __hmul2(h[e], f);
       reinterpret_cast<uint4*>(tile + n * kGradBlock * W * 2)[at] = v;
     }
+  }
+}
+
+// Asks L2 for what a block will read of a (chunk, value head).
+template <int PS, int DK>
+__device__ __forceinline__ void prefetch_kept(const DeltaParams& p, long long head, int tid) {
+  const int used = p.slabs * 16;
+  const auto ask = [&](const char* from, int bytes) {
+    for (int at = tid * 128; at < bytes; at += kGradThreads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + at));
+  };
+#pragma unroll
+  for (int n = 0; n < PS; ++n) {
+    const long long wide = static_cast<long long>(n) * p.rows * DK * 2, narrow = static_cast<long long>(n) * p.rows * kChunk * 2;
+    ask(p.states + kept_at<PS, DK>(p, head) + wide, used * DK * 2);
+    ask(p.dstates + kept_at<PS, DK>(p, head) + wide, used * DK * 2);
+    ask(p.us + kept_at<PS, kChunk>(p, head) + narrow, used * kChunk * 2);
+    ask(p.dxs + kept_at<PS, kChunk>(p, head) + narrow, used * kChunk * 2);
   }
 }
 
@@ -317,6 +348,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
   const int r0 = rb * 16 + (lane >> 2);
   const uint32_t kt = shared_u32(s.tile[0][0]), qt = shared_u32(s.tile[1][0]);
   const int group = p.hv / p.hk, used = p.slabs * 16;
+  prefetch_kept<PS, DK>(p, static_cast<long long>(chunk) * p.hv + kh * group, tid);
   {
     const uint4* from = reinterpret_cast<const uint4*>(p.tiles + (static_cast<long long>(chunk) * p.hk + kh) * L::kTiles);
 #pragma unroll
@@ -345,6 +377,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
       s.tail[tid] = expf((coef[kSumHi * kChunk + kChunk - 1] - hi) + (coef[kSumLo * kChunk + kChunk - 1] - lo));
     }
     const float decay = coef[kDecay * kChunk];
+    if (sub + 1 < group) prefetch_kept<PS, DK>(p, head_at + 1, tid);
     // do: 8 threads a row, 8 features each of both blocks; one scale a row
     const int o_row = tid >> 3, o_col = (tid & 7) * 8;
     float o[2][8] = {};
@@ -434,14 +467,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t at = tile_at<kChunk>(row + e, t >> 3) + (t & 7) * 2;
-          float x = 0.f;
 #pragma unroll
-          for (int n = 0; n < PS; ++n) x += __half2float(*reinterpret_cast<const __half*>(reinterpret_cast<const char*>(s.in.x) + n * kNarrow + at));
-          xv = fmaf(x, v[e], xv);
+          for (int n = 0; n < PS; ++n)
+            xv = fmaf(__half2float(*reinterpret_cast<const __half*>(reinterpret_cast<const char*>(s.in.x) + n * kNarrow + at)), v[e], xv);
         }
 #pragma unroll
         for (int i = 0; i < kGradBlock * DK / 8 / kGradThreads; ++i) {
-          float f[8] = {}, g[8] = {};
+          float f[8], g[8];
 #pragma unroll
           for (int n = 0; n < PS; ++n) {
             const uint4 a = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s.in.s) + n * kWide)[i * kGradThreads + tid];
@@ -449,14 +481,19 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 x = __half22float2(reinterpret_cast<const __half2*>(&a)[e]), y = __half22float2(reinterpret_cast<const __half2*>(&b)[e]);
-              f[2 * e] += x.x, f[2 * e + 1] += x.y, g[2 * e] += y.x, g[2 * e + 1] += y.y;
+              if (n == 0)
+                f[2 * e] = x.x, f[2 * e + 1] = x.y, g[2 * e] = y.x, g[2 * e + 1] = y.y;
+              else
+                f[2 * e] += x.x, f[2 * e + 1] += x.y, g[2 * e] += y.x, g[2 * e + 1] += y.y;
             }
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) sd = fmaf(f[e], g[e], sd);
         }
       }
-#pragma unroll
+      const auto products = [&](auto low) {
+      constexpr bool LOW = decltype(low)::value;
+#pragma unroll(PS > 1 ? 1 : kGradBlock / 16)
       for (int kk = 0; kk < kGradBlock / 16; ++kk) {
         uint32_t fo[PS][4], fu[PS][4], fx[PS][4], b[PS][4];
         planes_load<PS, false>(fo, ot + at_mk<kGradBlock>(lane, rb * 16, kk * 16), kNarrow);
@@ -466,15 +503,18 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
         for (int n = 0; n < NT / 2; ++n) {
           const uint32_t at = at_kn<DK>(lane, cg * (DK / 4) + n * 16, kk * 16);
           planes_load<PS, true>(b, st + at, kWide);
-          planes_product<PS, PS>(a_q[2 * n], a_q[2 * n + 1], fo, b);
-          planes_product<PS, PS>(a_x[2 * n], a_x[2 * n + 1], fx, b);
+          planes_product<PS, PS, LOW>(a_q[2 * n], a_q[2 * n + 1], fo, b);
+          planes_product<PS, PS, LOW>(a_x[2 * n], a_x[2 * n + 1], fx, b);
           planes_load<PS, true>(b, dt + at, kWide);
-          planes_product<PS, PS>(a_u[2 * n], a_u[2 * n + 1], fu, b);
+          planes_product<PS, PS, LOW>(a_u[2 * n], a_u[2 * n + 1], fu, b);
         }
         planes_load<PS, true>(b, ut + at_kn<kChunk>(lane, cg * 16, kk * 16), kNarrow);
-        planes_product<PS, PS>(a_p[0], a_p[1], fo, b);
-        planes_product<PS, PS>(a_a[0], a_a[1], fx, b);
+        planes_product<PS, PS, LOW>(a_p[0], a_p[1], fo, b);
+        planes_product<PS, PS, LOW>(a_a[0], a_a[1], fx, b);
       }
+      };
+      if constexpr (PS > 1) products(std::true_type{});
+      products(std::false_type{});
     }
 #pragma unroll
     for (int w = 16; w >= 1; w >>= 1) sd += __shfl_xor_sync(0xffffffffu, sd, w);
@@ -483,30 +523,33 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
 
     // parts of dq and dk that see the states, and their products with q and k
     float dot[4][2] = {};
+    float to_one[2], to_two[2], to_three[2], beta[2];  // of this lane's rows
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = r0 + h * 8;
+      to_one[h] = -s.down[i] * (common[3] * common[0]);
+      to_two[h] = p.scale * s.down[i] * (s.orow[i] * common[0]);
+      to_three[h] = s.tail[i] * (common[2] * common[1]);
+      beta[h] = s.beta[i];
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int i = r0 + h * 8;
         const uint32_t at = tile_at<DK>(i, cg * (DK / 32) + n) + (lane & 3) * 4;
-        float kv[2] = {}, qv[2] = {};
-#pragma unroll
-        for (int plane = 0; plane < IN; ++plane) {
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(s.tile[0][plane]) + at));
-          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(s.tile[1][plane]) + at));
-          kv[0] += a.x, kv[1] += a.y, qv[0] += b.x, qv[1] += b.y;
-        }
+        float kv[2], qv[2];
+        tile_pair<IN>(s.tile[0][0], L::kTile, at, kv);
+        tile_pair<IN>(s.tile[1][0], L::kTile, at, qv);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int at_e = 2 * h + e;
-          const float one = -s.down[i] * (a_x[n][at_e] * (common[3] * common[0]));
-          const float two = p.scale * s.down[i] * (a_q[n][at_e] * (s.orow[i] * common[0]));
-          const float three = s.tail[i] * (a_u[n][at_e] * (common[2] * common[1]));
+          const float one = to_one[h] * a_x[n][at_e], two = to_two[h] * a_q[n][at_e], three = to_three[h] * a_u[n][at_e];
           dot[0][h] = fmaf(kv[e], one, dot[0][h]);
           dot[1][h] = fmaf(qv[e], two, dot[1][h]);
           dot[2][h] = fmaf(kv[e], three, dot[2][h]);
           dq[n][at_e] += two;
-          dk[n][at_e] += fmaf(s.beta[i], one, three);
+          dk[n][at_e] += fmaf(beta[h], one, three);
         }
       }
     // sum of H = e^{G_C - G} k . (U D^T) over the chunk, before the rest joins that dot
@@ -514,21 +557,34 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
 
     // N, Gamma dA and B with the row factors of what they meet
     float sq[4][2][4], top[4] = {};
+    {
+      float row_hi[2], row_lo[2], row_n[2], row_q[2], row_k[2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = r0 + (e >> 1) * 8, j = cg * 16 + n * 8 + (lane & 3) * 2 + (e & 1);
-        const float gamma = j <= i ? expf((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j])) : 0.f;
-        const float nn = j <= i ? gamma * (p.scale * (a_p[n][e] * (s.orow[i] * common[2]))) : 0.f;
-        const float ga = j < i ? -gamma * (a_a[n][e] * (common[3] * common[2])) : 0.f;
-        sq[0][n][e] = nn * s.krow[j];
-        sq[1][n][e] = nn * s.qrow[i];
-        sq[2][n][e] = ga * s.krow[j];
-        sq[3][n][e] = s.beta[i] * ga * s.krow[i];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) top[w] = fmaxf(top[w], fabsf(sq[w][n][e]));
+      for (int h = 0; h < 2; ++h) {
+        const int i = r0 + h * 8;
+        row_hi[h] = s.hi[i], row_lo[h] = s.lo[i], row_q[h] = s.qrow[i], row_k[h] = beta[h] * s.krow[i];
+        row_n[h] = p.scale * (s.orow[i] * common[2]);
       }
+      const float to_a = -(common[3] * common[2]);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int j0 = cg * 16 + n * 8 + (lane & 3) * 2;
+        const float2 hi = *reinterpret_cast<const float2*>(&s.hi[j0]), lo = *reinterpret_cast<const float2*>(&s.lo[j0]),
+                     kj = *reinterpret_cast<const float2*>(&s.krow[j0]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int h = e >> 1, i = r0 + h * 8, j = j0 + (e & 1);
+          const float gamma = exp_fast((row_hi[h] - (e & 1 ? hi.y : hi.x)) + (row_lo[h] - (e & 1 ? lo.y : lo.x)));
+          const float nn = j <= i ? gamma * (row_n[h] * a_p[n][e]) : 0.f, ga = j < i ? gamma * (to_a * a_a[n][e]) : 0.f;
+          sq[0][n][e] = nn * (e & 1 ? kj.y : kj.x);
+          sq[1][n][e] = nn * row_q[h];
+          sq[2][n][e] = ga * (e & 1 ? kj.y : kj.x);
+          sq[3][n][e] = ga * row_k[h];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) top[w] = fmaxf(top[w], fabsf(sq[w][n][e]));
+        }
+      }
+    }
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const unsigned int m = __reduce_max_sync(0xffffffffu, __float_as_uint(top[w]));
@@ -558,7 +614,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
       float b_q[NT][4] = {}, b_n[NT][4] = {}, b_y[NT][4] = {}, b_t[NT][4] = {};
       const uint32_t base = shared_u32(s.square);
       constexpr uint32_t one = PS * kSq;
-#pragma unroll
+      const auto products = [&](auto low) {
+      constexpr bool LOW = decltype(low)::value;
+#pragma unroll(PS > 1 ? 1 : 4)
       for (int kk = 0; kk < 4; ++kk) {
         const uint32_t mk = at_mk<kChunk>(lane, rb * 16, kk * 16), km = at_km<kChunk>(lane, rb * 16, kk * 16);
         uint32_t a[PS][4], g[PS][4], b[IN][4];
@@ -568,8 +626,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
 #pragma unroll
           for (int n = 0; n < NT / 2; ++n) {
             planes_load<IN, true>(b, kt + at_kn<DK>(lane, cg * (DK / 4) + n * 16, kk * 16), L::kTile);
-            planes_product<PS, IN>(b_q[2 * n], b_q[2 * n + 1], a, b);
-            planes_product<PS, IN>(b_y[2 * n], b_y[2 * n + 1], g, b);
+            planes_product<PS, IN, LOW>(b_q[2 * n], b_q[2 * n + 1], a, b);
+            planes_product<PS, IN, LOW>(b_y[2 * n], b_y[2 * n + 1], g, b);
           }
         }
         if (kk >= rb) {
@@ -579,25 +637,24 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
           for (int n = 0; n < NT / 2; ++n) {
             const uint32_t at = at_kn<DK>(lane, cg * (DK / 4) + n * 16, kk * 16);
             planes_load<IN, true>(b, qt + at, L::kTile);
-            planes_product<PS, IN>(b_n[2 * n], b_n[2 * n + 1], a, b);
+            planes_product<PS, IN, LOW>(b_n[2 * n], b_n[2 * n + 1], a, b);
             planes_load<IN, true>(b, kt + at, L::kTile);
-            planes_product<PS, IN>(b_t[2 * n], b_t[2 * n + 1], g, b);
+            planes_product<PS, IN, LOW>(b_t[2 * n], b_t[2 * n + 1], g, b);
           }
         }
       }
+      };
+      if constexpr (PS > 1) products(std::true_type{});
+      products(std::false_type{});
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int i = r0 + h * 8;
           const uint32_t at = tile_at<DK>(i, cg * (DK / 32) + n) + (lane & 3) * 4;
-          float kv[2] = {}, qv[2] = {};
-#pragma unroll
-          for (int plane = 0; plane < IN; ++plane) {
-            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(s.tile[0][plane]) + at));
-            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(s.tile[1][plane]) + at));
-            kv[0] += x.x, kv[1] += x.y, qv[0] += y.x, qv[1] += y.y;
-          }
+          float kv[2], qv[2];
+          tile_pair<IN>(s.tile[0][0], L::kTile, at, kv);
+          tile_pair<IN>(s.tile[1][0], L::kTile, at, qv);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int at_e = 2 * h + e;
@@ -607,7 +664,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
             dot[2][h] = fmaf(kv[e], three, dot[2][h]);
             dot[3][h] = fmaf(kv[e], y, dot[3][h]);
             dq[n][at_e] += two;
-            dk[n][at_e] += fmaf(s.beta[i], y, three);
+            dk[n][at_e] += fmaf(beta[h], y, three);
           }
         }
     }

@@ -111,9 +111,6 @@ __device__ __forceinline__ int unit_of(int i, int id) { return (i & 1) + 4 * (i 
 
 __device__ __forceinline__ void head_sync(int head) { asm volatile("bar.sync %0, 128;" ::"r"(head + 1) : "memory"); }
 
-// e^x by the hardware's 2^x: off by 2^-22 |x| relative, that is below 2^-23 of 1.
-__device__ __forceinline__ float exp_fast(float x) { return exp2f(x * 1.4426950408889634f); }
-
 // c = sign a b, N x N each inside the 64 x 64 matrix; a thread computes R rows
 // of 4 columns.  LOWER_B / LOWER_A: that operand is lower triangular in blocks
 // of 16 and holds other values above.
