@@ -284,26 +284,39 @@ __device__ __forceinline__ void planes_load(uint32_t (&f)[PLANES][4], uint32_t a
     if (TRANS) ldsm_t(f[i], at + i * plane); else ldsm(f[i], at + i * plane);
 }
 
-// Rows [row0, row0 + 64) of kept planes into a tile, times their rows' ratios.
+// Rows [row0, row0 + 64) of kept planes: into registers, and from there, times
+// their rows' ratios, into a tile.
 template <int PS, int W>
-__device__ __forceinline__ void load_kept(const char* from, int rows, int row0, int used, const float* ratio, char* tile, int tid) {
-  constexpr int UNITS = kGradBlock * W / 8;
+struct Kept {
+  static constexpr int kUnits = kGradBlock * W / 8 / kGradThreads;
+  uint4 v[kUnits][PS];
+  __device__ __forceinline__ void fetch(const char* from, int rows, int row0, int used, int tid) {
 #pragma unroll
-  for (int i = 0; i < UNITS / kGradThreads; ++i) {
-    const int at = i * kGradThreads + tid, row = at / (W / 8);
-    const __half2 f = __float2half2_rn(row0 + row < used ? ratio[row0 + row] : 0.f);
+    for (int i = 0; i < kUnits; ++i) {
+      const int at = i * kGradThreads + tid;
 #pragma unroll
-    for (int n = 0; n < PS; ++n) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row0 + row < used)
-        v = __ldg(reinterpret_cast<const uint4*>(from + (static_cast<long long>(n) * rows + row0) * W * 2) + at);
-      __half2* h = reinterpret_cast<__half2*>(&v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = __hmul2(h[e], f);
-      reinterpret_cast<uint4*>(tile + n * kGradBlock * W * 2)[at] = v;
+      for (int n = 0; n < PS; ++n) {
+        v[i][n] = make_uint4(0, 0, 0, 0);
+        if (row0 + at / (W / 8) < used)
+          v[i][n] = __ldg(reinterpret_cast<const uint4*>(from + (static_cast<long long>(n) * rows + row0) * W * 2) + at);
+      }
     }
   }
-}
+  __device__ __forceinline__ void put(const float* ratio, int row0, int used, char* tile, int tid) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int at = i * kGradThreads + tid, row = row0 + at / (W / 8);
+      const __half2 f = __float2half2_rn(row < used ? ratio[row] : 0.f);
+#pragma unroll
+      for (int n = 0; n < PS; ++n) {
+        __half2* h = reinterpret_cast<__half2*>(&v[i][n]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = __hmul2(h[e], f);
+        reinterpret_cast<uint4*>(tile + n * kGradBlock * W * 2)[at] = v[i][n];
+      }
+    }
+  }
+};
 
 // Asks L2 for what a block will read of a (chunk, value head).
 template <int PS, int DK>
@@ -366,38 +379,56 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
     const int vh = kh * group + sub;
     const long long head_at = static_cast<long long>(chunk) * p.hv + vh;
     const float* coef = reinterpret_cast<const float*>(p.heads + head_at * L::kHead + L::kT + L::kP);
-    __syncthreads();
-    if (tid < 4) s.common[tid] = s.most[tid] = 0;
+    // everything that the head's first steps need is on its way before any of it is waited for
+    Kept<PS, DK> ks, kd;
+    Kept<PS, kChunk> ku, kx;
+    const auto fetch = [&](int v0) {
+      ks.fetch(p.states + kept_at<PS, DK>(p, head_at), p.rows, v0, used, tid);
+      kd.fetch(p.dstates + kept_at<PS, DK>(p, head_at), p.rows, v0, used, tid);
+      ku.fetch(p.us + kept_at<PS, kChunk>(p, head_at), p.rows, v0, used, tid);
+      kx.fetch(p.dxs + kept_at<PS, kChunk>(p, head_at), p.rows, v0, used, tid);
+    };
+    const float decay = __ldg(coef + kDecay * kChunk);
+    const int kind = tid >> 7, scale_row = tid & 127;
+    const float row_scale = scale_row < used ? __ldg(p.scales + (head_at * 4 + kind) * p.rows + scale_row) : 0.f;
+    float c_hi = 0.f, c_lo = 0.f, c_beta = 0.f, c_last = 0.f, c_last_lo = 0.f;
     if (tid < kChunk) {
-      const float hi = coef[kSumHi * kChunk + tid], lo = coef[kSumLo * kChunk + tid];
-      s.beta[tid] = coef[kBeta * kChunk + tid];
-      s.hi[tid] = hi;
-      s.lo[tid] = lo;
-      s.down[tid] = exp_sum(hi, lo);
-      s.tail[tid] = expf((coef[kSumHi * kChunk + kChunk - 1] - hi) + (coef[kSumLo * kChunk + kChunk - 1] - lo));
+      c_hi = __ldg(coef + kSumHi * kChunk + tid), c_lo = __ldg(coef + kSumLo * kChunk + tid);
+      c_beta = __ldg(coef + kBeta * kChunk + tid);
+      c_last = __ldg(coef + kSumHi * kChunk + kChunk - 1), c_last_lo = __ldg(coef + kSumLo * kChunk + kChunk - 1);
     }
-    const float decay = coef[kDecay * kChunk];
-    if (sub + 1 < group) prefetch_kept<PS, DK>(p, head_at + 1, tid);
     // do: 8 threads a row, 8 features each of both blocks; one scale a row
     const int o_row = tid >> 3, o_col = (tid & 7) * 8;
     float o[2][8] = {};
-    {
+    if (o_row < c.len) {
       const T* from = static_cast<const T*>(p.d_o) + c.batch * p.do_batch + (c.token + o_row) * p.do_token + vh * p.do_head;
-      if (o_row < c.len)
+      constexpr int V = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int col = b * kGradBlock + o_col;
-          constexpr int V = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;
-          if (p.vec_do) {
+      for (int b = 0; b < 2; ++b) {
+        const int col = b * kGradBlock + o_col;
+        if (p.vec_do) {
 #pragma unroll
-            for (int e = 0; e < 8; e += V)
-              if (col + e < p.dv) load<T, V>(from + col + e, *reinterpret_cast<float(*)[V]>(&o[b][e]));
-          } else {
+          for (int e = 0; e < 8; e += V)
+            if (col + e < p.dv) load<T, V>(from + col + e, *reinterpret_cast<float(*)[V]>(&o[b][e]));
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (col + e < p.dv) o[b][e] = up(from[col + e]);
-          }
+          for (int e = 0; e < 8; ++e)
+            if (col + e < p.dv) o[b][e] = up(from[col + e]);
         }
+      }
+    }
+    fetch(0);
+    if (sub + 1 < group) prefetch_kept<PS, DK>(p, head_at + 1, tid);
+    __syncthreads();  // the last head is done with
+    if (tid < 4) s.common[tid] = s.most[tid] = 0;
+    if (tid < kChunk) {
+      s.beta[tid] = c_beta;
+      s.hi[tid] = c_hi;
+      s.lo[tid] = c_lo;
+      s.down[tid] = exp_sum(c_hi, c_lo);
+      s.tail[tid] = expf((c_last - c_hi) + (c_last_lo - c_lo));
+    }
+    {
       float m = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaxf(fabsf(o[0][e]), fabsf(o[1][e])));
@@ -409,8 +440,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
       for (int e = 0; e < 8; ++e) o[0][e] *= f.f, o[1][e] *= f.f;
     }
     // scales of the kept planes: the largest of each kind is the common one
-    const int kind = tid >> 7, scale_row = tid & 127;
-    const float row_scale = scale_row < used ? p.scales[(head_at * 4 + kind) * p.rows + scale_row] : 0.f;
     {
       const unsigned int m = __reduce_max_sync(0xffffffffu, __float_as_uint(row_scale));
       // non-negative floats order as integers: the maximum does not depend on the order
@@ -427,12 +456,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
     float sd = 0.f, xv = 0.f;
 #pragma unroll 1
     for (int block = 0; block * kGradBlock < used; ++block) {
-      __syncthreads();
       const int v0 = block * kGradBlock;
-      load_kept<PS, DK>(p.states + kept_at<PS, DK>(p, head_at), p.rows, v0, used, s.ratio[0], reinterpret_cast<char*>(s.in.s), tid);
-      load_kept<PS, DK>(p.dstates + kept_at<PS, DK>(p, head_at), p.rows, v0, used, s.ratio[1], reinterpret_cast<char*>(s.in.d), tid);
-      load_kept<PS, kChunk>(p.us + kept_at<PS, kChunk>(p, head_at), p.rows, v0, used, s.ratio[2], reinterpret_cast<char*>(s.in.u), tid);
-      load_kept<PS, kChunk>(p.dxs + kept_at<PS, kChunk>(p, head_at), p.rows, v0, used, s.ratio[3], reinterpret_cast<char*>(s.in.x), tid);
+      if (block) fetch(v0);
+      __syncthreads();
+      ks.put(s.ratio[0], v0, used, reinterpret_cast<char*>(s.in.s), tid);
+      kd.put(s.ratio[1], v0, used, reinterpret_cast<char*>(s.in.d), tid);
+      ku.put(s.ratio[2], v0, used, reinterpret_cast<char*>(s.in.u), tid);
+      kx.put(s.ratio[3], v0, used, reinterpret_cast<char*>(s.in.x), tid);
       {
         Vec<uint32_t, 4> plane[2];
 #pragma unroll
