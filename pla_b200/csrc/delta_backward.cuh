@@ -122,7 +122,6 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
     shared_of(m.most_d, m0, lane, most_g);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      if (VB == 64 && kk < wn) continue;  // the other blocks are zero
       uint32_t hi[4], lo[4];
       float bx[2][4];
       tile_operand<PO>(yw[kk] + (wt - yt), M::kNarrow, hi, lo);
@@ -143,7 +142,6 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
     shared_of(m.scale_a, m0, lane, back);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      if (VB == 64 && kk < wn) continue;  // the other blocks are zero
       uint32_t hi[4], lo[4];
       float bx[2][4];
       tile_operand<PS>(yw[kk], M::kNarrow, hi, lo);

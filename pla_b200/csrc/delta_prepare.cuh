@@ -40,28 +40,30 @@ struct PrepShared {
   unsigned int bound[HEADS][4];       // kBounds
 };
 
-// Rows of q and k as planes, in shared memory and in the workspace; eight
-// rows of both are in flight at a time.
+// Rows of q and k as planes, in shared memory and in the workspace; a warp's
+// rows of both are all in flight at once (fp32: eight at a time).
 template <typename T, int DK, int HEADS, typename S>
 __device__ __forceinline__ void prepare_rows(const DeltaParams& p, const T* k, const T* q, int len, int lane, int warp, S& s,
                                              char* out) {
-  constexpr int IN = DeltaType<T>::kIn, E = DK / 32, ROWS = kChunk / (4 * HEADS), U = 8;
+  constexpr int IN = DeltaType<T>::kIn, E = DK / 32, ROWS = kChunk / (4 * HEADS), U = sizeof(T) == 2 ? ROWS : 8;
 #pragma unroll 1
   for (int base = 0; base < ROWS; base += U) {
-    float f[2][U][E] = {};
+    Vec<T, E> raw[2][U];
 #pragma unroll
     for (int side = 0; side < 2; ++side)
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int row = warp * ROWS + base + i;
+#pragma unroll
+        for (int e = 0; e < E; ++e) raw[side][i].e[e] = down<T>(0.f);
         if (row < len) {
-          const T* r = side ? q + row * p.q_token : k + row * p.k_token;
+          const T* r = (side ? q + row * p.q_token : k + row * p.k_token) + lane * E;
           if (p.vec_qk) {
-            if (lane * E < p.dk) load<T, E>(r + lane * E, f[side][i]);
+            if (lane * E < p.dk) raw[side][i] = *reinterpret_cast<const Vec<T, E>*>(r);
           } else {
 #pragma unroll
             for (int e = 0; e < E; ++e)
-              if (lane * E + e < p.dk) f[side][i][e] = up(r[lane * E + e]);
+              if (lane * E + e < p.dk) raw[side][i].e[e] = r[e];
           }
         }
       }
@@ -70,9 +72,10 @@ __device__ __forceinline__ void prepare_rows(const DeltaParams& p, const T* k, c
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int row = warp * ROWS + base + i;
-        float m = 0.f;
+        float f[E], m = 0.f;
+        unpack(raw[side][i], f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) m = fmaxf(m, fabsf(f[side][i][e]));
+        for (int e = 0; e < E; ++e) m = fmaxf(m, fabsf(f[e]));
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const Pow2 scale = pow2_for(m);
@@ -82,8 +85,7 @@ __device__ __forceinline__ void prepare_rows(const DeltaParams& p, const T* k, c
         }
         Vec<uint32_t, E / 2> plane[2];
 #pragma unroll
-        for (int e = 0; e < E / 2; ++e)
-          split<IN>(f[side][i][2 * e] * scale.f, f[side][i][2 * e + 1] * scale.f, &plane[0].e[e], &plane[1].e[e]);
+        for (int e = 0; e < E / 2; ++e) split<IN>(f[2 * e] * scale.f, f[2 * e + 1] * scale.f, &plane[0].e[e], &plane[1].e[e]);
         const uint32_t at = tile_at<DK>(row, lane * E / 8) + (lane * E % 8) * 2;
 #pragma unroll
         for (int n = 0; n < IN; ++n) {
@@ -164,7 +166,7 @@ __device__ __forceinline__ void load_gates(const DeltaParams& p, const ChunkAt& 
 }
 
 template <typename T, int DK, int PS, int PO, int HEADS>
-__global__ void __launch_bounds__(128 * HEADS, HEADS == 2 ? 3 : 5) delta_prepare(DeltaParams p) {
+__global__ void __launch_bounds__(128 * HEADS, 3) delta_prepare(DeltaParams p) {
   using L = DeltaLayout<T, DK, PS, PO>;
   extern __shared__ __align__(16) char shared_bytes[];
   PrepShared<T, DK, HEADS>& s = *reinterpret_cast<PrepShared<T, DK, HEADS>*>(shared_bytes);

@@ -2,7 +2,7 @@
 // (delta_common.cuh has the mathematics).
 //
 // The columns of S (one per value feature) never meet, so a block takes VB of
-// them (16, 32 or 64) through the whole sequence on its own.  Every product of
+// them (16 or 32) through the whole sequence on its own.  Every product of
 // a chunk has the value features as its rows,
 //     (K S)^T = S^T K^T,  U^T = X^T T^T,  O^T = S^T Q^T + U^T P^T,  S^T += U^T K,
 // so that K, Q, T and P are always the right operand, read by ldmatrix from
@@ -14,7 +14,10 @@
 // instructions a warp, and operands pass between the warps through shared
 // memory as planes (one barrier a step).  One warp that kept all of S^T in
 // registers instead needed no barrier, but its 400 products and 1500 other
-// instructions a chunk took 8.6 us where this takes KSWEEP us (bf16, Dk = 128).
+// instructions a chunk took 8.6 us where this takes 2.8 us (bf16, Dk = 128).
+// A chunk's 112 products a warp are a third of that; the rest is the wait for
+// operands and barriers, which more warps an SM or more products at a time do
+// not shorten.
 //
 // A row's planes take one scale wherever a bound gives it before the warps
 // have met: |U| <= max_i sum_j |T_ij| max|X| (delta_prepare has the sums), and
@@ -536,13 +539,13 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
       tile_write<PS, kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, x, fx);
     }
     __syncthreads();
-    // U^T = X^T T^T, T lower triangular
+    // U^T = X^T T^T; T is lower triangular, but the warp with the last tokens needs every step,
+    // and steps without a branch overlap
     float u[2][4] = {};
     float4 back[2];
     shared_of(m.scale_a, m0, lane, back);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      if (VB == 64 && kk > wn) break;  // T's other blocks are zero
       uint32_t hi[4], lo[4];
       float bu[2][4];
       tile_operand<PS>(xw[kk], M::kNarrow, hi, lo);
@@ -592,7 +595,6 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
         float pu[2][4];
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
-          if (VB == 64 && kk > wn) break;
           uint32_t hi[4], lo[4];
           tile_operand<PO>(xw[kk] + (vt - xt), M::kNarrow, hi, lo);
           product<PO, PO, false>(pu[0], pu[1], hi, lo, pt + tw[kk], L::kSquare, kk == 0);

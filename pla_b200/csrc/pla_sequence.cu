@@ -422,25 +422,23 @@ struct SweepShape {
 };
 
 // Value features of a sweep's block.  A block's time is the latency of its
-// chunks' chain whatever it holds, so while every block has an SM of its own:
-// the fewest features that still leave it so.  With more blocks than SMs two
-// of 32 features side by side fill each other's waits, if their shared memory
-// fits; else 64 features share one copy of a chunk's tiles.
-//   8192 tokens x 32 heads of 128, bf16: SWEEPRULE
-// f(shape)
+// chunks' chain, nearly whatever it holds, so while every block has an SM of
+// its own: the fewest features that still leave it so (1001 tokens x 16 heads
+// of 128, fp16: 28 us with 16, 42 with 32; 4096 tokens x 32 heads, bf16: 177 us
+// with 32, 291 with 64).  With more blocks than SMs: of a batch, whose rows are
+// equally long, two blocks of 32 an SM, if they fit, fill each other's waits
+// (8 x 2048 tokens x 32 heads, bf16: 565 us; one block of 32: 620, of 64: 588);
+// of a ragged batch one block of 32, because the longest sequence's blocks, the
+// first to start, decide (16383 tokens in three, 32 heads: 631 us; two of 32:
+// 692, one of 64: 650).  f(shape)
 template <typename T, int DK, int PS, int PO, bool BACK, typename F>
 int with_columns(const DeltaParams& p, int sms, F&& f) {
   using Two = SweepShape<T, DK, PS, PO, 32, 2, BACK>;
-  using Wide = SweepShape<T, DK, PS, PO, 64, 1, BACK>;
   const long long heads = static_cast<long long>(p.sequences) * p.hv;
   if (p.dv <= 16 || heads * ((p.dv + 15) / 16) <= sms) return f(SweepShape<T, DK, PS, PO, 16, 1, BACK>{});
-  if (p.dv <= 32 || heads * ((p.dv + 31) / 32) <= sms) return f(SweepShape<T, DK, PS, PO, 32, 1, BACK>{});
   if constexpr (Two::kStages >= 1)
-    return f(Two{});
-  else if constexpr (Wide::kStages >= 2)
-    return f(Wide{});
-  else
-    return f(SweepShape<T, DK, PS, PO, 32, 1, BACK>{});
+    if (!p.cu && heads * ((p.dv + 31) / 32) > sms) return f(Two{});
+  return f(SweepShape<T, DK, PS, PO, 32, 1, BACK>{});
 }
 
 template <typename T, int DK, int PS, int PO, bool KEEP>
