@@ -30,7 +30,6 @@ NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-    "-split-compile=0",  # a unit's kernels are optimised side by side
 ]
 LINK_FLAGS = ["-shared", "-Xlinker", "-soname=libpla_b200.so"]
 

@@ -11,7 +11,7 @@
 // eight rows is in flight, each refilled as soon as it is used.  Four channels
 // (8 bytes a 16-bit load) and not eight: eight took 148 registers a thread,
 // which left 8 warps an SM and too few bytes in flight (140 us for 8191 x 8192
-// bf16, against CAUSALFWD).  The products are summed in fp32 in tap
+// bf16, against 59).  The products are summed in fp32 in tap
 // order, two channels an instruction, and rounded once.
 //
 // Backward, with dp[t] = dy[t] act'(p[t]) recomputed from x:
@@ -20,7 +20,9 @@
 // K pending dx it reaches inside the same sequence, and keeps dw / db of its
 // own strip in registers.  The strips of a block are added in shared memory,
 // the blocks' partial sums in a second kernel, both in a fixed order: no
-// atomics, so the same inputs give the same bits.
+// atomics, so the same inputs give the same bits.  2 x 4096 x 4096 bf16: 74 us,
+// 2.7 TB/s (three passes over the data); two channels a thread, because it
+// holds five times the forward's registers.
 #pragma once
 
 #include "seq_common.cuh"
