@@ -258,14 +258,16 @@ int norm_lanes(const pla_qk_norm* a, bool wide) { return !wide || a->dim > 128 ?
 
 // Blocks of one side in the backward pass: a number of groups that is a
 // multiple of the heads (a group keeps its head), a few turns each so that a
-// block's partial sum is small beside what it reads, no more than the device
-// holds at a time.
+// block's partial sum is small beside what it reads, and both sides together
+// no more than run at a time, each by its share of the heads (4094 tokens of 32
+// heads of 96, fp16: 36 us; twice as many blocks 37, half as many again 45).
 int norm_side_blocks(const pla_qk_norm* a, int heads, int lanes) {
   const long long rows = static_cast<long long>(a->batch) * a->tokens * heads;
   if (!rows) return 0;
   const int groups = kNormThreads / lanes, step = heads / std::gcd(heads, groups);
-  const long long want = std::min<long long>((rows + groups * 4 - 1) / (groups * 4), 148 * 4);
-  return static_cast<int>(std::max<long long>(1, (want + step - 1) / step) * step);
+  const long long most = 148ll * 2 * heads / (static_cast<long long>(a->q.heads) + a->k.heads);
+  const long long want = std::min((rows + groups * 4 - 1) / (groups * 4), most);
+  return static_cast<int>(std::max<long long>(1, want / step) * step);
 }
 
 // ---- gated delta rule ------------------------------------------------------
@@ -641,13 +643,17 @@ int pla_qk_norm_rotate_forward(const pla_qk_norm* a, pla_stream_t stream) {
   p.units[0] = (a->q.heads + hb - 1) / hb;
   p.units[1] = (a->k.heads + hb - 1) / hb;
   const int units = p.units[0] + p.units[1];
-  // a few times the blocks that the device holds at a time, each group walking tokens
   const long long whole = (static_cast<long long>(a->tokens) * units + groups - 1) / groups;
-  const long long share = std::max<long long>(1, sms * 8ll / a->batch);
-  // a number of groups that is a multiple of the units, so that a group keeps its unit
+  // Several heads a group: no more blocks than run at a time, two an SM, each group walking tokens; one block more
+  // is a second walk (8192 tokens of 40 heads of 128, bf16: 45 us; 300 blocks on 296 places 68; 1180 blocks 50).
+  // Where batch rows leave an eighth of the places empty that way, and with single heads a group, whose blocks are
+  // lighter (8192 tokens of 16 heads of 250, fp16: 69 us, with two an SM 82): eight an SM.  Always a number of
+  // groups that is a multiple of the units, so that a group keeps its unit.
   const int step = units / std::gcd(units, groups);
-  const long long blocks = whole <= share ? whole : (share + step - 1) / step * step;
-  p.stride = whole <= share ? a->tokens : static_cast<int>(blocks * groups / units);
+  long long blocks = hb > 1 ? sms * 2ll / a->batch / step * step : 0;
+  if (blocks * a->batch * 8 < sms * 2ll * 7) blocks = std::max<long long>(1, (sms * 8ll / a->batch + step - 1) / step) * step;
+  p.stride = whole <= blocks ? a->tokens : static_cast<int>(blocks * groups / units);
+  blocks = std::min(blocks, whole);
   const dim3 grid(static_cast<int>(blocks), a->batch);
   if (!wide)
     return with_type(a->dtype, [&](auto zero) {

@@ -17,10 +17,12 @@
 // tokens with their weights in registers: the set's loads are in flight
 // together, the next token's while this one's are worked on, and share the
 // token's cosines and sines.  All arithmetic is fp32 with one rounding at the
-// end.  8192 tokens of 40 heads of 128 in bf16: 50 us, 3.4 TB/s, 52 % of the
+// end.  8192 tokens of 40 heads of 128 in bf16: 45 us, 3.7 TB/s, 57 % of the
 // copy rate; what holds it there is latency (16 warps an SM at 118 registers,
-// 50 % of issue slots), not a pipe.  One token a group without the walk and
-// with 64-bit divisions took 68 us; three blocks an SM at 80 registers spill.
+// half of the issue slots), not a pipe.  One token a group without the walk and
+// with 64-bit divisions took 68 us; three blocks an SM at 80 registers spill;
+// asynchronous copies through shared memory two tokens ahead leave three blocks
+// an SM room and still took 52 us.
 #pragma once
 
 #include "seq_common.cuh"
@@ -153,7 +155,7 @@ __device__ __forceinline__ float group_sum(float v) {
 // 1 / sqrt(v): the hardware's approximation (2^-22) and one Newton step, which
 // leaves a few units of the last place.  No branch, so that the heads of a
 // group overlap (1.f / sqrtf(v) has two; with them 8192 tokens of 40 heads of
-// 128 in bf16 took 56 us, against 50).
+// 128 in bf16 took 56 us where this took 50).
 __device__ __forceinline__ float inverse_root(float v) {
   const float r = rsqrtf(v);
   const float better = r * fmaf(-0.5f * v * r, r, 1.5f);
@@ -360,18 +362,19 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_backward4(NormParams p) 
   int row = group / side.heads;  // batch row and token as one number
   const int h = group - row * side.heads;
   int b = row / p.tokens, t = row - b * p.tokens;
+  const int on_b = stride / p.tokens, on_t = stride - on_b * p.tokens;
   const T* x = static_cast<const T*>(side.x) + h * side.x_head;
   const T* dy = static_cast<const T*>(side.dy) + h * side.dy_head;
   // the next token's head and angles are fetched while this one's are worked on; past the end, the first's
   Raw4<T> x_next, dy_next;
   float c_next[4], s_next[4];
   const auto fetch = [&](int at_row) {
-    while (t >= p.tokens) t -= p.tokens, ++b;
     const int bb = at_row < rows ? b : 0, tt = at_row < rows ? t : 0;
     x_next = raw4(x + bb * side.x_batch + tt * side.x_token, lane);
     dy_next = raw4(dy + bb * side.dy_batch + tt * side.dy_token, lane);
     angles4(p, lane, table_row(p, bb, tt), c_next, s_next);
-    t += stride;
+    t += on_t, b += on_b;
+    if (t >= p.tokens) t -= p.tokens, ++b;
   };
   fetch(row);
   // `stride` tokens on for every turn; a warp's groups make the same number of turns

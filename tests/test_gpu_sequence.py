@@ -251,6 +251,26 @@ def test_norm_strided_views_of_one_projection():
             assert float((a.double() - b.double()).abs().max()) <= 4 * half(dtype) * 8  # other lanes, another order of sums
 
 
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_norm_of_many_short_rows_equals_one_long_row(tokens):
+    # a row's arithmetic does not depend on how rows are counted: equal bits
+    g = torch.Generator().manual_seed(5)
+    n = 601 * tokens
+    q, k = rand(g, 1, n, 3, 128, dtype=BF16), rand(g, 1, n, 1, 128, dtype=BF16)
+    dq, dk = rand(g, *q.shape, dtype=BF16), rand(g, *k.shape, dtype=BF16)
+    angle = torch.randn(50, 64, generator=g)
+    pos = torch.randint(0, 50, (1, n), generator=g)
+    kw = dict(cos=gpu(angle.cos()), sin=gpu(angle.sin()))
+
+    def run(*shape):
+        leaves = [gpu(t.reshape(*shape, *t.shape[2:])).requires_grad_() for t in (q, k)]
+        out = P.qk_norm_rotate(*leaves, positions=gpu(pos.reshape(shape)), **kw)
+        return *out, *torch.autograd.grad(out, leaves, [gpu(t.reshape(*shape, *t.shape[2:])) for t in (dq, dk)])
+
+    for a, b in zip(run(601, tokens), run(1, n)):
+        assert torch.equal(a.flatten(0, 1), b.flatten(0, 1))
+
+
 def test_norm_positions_outside_the_tables_are_nan_and_zero_rows_finite():
     q = torch.zeros(1, 4, 2, 64, device=DEV, dtype=BF16)
     q[:, 2] = 1
