@@ -75,7 +75,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     pairs (i, i + R / 2), or (2i, 2i + 1) with ``interleaved``, by row
     ``positions`` ([T], [1, T] or [B, T] integers; the token's number if
     None).  A position outside the tables gives NaN in the rotated features.
-    D is at most 256.  Differentiable in q, k and the weights.
+    D is at most 256, B at most 65535.  Differentiable in q, k and the weights.
     """
     if norm not in ("rms", "l2"):
         raise ValueError('norm must be "rms" or "l2"')
