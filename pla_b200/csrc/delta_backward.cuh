@@ -20,10 +20,10 @@
 namespace pla {
 namespace seq {
 
-template <typename T, int DK, int PS, int PO, int VB, int STAGES, int PER_SM>
+template <typename T, int DK, int VB, int STAGES, int PER_SM>
 __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p) {
-  using L = DeltaLayout<T, DK, PS, PO>;
-  using M = SweepShared<T, DK, PS, PO, VB, true>;
+  using L = DeltaLayout<T, DK>;
+  using M = SweepShared<T, DK, VB, true>;
   constexpr int IN = L::kIn, QN = DK / 32, kPitch = Slab<T, VB>::kPitch;
   extern __shared__ __align__(128) char shared_bytes[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
     shared_of(m.most_s, m0, lane, all);
     fd[0] = scale_below(most_of(all[0]));
     fd[1] = scale_below(most_of(all[1]));
-    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, fd);
+    tile_write<DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, fd);
   }
 
   for (int turn = 0; turn < a.chunks; ++turn) {
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
     __syncthreads();  // planes of D and this chunk's do are there; the other slab is free
     if (c > 0)
       slab_fetch<T, VB>(m.slab[~turn & 1], d_o + (c - 1) * kChunk * p.do_token, p.do_token, kChunk, a.width, p.vec_do);
-    keep_tile<PS, VB, DK>(m.s, m.keep_s, p.dstates + kept_at<PS, DK>(p, head_at), p.scales + (head_at * 4 + 1) * p.rows, p.rows,
+    keep_tile<VB, DK>(m.s, m.keep_s, p.dstates + kept_at<DK>(p, head_at), p.scales + (head_at * 4 + 1) * p.rows, p.rows,
                           a.column);
     const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
     const char* coef = stage + L::kTiles + L::kT + L::kP;
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
       row_max(f, top);
       const Pow2 fw[2] = {pow2_for(top[0]), pow2_for(top[1])};
       share(m.scale_c, wn, m0, lane, fw[0].inverse, fw[1].inverse);
-      tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, f, fw);
+      tile_write<kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, f, fw);
       coef_read(coef, kOutQ, wn * 2, lane, w);
       scale_columns(g, w);
       row_max(g, top);
@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
 #pragma unroll
     for (int kk = 0; kk < DK / 16; ++kk) {
       uint32_t hi[4], lo[4];
-      tile_operand<PS>(dw[kk], M::kWide, hi, lo);
-      product<PS, IN, false>(du[0], du[1], hi, lo, kt + kw[kk], L::kTile, kk == 0);
+      tile_operand(dw[kk], M::kWide, hi, lo);
+      product<IN, false>(du[0], du[1], hi, lo, kt + kw[kk], L::kTile, kk == 0);
     }
     float4 most[2];
     shared_of(m.most_s, m0, lane, most);
@@ -124,8 +124,8 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
     for (int kk = 0; kk < 4; ++kk) {
       uint32_t hi[4], lo[4];
       float bx[2][4];
-      tile_operand<PO>(yw[kk] + (wt - yt), M::kNarrow, hi, lo);
-      product<PO, PO, true>(bx[0], bx[1], hi, lo, pt + ts + kk * 16 * kChunk * 2, L::kSquare, true);
+      tile_operand(yw[kk] + (wt - yt), M::kNarrow, hi, lo);
+      product<kPlanes, true>(bx[0], bx[1], hi, lo, pt + ts + kk * 16 * kChunk * 2, L::kSquare, true);
       add_scaled(du, bx, element(back[0], kk), element(back[1], kk));
     }
     coef_read(coef, kTRow, wn * 2, lane, w);
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
       row_max(du, top);
       const Pow2 fy[2] = {pow2_for(top[0]), pow2_for(top[1])};
       share(m.scale_a, wn, m0, lane, fy[0].inverse, fy[1].inverse);
-      tile_write<PS, kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, du, fy);
+      tile_write<kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, du, fy);
     }
     __syncthreads();
     // dX^T = (T^T dU)^T
@@ -144,14 +144,14 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
     for (int kk = 0; kk < 4; ++kk) {
       uint32_t hi[4], lo[4];
       float bx[2][4];
-      tile_operand<PS>(yw[kk], M::kNarrow, hi, lo);
-      product<PS, PS, true>(bx[0], bx[1], hi, lo, tt + ts + kk * 16 * kChunk * 2, L::kSquare, true);
+      tile_operand(yw[kk], M::kNarrow, hi, lo);
+      product<kPlanes, true>(bx[0], bx[1], hi, lo, tt + ts + kk * 16 * kChunk * 2, L::kSquare, true);
       add_scaled(x, bx, element(back[0], kk), element(back[1], kk));
     }
     const float bound_x[2] = {kSumTop * kPlaneTop * most_of(back[0]), kSumTop * kPlaneTop * most_of(back[1])};
-    // dX is kept, at a scale from its bound; do' is done with, and PO = PS
+    // dX is kept, at a scale from its bound; do' is done with
     const Pow2 fk[2] = {scale_below(bound_x[0]), scale_below(bound_x[1])};
-    tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, x, fk);
+    tile_write<kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, x, fk);
     if (wn == 0 && (lane & 3) == 0) {
       m.keep_c[m0 + (lane >> 2)] = fk[0].inverse;
       m.keep_c[m0 + (lane >> 2) + 8] = fk[1].inverse;
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
       bound_f[h] = fmaxf(most_of(most_g[h]), bounds.z * bound_x[h]);
       ff[h] = scale_below(bound_f[h]);
     }
-    tile_write<PS, kChunk>(m.d, M::kNarrow, m0, wn * 16, lane, g, ff);
+    tile_write<kChunk>(m.d, M::kNarrow, m0, wn * 16, lane, g, ff);
     {
       float out[2][4];
       float2 b[2];
@@ -177,26 +177,26 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
           out[n][e] = (e & 1 ? b[n].y : b[n].x) * x[n][e];
           x[n][e] *= e & 1 ? -w[n].y : -w[n].x;
         }
-      tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, x, ff);
+      tile_write<kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, x, ff);
       strip_store<T, kPitch>(m.slab[turn & 1] + wn * 16 * kPitch + m0 * sizeof(T), lane, out, dv + (c * kChunk + wn * 16) * dv_step + m0, dv_step, len - wn * 16, a.width - m0,
                      p.vec_o);
     }
     __syncthreads();
-    keep_tile<PO, VB, kChunk>(m.c, m.keep_c, p.dxs + kept_at<PO, kChunk>(p, head_at), p.scales + (head_at * 4 + 3) * p.rows,
+    keep_tile<VB, kChunk>(m.c, m.keep_c, p.dxs + kept_at<kChunk>(p, head_at), p.scales + (head_at * 4 + 3) * p.rows,
                               p.rows, a.column);
     // D = e^{G_C} D + (e^G do')^T Q - (beta e^G dX)^T K
     float bs[QN][4];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       uint32_t hi[4], lo[4];
-      tile_operand<PS>(yw[kk] + (ft - yt), M::kNarrow, hi, lo);
+      tile_operand(yw[kk] + (ft - yt), M::kNarrow, hi, lo);
 #pragma unroll
       for (int n = 0; n < QN / 2; ++n)
-        product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, qt + ks[n] + kk * 16 * DK * 2, L::kTile, kk == 0);
-      tile_operand<PS>(yw[kk] + (xt - yt), M::kNarrow, hi, lo);
+        product<IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, qt + ks[n] + kk * 16 * DK * 2, L::kTile, kk == 0);
+      tile_operand(yw[kk] + (xt - yt), M::kNarrow, hi, lo);
 #pragma unroll
       for (int n = 0; n < QN / 2; ++n)
-        product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile, false);
+        product<IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile, false);
     }
 #pragma unroll
     for (int n = 0; n < QN; ++n)
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
       for (int e = 0; e < 4; ++e) d[n][e] = fmaf(bs[n][e], ff[e >> 1].inverse, decay * d[n][e]);
 #pragma unroll
     for (int h = 0; h < 2; ++h) fd[h] = scale_below(fmaf(decay, most_of(most[h]), 2 * kSumTop * bound_f[h]));
-    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, fd);
+    tile_write<DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, d, fd);
     row_max(d, top);
     share(m.most_s, wn, m0, lane, top[0], top[1]);
     ring.next(p, turn + STAGES < a.chunks ? a.first + a.chunks - 1 - turn - STAGES : -1, a.kh, a.vh);
@@ -223,17 +223,17 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
 constexpr int kGradThreads = 512;
 constexpr int kGradBlock = 64;  // value features at a time
 
-template <typename T, int DK, int PS>
+template <typename T, int DK>
 struct GradShared {
   static constexpr int IN = DeltaType<T>::kIn;
   alignas(128) __half tile[2][IN][kChunk * DK];  // K, Q planes
   union {
     struct {
-      alignas(128) __half s[PS][kGradBlock * DK], d[PS][kGradBlock * DK];               // S^T, D^T
-      __half u[PS][kGradBlock * kChunk], x[PS][kGradBlock * kChunk];                    // U^T, dX^T
-      __half o[PS][kChunk * kGradBlock];                                                // do
+      alignas(128) __half s[kPlanes][kGradBlock * DK], d[kPlanes][kGradBlock * DK];               // S^T, D^T
+      __half u[kPlanes][kGradBlock * kChunk], x[kPlanes][kGradBlock * kChunk];                    // U^T, dX^T
+      __half o[kPlanes][kChunk * kGradBlock];                                                // do
     } in;
-    alignas(128) __half square[4][PS][kChunk * kChunk];  // N f_k, N f_q (rows), Gamma dA f_k, B f_k (rows)
+    alignas(128) __half square[4][kPlanes][kChunk * kChunk];  // N f_k, N f_q (rows), Gamma dA f_k, B f_k (rows)
   };
   alignas(16) float krow[kChunk];
   float qrow[kChunk], orow[kChunk];
@@ -251,16 +251,16 @@ __device__ __forceinline__ float quad_sum(float v) {
 }
 
 // d0, d1 += A B over planes, lo x lo left out.  The tensor cores cut a sum's
-// last bits at every step, towards zero, so with two planes the small products
-// are summed first (LOW) over all steps and the large ones after them: a third
-// of the cuts happen at full size.
-template <int PA, int PB, bool LOW>
-__device__ __forceinline__ void planes_product(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[PA][4], const uint32_t (&b)[PB][4]) {
+// last bits at every step, towards zero, so the small products are summed first
+// (LOW) over all steps and the large ones after them: a third of the cuts happen
+// at full size.
+template <int PB, bool LOW>
+__device__ __forceinline__ void planes_product(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[kPlanes][4], const uint32_t (&b)[PB][4]) {
 #pragma unroll
-  for (int i = 0; i < PA; ++i)
+  for (int i = 0; i < kPlanes; ++i)
 #pragma unroll
     for (int j = 0; j < PB; ++j) {
-      if (i + j >= (PA > PB ? PA : PB) || LOW != (i + j > 0)) continue;
+      if (i + j >= kPlanes || LOW != (i + j > 0)) continue;
       mma(d0, a[i], b[j][0], b[j][1]);
       mma(d1, a[i], b[j][2], b[j][3]);
     }
@@ -284,16 +284,16 @@ __device__ __forceinline__ void planes_load(uint32_t (&f)[PLANES][4], uint32_t a
 
 // Rows [row0, row0 + 64) of kept planes: into registers, and from there, times
 // their rows' ratios, into a tile.
-template <int PS, int W>
+template <int W>
 struct Kept {
   static constexpr int kUnits = kGradBlock * W / 8 / kGradThreads;
-  uint4 v[kUnits][PS];
+  uint4 v[kUnits][kPlanes];
   __device__ __forceinline__ void fetch(const char* from, int rows, int row0, int used, int tid) {
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
       const int at = i * kGradThreads + tid;
 #pragma unroll
-      for (int n = 0; n < PS; ++n) {
+      for (int n = 0; n < kPlanes; ++n) {
         v[i][n] = make_uint4(0, 0, 0, 0);
         if (row0 + at / (W / 8) < used)
           v[i][n] = __ldg(reinterpret_cast<const uint4*>(from + (static_cast<long long>(n) * rows + row0) * W * 2) + at);
@@ -306,7 +306,7 @@ struct Kept {
       const int at = i * kGradThreads + tid, row = row0 + at / (W / 8);
       const __half2 f = __float2half2_rn(row < used ? ratio[row] : 0.f);
 #pragma unroll
-      for (int n = 0; n < PS; ++n) {
+      for (int n = 0; n < kPlanes; ++n) {
         __half2* h = reinterpret_cast<__half2*>(&v[i][n]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) h[e] = __hmul2(h[e], f);
@@ -317,19 +317,19 @@ struct Kept {
 };
 
 // Asks L2 for what a block will read of a (chunk, value head).
-template <int PS, int DK>
+template <int DK>
 __device__ __forceinline__ void prefetch_kept(const DeltaParams& p, long long head, int tid) {
   const int used = p.slabs * 16;
   const auto ask = [&](const char* from, int bytes) {
     for (int at = tid * 128; at < bytes; at += kGradThreads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + at));
   };
 #pragma unroll
-  for (int n = 0; n < PS; ++n) {
+  for (int n = 0; n < kPlanes; ++n) {
     const long long wide = static_cast<long long>(n) * p.rows * DK * 2, narrow = static_cast<long long>(n) * p.rows * kChunk * 2;
-    ask(p.states + kept_at<PS, DK>(p, head) + wide, used * DK * 2);
-    ask(p.dstates + kept_at<PS, DK>(p, head) + wide, used * DK * 2);
-    ask(p.us + kept_at<PS, kChunk>(p, head) + narrow, used * kChunk * 2);
-    ask(p.dxs + kept_at<PS, kChunk>(p, head) + narrow, used * kChunk * 2);
+    ask(p.states + kept_at<DK>(p, head) + wide, used * DK * 2);
+    ask(p.dstates + kept_at<DK>(p, head) + wide, used * DK * 2);
+    ask(p.us + kept_at<kChunk>(p, head) + narrow, used * kChunk * 2);
+    ask(p.dxs + kept_at<kChunk>(p, head) + narrow, used * kChunk * 2);
   }
 }
 
@@ -344,13 +344,13 @@ __device__ __forceinline__ void store_row(T* to, const float (&f)[N], int count,
   }
 }
 
-template <typename T, int DK, int PS, int PO>
+template <typename T, int DK>
 __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p) {
-  using L = DeltaLayout<T, DK, PS, PO>;
+  using L = DeltaLayout<T, DK>;
   constexpr int IN = L::kIn, NT = DK / 32;  // column tiles of a warp
   constexpr uint32_t kWide = kGradBlock * DK * 2, kNarrow = kGradBlock * kChunk * 2, kSq = kChunk * kChunk * 2;
   extern __shared__ __align__(128) char shared_bytes[];
-  GradShared<T, DK, PS>& s = *reinterpret_cast<GradShared<T, DK, PS>*>(shared_bytes);
+  GradShared<T, DK>& s = *reinterpret_cast<GradShared<T, DK>*>(shared_bytes);
   const int chunk = blockIdx.x / p.hk, kh = blockIdx.x % p.hk;
   ChunkAt c;
   if (!chunk_at(p, chunk, &c)) return;
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
   const int r0 = rb * 16 + (lane >> 2);
   const uint32_t kt = shared_u32(s.tile[0][0]), qt = shared_u32(s.tile[1][0]);
   const int group = p.hv / p.hk, used = p.slabs * 16;
-  prefetch_kept<PS, DK>(p, static_cast<long long>(chunk) * p.hv + kh * group, tid);
+  prefetch_kept<DK>(p, static_cast<long long>(chunk) * p.hv + kh * group, tid);
   {
     const uint4* from = reinterpret_cast<const uint4*>(p.tiles + (static_cast<long long>(chunk) * p.hk + kh) * L::kTiles);
 #pragma unroll
@@ -378,13 +378,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
     const long long head_at = static_cast<long long>(chunk) * p.hv + vh;
     const float* coef = reinterpret_cast<const float*>(p.heads + head_at * L::kHead + L::kT + L::kP);
     // everything that the head's first steps need is on its way before any of it is waited for
-    Kept<PS, DK> ks, kd;
-    Kept<PS, kChunk> ku, kx;
+    Kept<DK> ks, kd;
+    Kept<kChunk> ku, kx;
     const auto fetch = [&](int v0) {
-      ks.fetch(p.states + kept_at<PS, DK>(p, head_at), p.rows, v0, used, tid);
-      kd.fetch(p.dstates + kept_at<PS, DK>(p, head_at), p.rows, v0, used, tid);
-      ku.fetch(p.us + kept_at<PS, kChunk>(p, head_at), p.rows, v0, used, tid);
-      kx.fetch(p.dxs + kept_at<PS, kChunk>(p, head_at), p.rows, v0, used, tid);
+      ks.fetch(p.states + kept_at<DK>(p, head_at), p.rows, v0, used, tid);
+      kd.fetch(p.dstates + kept_at<DK>(p, head_at), p.rows, v0, used, tid);
+      ku.fetch(p.us + kept_at<kChunk>(p, head_at), p.rows, v0, used, tid);
+      kx.fetch(p.dxs + kept_at<kChunk>(p, head_at), p.rows, v0, used, tid);
     };
     const float decay = __ldg(coef + kDecay * kChunk);
     const int kind = tid >> 7, scale_row = tid & 127;
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
       }
     }
     fetch(0);
-    if (sub + 1 < group) prefetch_kept<PS, DK>(p, head_at + 1, tid);
+    if (sub + 1 < group) prefetch_kept<DK>(p, head_at + 1, tid);
     __syncthreads();  // the last head is done with
     if (tid < 4) s.common[tid] = s.most[tid] = 0;
     if (tid < kChunk) {
@@ -462,12 +462,12 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
       ku.put(s.ratio[2], v0, used, reinterpret_cast<char*>(s.in.u), tid);
       kx.put(s.ratio[3], v0, used, reinterpret_cast<char*>(s.in.x), tid);
       {
-        Vec<uint32_t, 4> plane[2];
+        Vec<uint32_t, 4> plane[kPlanes];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          split<PS>(block ? o[1][2 * e] : o[0][2 * e], block ? o[1][2 * e + 1] : o[0][2 * e + 1], &plane[0].e[e], &plane[1].e[e]);
+          split(block ? o[1][2 * e] : o[0][2 * e], block ? o[1][2 * e + 1] : o[0][2 * e + 1], &plane[0].e[e], &plane[1].e[e]);
 #pragma unroll
-        for (int n = 0; n < PS; ++n)
+        for (int n = 0; n < kPlanes; ++n)
           *reinterpret_cast<Vec<uint32_t, 4>*>(reinterpret_cast<char*>(s.in.o) + n * kNarrow + tile_at<kGradBlock>(o_row, tid & 7)) = plane[n];
       }
       float v[8] = {};  // of token tid & 63, eight features
@@ -496,14 +496,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
         for (int e = 0; e < 8; ++e) {
           const uint32_t at = tile_at<kChunk>(row + e, t >> 3) + (t & 7) * 2;
 #pragma unroll
-          for (int n = 0; n < PS; ++n)
+          for (int n = 0; n < kPlanes; ++n)
             xv = fmaf(__half2float(*reinterpret_cast<const __half*>(reinterpret_cast<const char*>(s.in.x) + n * kNarrow + at)), v[e], xv);
         }
 #pragma unroll
         for (int i = 0; i < kGradBlock * DK / 8 / kGradThreads; ++i) {
           float f[8], g[8];
 #pragma unroll
-          for (int n = 0; n < PS; ++n) {
+          for (int n = 0; n < kPlanes; ++n) {
             const uint4 a = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s.in.s) + n * kWide)[i * kGradThreads + tid];
             const uint4 b = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s.in.d) + n * kWide)[i * kGradThreads + tid];
 #pragma unroll
@@ -521,27 +521,27 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
       }
       const auto products = [&](auto low) {
       constexpr bool LOW = decltype(low)::value;
-#pragma unroll(PS > 1 ? 1 : kGradBlock / 16)
+#pragma unroll 1
       for (int kk = 0; kk < kGradBlock / 16; ++kk) {
-        uint32_t fo[PS][4], fu[PS][4], fx[PS][4], b[PS][4];
-        planes_load<PS, false>(fo, ot + at_mk<kGradBlock>(lane, rb * 16, kk * 16), kNarrow);
-        planes_load<PS, true>(fu, ut + at_km<kChunk>(lane, rb * 16, kk * 16), kNarrow);
-        planes_load<PS, true>(fx, xt + at_km<kChunk>(lane, rb * 16, kk * 16), kNarrow);
+        uint32_t fo[kPlanes][4], fu[kPlanes][4], fx[kPlanes][4], b[kPlanes][4];
+        planes_load<kPlanes, false>(fo, ot + at_mk<kGradBlock>(lane, rb * 16, kk * 16), kNarrow);
+        planes_load<kPlanes, true>(fu, ut + at_km<kChunk>(lane, rb * 16, kk * 16), kNarrow);
+        planes_load<kPlanes, true>(fx, xt + at_km<kChunk>(lane, rb * 16, kk * 16), kNarrow);
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) {
           const uint32_t at = at_kn<DK>(lane, cg * (DK / 4) + n * 16, kk * 16);
-          planes_load<PS, true>(b, st + at, kWide);
-          planes_product<PS, PS, LOW>(a_q[2 * n], a_q[2 * n + 1], fo, b);
-          planes_product<PS, PS, LOW>(a_x[2 * n], a_x[2 * n + 1], fx, b);
-          planes_load<PS, true>(b, dt + at, kWide);
-          planes_product<PS, PS, LOW>(a_u[2 * n], a_u[2 * n + 1], fu, b);
+          planes_load<kPlanes, true>(b, st + at, kWide);
+          planes_product<kPlanes, LOW>(a_q[2 * n], a_q[2 * n + 1], fo, b);
+          planes_product<kPlanes, LOW>(a_x[2 * n], a_x[2 * n + 1], fx, b);
+          planes_load<kPlanes, true>(b, dt + at, kWide);
+          planes_product<kPlanes, LOW>(a_u[2 * n], a_u[2 * n + 1], fu, b);
         }
-        planes_load<PS, true>(b, ut + at_kn<kChunk>(lane, cg * 16, kk * 16), kNarrow);
-        planes_product<PS, PS, LOW>(a_p[0], a_p[1], fo, b);
-        planes_product<PS, PS, LOW>(a_a[0], a_a[1], fx, b);
+        planes_load<kPlanes, true>(b, ut + at_kn<kChunk>(lane, cg * 16, kk * 16), kNarrow);
+        planes_product<kPlanes, LOW>(a_p[0], a_p[1], fo, b);
+        planes_product<kPlanes, LOW>(a_a[0], a_a[1], fx, b);
       }
       };
-      if constexpr (PS > 1) products(std::true_type{});
+      products(std::true_type{});
       products(std::false_type{});
     }
 #pragma unroll
@@ -630,10 +630,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t hi, lo;
-          split<PS>(sq[w][n][2 * h] * f[w].f, sq[w][n][2 * h + 1] * f[w].f, &hi, &lo);
+          split(sq[w][n][2 * h] * f[w].f, sq[w][n][2 * h + 1] * f[w].f, &hi, &lo);
           char* to = reinterpret_cast<char*>(s.square[w]);
           *reinterpret_cast<uint32_t*>(to + at) = hi;
-          if (PS > 1) *reinterpret_cast<uint32_t*>(to + kSq + at) = lo;
+          *reinterpret_cast<uint32_t*>(to + kSq + at) = lo;
         }
       }
     __syncthreads();
@@ -641,38 +641,38 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
     {
       float b_q[NT][4] = {}, b_n[NT][4] = {}, b_y[NT][4] = {}, b_t[NT][4] = {};
       const uint32_t base = shared_u32(s.square);
-      constexpr uint32_t one = PS * kSq;
+      constexpr uint32_t one = kPlanes * kSq;
       const auto products = [&](auto low) {
       constexpr bool LOW = decltype(low)::value;
-#pragma unroll(PS > 1 ? 1 : 4)
+#pragma unroll 1
       for (int kk = 0; kk < 4; ++kk) {
         const uint32_t mk = at_mk<kChunk>(lane, rb * 16, kk * 16), km = at_km<kChunk>(lane, rb * 16, kk * 16);
-        uint32_t a[PS][4], g[PS][4], b[IN][4];
+        uint32_t a[kPlanes][4], g[kPlanes][4], b[IN][4];
         if (kk <= rb) {
-          planes_load<PS, false>(a, base + mk, kSq);
-          planes_load<PS, false>(g, base + 2 * one + mk, kSq);
+          planes_load<kPlanes, false>(a, base + mk, kSq);
+          planes_load<kPlanes, false>(g, base + 2 * one + mk, kSq);
 #pragma unroll
           for (int n = 0; n < NT / 2; ++n) {
             planes_load<IN, true>(b, kt + at_kn<DK>(lane, cg * (DK / 4) + n * 16, kk * 16), L::kTile);
-            planes_product<PS, IN, LOW>(b_q[2 * n], b_q[2 * n + 1], a, b);
-            planes_product<PS, IN, LOW>(b_y[2 * n], b_y[2 * n + 1], g, b);
+            planes_product<IN, LOW>(b_q[2 * n], b_q[2 * n + 1], a, b);
+            planes_product<IN, LOW>(b_y[2 * n], b_y[2 * n + 1], g, b);
           }
         }
         if (kk >= rb) {
-          planes_load<PS, true>(a, base + one + km, kSq);
-          planes_load<PS, true>(g, base + 3 * one + km, kSq);
+          planes_load<kPlanes, true>(a, base + one + km, kSq);
+          planes_load<kPlanes, true>(g, base + 3 * one + km, kSq);
 #pragma unroll
           for (int n = 0; n < NT / 2; ++n) {
             const uint32_t at = at_kn<DK>(lane, cg * (DK / 4) + n * 16, kk * 16);
             planes_load<IN, true>(b, qt + at, L::kTile);
-            planes_product<PS, IN, LOW>(b_n[2 * n], b_n[2 * n + 1], a, b);
+            planes_product<IN, LOW>(b_n[2 * n], b_n[2 * n + 1], a, b);
             planes_load<IN, true>(b, kt + at, L::kTile);
-            planes_product<PS, IN, LOW>(b_t[2 * n], b_t[2 * n + 1], g, b);
+            planes_product<IN, LOW>(b_t[2 * n], b_t[2 * n + 1], g, b);
           }
         }
       }
       };
-      if constexpr (PS > 1) products(std::true_type{});
+      products(std::true_type{});
       products(std::false_type{});
 #pragma unroll
       for (int n = 0; n < NT; ++n)

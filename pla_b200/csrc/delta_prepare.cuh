@@ -97,13 +97,12 @@ __device__ __forceinline__ void prepare_rows(const DeltaParams& p, const T* k, c
 }
 
 // Eight columns of a row as planes.
-template <int PLANES>
 __device__ __forceinline__ void store_unit(char* out, int row, int unit, const float (&f)[8], float scale) {
-  Vec<uint32_t, 4> plane[2];
+  Vec<uint32_t, 4> plane[kPlanes];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) split<PLANES>(f[2 * e] * scale, f[2 * e + 1] * scale, &plane[0].e[e], &plane[1].e[e]);
+  for (int e = 0; e < 4; ++e) split(f[2 * e] * scale, f[2 * e + 1] * scale, &plane[0].e[e], &plane[1].e[e]);
 #pragma unroll
-  for (int n = 0; n < PLANES; ++n)
+  for (int n = 0; n < kPlanes; ++n)
     *reinterpret_cast<Vec<uint32_t, 4>*>(out + n * kChunk * kChunk * 2 + tile_at<kChunk>(row, unit)) = plane[n];
 }
 
@@ -165,9 +164,9 @@ __device__ __forceinline__ void load_gates(const DeltaParams& p, const ChunkAt& 
   }
 }
 
-template <typename T, int DK, int PS, int PO, int HEADS>
+template <typename T, int DK, int HEADS>
 __global__ void __launch_bounds__(128 * HEADS, 3) delta_prepare(DeltaParams p) {
-  using L = DeltaLayout<T, DK, PS, PO>;
+  using L = DeltaLayout<T, DK>;
   extern __shared__ __align__(16) char shared_bytes[];
   PrepShared<T, DK, HEADS>& s = *reinterpret_cast<PrepShared<T, DK, HEADS>*>(shared_bytes);
   const int chunk = blockIdx.x / p.hk, kh = blockIdx.x % p.hk;
@@ -294,7 +293,7 @@ __global__ void __launch_bounds__(128 * HEADS, 3) delta_prepare(DeltaParams p) {
             av[e] = j < row ? b * (decay * s.kk[row][j]) : 0.f;
           }
         }
-        store_unit<PO>(head + L::kT, row, unit, pv, f.f);
+        store_unit(head + L::kT, row, unit, pv, f.f);
         *reinterpret_cast<float4*>(&t[row][unit * 8]) = make_float4(av[0], av[1], av[2], av[3]);
         *reinterpret_cast<float4*>(&t[row][unit * 8 + 4]) = make_float4(av[4], av[5], av[6], av[7]);
       }
@@ -368,7 +367,7 @@ __global__ void __launch_bounds__(128 * HEADS, 3) delta_prepare(DeltaParams p) {
       }
       if (!(id & 1)) coef[kTail * kChunk + row] = tail;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) store_unit<PS>(head, row, unit_of(i, id), v[i], f.f);
+      for (int i = 0; i < 4; ++i) store_unit(head, row, unit_of(i, id), v[i], f.f);
       if (!(id & 1)) coef[kTRow * kChunk + row] = f.inverse;
     }
     if (id < kChunk) {

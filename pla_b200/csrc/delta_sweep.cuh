@@ -14,10 +14,10 @@
 // instructions a warp, and operands pass between the warps through shared
 // memory as planes (one barrier a step).  One warp that kept all of S^T in
 // registers instead needed no barrier, but its 400 products and 1500 other
-// instructions a chunk took 8.6 us where this takes 2.8 us (bf16, Dk = 128).
-// A chunk's 112 products a warp are a third of that; the rest is the wait for
-// operands and barriers, which more warps an SM or more products at a time do
-// not shorten.
+// instructions a chunk took 8.6 us where this took 2.8 us (bf16, Dk = 128, one
+// plane for the outputs; 3.0 us with two).  A chunk's 144 products a warp are
+// 40 % of that; the rest is the wait for operands and barriers, which more warps
+// an SM or more products at a time do not shorten.
 //
 // A row's planes take one scale wherever a bound gives it before the warps
 // have met: |U| <= max_i sum_j |T_ij| max|X| (delta_prepare has the sums), and
@@ -190,7 +190,7 @@ __device__ __forceinline__ void row_max(const float (&f)[N][4], float (&m)[2]) {
 
 // Accumulators of 16 rows x 8 N columns, times a scale for each row, as planes
 // of a tile of W columns.
-template <int PLANES, int W, int N>
+template <int W, int N>
 __device__ __forceinline__ void tile_write(char* tile, uint32_t plane, int row0, int col0, int lane, const float (&f)[N][4],
                                            const Pow2 (&s)[2]) {
 #pragma unroll
@@ -199,10 +199,10 @@ __device__ __forceinline__ void tile_write(char* tile, uint32_t plane, int row0,
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       uint32_t hi, lo;
-      split<PLANES>(f[n][2 * h] * s[h].f, f[n][2 * h + 1] * s[h].f, &hi, &lo);
+      split(f[n][2 * h] * s[h].f, f[n][2 * h + 1] * s[h].f, &hi, &lo);
       const uint32_t at = tile_at<W>(row, (col0 >> 3) + n) + (lane & 3) * 4;
       *reinterpret_cast<uint32_t*>(tile + at) = hi;
-      if (PLANES > 1) *reinterpret_cast<uint32_t*>(tile + plane + at) = lo;
+      *reinterpret_cast<uint32_t*>(tile + plane + at) = lo;
     }
   }
 }
@@ -221,10 +221,9 @@ __device__ __forceinline__ float most_of(float4 v) { return fmaxf(fmaxf(v.x, v.y
 __device__ __forceinline__ float element(const float4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // Left operand: 16 x 16 of a tile's planes.
-template <int PLANES>
 __device__ __forceinline__ void tile_operand(uint32_t at, uint32_t plane, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
   ldsm(hi, at);
-  if (PLANES > 1) ldsm(lo, at + plane);
+  ldsm(lo, at + plane);
 }
 
 // f += g, row by row times a factor.
@@ -251,9 +250,9 @@ __device__ __forceinline__ void scale_columns(float (&f)[N][4], const float2 (&w
   }
 }
 
-// d0, d1 (+)= A B for two column tiles: A in PA planes (hi, lo), B in PB planes
+// d0, d1 (+)= A B for two column tiles: A in two planes (hi, lo), B in PB planes
 // `apart` bytes apart at `at`; the product of two lo planes is left out.
-template <int PA, int PB, bool TRANS>
+template <int PB, bool TRANS>
 __device__ __forceinline__ void product(float (&d0)[4], float (&d1)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
                                         uint32_t at, uint32_t apart, bool first) {
   uint32_t b[4];
@@ -265,10 +264,8 @@ __device__ __forceinline__ void product(float (&d0)[4], float (&d1)[4], const ui
     mma(d0, hi, b[0], b[1]);
     mma(d1, hi, b[2], b[3]);
   }
-  if (PA > 1) {
-    mma(d0, lo, b[0], b[1]);
-    mma(d1, lo, b[2], b[3]);
-  }
+  mma(d0, lo, b[0], b[1]);
+  mma(d1, lo, b[2], b[3]);
   if (PB > 1) {
     if (TRANS) ldsm_t(b, at + apart); else ldsm(b, at + apart);
     mma(d0, hi, b[0], b[1]);
@@ -382,12 +379,12 @@ __device__ __forceinline__ void state_store(float* to, const DeltaParams& p, con
 }
 // A block's planes of a tile and the inverses of their rows' scales to the
 // workspace: VB rows of W columns of plane after plane.
-template <int PLANES, int VB, int W>
+template <int VB, int W>
 __device__ __forceinline__ void keep_tile(const char* tile, const float* scale, char* to, float* scales, int rows, int column) {
   constexpr int UNITS = VB * W * 2 / 16;
   char* at = to + static_cast<long long>(column) * W * 2;
 #pragma unroll
-  for (int n = 0; n < PLANES; ++n)
+  for (int n = 0; n < kPlanes; ++n)
 #pragma unroll
     for (int i = 0; i < UNITS / (VB * 8); ++i) {
       const int u = i * VB * 8 + threadIdx.x;
@@ -397,9 +394,9 @@ __device__ __forceinline__ void keep_tile(const char* tile, const float* scale, 
   if (threadIdx.x < VB) scales[column + threadIdx.x] = scale[threadIdx.x];
 }
 // Where a (chunk, value head) keeps what: bytes of the planes, floats of the scales.
-template <int PLANES, int W>
+template <int W>
 __device__ __forceinline__ long long kept_at(const DeltaParams& p, long long head) {
-  return head * PLANES * p.rows * W * 2;
+  return head * kPlanes * p.rows * W * 2;
 }
 
 template <int N>
@@ -413,14 +410,14 @@ constexpr int kSweepRing = 128;  // bytes of the ring's barriers
 
 // Shared memory of a sweep behind the ring: planes of S, X, U and what else
 // the steps hand on.
-template <typename T, int DK, int PS, int PO, int VB, bool BACK>
+template <typename T, int DK, int VB, bool BACK>
 struct SweepShared {
   static constexpr uint32_t kWide = VB * DK * 2, kNarrow = VB * kChunk * 2;
-  alignas(128) char s[PS * kWide];
-  char a[PS * kNarrow];  // X; back: Y
-  char b[PS * kNarrow];  // e^{G_C - G} U; back: beta e^G dX
-  char c[PO * kNarrow];  // U; back: do' with P's weights, then dX
-  char d[BACK ? PS * kNarrow : 128];  // back: e^G do'
+  alignas(128) char s[kPlanes * kWide];
+  char a[kPlanes * kNarrow];  // X; back: Y
+  char b[kPlanes * kNarrow];  // e^{G_C - G} U; back: beta e^G dX
+  char c[kPlanes * kNarrow];  // U; back: do' with P's weights, then dX
+  char d[BACK ? kPlanes * kNarrow : 128];  // back: e^G do'
   alignas(16) float most_s[VB * 4];   // largest of S's rows, by warp
   alignas(16) float scale_a[VB * 4];  // inverses of the scales of X (Y), by warp
   alignas(16) float scale_c[VB * 4];  // back: of do'
@@ -438,10 +435,10 @@ __device__ __forceinline__ Pow2 scale_below(float bound) {
 }
 
 // KEEP: store S at every chunk's start and U for the backward pass instead of O.
-template <typename T, int DK, int PS, int PO, int VB, int STAGES, int PER_SM, bool KEEP>
+template <typename T, int DK, int VB, int STAGES, int PER_SM, bool KEEP>
 __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
-  using L = DeltaLayout<T, DK, PS, PO>;
-  using M = SweepShared<T, DK, PS, PO, VB, false>;
+  using L = DeltaLayout<T, DK>;
+  using M = SweepShared<T, DK, VB, false>;
   constexpr int IN = L::kIn, QN = DK / 32;  // column tiles of a quarter of Dk
   constexpr int kPitch = Slab<T, VB>::kPitch;
   extern __shared__ __align__(128) char shared_bytes[];
@@ -485,7 +482,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
     shared_of(m.most_s, m0, lane, all);
     fs[0] = scale_below(most_of(all[0]));
     fs[1] = scale_below(most_of(all[1]));
-    tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, fs);
+    tile_write<DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, fs);
   }
 
   for (int c = 0; c < a.chunks; ++c) {
@@ -502,7 +499,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
       slab_fetch<T, VB>(m.slab[~c & 1], v + (c + 1) * kChunk * p.v_token, p.v_token, min(kChunk, a.len - (c + 1) * kChunk),
                         a.width, p.vec_v);
     if (KEEP)
-      keep_tile<PS, VB, DK>(m.s, m.keep_s, p.states + kept_at<PS, DK>(p, head_at), p.scales + head_at * 4 * p.rows, p.rows,
+      keep_tile<VB, DK>(m.s, m.keep_s, p.states + kept_at<DK>(p, head_at), p.scales + head_at * 4 * p.rows, p.rows,
                             a.column);
     const uint32_t kt = shared_u32(stage), qt = kt + IN * L::kTile, tt = kt + L::kTiles, pt = tt + L::kT;
     const char* coef = stage + L::kTiles + L::kT + L::kP;
@@ -514,9 +511,9 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
 #pragma unroll
     for (int kk = 0; kk < DK / 16; ++kk) {
       uint32_t hi[4], lo[4];
-      tile_operand<PS>(sw[kk], M::kWide, hi, lo);
-      product<PS, IN, false>(x[0], x[1], hi, lo, kt + kw[kk], L::kTile, kk == 0);
-      if (!KEEP) product<PO, IN, false>(q[0], q[1], hi, lo, qt + kw[kk], L::kTile, kk == 0);
+      tile_operand(sw[kk], M::kWide, hi, lo);
+      product<IN, false>(x[0], x[1], hi, lo, kt + kw[kk], L::kTile, kk == 0);
+      if (!KEEP) product<IN, false>(q[0], q[1], hi, lo, qt + kw[kk], L::kTile, kk == 0);
     }
     float4 most[2];
     shared_of(m.most_s, m0, lane, most);
@@ -536,7 +533,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
       row_max(x, top);
       const Pow2 fx[2] = {pow2_for(top[0]), pow2_for(top[1])};
       share(m.scale_a, wn, m0, lane, fx[0].inverse, fx[1].inverse);
-      tile_write<PS, kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, x, fx);
+      tile_write<kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, x, fx);
     }
     __syncthreads();
     // U^T = X^T T^T; T is lower triangular, but the warp with the last tokens needs every step,
@@ -548,15 +545,15 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
     for (int kk = 0; kk < 4; ++kk) {
       uint32_t hi[4], lo[4];
       float bu[2][4];
-      tile_operand<PS>(xw[kk], M::kNarrow, hi, lo);
-      product<PS, PS, false>(bu[0], bu[1], hi, lo, tt + tw[kk], L::kSquare, true);
+      tile_operand(xw[kk], M::kNarrow, hi, lo);
+      product<kPlanes, false>(bu[0], bu[1], hi, lo, tt + tw[kk], L::kSquare, true);
       add_scaled(u, bu, element(back[0], kk), element(back[1], kk));
     }
     coef_read(coef, kTRow, wn * 2, lane, w);
     scale_columns(u, w);
     const float bound_x[2] = {most_of(back[0]) * kPlaneTop, most_of(back[1]) * kPlaneTop};
     const Pow2 fu[2] = {scale_below(bounds.x * bound_x[0]), scale_below(bounds.x * bound_x[1])};
-    tile_write<PO, kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, u, fu);
+    tile_write<kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, u, fu);
     if (KEEP && wn == 0 && (lane & 3) == 0) {
       m.keep_c[m0 + (lane >> 2)] = fu[0].inverse;
       m.keep_c[m0 + (lane >> 2) + 8] = fu[1].inverse;
@@ -565,10 +562,10 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
     scale_columns(u, w);
     const float bound_u[2] = {bounds.y * bound_x[0], bounds.y * bound_x[1]};
     const Pow2 ft[2] = {scale_below(bound_u[0]), scale_below(bound_u[1])};
-    tile_write<PS, kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, u, ft);
+    tile_write<kChunk>(m.b, M::kNarrow, m0, wn * 16, lane, u, ft);
     __syncthreads();
-    if (KEEP)  // here PO = PS
-      keep_tile<PO, VB, kChunk>(m.c, m.keep_c, p.us + kept_at<PO, kChunk>(p, head_at), p.scales + (head_at * 4 + 2) * p.rows,
+    if (KEEP)
+      keep_tile<VB, kChunk>(m.c, m.keep_c, p.us + kept_at<kChunk>(p, head_at), p.scales + (head_at * 4 + 2) * p.rows,
                                 p.rows, a.column);
     // S^T = e^{G_C} S^T + (e^{G_C - G} U)^T K
     {
@@ -576,10 +573,10 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         uint32_t hi[4], lo[4];
-        tile_operand<PS>(xw[kk] + (ut - xt), M::kNarrow, hi, lo);
+        tile_operand(xw[kk] + (ut - xt), M::kNarrow, hi, lo);
 #pragma unroll
         for (int n = 0; n < QN / 2; ++n)
-          product<PS, IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile, kk == 0);
+          product<IN, true>(bs[2 * n], bs[2 * n + 1], hi, lo, kt + ks[n] + kk * 16 * DK * 2, L::kTile, kk == 0);
       }
 #pragma unroll
       for (int n = 0; n < QN; ++n)
@@ -588,7 +585,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
       const Pow2 old[2] = {fs[0], fs[1]};
 #pragma unroll
       for (int h = 0; h < 2; ++h) fs[h] = scale_below(fmaf(decay, most_of(most[h]), kSumTop * bound_u[h]));
-      tile_write<PS, DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, fs);
+      tile_write<DK>(m.s, M::kWide, m0, wn * (DK / 4), lane, s, fs);
       row_max(s, top);
       share(m.most_s, wn, m0, lane, top[0], top[1]);
       if (!KEEP) {  // O^T = (Q S)^T + U^T P^T, each with its weights
@@ -596,8 +593,8 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           uint32_t hi[4], lo[4];
-          tile_operand<PO>(xw[kk] + (vt - xt), M::kNarrow, hi, lo);
-          product<PO, PO, false>(pu[0], pu[1], hi, lo, pt + tw[kk], L::kSquare, kk == 0);
+          tile_operand(xw[kk] + (vt - xt), M::kNarrow, hi, lo);
+          product<kPlanes, false>(pu[0], pu[1], hi, lo, pt + tw[kk], L::kSquare, kk == 0);
         }
         float2 wq[2];
         coef_read(coef, kOutQ, wn * 2, lane, wq);

@@ -291,9 +291,9 @@ struct DeltaSizes {
 };
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-template <typename T, int DK, int PS, int PO>
+template <typename T, int DK>
 DeltaSizes delta_sizes_of(const pla_delta* a, bool backward) {
-  using L = DeltaLayout<T, DK, PS, PO>;
+  using L = DeltaLayout<T, DK>;
   DeltaSizes s;
   s.chunks = a->cu_seqlens ? a->tokens / kChunk + static_cast<long long>(a->sequences)
                            : static_cast<long long>(a->batch) * ((a->tokens + kChunk - 1) / kChunk);
@@ -302,35 +302,18 @@ DeltaSizes delta_sizes_of(const pla_delta* a, bool backward) {
   s.heads = up256(static_cast<size_t>(s.chunks) * a->hv * L::kHead);
   if (backward) {
     const size_t rows = static_cast<size_t>(s.chunks) * a->hv * ((a->dv + 63) / 64) * 64;
-    s.states = up256(rows * PS * DK * 2);
-    s.us = up256(rows * PS * kChunk * 2);
+    s.states = up256(rows * kPlanes * DK * 2);
+    s.us = up256(rows * kPlanes * kChunk * 2);
     s.scales = up256(rows * 4 * sizeof(float));
   }
   s.total = s.plan + s.tiles + s.heads + 2 * s.states + 2 * s.us + s.scales;
   return s;
 }
 
-// f(element type, padded Dk, planes of states, planes of outputs).  Forward:
-// states come back in fp32, so their operands keep 22 bits; what only a bf16
-// output sees takes one fp16 plane (2^-12 beside a rounding of 2^-9).
+// f(element type, padded Dk)
 template <typename F>
 int with_delta(const pla_delta* a, F&& f) {
-  return with_type(a->dtype, [&](auto zero) {
-    using T = decltype(zero);
-    constexpr int PO = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
-    return a->dk <= 64 ? f(zero, Int<64>{}, Int<2>{}, Int<PO>{}) : f(zero, Int<128>{}, Int<2>{}, Int<PO>{});
-  });
-}
-// Backward: one plane everywhere if every gradient is rounded to bf16, else two.
-template <typename F>
-int with_delta_gradient(const pla_delta* a, bool fp32_result, F&& f) {
-  return with_type(a->dtype, [&](auto zero) {
-    using T = decltype(zero);
-    if constexpr (std::is_same<T, __nv_bfloat16>::value)
-      if (!fp32_result)
-        return a->dk <= 64 ? f(zero, Int<64>{}, Int<1>{}, Int<1>{}) : f(zero, Int<128>{}, Int<1>{}, Int<1>{});
-    return a->dk <= 64 ? f(zero, Int<64>{}, Int<2>{}, Int<2>{}) : f(zero, Int<128>{}, Int<2>{}, Int<2>{});
-  });
+  return with_type(a->dtype, [&](auto zero) { return a->dk <= 64 ? f(zero, Int<64>{}) : f(zero, Int<128>{}); });
 }
 
 DeltaParams delta_params(const pla_delta* a, const DeltaSizes& s) {
@@ -388,7 +371,7 @@ DeltaParams delta_params(const pla_delta* a, const DeltaSizes& s) {
   return p;
 }
 
-template <typename T, int DK, int PS, int PO>
+template <typename T, int DK>
 int launch_prepare(const DeltaParams& p, cudaStream_t stream) {
   if (p.cu) {
     delta_plan<<<1, 1024, 0, stream>>>(p.cu, p.tokens, p.sequences, p.plan, p.table, p.chunk_bound);
@@ -400,19 +383,19 @@ int launch_prepare(const DeltaParams& p, cudaStream_t stream) {
   const auto go = [&](auto heads) {
     constexpr int HEADS = decltype(heads)::value;
     const size_t shared = sizeof(PrepShared<T, DK, HEADS>);
-    const int st = allow_shared<delta_prepare<T, DK, PS, PO, HEADS>>(shared);
+    const int st = allow_shared<delta_prepare<T, DK, HEADS>>(shared);
     if (st != PLA_OK) return st;
-    delta_prepare<T, DK, PS, PO, HEADS><<<p.chunk_bound * p.hk, 128 * HEADS, shared, stream>>>(p);
+    delta_prepare<T, DK, HEADS><<<p.chunk_bound * p.hk, 128 * HEADS, shared, stream>>>(p);
     return launched("delta_prepare");
   };
   return p.hv > p.hk ? go(Int<2>{}) : go(Int<1>{});  // two value heads of a key head side by side
 }
 
 // Stages of the ring and shared memory of a sweep; PER_SM blocks fit an SM.
-template <typename T, int DK, int PS, int PO, int VB, int PER_SM, bool BACK>
+template <typename T, int DK, int VB, int PER_SM, bool BACK>
 struct SweepShape {
-  using L = DeltaLayout<T, DK, PS, PO>;
-  static constexpr size_t kHeld = kSweepRing + sizeof(SweepShared<T, DK, PS, PO, VB, BACK>);
+  using L = DeltaLayout<T, DK>;
+  static constexpr size_t kHeld = kSweepRing + sizeof(SweepShared<T, DK, VB, BACK>);
   static constexpr size_t kMost = 227 * 1024 / PER_SM - (PER_SM > 1 ? 1024 : 0);  // 1 KB of a block is the system's
   static constexpr size_t kRoom = kHeld < kMost ? (kMost - kHeld) / L::kStage : 0;
   static constexpr int kStages = kRoom < 3 ? kRoom : 3;
@@ -426,47 +409,47 @@ struct SweepShape {
 // Value features of a sweep's block.  A block's time is the latency of its
 // chunks' chain, nearly whatever it holds, so while every block has an SM of
 // its own: the fewest features that still leave it so (1001 tokens x 16 heads
-// of 128, fp16: 28 us with 16, 42 with 32; 4096 tokens x 32 heads, bf16: 177 us
-// with 32, 291 with 64).  With more blocks than SMs: of a batch, whose rows are
-// equally long, two blocks of 32 an SM, if they fit, fill each other's waits
-// (8 x 2048 tokens x 32 heads, bf16: 565 us; one block of 32: 620, of 64: 588);
-// of a ragged batch one block of 32, because the longest sequence's blocks, the
-// first to start, decide (16383 tokens in three, 32 heads: 631 us; two of 32:
-// 692, one of 64: 650).  f(shape)
-template <typename T, int DK, int PS, int PO, bool BACK, typename F>
+// of 128, fp16: 28 us with 16, 42 with 32).  With more blocks than SMs: of a
+// batch, whose rows are equally long, two blocks of 32 an SM, if they fit (16-bit
+// inputs, Dk up to 64), fill each other's waits (8 x 2048 tokens x 32 heads of 64 x
+// 128, bf16: 500 us, back 620; one block: 561 and 705); of a ragged batch one
+// block of 32, because the longest sequence's blocks, the first to start, decide
+// (16383 tokens in three, 32 heads of 128, when outputs had one plane and two
+// blocks fit: 631 us against 692).  f(shape)
+template <typename T, int DK, bool BACK, typename F>
 int with_columns(const DeltaParams& p, int sms, F&& f) {
-  using Two = SweepShape<T, DK, PS, PO, 32, 2, BACK>;
+  using Two = SweepShape<T, DK, 32, 2, BACK>;
   const long long heads = static_cast<long long>(p.sequences) * p.hv;
-  if (p.dv <= 16 || heads * ((p.dv + 15) / 16) <= sms) return f(SweepShape<T, DK, PS, PO, 16, 1, BACK>{});
+  if (p.dv <= 16 || heads * ((p.dv + 15) / 16) <= sms) return f(SweepShape<T, DK, 16, 1, BACK>{});
   if constexpr (Two::kStages >= 1)
     if (!p.cu && heads * ((p.dv + 31) / 32) > sms) return f(Two{});
-  return f(SweepShape<T, DK, PS, PO, 32, 1, BACK>{});
+  return f(SweepShape<T, DK, 32, 1, BACK>{});
 }
 
-template <typename T, int DK, int PS, int PO, bool KEEP>
+template <typename T, int DK, bool KEEP>
 int launch_sweep(const DeltaParams& p, int sms, cudaStream_t stream) {
-  return with_columns<T, DK, PS, PO, false>(p, sms, [&](auto shape) {
+  return with_columns<T, DK, false>(p, sms, [&](auto shape) {
     using S = decltype(shape);
     constexpr int VB = S::kColumns;
     static_assert(S::kStages >= 1, "no room for a chunk's tiles");
     const long long grid = S::grid(p);
     if (grid > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
-    const int st = allow_shared<delta_sweep<T, DK, PS, PO, VB, S::kStages, S::kPerSm, KEEP>>(S::kShared);
+    const int st = allow_shared<delta_sweep<T, DK, VB, S::kStages, S::kPerSm, KEEP>>(S::kShared);
     if (st != PLA_OK) return st;
-    delta_sweep<T, DK, PS, PO, VB, S::kStages, S::kPerSm, KEEP><<<static_cast<int>(grid), VB * 8, S::kShared, stream>>>(p);
+    delta_sweep<T, DK, VB, S::kStages, S::kPerSm, KEEP><<<static_cast<int>(grid), VB * 8, S::kShared, stream>>>(p);
     return launched("delta_sweep");
   });
 }
 
-template <typename T, int DK, int PS, int PO>
+template <typename T, int DK>
 int launch_gradient(const DeltaParams& p, int sms, cudaStream_t stream) {
-  int st = with_columns<T, DK, PS, PO, true>(p, sms, [&](auto shape) {
+  int st = with_columns<T, DK, true>(p, sms, [&](auto shape) {
     using S = decltype(shape);
     constexpr int VB = S::kColumns;
     static_assert(S::kStages >= 1, "no room for a chunk's tiles");
-    const int st = allow_shared<delta_sweep_back<T, DK, PS, PO, VB, S::kStages, S::kPerSm>>(S::kShared);
+    const int st = allow_shared<delta_sweep_back<T, DK, VB, S::kStages, S::kPerSm>>(S::kShared);
     if (st != PLA_OK) return st;
-    delta_sweep_back<T, DK, PS, PO, VB, S::kStages, S::kPerSm><<<static_cast<int>(S::grid(p)), VB * 8, S::kShared, stream>>>(p);
+    delta_sweep_back<T, DK, VB, S::kStages, S::kPerSm><<<static_cast<int>(S::grid(p)), VB * 8, S::kShared, stream>>>(p);
     return launched("delta_sweep_back");
   });
   if (st != PLA_OK) return st;
@@ -475,9 +458,9 @@ int launch_gradient(const DeltaParams& p, int sms, cudaStream_t stream) {
     if ((st = launched("delta_clear_rows")) != PLA_OK) return st;
   }
   if (!p.chunk_bound) return PLA_OK;
-  const size_t shared = sizeof(GradShared<T, DK, PS>);
-  if ((st = allow_shared<delta_gradient<T, DK, PS, PO>>(shared)) != PLA_OK) return st;
-  delta_gradient<T, DK, PS, PO><<<p.chunk_bound * p.hk, kGradThreads, shared, stream>>>(p);
+  const size_t shared = sizeof(GradShared<T, DK>);
+  if ((st = allow_shared<delta_gradient<T, DK>>(shared)) != PLA_OK) return st;
+  delta_gradient<T, DK><<<p.chunk_bound * p.hk, kGradThreads, shared, stream>>>(p);
   return launched("delta_gradient");
 }
 
@@ -728,14 +711,11 @@ int pla_qk_norm_rotate_backward(const pla_qk_norm* a, void* workspace, size_t wo
 size_t pla_gated_delta_rule_workspace(const pla_delta* a, int backward) {
   if (check_delta(a) != PLA_OK) return 0;
   size_t bytes = 0;
-  const auto size = [&](auto zero, auto dk, auto ps, auto po) {
-    bytes = delta_sizes_of<decltype(zero), decltype(dk)::value, decltype(ps)::value, decltype(po)::value>(a, backward != 0).total;
+  const auto size = [&](auto zero, auto dk) {
+    bytes = delta_sizes_of<decltype(zero), decltype(dk)::value>(a, backward != 0).total;
     return 0;
   };
-  if (backward)
-    with_delta_gradient(a, true, size);
-  else
-    with_delta(a, size);
+  with_delta(a, size);
   return bytes;
 }
 
@@ -758,17 +738,17 @@ int pla_gated_delta_rule_forward(const pla_delta* a, pla_stream_t stream) {
   if (!a->hv || !a->dv || !a->sequences) return PLA_OK;
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
-  return with_delta(a, [&](auto zero, auto dk, auto ps, auto po) {
+  return with_delta(a, [&](auto zero, auto dk) {
     using T = decltype(zero);
-    constexpr int DK = decltype(dk)::value, PS = decltype(ps)::value, PO = decltype(po)::value;
-    const DeltaSizes s = delta_sizes_of<T, DK, PS, PO>(a, false);
+    constexpr int DK = decltype(dk)::value;
+    const DeltaSizes s = delta_sizes_of<T, DK>(a, false);
     if (s.chunks > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
     if (s.total && (a->workspace_bytes < s.total || !a->workspace || !aligned_to(a->workspace, 256)))
       return static_cast<int>(PLA_ERR_INVALID_ARGUMENT);
     const DeltaParams p = delta_params(a, s);
-    const int st = launch_prepare<T, DK, PS, PO>(p, as_stream(stream));
+    const int st = launch_prepare<T, DK>(p, as_stream(stream));
     if (st != PLA_OK) return st;
-    return launch_sweep<T, DK, PS, PO, false>(p, sms, as_stream(stream));
+    return launch_sweep<T, DK, false>(p, sms, as_stream(stream));
   });
 }
 
@@ -797,11 +777,10 @@ int pla_gated_delta_rule_backward(const pla_delta* a, const pla_delta_gradient* 
   if (!a->hv || !a->dv || !a->sequences) return PLA_OK;
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
-  const bool fp32_result = a->gates32 || g->dstate_in || g->dstate_out;
-  return with_delta_gradient(a, fp32_result, [&](auto zero, auto dk, auto ps, auto po) {
+  return with_delta(a, [&](auto zero, auto dk) {
     using T = decltype(zero);
-    constexpr int DK = decltype(dk)::value, PS = decltype(ps)::value, PO = decltype(po)::value;
-    const DeltaSizes s = delta_sizes_of<T, DK, PS, PO>(a, true);
+    constexpr int DK = decltype(dk)::value;
+    const DeltaSizes s = delta_sizes_of<T, DK>(a, true);
     if (s.chunks > kMaxGrid) return static_cast<int>(PLA_ERR_TOO_LARGE);
     if (s.total && (a->workspace_bytes < s.total || !a->workspace || !aligned_to(a->workspace, 256)))
       return static_cast<int>(PLA_ERR_INVALID_ARGUMENT);
@@ -815,10 +794,10 @@ int pla_gated_delta_rule_backward(const pla_delta* a, const pla_delta_gradient* 
     p.vec_do = a->dv % whole == 0 && aligned_to(g->d_o, 16) && !((g->do_batch | g->do_token | g->do_head) % whole);
     p.vec_o = aligned_to(g->dv, 16) && a->dv % whole == 0;
     p.state_out = nullptr;
-    int st = launch_prepare<T, DK, PS, PO>(p, as_stream(stream));
+    int st = launch_prepare<T, DK>(p, as_stream(stream));
     if (st != PLA_OK) return st;
-    if ((st = launch_sweep<T, DK, PS, PO, true>(p, sms, as_stream(stream))) != PLA_OK) return st;
-    return launch_gradient<T, DK, PS, PO>(p, sms, as_stream(stream));
+    if ((st = launch_sweep<T, DK, true>(p, sms, as_stream(stream))) != PLA_OK) return st;
+    return launch_gradient<T, DK>(p, sms, as_stream(stream));
   });
 }
 

@@ -1,0 +1,45 @@
+"""The sequence operators on a GPU where small calls do not reach: results to
+the last bit that their type holds, and the paths that large calls take.
+
+Tolerances.  The error of a vector bounds that of each of its elements, so a
+result of a 16-bit type is held element by element to one rounding of the
+element, h(t) = finfo(t).eps / 2, and the fp32 error of its token's vector:
+tests/test_gpu_sequence.py derives 2.4e-5 of the vector's norm for the delta
+rule, 4.8e-5 for its gradients and four times that for the gates'."""
+import pytest
+import torch
+
+import pla_b200 as P
+from tests import sequence_reference as R
+from tests import test_gpu_sequence as S
+from tests.test_gpu_sequence import BF16, DEV, F16, F32, f64, gpu, half, rand
+
+pytestmark = pytest.mark.gpu
+
+
+def by_element(got, want, dtype, tol, what):
+    """One rounding of each element and ``tol`` of the norm over the last dimension (the average row's if that is larger)."""
+    size = want.norm(dim=-1, keepdim=True)
+    S.within(got, want, half(dtype) * want.abs() + tol * torch.maximum(size, size.square().mean().sqrt()), what)
+
+
+# ---- bf16 results are fp32 results, rounded once ----------------------------
+ROUNDED = [c[:8] + (None,) for c in S.DELTA if c[1] > 1 and c[4] > 32]
+
+
+@pytest.mark.parametrize("case", ROUNDED)
+def test_delta_bf16_outputs_are_rounded_once(case):
+    q, k, v, g, beta, s, cu = S.delta_inputs(case, BF16, seed=101)
+    want, _ = R.gated_delta_rule(*(f64(t) for t in (q, k, v, g, beta)), cu=cu, state=f64(s))
+    o = P.gated_delta_rule(*(gpu(t) for t in (q, k, v, g, beta)), cu_seqlens=gpu(cu), state=gpu(s))
+    by_element(o, want, BF16, S.FORWARD[F32], "o")
+
+
+@pytest.mark.parametrize("case", ROUNDED)
+def test_delta_bf16_gradients_are_rounded_once(case):
+    got, want = S.delta_gradients(case, BF16, 102, False)
+    for name, a, b in zip("q k v g beta".split(), got, want):
+        gate = name in ("g", "beta")
+        if gate:  # over a head's tokens, as there
+            a, b = a.transpose(1, 2), b.transpose(1, 2)
+        by_element(a, b, BF16, S.BACKWARD[F32] * (4 if gate else 1), "d" + name)
