@@ -7,7 +7,7 @@
 // allocator, the launch on the current stream, a Meta kernel per op.  The
 // three training ops carry a C++ autograd function whose backward is an op of
 // its own, so autograd, fake tensors and graph capture see the same calls; a
-// second derivative raises.
+// second derivative and a forward-mode one raise.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -543,6 +543,17 @@ bool wants_gradient(const Ts&... ts) {
   };
   return at::GradMode::is_enabled() && (one(ts) || ...);
 }
+// There is no forward-mode formula: a tangent raises (it does not ask for a gradient, so it would be dropped).
+template <typename... Ts>
+void refuse_tangents(const char* op, const Ts&... ts) {
+  const auto one = [](const auto& t) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(t)>, Tensor>)
+      return t._fw_grad(0).defined();
+    else
+      return t && t->defined() && t->_fw_grad(0).defined();
+  };
+  TORCH_CHECK_NOT_IMPLEMENTED(!(one(ts) || ...), op, ": forward-mode derivatives are not implemented");
+}
 Tensor grad_if(const Tensor& g, const Tensor& input) { return input.defined() ? g : Tensor(); }
 
 std::tuple<Tensor, Tensor> causal_below(const Tensor& x, const Tensor& w, const optional<Tensor>& b, bool silu,
@@ -572,6 +583,7 @@ struct CausalFunction : torch::autograd::Function<CausalFunction> {
 };
 std::tuple<Tensor, Tensor> causal_autograd(const Tensor& x, const Tensor& w, const optional<Tensor>& b, bool silu,
                                            const optional<Tensor>& cu, const optional<Tensor>& state, bool return_state) {
+  refuse_tangents(kCausal, x, w, b, state);
   if (!wants_gradient(x, w, b, state)) return causal_below(x, w, b, silu, cu, state, return_state);
   auto r = CausalFunction::apply(x, w, b, silu, cu, state, return_state);
   return {r[0], r[1]};
@@ -608,6 +620,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 std::tuple<Tensor, Tensor> norm_autograd(const Tensor& q, const Tensor& k, const optional<Tensor>& wq, const optional<Tensor>& wk,
                                          const optional<Tensor>& cos, const optional<Tensor>& sin, const optional<Tensor>& pos,
                                          bool l2, double eps, bool interleaved) {
+  refuse_tangents(kNorm, q, k, wq, wk, cos, sin);
   TORCH_CHECK(!wants_gradient(cos, sin), kNorm, ": the tables have no gradient");
   if (!wants_gradient(q, k, wq, wk)) return norm_below(q, k, wq, wk, cos, sin, pos, l2, eps, interleaved);
   auto r = NormFunction::apply(q, k, wq, wk, cos, sin, pos, l2, eps, interleaved);
@@ -644,6 +657,7 @@ struct DeltaFunction : torch::autograd::Function<DeltaFunction> {
 std::tuple<Tensor, Tensor> delta_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
                                           double scale, const optional<Tensor>& cu, const optional<Tensor>& state,
                                           bool return_state) {
+  refuse_tangents(kDelta, q, k, v, g, beta, state);
   if (!wants_gradient(q, k, v, g, beta, state)) return delta_below(q, k, v, g, beta, scale, cu, state, return_state);
   auto r = DeltaFunction::apply(q, k, v, g, beta, scale, cu, state, return_state);
   return {r[0], r[1]};
@@ -674,6 +688,7 @@ struct NoGradient : torch::autograd::Function<NoGradient> {
 Tensor causal_step_autograd(const Tensor& x, const Tensor& state, const Tensor& w, const optional<Tensor>& b, bool silu) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && state.requires_grad()),
               "causal_depthwise_step: state is updated in place and must not require grad");
+  refuse_tangents("causal_depthwise_step", x, state, w, b);
   Tensor y = step_below<decltype(causal_step_cuda)>("pla_b200::causal_depthwise_step", state, x, state, w, b, silu);
   return wants_gradient(x, w, b) ? NoGradient::apply(y, x, w, b, optional<Tensor>(), optional<Tensor>()) : y;
 }
@@ -681,6 +696,7 @@ Tensor delta_step_autograd(const Tensor& q, const Tensor& k, const Tensor& v, co
                            const Tensor& state, double scale) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && state.requires_grad()),
               "gated_delta_rule_step: state is updated in place and must not require grad");
+  refuse_tangents("gated_delta_rule_step", q, k, v, g, beta, state);
   Tensor o = step_below<decltype(delta_step_cuda)>("pla_b200::gated_delta_rule_step", state, q, k, v, g, beta, state, scale);
   return wants_gradient(q, k, v, g, beta) ? NoGradient::apply(o, q, k, optional<Tensor>(v), optional<Tensor>(g), optional<Tensor>(beta)) : o;
 }

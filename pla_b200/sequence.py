@@ -23,7 +23,7 @@ no gradient.
 Dtypes: float32, bfloat16, float16; sums, norms and delta-rule states are
 fp32.  Every call runs as ``torch.ops.pla_b200.*`` on the current stream and
 can be captured in a CUDA graph.  A CPU tensor raises: there is no fallback.
-A second derivative raises.
+A second derivative and a forward-mode one raise.
 """
 from __future__ import annotations
 

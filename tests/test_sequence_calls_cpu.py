@@ -1,0 +1,44 @@
+"""Calls of the sequence operators that need no GPU to be judged: what is
+refused, what is laid out, what the sources promise."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import pla_b200 as P
+
+
+def meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, device="meta", dtype=dtype)
+
+
+def operators():
+    """name, call, its differentiable arguments."""
+    g, g1 = meta(1, 9, 4), meta(3, 4)
+    f32 = torch.float32
+    return [
+        ("causal_depthwise", lambda x, w, b, s: P.causal_depthwise(x, w, b, state=s),
+         [meta(2, 9, 24), meta(24, 4), meta(24), meta(2, 3, 24)]),
+        ("causal_depthwise_step", lambda x, w, b, s: P.causal_depthwise_step(x, s, w, b),
+         [meta(3, 24), meta(24, 4), meta(24), meta(3, 3, 24)]),
+        ("qk_norm_rotate", lambda q, k, wq, wk, c, s: P.qk_norm_rotate(q, k, wq, wk, cos=c, sin=s),
+         [meta(1, 9, 4, 64), meta(1, 9, 2, 64), meta(64), meta(64), meta(9, 16, dtype=f32), meta(9, 16, dtype=f32)]),
+        ("gated_delta_rule", lambda q, k, v, g, b, s: P.gated_delta_rule(q, k, v, g, b, state=s),
+         [meta(1, 9, 2, 64), meta(1, 9, 2, 64), meta(1, 9, 4, 32), g, g.clone(), meta(1, 4, 64, 32, dtype=f32)]),
+        ("gated_delta_rule_step", lambda q, k, v, g, b, s: P.gated_delta_rule_step(q, k, v, g, b, s),
+         [meta(3, 2, 64), meta(3, 2, 64), meta(3, 4, 32), g1, g1.clone(), meta(3, 4, 64, 32, dtype=f32)]),
+    ]
+
+
+# ---- forward-mode derivatives ----------------------------------------------
+@pytest.mark.parametrize("name,call,args", operators(), ids=lambda v: v if isinstance(v, str) else "")
+def test_forward_mode_derivatives_raise(name, call, args):
+    """There is no forward-mode formula: a tangent is refused, not dropped."""
+    call(*args)
+    for i in range(len(args)):
+        for needs_grad in (False, True):
+            with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+                dual = forward_ad.make_dual(args[i].detach().clone(), torch.empty_like(args[i]))
+                rest = [a.detach().clone().requires_grad_() if needs_grad and j == 0 and i else a for j, a in enumerate(args)]
+                call(*[dual if j == i else a for j, a in enumerate(rest)])
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda a: call(a, *args[1:]), (args[0],), (torch.empty_like(args[0]),))
