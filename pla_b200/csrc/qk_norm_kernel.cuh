@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_forward4(NormParams p) {
     }
     pairs_of<INTER>(f, g, lane.adjacent, wa, wb);
   }
-  const float per = p.l2 ? 1.f : 1.f / p.dim, counted = lane.there ? 1.f : 0.f;
+  const float per = p.l2 ? 1.f : 1.f / p.dim;
   Raw4<T> next[HB];
   float c_next[4], s_next[4];
   // past the end the last token, and past the heads the last head, are fetched again
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_forward4(NormParams p) {
     for (int h = 0; h < HB; ++h) {
       unpack4<T, INTER>(raw[h], lane, xa[h], xb[h]);
       const float2 f = both(fma2(xa[h][0], xa[h][0], fma2(xb[h][0], xb[h][0], fma2(xa[h][1], xa[h][1], mul2(xb[h][1], xb[h][1])))));
-      sum[h] = (f.x + f.y) * counted;
+      sum[h] = lane.there ? f.x + f.y : 0.f;  // not times 0: the sum may be infinite
     }
 #pragma unroll
     for (int o = LANES / 2; o >= 1; o >>= 1)
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_backward4(NormParams p) 
     }
     pairs_of<INTER>(f, g, lane.adjacent, wa, wb);
   }
-  const float per = p.l2 ? 1.f : 1.f / p.dim, counted = lane.there ? 1.f : 0.f;
+  const float per = p.l2 ? 1.f : 1.f / p.dim;
   const int rows = p.batch * p.tokens, stride = p.side_stride[which];  // rows below 2^30
   const int group = block * GROUPS + in_block;
   int row = group / side.heads;  // batch row and token as one number
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_backward4(NormParams p) 
       dots = fma2(mul2(da[i], wa[i]), xa[i], fma2(mul2(db[i], wb[i]), xb[i], dots));
     }
     const float2 q = both(squares), d = both(dots);
-    const float square = group_sum<LANES>((q.x + q.y) * counted);
+    const float square = group_sum<LANES>(lane.there ? q.x + q.y : 0.f);
     const float dot = group_sum<LANES>(lane.there ? d.x + d.y : 0.f);
     if (row >= rows) continue;
     const float r = inverse_root(fmaf(square, per, p.eps));

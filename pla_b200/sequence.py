@@ -74,7 +74,8 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     ``sin`` are float32 tables [P, R / 2]: the first R features are rotated in
     pairs (i, i + R / 2), or (2i, 2i + 1) with ``interleaved``, by row
     ``positions`` ([T], [1, T] or [B, T] integers; the token's number if
-    None).  A position outside the tables gives NaN in the rotated features.
+    None).  A position outside the tables gives NaN in the rotated features; a
+    head whose squares overflow float32 (values above about 1e19) gives 0.
     D is at most 256, B at most 65535.  Differentiable in q, k and the weights.
     """
     if norm not in ("rms", "l2"):

@@ -43,3 +43,23 @@ def test_delta_bf16_gradients_are_rounded_once(case):
         if gate:  # over a head's tokens, as there
             a, b = a.transpose(1, 2), b.transpose(1, 2)
         by_element(a, b, BF16, S.BACKWARD[F32] * (4 if gate else 1), "d" + name)
+
+
+# ---- norms of values that overflow, infinities -------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [6, 32, 64, 80, 96, 128, 192, 256])
+def test_norm_of_a_head_whose_squares_overflow_is_zero(dim, dtype):
+    """1e20^2 is not a float: 1 / sqrt(inf) = 0, times finite values, whatever part of its group a head fills."""
+    q = torch.ones(1, 3, 2, dim, device=DEV, dtype=dtype)
+    q[0, 1, 1] = 1e20
+    k = q.clone()
+    w = torch.ones(dim, device=DEV, dtype=dtype)
+    leaves = [t.requires_grad_() for t in (q, k, w)]
+    out = P.qk_norm_rotate(q, k, w, w)
+    grads = torch.autograd.grad(out, leaves, [torch.ones_like(t) for t in out])
+    for t in out:
+        # 1 / sqrt(1 + eps) is 5e-7 below 1, and a root and two products a few units of 2^-24
+        assert not t[0, 1, 1].any() and float((t[0, ::2] - 1).abs().max()) <= 1e-6
+    for t in grads[:2]:
+        assert not t[0, 1, 1].any() and bool(torch.isfinite(t).all())
+    assert bool(torch.isfinite(grads[2]).all())
