@@ -274,8 +274,10 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_forward4(NormParams p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const Pair na = mul2(xa[h][i], rr), nb = mul2(xb[h][i], rr);
-        oa[i] = fma2(na, ac[i], mul2(nb, bs[i]));
-        ob[i] = fma2(nb, bc[i], mul2(na, as[i]));
+        Pair from_b = pair(0.f, 0.f), from_a = from_b;  // nothing without rotation: the partner may be infinite
+        if (lane.turned) from_b = mul2(nb, bs[i]), from_a = mul2(na, as[i]);
+        oa[i] = fma2(na, ac[i], from_b);
+        ob[i] = fma2(nb, bc[i], from_a);
       }
       if (t < end && h < heads && lane.there) store4<T, INTER>(to, lane, oa, ob);
       to += p.dim;
@@ -390,9 +392,11 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_backward4(NormParams p) 
     if (turn + stride < rows) fetch(row + stride);
     Pair squares = pair(0.f, 0.f), dots = pair(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {  // rotated back; cos 1, sin 0 where there is no rotation
-      da[i] = fma2(ya[i], c[i], mul2(yb[i], s[i]));
-      db[i] = fma2(yb[i], c[i], mul2(ya[i], n[i]));
+    for (int i = 0; i < 2; ++i) {  // rotated back; without rotation cos is 1 and the partner left out
+      Pair from_b = pair(0.f, 0.f), from_a = from_b;
+      if (lane.turned) from_b = mul2(yb[i], s[i]), from_a = mul2(ya[i], n[i]);
+      da[i] = fma2(ya[i], c[i], from_b);
+      db[i] = fma2(yb[i], c[i], from_a);
       squares = fma2(xa[i], xa[i], fma2(xb[i], xb[i], squares));
       dots = fma2(mul2(da[i], wa[i]), xa[i], fma2(mul2(db[i], wb[i]), xb[i], dots));
     }

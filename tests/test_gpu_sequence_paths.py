@@ -63,3 +63,28 @@ def test_norm_of_a_head_whose_squares_overflow_is_zero(dim, dtype):
     for t in grads[:2]:
         assert not t[0, 1, 1].any() and bool(torch.isfinite(t).all())
     assert bool(torch.isfinite(grads[2]).all())
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rot", [(64, 32), (128, 0), (96, 64), (33, 10)])
+def test_norm_unrotated_features_do_not_meet(dim, rot, interleaved):
+    """An infinity in a feature that is not rotated stays there: in the weight, and for dw in the gradient."""
+    g = torch.Generator().manual_seed(111)
+    q, k = gpu(rand(g, 1, 5, 2, dim)), gpu(rand(g, 1, 5, 2, dim))
+    cos, sin = (torch.ones(5, rot // 2, device=DEV), torch.zeros(5, rot // 2, device=DEV)) if rot else (None, None)
+    call = lambda *a: P.qk_norm_rotate(*a, cos=cos, sin=sin, interleaved=interleaved)  # noqa: E731
+    w = torch.ones(dim, device=DEV)
+    rest = dim - rot
+    for bad in (rot, rot + rest // 2, dim - 1):
+        others = [i for i in range(dim) if i != bad]
+        odd = w.clone()
+        odd[bad] = float("inf")
+        for got, want in zip(call(q, k, odd, odd), call(q, k, w, w)):
+            assert torch.equal(got[..., others], want[..., others]) and not torch.isfinite(got[..., bad]).any()
+        leaves = [w.clone().requires_grad_(), w.clone().requires_grad_()]
+        dy = torch.ones_like(q)
+        want = torch.autograd.grad(call(q, k, *leaves), leaves, (dy, dy))
+        dy = dy.clone()
+        dy[0, 3, 1, bad] = float("nan")
+        for a, b in zip(torch.autograd.grad(call(q, k, *leaves), leaves, (dy, dy)), want):
+            assert torch.equal(a[others], b[others]) and bool(torch.isnan(a[bad]))
