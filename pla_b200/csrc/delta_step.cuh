@@ -41,7 +41,8 @@ constexpr int kStepWarps = 8;
 // lane.  The state follows the other shared memory.
 template <typename T>
 __global__ void __launch_bounds__(kStepWarps * 32, 3) delta_step(DeltaStepParams p) {
-  __shared__ float sq[128], sk[128], su[128];
+  __shared__ float sq[128], sk[128];
+  __shared__ __align__(16) float su[128];  // read four values at a time
   __shared__ __align__(16) float part[2][kStepWarps][128];
   __shared__ uint64_t full;
   extern __shared__ __align__(128) float held[];

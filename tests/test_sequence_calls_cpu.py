@@ -1,10 +1,16 @@
 """Calls of the sequence operators that need no GPU to be judged: what is
 refused, what is laid out, what the sources promise."""
+import glob
+import os
+import re
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import pla_b200 as P
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def meta(*shape, dtype=torch.bfloat16):
@@ -42,3 +48,25 @@ def test_forward_mode_derivatives_raise(name, call, args):
                 call(*[dual if j == i else a for j, a in enumerate(rest)])
     with pytest.raises(NotImplementedError):
         torch.func.jvp(lambda a: call(a, *args[1:]), (args[0],), (torch.empty_like(args[0]),))
+
+
+# ---- alignment ---------------------------------------------------------------
+def shared_arrays_read_as_vectors(text):
+    """Names of __shared__ arrays of scalars that a vector access names and no declaration aligns."""
+    bare = set()
+    for line in re.findall(r"^\s*__shared__ ([^;]*);", text, re.M):
+        if "__align__" in line or "alignas" in line:
+            continue
+        bare |= set(re.findall(r"(\w+)(?=\s*(?:\[|,|$))", re.sub(r"\[[^\]]*\]", "[", line.split(None, 1)[1])))
+    vector = re.findall(r"reinterpret_cast<(?:const )?(?:float[24]|uint[24]|int[24]|Vec<[^>]*>)\s*\*>\(&?(\w+)", text)
+    vector += re.findall(r"\b(?:load|store)<\w+, [248]>\(&?(\w+)", text)
+    return bare & set(vector)
+
+
+def test_shared_arrays_that_are_read_as_vectors_are_aligned():
+    assert shared_arrays_read_as_vectors("__shared__ float a[4], su[128];\n reinterpret_cast<const float4*>(su + c)") == {"su"}
+    assert not shared_arrays_read_as_vectors("__shared__ __align__(16) float su[128];\n reinterpret_cast<const float4*>(su + c)")
+    for path in sorted(glob.glob(os.path.join(ROOT, "pla_b200", "csrc", "*.cu*"))):
+        # a kernel's declarations reach to its end
+        for kernel in open(path).read().split("__global__")[1:]:
+            assert not shared_arrays_read_as_vectors(kernel), path
