@@ -306,6 +306,8 @@ PLA_API int pla_stencil7x7_band_step_halo(const void* in, const float* taps, con
  * linearly).  No reference counterpart.  dtype is f32 / bf16 / f16; sums,
  * norms and states are fp32.  Strides are in elements; the innermost
  * dimension is dense.  Outputs are dense and must not overlap an input.
+ * Tensors need no more than their elements' alignment (whole vectors are moved
+ * where addresses and strides allow it); workspaces as stated.
  *
  * A ragged batch is one batch row (batch == 1) of `tokens` tokens cut by
  * cu_seqlens, an int32 device array of sequences + 1 ascending entries that

@@ -761,8 +761,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
       if (t >= c.len || col >= p.dk) continue;
       const long long at = ((static_cast<long long>(c.batch) * p.tokens + c.token + t) * p.hk + kh) * p.dk + col;
       const float q2[2] = {dq[n][2 * h], dq[n][2 * h + 1]}, k2[2] = {dk[n][2 * h], dk[n][2 * h + 1]};
-      store_row(static_cast<T*>(p.dq) + at, q2, p.dk - col, p.dk % 2 == 0);
-      store_row(static_cast<T*>(p.dk_out) + at, k2, p.dk - col, p.dk % 2 == 0);
+      store_row(static_cast<T*>(p.dq) + at, q2, p.dk - col, p.pair_qk);
+      store_row(static_cast<T*>(p.dk_out) + at, k2, p.dk - col, p.pair_qk);
     }
 }
 

@@ -78,7 +78,7 @@ struct DeltaParams {
   int rows;          // dv rounded up to 64
   void *dq, *dk_out, *dv_out, *dg, *dbeta;
   int slabs;         // ceil(dv / 16)
-  int vec_qk, vec_v, vec_o, vec_do;
+  int vec_qk, vec_v, vec_o, vec_do, pair_qk;  // whole accesses: of 16 bytes (q, k: 4 elements; dq, dk: 2)
 };
 
 struct ChunkAt {

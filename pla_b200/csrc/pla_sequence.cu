@@ -793,6 +793,7 @@ int pla_gated_delta_rule_backward(const pla_delta* a, const pla_delta_gradient* 
     const int whole = static_cast<int>(16 / es);
     p.vec_do = a->dv % whole == 0 && aligned_to(g->d_o, 16) && !((g->do_batch | g->do_token | g->do_head) % whole);
     p.vec_o = aligned_to(g->dv, 16) && a->dv % whole == 0;
+    p.pair_qk = a->dk % 2 == 0 && aligned_to(g->dq, 2 * es) && aligned_to(g->dk, 2 * es);
     p.state_out = nullptr;
     int st = launch_prepare<T, DK>(p, as_stream(stream));
     if (st != PLA_OK) return st;

@@ -6,10 +6,13 @@ result of a 16-bit type is held element by element to one rounding of the
 element, h(t) = finfo(t).eps / 2, and the fp32 error of its token's vector:
 tests/test_gpu_sequence.py derives 2.4e-5 of the vector's norm for the delta
 rule, 4.8e-5 for its gradients and four times that for the gates'."""
+import ctypes
+
 import pytest
 import torch
 
 import pla_b200 as P
+from pla_b200 import _lib
 from tests import sequence_reference as R
 from tests import test_gpu_sequence as S
 from tests.test_gpu_sequence import BF16, DEV, F16, F32, f64, gpu, half, rand
@@ -88,3 +91,38 @@ def test_norm_unrotated_features_do_not_meet(dim, rot, interleaved):
         dy[0, 3, 1, bad] = float("nan")
         for a, b in zip(torch.autograd.grad(call(q, k, *leaves), leaves, (dy, dy)), want):
             assert torch.equal(a[others], b[others]) and bool(torch.isnan(a[bad]))
+
+
+# ---- C callers ---------------------------------------------------------------
+CODE = {F32: _lib.PLA_F32, BF16: _lib.PLA_BF16, F16: _lib.PLA_F16}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_delta_tensors_that_start_anywhere(dtype):
+    """A C caller's tensors are aligned to their elements only: the same bits as from torch's."""
+    q, k, v, g, beta, _, _ = (gpu(t) for t in S.delta_inputs((1, 100, 1, 2, 64, 32, False, None, F32), dtype, seed=121))
+    d_o = gpu(rand(torch.Generator().manual_seed(122), *v.shape, dtype=dtype))
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, g, beta)]
+    o = P.gated_delta_rule(*leaves, scale=0.125)
+    want = [o.detach(), *torch.autograd.grad(o, leaves, d_o)]
+
+    def odd(t):  # one element behind an aligned address
+        return torch.empty(t.numel() + 1, device=DEV, dtype=t.dtype)[1:].view(t.shape).copy_(t)
+
+    q, k, v, g, beta, d_o = (odd(t) for t in (q, k, v, g, beta, d_o))
+    got = [odd(torch.zeros_like(t)) for t in want]
+    a = _lib.Delta(**{n: t.data_ptr() for n, t in zip(("q", "k", "v", "g", "beta", "o"), (q, k, v, g, beta, got[0]))},
+                   batch=1, tokens=100, sequences=1, hk=1, hv=2, dk=64, dv=32, gates32=1, dtype=CODE[dtype], scale=0.125)
+    for name, t in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta)):
+        for part, stride in zip(("batch", "token", "head"), t.stride()):
+            setattr(a, f"{name}_{part}", stride)
+    L, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    size = max(L.pla_gated_delta_rule_workspace(ctypes.byref(a), back) for back in (0, 1))
+    work = torch.empty(size, device=DEV, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = work.data_ptr(), size
+    assert L.pla_gated_delta_rule_forward(ctypes.byref(a), stream) == 0
+    grad = _lib.DeltaGradient(d_o=d_o.data_ptr(), do_batch=d_o.stride(0), do_token=d_o.stride(1), do_head=d_o.stride(2),
+                              **{n: t.data_ptr() for n, t in zip(("dq", "dk", "dv", "dg", "dbeta"), got[1:])})
+    assert L.pla_gated_delta_rule_backward(ctypes.byref(a), ctypes.byref(grad), stream) == 0
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
