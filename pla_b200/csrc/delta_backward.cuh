@@ -265,15 +265,16 @@ __device__ __forceinline__ void planes_product(float (&d0)[4], float (&d1)[4], c
       mma(d1, a[i], b[j][2], b[j][3]);
     }
 }
-// Two neighbours of a tile as the sum of its planes.
+// Two neighbours of a tile as the sum of its planes, times their row's factor.
 template <int PLANES>
-__device__ __forceinline__ void tile_pair(const __half* tile, uint32_t plane, uint32_t at, float (&f)[2]) {
+__device__ __forceinline__ void tile_pair(const __half* tile, uint32_t plane, uint32_t at, float row, float (&f)[2]) {
 #pragma unroll
   for (int i = 0; i < PLANES; ++i) {
     const float2 v = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const char*>(tile) + i * plane + at));
     f[0] = i ? f[0] + v.x : v.x;
     f[1] = i ? f[1] + v.y : v.y;
   }
+  f[0] *= row, f[1] *= row;
 }
 template <int PLANES, bool TRANS>
 __device__ __forceinline__ void planes_load(uint32_t (&f)[PLANES][4], uint32_t at, uint32_t plane) {
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
           const uint32_t at = tile_at<kChunk>(row + e, t >> 3) + (t & 7) * 2;
 #pragma unroll
           for (int n = 0; n < kPlanes; ++n)
-            xv = fmaf(__half2float(*reinterpret_cast<const __half*>(reinterpret_cast<const char*>(s.in.x) + n * kNarrow + at)), v[e], xv);
+            xv = fmaf(common[3] * __half2float(*reinterpret_cast<const __half*>(reinterpret_cast<const char*>(s.in.x) + n * kNarrow + at)), v[e], xv);
         }
 #pragma unroll
         for (int i = 0; i < kGradBlock * DK / 8 / kGradThreads; ++i) {
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
 
     // parts of dq and dk that see the states, and their products with q and k
     float dot[4][2] = {};
-    float to_one[2], to_two[2], to_three[2], beta[2];  // of this lane's rows
+    float to_one[2], to_two[2], to_three[2], beta[2], k_row[2], q_row[2];  // of this lane's rows
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int i = r0 + h * 8;
@@ -559,6 +560,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
       to_two[h] = p.scale * s.down[i] * (s.orow[i] * common[0]);
       to_three[h] = s.tail[i] * (common[2] * common[1]);
       beta[h] = s.beta[i];
+      k_row[h] = s.krow[i], q_row[h] = s.qrow[i];
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -567,8 +569,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
         const int i = r0 + h * 8;
         const uint32_t at = tile_at<DK>(i, cg * (DK / 32) + n) + (lane & 3) * 4;
         float kv[2], qv[2];
-        tile_pair<IN>(s.tile[0][0], L::kTile, at, kv);
-        tile_pair<IN>(s.tile[1][0], L::kTile, at, qv);
+        tile_pair<IN>(s.tile[0][0], L::kTile, at, k_row[h], kv);
+        tile_pair<IN>(s.tile[1][0], L::kTile, at, q_row[h], qv);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int at_e = 2 * h + e;
@@ -581,16 +583,16 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
         }
       }
     // sum of H = e^{G_C - G} k . (U D^T) over the chunk, before the rest joins that dot
-    float h_part = quad_sum(dot[2][0]) * s.krow[r0] + quad_sum(dot[2][1]) * s.krow[r0 + 8];
+    float h_part = quad_sum(dot[2][0]) + quad_sum(dot[2][1]);
 
     // N, Gamma dA and B with the row factors of what they meet
     float sq[4][2][4], top[4] = {};
     {
-      float row_hi[2], row_lo[2], row_n[2], row_q[2], row_k[2];
+      float row_hi[2], row_lo[2], row_n[2], row_k[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int i = r0 + h * 8;
-        row_hi[h] = s.hi[i], row_lo[h] = s.lo[i], row_q[h] = s.qrow[i], row_k[h] = beta[h] * s.krow[i];
+        row_hi[h] = s.hi[i], row_lo[h] = s.lo[i], row_k[h] = beta[h] * k_row[h];
         row_n[h] = p.scale * (s.orow[i] * common[2]);
       }
       const float to_a = -(common[3] * common[2]);
@@ -605,7 +607,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
           const float gamma = exp_fast((row_hi[h] - (e & 1 ? hi.y : hi.x)) + (row_lo[h] - (e & 1 ? lo.y : lo.x)));
           const float nn = j <= i ? gamma * (row_n[h] * a_p[n][e]) : 0.f, ga = j < i ? gamma * (to_a * a_a[n][e]) : 0.f;
           sq[0][n][e] = nn * (e & 1 ? kj.y : kj.x);
-          sq[1][n][e] = nn * row_q[h];
+          sq[1][n][e] = nn * q_row[h];
           sq[2][n][e] = ga * (e & 1 ? kj.y : kj.x);
           sq[3][n][e] = ga * row_k[h];
 #pragma unroll
@@ -681,8 +683,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
           const int i = r0 + h * 8;
           const uint32_t at = tile_at<DK>(i, cg * (DK / 32) + n) + (lane & 3) * 4;
           float kv[2], qv[2];
-          tile_pair<IN>(s.tile[0][0], L::kTile, at, kv);
-          tile_pair<IN>(s.tile[1][0], L::kTile, at, qv);
+          tile_pair<IN>(s.tile[0][0], L::kTile, at, k_row[h], kv);
+          tile_pair<IN>(s.tile[1][0], L::kTile, at, q_row[h], qv);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int at_e = 2 * h + e;
@@ -701,7 +703,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int i = r0 + h * 8;
-        const float v = quad_sum(dot[w][h]) * (w == 1 ? s.qrow[i] : s.krow[i]);
+        const float v = quad_sum(dot[w][h]);
         if ((lane & 3) == 0) s.dots[cg][w][i] = v;
       }
     // H summed over this warp's rows (a lane of each quad)
@@ -721,7 +723,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
         for (int w = 0; w < 4; ++w) v[w] = (s.dots[0][w][t] + s.dots[1][w][t]) + (s.dots[2][w][t] + s.dots[3][w][t]);
         const float with_v = ((s.xv[0][t] + s.xv[1][t]) + (s.xv[2][t] + s.xv[3][t])) + ((s.xv[4][t] + s.xv[5][t]) + (s.xv[6][t] + s.xv[7][t]));
         dg[e] = s.beta[t] * (v[0] + v[3]) + v[1] - v[2];
-        const float db = (v[0] + v[3]) + common[3] * with_v;
+        const float db = (v[0] + v[3]) + with_v;
         if (t < c.len) {
           const long long at = (static_cast<long long>(c.batch) * p.tokens + c.token + t) * p.hv + vh;
           if (p.gates32)

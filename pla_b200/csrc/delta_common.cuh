@@ -177,7 +177,7 @@ struct Pow2 {
 };
 __device__ __forceinline__ Pow2 pow2_for(float largest) {
   int e = static_cast<int>((__float_as_uint(largest) >> 23) & 0xff);
-  e = min(max(e, 32), 240);  // f in [2^-101, 2^107]
+  e = min(max(e, 32), 254);  // f in [2^-115, 2^107]
   return {__int_as_float((127 + 12 - e + 127) << 23), __int_as_float((e - 12) << 23)};
 }
 

@@ -428,6 +428,10 @@ struct SweepShared {
 
 // |A B| over 64 tokens with one operand's planes below 2^13.
 constexpr float kPlaneTop = 8192.f, kSumTop = 64.f * kPlaneTop;
+// A row of T has its largest near 2^12, and at least 1 of T itself is 1: X's
+// scales are handed on divided by that, so that sums of T X times them are no
+// larger than U and reach the end of the float range.
+constexpr float kTTop = 4096.f;
 // Scale for what lies below `bound`: brings it below 2^15.
 __device__ __forceinline__ Pow2 scale_below(float bound) {
   const Pow2 s = pow2_for(bound);
@@ -532,7 +536,7 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
     {
       row_max(x, top);
       const Pow2 fx[2] = {pow2_for(top[0]), pow2_for(top[1])};
-      share(m.scale_a, wn, m0, lane, fx[0].inverse, fx[1].inverse);
+      share(m.scale_a, wn, m0, lane, fx[0].inverse / kTTop, fx[1].inverse / kTTop);
       tile_write<kChunk>(m.a, M::kNarrow, m0, wn * 16, lane, x, fx);
     }
     __syncthreads();
@@ -550,8 +554,10 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
       add_scaled(u, bu, element(back[0], kk), element(back[1], kk));
     }
     coef_read(coef, kTRow, wn * 2, lane, w);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) w[n].x *= kTTop, w[n].y *= kTTop;
     scale_columns(u, w);
-    const float bound_x[2] = {most_of(back[0]) * kPlaneTop, most_of(back[1]) * kPlaneTop};
+    const float bound_x[2] = {most_of(back[0]) * (kTTop * kPlaneTop), most_of(back[1]) * (kTTop * kPlaneTop)};
     const Pow2 fu[2] = {scale_below(bounds.x * bound_x[0]), scale_below(bounds.x * bound_x[1])};
     tile_write<kChunk>(m.c, M::kNarrow, m0, wn * 16, lane, u, fu);
     if (KEEP && wn == 0 && (lane & 3) == 0) {
@@ -603,8 +609,8 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            q[n][e] = (e & 1 ? wq[n].y : wq[n].x) * (q[n][e] * old[e >> 1].inverse) +
-                      (e & 1 ? w[n].y : w[n].x) * (pu[n][e] * fu[e >> 1].inverse);
+            q[n][e] = ((e & 1 ? wq[n].y : wq[n].x) * old[e >> 1].inverse) * q[n][e] +
+                      ((e & 1 ? w[n].y : w[n].x) * fu[e >> 1].inverse) * pu[n][e];
         strip_store<T, kPitch>(m.slab[c & 1] + wn * 16 * kPitch + m0 * sizeof(T), lane, q, o + (c * kChunk + wn * 16) * o_step + m0, o_step, len - wn * 16, a.width - m0,
                        p.vec_o);
       }

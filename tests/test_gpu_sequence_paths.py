@@ -126,3 +126,28 @@ def test_delta_tensors_that_start_anywhere(dtype):
     assert L.pla_gated_delta_rule_backward(ctypes.byref(a), ctypes.byref(grad), stream) == 0
     for x, y in zip(got, want):
         assert torch.equal(x, y)
+
+
+# ---- values near the end of the float range ----------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_delta_values_near_the_end_of_the_range(dtype):
+    """The planes' scales reach every float: columns of v and of the state of 1e36 give what smaller ones give."""
+    q, k, v, g, beta, s, _ = S.delta_inputs((1, 150, 1, 2, 64, 32, True, None, F32), dtype, seed=131)
+    v[..., 5] *= 1e36
+    v[..., 6] *= 1e-30
+    s[..., 5] *= 1e36
+    s[..., 7] *= 1e36
+    want, last = R.gated_delta_rule(*(f64(t) for t in (q, k, v, g, beta)), cu=None, state=f64(s))
+    o, state = P.gated_delta_rule(*(gpu(t) for t in (q, k, v, g, beta)), state=gpu(s), return_state=True)
+    for c in range(32):  # columns never meet: each against its own size
+        S.token_norms(o[..., c].transpose(1, 2), want[..., c].transpose(1, 2), S.FORWARD[dtype], f"o, column {c}")
+        S.token_norms(state[..., c], last[..., c], S.FORWARD[F32], f"state, column {c}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_delta_gradients_near_the_end_of_the_range(dtype):
+    def change(q, k, v, g, beta):
+        v[..., 5] *= 4e35
+
+    got, want = S.delta_gradients((1, 30, 1, 2, 64, 32, True, None, F32), dtype, 132, True, change)
+    S.check_delta_gradients(got, want, dtype, F32, False)
