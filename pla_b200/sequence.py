@@ -150,7 +150,7 @@ class DeltaMixer(torch.nn.Module):
         """Zero states of n sequences: the convolution's inputs and the delta rule's fp32 state."""
         w = self.in_proj.weight
         return (torch.zeros(n, self.conv.weight.shape[-1] - 1, sum(self.widths), device=w.device, dtype=w.dtype),
-                torch.zeros(n, self.value_heads, self.head_dim, self.value_dim, device=w.device))
+                torch.zeros(n, self.value_heads, self.head_dim, self.value_dim, device=w.device, dtype=torch.float32))
 
     def _gates(self, x):
         a, b = self.gate_proj(x).float().chunk(2, -1)
@@ -173,7 +173,18 @@ class DeltaMixer(torch.nn.Module):
             return self.out_proj(o[0].flatten(-2)), (conv_state, o[1])
         return self.out_proj(o.flatten(-2))
 
+    def _check_delta_state(self, s: torch.Tensor, n: int) -> None:
+        # what gated_delta_rule_step would refuse, before the convolution's state has moved on
+        shape = (n, self.value_heads, self.head_dim, self.value_dim)
+        if s.shape != shape or s.dtype != torch.float32:
+            raise ValueError(f"the delta rule's state must be float32 {list(shape)}, got {s.dtype} {list(s.shape)}")
+        if n and not (s.is_contiguous() or s[0].is_contiguous() and (n == 1 or s.stride(0) >= s[0].numel())):
+            raise ValueError("each sequence's delta rule state must be dense and its own: it is updated in place")
+        if s.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the delta rule's state is updated in place and must not require grad")
+
     def step(self, x: torch.Tensor, state: tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
+        self._check_delta_state(state[1], x.shape[0])
         h = causal_depthwise_step(self.in_proj(x), state[0], self.conv.weight, self.conv.bias, silu=True)
         q, k, v = self._heads(h)
         q, k = (t[:, 0] for t in qk_norm_rotate(q[:, None], k[:, None], norm="l2"))

@@ -70,3 +70,28 @@ def test_shared_arrays_that_are_read_as_vectors_are_aligned():
         # a kernel's declarations reach to its end
         for kernel in open(path).read().split("__global__")[1:]:
             assert not shared_arrays_read_as_vectors(kernel), path
+
+
+# ---- the block -----------------------------------------------------------------
+def test_mixer_states_do_not_follow_the_default_dtype():
+    m = P.DeltaMixer(32, 2, head_dim=16, value_heads=4, value_dim=8)
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        conv, delta = m.new_state(3)
+    finally:
+        torch.set_default_dtype(before)
+    assert conv.dtype == m.in_proj.weight.dtype and delta.dtype == torch.float32
+
+
+def test_mixer_step_refuses_a_state_before_it_changes_any():
+    m = P.DeltaMixer(32, 2, head_dim=16, value_heads=4, value_dim=8).to("meta")
+    x, (conv, delta) = meta(3, 32, dtype=torch.float32), m.new_state(3)
+    version = conv._version
+    m.step(x, (conv, delta))
+    assert conv._version > version
+    version = conv._version
+    for bad in (delta.bfloat16(), delta[:2], delta[:, :2], delta.transpose(2, 3), delta[:1].expand(3, -1, -1, -1), delta.requires_grad_()):
+        with pytest.raises((ValueError, RuntimeError)):
+            m.step(x, (conv, bad))
+        assert conv._version == version
