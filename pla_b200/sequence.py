@@ -126,7 +126,8 @@ class DeltaMixer(torch.nn.Module):
     fp32; ``out_proj`` maps the heads back.  ``forward`` takes [B, T, dim] (or
     a ragged [1, T, dim] with ``cu_seqlens``); ``step`` takes [N, dim] and a
     state from ``new_state`` or ``forward(..., return_state=True)``, which it
-    updates in place.
+    updates in place.  Under ``torch.autocast`` the operators run in its dtype,
+    and so do the convolution's states.
     """
 
     def __init__(self, dim: int, num_heads: int, head_dim: int = 128, value_heads: int | None = None,
@@ -149,8 +150,12 @@ class DeltaMixer(torch.nn.Module):
     def new_state(self, n: int) -> tuple[torch.Tensor, torch.Tensor]:
         """Zero states of n sequences: the convolution's inputs and the delta rule's fp32 state."""
         w = self.in_proj.weight
-        return (torch.zeros(n, self.conv.weight.shape[-1] - 1, sum(self.widths), device=w.device, dtype=w.dtype),
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else w.dtype
+        return (torch.zeros(n, self.conv.weight.shape[-1] - 1, sum(self.widths), device=w.device, dtype=dtype),
                 torch.zeros(n, self.value_heads, self.head_dim, self.value_dim, device=w.device, dtype=torch.float32))
+
+    def _taps(self, dtype):  # under autocast the projections' results are not of the weights' dtype
+        return self.conv.weight.to(dtype), self.conv.bias.to(dtype)
 
     def _gates(self, x):
         a, b = self.gate_proj(x).float().chunk(2, -1)
@@ -164,8 +169,9 @@ class DeltaMixer(torch.nn.Module):
 
     def forward(self, x: torch.Tensor, cu_seqlens: torch.Tensor | None = None, state=None, return_state: bool = False):
         before = (None, None) if state is None else state
-        h, conv_state = causal_depthwise(self.in_proj(x), self.conv.weight, self.conv.bias, silu=True,
-                                         cu_seqlens=cu_seqlens, state=before[0], return_state=True)
+        h = self.in_proj(x)
+        h, conv_state = causal_depthwise(h, *self._taps(h.dtype), silu=True, cu_seqlens=cu_seqlens, state=before[0],
+                                         return_state=True)
         q, k, v = self._heads(h)
         q, k = qk_norm_rotate(q, k, norm="l2")
         o = gated_delta_rule(q, k, v, *self._gates(x), cu_seqlens=cu_seqlens, state=before[1], return_state=return_state)
@@ -185,7 +191,8 @@ class DeltaMixer(torch.nn.Module):
 
     def step(self, x: torch.Tensor, state: tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
         self._check_delta_state(state[1], x.shape[0])
-        h = causal_depthwise_step(self.in_proj(x), state[0], self.conv.weight, self.conv.bias, silu=True)
+        h = self.in_proj(x)
+        h = causal_depthwise_step(h, state[0], *self._taps(h.dtype), silu=True)
         q, k, v = self._heads(h)
         q, k = (t[:, 0] for t in qk_norm_rotate(q[:, None], k[:, None], norm="l2"))
         return self.out_proj(gated_delta_rule_step(q, k, v, *self._gates(x), state[1]).flatten(-2))

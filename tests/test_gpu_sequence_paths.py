@@ -151,3 +151,39 @@ def test_delta_gradients_near_the_end_of_the_range(dtype):
 
     got, want = S.delta_gradients((1, 30, 1, 2, 64, 32, True, None, F32), dtype, 132, True, change)
     S.check_delta_gradients(got, want, dtype, F32, False)
+
+
+# ---- the block -----------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_mixer_under_autocast_is_the_mixer_of_that_dtype(dtype):
+    """fp32 weights under autocast: the calls of a block whose products and operators are of that dtype, with the same bits
+    (its gates' constants stay fp32)."""
+    m = S.make_mixer()
+    cast = S.make_mixer().to(dtype)
+    cast.A_log.data, cast.dt_bias.data = m.A_log.data.clone(), m.dt_bias.data.clone()
+    x = gpu(rand(torch.Generator().manual_seed(141), 2, 70, 48))
+    with torch.no_grad():
+        want, end = cast(x.to(dtype), return_state=True)
+        steps, first = cast.new_state(2), None
+        first = cast.step(x[:, 0].to(dtype), steps)
+        with torch.autocast("cuda", dtype):
+            y, state = m(x, return_state=True)
+            held = m.new_state(2)
+            one = m.step(x[:, 0], held)
+    for a, b in zip((y, *state, one, *held), (want, *end, first, *steps)):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_mixer_trains_under_autocast():
+    m = S.make_mixer()
+    cast = S.make_mixer().to(BF16)
+    cast.A_log.data, cast.dt_bias.data = m.A_log.data.clone(), m.dt_bias.data.clone()
+    x = gpu(rand(torch.Generator().manual_seed(142), 2, 70, 48, dtype=BF16))
+    with torch.autocast("cuda", BF16):
+        y = m(x)
+    y.backward(torch.ones_like(y))
+    z = cast(x)
+    z.backward(torch.ones_like(z))
+    assert torch.equal(y, z)
+    for (name, a), b in zip(m.named_parameters(), cast.parameters()):
+        assert a.grad.dtype == F32 and torch.equal(a.grad.to(b.dtype), b.grad), name
