@@ -194,5 +194,5 @@ class DeltaMixer(torch.nn.Module):
         h = self.in_proj(x)
         h = causal_depthwise_step(h, state[0], *self._taps(h.dtype), silu=True)
         q, k, v = self._heads(h)
-        q, k = (t[:, 0] for t in qk_norm_rotate(q[:, None], k[:, None], norm="l2"))
+        q, k = (t[0] for t in qk_norm_rotate(q[None], k[None], norm="l2"))  # no positions: any number of sequences as one row
         return self.out_proj(gated_delta_rule_step(q, k, v, *self._gates(x), state[1]).flatten(-2))
