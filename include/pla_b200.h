@@ -473,7 +473,8 @@ PLA_API int pla_ipc_close(void* ptr, uint64_t offset);
 
 /*
  * Device-side fault word of the current device: bit 0 = an mbarrier wait in a
- * kernel gave up after its time bound; bit 1 = a wait for a neighbouring
+ * kernel gave up after its time bound (its output is incomplete; a delta rule
+ * step leaves that head's state as it was); bit 1 = a wait for a neighbouring
  * GPU's halo flag gave up.  Reading it synchronises the
  * device.  pla_clear_device_faults() zeroes it.
  */

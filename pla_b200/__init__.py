@@ -11,6 +11,7 @@ replace ``data/depthwise_conv_7x7.py`` and ``data/stencil_7x7.py``.
   ``gated_delta_rule()`` with their gradients, and the single-token forms ``causal_depthwise_step()``,
   ``gated_delta_rule_step()``; ``DeltaMixer`` chains them
 * ``pla_b200.iterate``   — ``stencil7x7_iterate()``, ``BandedStencil`` (multi-GPU)
+* ``check_faults()``      — raises if a kernel gave up a bounded wait
 
 All compute goes through the C ABI in ``include/pla_b200.h``
 (``libpla_b200.so``, built by ``python -m pla_b200.build``).  The functional
@@ -26,6 +27,7 @@ try:  # registered at import so that compiled code never traces the loading
 except ImportError:  # not built yet (e.g. while pla_b200.build runs): the ops raise when called
     pass
 
+from ._lib import check_faults
 from .depthwise import DepthwiseLayerNorm, depthwise7x7, depthwise7x7_layernorm, depthwise7x7_many, depthwise_kxk
 from .iterate import BandedStencil, band_rows, stencil7x7_iterate
 from .sequence import (DeltaMixer, causal_depthwise, causal_depthwise_step, gated_delta_rule, gated_delta_rule_step,
@@ -34,4 +36,4 @@ from .stencil import stencil7x7
 
 __all__ = ["stencil7x7", "depthwise7x7", "depthwise7x7_many", "depthwise_kxk", "depthwise7x7_layernorm", "DepthwiseLayerNorm",
            "stencil7x7_iterate", "BandedStencil", "band_rows", "causal_depthwise", "causal_depthwise_step",
-           "qk_norm_rotate", "gated_delta_rule", "gated_delta_rule_step", "DeltaMixer"]
+           "qk_norm_rotate", "gated_delta_rule", "gated_delta_rule_step", "DeltaMixer", "check_faults"]

@@ -6,6 +6,7 @@ CPU or eager-PyTorch fallback anywhere in this package.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -162,6 +163,21 @@ def check(status: int, what: str) -> None:
         msg = L.pla_status_string(status).decode()
         detail = L.pla_last_cuda_error().decode()
         raise PlaError(f"{what}: {msg}" + (f" ({detail})" if detail and status == 4 else ""))
+
+
+def check_faults(device=None) -> None:
+    """Raise ``PlaError`` if a kernel on ``device`` (the current one if None) gave up a bounded wait (synchronises).
+
+    Kernels that wait (for an asynchronous copy, for a neighbour's halo) do so
+    for about two seconds at most, then record it and end; what they had to
+    write is then incomplete.  The word stays set until
+    ``pla_clear_device_faults``.
+    """
+    v = ctypes.c_uint(0)
+    with contextlib.nullcontext() if device is None else torch.cuda.device(device):
+        check(lib().pla_read_device_faults(ctypes.byref(v)), "pla_read_device_faults")
+    if v.value:
+        raise PlaError(f"device fault word {v.value:#x}: a bounded wait in a kernel timed out")
 
 
 def stream_ptr(device: torch.device) -> int:

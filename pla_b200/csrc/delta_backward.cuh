@@ -70,8 +70,9 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
       m.keep_s[m0 + (lane >> 2) + 8] = fd[1].inverse;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    const char* stage = ring.wait();
-    __syncthreads();  // planes of D and this chunk's do are there; the other slab is free
+    // planes of D and this chunk's do are there; the other slab is free
+    if (!__syncthreads_and(ring.wait())) return ring.give_up(a.chunks - turn);
+    const char* stage = ring.stage();
     if (c > 0)
       slab_fetch<T, VB>(m.slab[~turn & 1], d_o + (c - 1) * kChunk * p.do_token, p.do_token, kChunk, a.width, p.vec_do);
     keep_tile<VB, DK>(m.s, m.keep_s, p.dstates + kept_at<DK>(p, head_at), p.scales + (head_at * 4 + 1) * p.rows, p.rows,

@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) delta_step(DeltaStepParams
   // lanes_row lanes a row, the warp's rows 32 / lanes_row at a time
   const int lanes_row = p.dv / 4, at_once = 32 / lanes_row, sub = lane / lanes_row, col = lane % lanes_row * 4;
   const int step = at_once * kStepWarps;
-  barrier_wait(&full, 0);
+  const bool there = barrier_wait(&full, 0);
   float with_k[4] = {}, with_q[4] = {};
 #pragma unroll 4
   for (int row = warp * at_once + sub; row < p.dk; row += step) {
@@ -93,7 +93,10 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) delta_step(DeltaStepParams
     store<float, 4>(&part[0][warp][col], with_k);
     store<float, 4>(&part[1][warp][col], with_q);
   }
-  __syncthreads();
+  if (!__syncthreads_and(there)) {  // the state stays as it was
+    if (tid == 0) barrier_wait(&full, 0);  // more time for the copy: the block's shared memory is held meanwhile
+    return;
+  }
   if (tid < p.dv) {
     float a = 0.f, c = 0.f;
 #pragma unroll

@@ -55,19 +55,20 @@ __device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// Waits about two seconds at most; then records the fault and lets the caller
-// carry on (its results are undefined, the host sees the fault word).
-__device__ __forceinline__ void barrier_wait(uint64_t* bar, uint32_t parity) {
-  if (barrier_try(bar, parity)) return;
+// Waits about two seconds at most; then records the fault, which the host reads,
+// and returns false: the caller's block ends without using what did not come.
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity) {
+  if (barrier_try(bar, parity)) return true;
   uint64_t t0, t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
   do {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i)
-      if (barrier_try(bar, parity)) return;
+      if (barrier_try(bar, parity)) return true;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   } while (t - t0 < 2000000000ull);
   atomicOr(&g_sequence_faults, 1u);
+  return false;
 }
 __device__ __forceinline__ void bulk_copy(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -273,6 +274,17 @@ __device__ __forceinline__ void product(float (&d0)[4], float (&d1)[4], const ui
   }
 }
 
+// Thread 0 gives `count` copies in flight their time, from stage `at` on; the
+// block's shared memory is held until it returns.  (Not inlined: the sweeps need
+// the registers.)
+static __device__ __noinline__ void drain(uint64_t* full, int at, int filled, int stages, int count) {
+  if (threadIdx.x != 0) return;
+  for (int i = 0; i < count; ++i) {
+    barrier_wait(full + at, filled & 1);
+    if (++at == stages) at = 0, ++filled;
+  }
+}
+
 // Copies of the chunks' tiles into a ring of stages.  Thread 0 issues them; a
 // stage is refilled when every warp has arrived at its `empty` barrier.
 template <typename L, int STAGES>
@@ -300,17 +312,16 @@ struct Ring {
     bulk_copy(to, p.tiles + (static_cast<long long>(chunk) * p.hk + kh) * L::kTiles, L::kTiles, full + stage);
     bulk_copy(to + L::kTiles, p.heads + (static_cast<long long>(chunk) * p.hv + vh) * L::kHead, L::kHead, full + stage);
   }
-  __device__ __forceinline__ const char* wait() {
-    barrier_wait(full + at, filled & 1);
-    return stages + at * L::kStage;
-  }
+  __device__ __forceinline__ const char* stage() const { return stages + at * L::kStage; }
+  __device__ __forceinline__ bool wait() { return barrier_wait(full + at, filled & 1); }
+  // A wait ran out, `left` chunks (this one among them) are not worked on.
+  __device__ __forceinline__ void give_up(int left) const { drain(full, at, filled, STAGES, min(STAGES, left)); }
   // This chunk's stage is done with; chunk `refill` (if >= 0) takes its place.
   __device__ __forceinline__ void next(const DeltaParams& p, int refill, int kh, int vh) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) barrier_arrive(empty + at);
     if (threadIdx.x == 0 && refill >= 0) {
-      barrier_wait(empty + at, filled & 1);
-      fill(p, at, refill, kh, vh);
+      if (barrier_wait(empty + at, filled & 1)) fill(p, at, refill, kh, vh);  // else the wait for it runs out too
     }
     __syncwarp();
     if (++at == STAGES) {
@@ -497,8 +508,9 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep(DeltaParams p) {
       m.keep_s[m0 + (lane >> 2) + 8] = fs[1].inverse;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    const char* stage = ring.wait();
-    __syncthreads();  // planes of S and this chunk's v are there; the other slab is free
+    // planes of S and this chunk's v are there; the other slab is free
+    if (!__syncthreads_and(ring.wait())) return ring.give_up(a.chunks - c);
+    const char* stage = ring.stage();
     if (c + 1 < a.chunks)
       slab_fetch<T, VB>(m.slab[~c & 1], v + (c + 1) * kChunk * p.v_token, p.v_token, min(kChunk, a.len - (c + 1) * kChunk),
                         a.width, p.vec_v);

@@ -200,11 +200,7 @@ class BandedStencil:
 
     def check_faults(self) -> None:
         """Raise if a kernel on this device gave up a bounded wait (synchronises)."""
-        v = ctypes.c_uint(0)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.lib().pla_read_device_faults(ctypes.byref(v)), "pla_read_device_faults")
-        if v.value:
-            raise _lib.PlaError(f"device fault word {v.value:#x}: a bounded wait in a kernel timed out")
+        _lib.check_faults(self.device)
 
     def _global(self, peer: int) -> int:
         return peer if self.group is None else dist.get_global_rank(self.group, peer)

@@ -23,7 +23,9 @@ no gradient.
 Dtypes: float32, bfloat16, float16; sums, norms and delta-rule states are
 fp32.  Every call runs as ``torch.ops.pla_b200.*`` on the current stream and
 can be captured in a CUDA graph.  A CPU tensor raises: there is no fallback.
-A second derivative and a forward-mode one raise.
+A second derivative and a forward-mode one raise.  A kernel of the delta rule
+whose copies do not arrive within two seconds ends with its results incomplete
+(a single token's state unchanged); ``pla_b200.check_faults()`` raises then.
 """
 from __future__ import annotations
 

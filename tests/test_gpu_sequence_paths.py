@@ -198,3 +198,7 @@ def test_mixer_steps_any_number_of_sequences():
     for a, b in ((y[-40:], z), (state[0][-40:], part[0]), (state[1][-40:], part[1])):
         # matrix products of other shapes may sum in another order: a few roundings, as in a prompt and its steps
         assert float((a - b).norm() / b.norm()) <= 16 * half(BF16)
+
+
+def test_no_wait_ran_out():
+    P.check_faults(DEV)

@@ -9,6 +9,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import pla_b200 as P
+from pla_b200 import _lib
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -95,3 +96,34 @@ def test_mixer_step_refuses_a_state_before_it_changes_any():
         with pytest.raises((ValueError, RuntimeError)):
             m.step(x, (conv, bad))
         assert conv._version == version
+
+
+# ---- waits that run out ----------------------------------------------------------
+def test_check_faults_raises_for_a_set_word(monkeypatch):
+    class Library:
+        word, status = 0, 0
+
+        def pla_read_device_faults(self, to):
+            to._obj.value = self.word
+            return self.status
+
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+    real, fake = _lib.lib(), Library()
+    monkeypatch.setattr(_lib, "lib", lambda: fake)
+    P.check_faults()
+    fake.word = 1
+    with pytest.raises(_lib.PlaError, match="0x1"):
+        P.check_faults()
+    fake.word, fake.status = 0, 4
+    with pytest.raises(_lib.PlaError, match="pla_read_device_faults"):
+        P.check_faults()
+
+
+def test_no_wait_of_a_kernel_goes_unread():
+    """Every bounded wait's outcome is used, but those that only give copies in flight their time."""
+    text = "".join(open(p).read() for p in sorted(glob.glob(os.path.join(ROOT, "pla_b200", "csrc", "delta_*.cuh"))))
+    bare = [line.strip() for line in text.splitlines() if re.match(r"\s*(\w+\.)?(barrier_wait|wait)\(", line)]
+    drain = re.search(r"void drain\(.*?\n}", text, re.S).group(0)
+    assert all(line in drain for line in bare), bare
