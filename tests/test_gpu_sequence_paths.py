@@ -202,3 +202,144 @@ def test_mixer_steps_any_number_of_sequences():
 
 def test_no_wait_ran_out():
     P.check_faults(DEV)
+
+
+# ---- the kernels and loops that only large calls reach -----------------------
+# Compared as in tests/test_gpu_sequence.py, with its tolerances, which do not depend on sizes: sums over tokens there are
+# bounded relative to the sum of their terms' magnitudes.  The 64-bit forms run on the GPU.
+LONG_CONV = [  # batch, tokens, channels, taps, silu, bias, state, cu
+    (1, 1811, 8192, 4, True, True, True, [0, 5, 40, 41, 41, 300, 1000, 1800]),   # strips of 32 forward, 64 back
+    (2, 921, 4096, 3, True, False, True, None),                                  # strips of 16 (fp32: 32), 32 back
+    (1, 1795, 2049, 2, False, True, False, [0, 700, 1795]),                      # single channels a thread
+    (1, 4003, 96, 4, True, True, True, [min(4003, 2 * i - i // 3) for i in range(2402)]),  # thousands of sequences
+]
+
+
+def convolution(x, w, b, silu, cu, state):
+    """The definition, a sequence at a time; y and the states after."""
+    K, ys, last, at = w.shape[-1], [], [], 0
+    for n, (r, a, e) in enumerate(R.spans(x, cu)):
+        seen = torch.cat([x.new_zeros(K - 1, x.shape[-1]) if state is None else state[n], x[r, a:e]])
+        p = sum(w[:, j] * seen[j:j + e - a] for j in range(K))
+        p = p if b is None else p + b
+        ys.append(p * torch.sigmoid(p) if silu else p)
+        last.append(seen[e - a:])
+        at = e
+    y = torch.stack(ys) if cu is None else torch.cat(ys + [x.new_zeros(x.shape[1] - at, x.shape[-1])])[None]
+    return y, torch.stack(last)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("case", LONG_CONV, ids=lambda c: "x".join(map(str, c[:4])))
+def test_long_convolutions(case, dtype):
+    silu = case[4]
+    x, w, b, s, cu = S.conv_inputs(case, dtype, seed=161)
+    there = [i for i, t in enumerate((x, w, b, s)) if t is not None]
+    leaves = [f64(gpu(t), True) for t in (x, w, b, s)]
+    y, last = convolution(*leaves[:3], silu, cu, leaves[3])
+    gen = torch.Generator().manual_seed(162)
+    dy, dlast = rand(gen, *y.shape, dtype=dtype), rand(gen, *last.shape, dtype=dtype)
+    grads = torch.autograd.grad((y, last), [leaves[i] for i in there], (f64(gpu(dy)), f64(gpu(dlast))))
+    mine = [None if t is None else gpu(t).requires_grad_() for t in (x, w, b, s)]
+    out, state = P.causal_depthwise(*mine[:3], silu=silu, cu_seqlens=gpu(cu), state=mine[3], return_state=True)
+    got = torch.autograd.grad((out, state), [mine[i] for i in there], (gpu(dy), gpu(dlast)))
+    # magnitudes: every term positive, slopes at most 1.1
+    pos = [None if t is None else t.detach().abs().requires_grad_() for t in leaves]
+    py, pl = convolution(*pos[:3], False, cu, pos[3])
+    mags = torch.autograd.grad((py, pl), [pos[i] for i in there], (1.1 * f64(gpu(dy)).abs(), f64(gpu(dlast)).abs()))
+    # below 2^-14 an fp16 is a multiple of 2^-24, and its rounding off by up to 2^-25
+    step = 2 ** -25 if dtype == F16 else 0
+    S.within(out, y.detach().cpu(), (S.conv_bound(dtype, y.detach(), py.detach()) + step).cpu(), "y")
+    assert torch.equal(state.detach().double(), last.detach())  # copies
+    for i, a, want, mag in zip(there, got, grads, mags):
+        S.within(a, want.cpu(), (half(dtype) * want.abs() + 2 ** -15 * mag + step).cpu(), "x w b state".split()[i])
+
+
+LARGE_NORM = [  # B, T, Hq, Hk, D, rot, l2, weight, interleaved, position bytes
+    (1, 4801, 5, 3, 128, 64, False, True, False, 8),     # heads in fours (fp32 twos) and a partial last group of them
+    (1, 4801, 6, 3, 96, 96, False, True, True, 4),       # heads that do not fill their lanes
+    (2, 5003, 9, 2, 64, 0, True, False, False, 0),       # as a block of this library calls it
+    (3, 1601, 7, 1, 256, 128, False, True, False, 8),
+    (1, 3001, 6, 5, 250, 100, False, True, False, 8),    # single pairs a lane, a walk over tokens
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("case", LARGE_NORM, ids=lambda c: "x".join(map(str, c[:6])))
+def test_large_norms(case, dtype):
+    S.test_norm_forward_and_gradients(case, dtype)
+
+
+LARGE_DELTA = [  # n, T, Hk, Hv, Dk, Dv, state, cu, gates
+    (1, 200, 10, 20, 128, 128, True, None, F32),                       # 32 columns a block
+    (2, 150, 10, 20, 64, 128, True, None, None),                       # the same, two blocks an SM (16-bit types)
+    (4, 130, 4, 20, 40, 40, False, None, None),                        # a last block of 8 columns
+    (1, 300, 5, 20, 64, 100, True, [0, 70, 70, 150, 290], F32),        # a ragged batch, a last block of 4
+    (1, 260, 20, 20, 128, 128, False, [0, 3, 260], None),
+]
+MANY = [[min(2500, 2 * i - i // 3) for i in range(1301)], [min(4003, 2 * i - i // 3) for i in range(2402)]]
+
+
+def check_delta(case, dtype, with_state):
+    inputs = S.delta_inputs(case, dtype, seed=171)
+    cu = inputs[6]
+    there = [i for i, t in enumerate(inputs[:6]) if t is not None]
+    leaves = [f64(gpu(t), True) for t in inputs[:6]]
+    o, last = R.gated_delta_rule(*leaves[:5], cu=cu, state=leaves[5])
+    gen = torch.Generator().manual_seed(172)
+    d_o, ds = rand(gen, *o.shape, dtype=dtype), rand(gen, *last.shape, scale=0.5)
+    pick = slice(0, 2 if with_state else 1)
+    wants = torch.autograd.grad((o, last)[pick], [leaves[i] for i in there], (f64(gpu(d_o)), f64(gpu(ds)))[pick])
+    mine = [None if t is None else gpu(t).requires_grad_() for t in inputs[:6]]
+    out, state = P.gated_delta_rule(*mine[:5], cu_seqlens=gpu(cu), state=mine[5], return_state=True)
+    got = torch.autograd.grad((out, state)[pick], [mine[i] for i in there], (gpu(d_o), gpu(ds))[pick])
+    S.token_norms(out, o.detach().cpu(), half(dtype) + S.FORWARD[F32], "o")
+    S.token_norms(state, last.detach().cpu(), S.FORWARD[F32], "state")
+    for i, a, want in zip(there, got, wants):
+        name, tol = "q k v g beta state".split()[i], S.BACKWARD[F32]
+        if name in ("g", "beta"):  # relative to the largest of a head, as there
+            a, want, tol = a.transpose(1, 2), want.transpose(1, 2), 4 * tol
+        S.token_norms(a, want.cpu(), (half(a.dtype) if a.dtype != F32 else 0) + tol, "d" + name)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("case", LARGE_DELTA, ids=lambda c: "x".join(map(str, c[:6])))
+def test_delta_of_many_heads(case, dtype):
+    check_delta(case, dtype, True)
+    if case[8] is None:
+        check_delta(case, dtype, False)
+
+
+@pytest.mark.parametrize("cu", MANY, ids=lambda c: str(len(c) - 1))
+def test_delta_of_many_sequences(cu):
+    """More sequences than the plan's threads, and more than it orders by length."""
+    check_delta((1, cu[-1] + 9, 1, 2, 16, 16, True, cu, F32), BF16, True)
+
+
+def test_the_cases_above_reach_the_kernels_of_large_calls():
+    from torch.profiler import ProfilerActivity, profile
+
+    def forward_and_back(leaves, f):
+        leaves = [None if t is None else gpu(t).requires_grad_(t.is_floating_point()) for t in leaves]
+        y = f(*leaves)
+        y = y if isinstance(y, tuple) else (y,)
+        torch.autograd.grad(y, [t for t in leaves if t is not None and t.requires_grad], y)
+
+    with profile(activities=[ProfilerActivity.CUDA]) as run:
+        for case in LARGE_DELTA:
+            q, k, v, g, beta, _, cu = S.delta_inputs(case, BF16)
+            forward_and_back((q, k, v, g, beta), lambda *a: P.gated_delta_rule(*a, cu_seqlens=gpu(cu)))
+        for case, dtype in ((LARGE_NORM[0], BF16), (LARGE_NORM[0], F32), (LARGE_NORM[1], BF16), (LARGE_NORM[2], F16)):
+            q, k, wq, wk, cos, sin, pos = S.norm_inputs(case, dtype)
+            kw = dict(cos=gpu(cos), sin=gpu(sin), positions=gpu(pos), norm="l2" if case[6] else "rms", interleaved=case[8])
+            forward_and_back((q, k, wq, wk), lambda *a: P.qk_norm_rotate(*a, **kw))
+        torch.cuda.synchronize()
+    names = " ".join({e.key for e in run.key_averages()})
+    if "pla::" not in names:
+        pytest.skip("the profiler records no kernels here")
+    for name in ("delta_sweep<__nv_bfloat16, 128, 32, 2, 1, false>", "delta_sweep<__nv_bfloat16, 64, 32, 1, 2, false>",
+                 "delta_sweep<__nv_bfloat16, 64, 32, 3, 1, false>", "delta_sweep<__nv_bfloat16, 64, 32, 1, 2, true>",
+                 "delta_sweep_back<__nv_bfloat16, 128, 32, 2, 1>", "delta_sweep_back<__nv_bfloat16, 64, 32, 1, 2>",
+                 "qk_norm_forward4<__nv_bfloat16, 16, 4, false>", "qk_norm_forward4<float, 16, 2, false>",
+                 "qk_norm_forward4<__nv_bfloat16, 16, 4, true>", "qk_norm_forward4<__half, 8, 4, false>"):
+        assert name in names, name
