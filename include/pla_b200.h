@@ -413,7 +413,9 @@ PLA_API int pla_qk_norm_rotate_backward(const pla_qk_norm* a, void* workspace, s
  * tokens, hv], both of dtype or both fp32 (gates32); o dense like v;
  * state_out [sequences, hv, dk, dv] fp32 or NULL.  dk, dv <= 128, hv a
  * multiple of hk.  It is stable for |k| up to about 1 and beta in [0, 2]; a g
- * below -200 is taken as -200 (its decay is 0 in fp32 either way).
+ * below -200 is taken as -200 (its decay is 0 in fp32 either way).  Tokens are
+ * worked on in chunks of 64 from a sequence's start: a value that is not finite
+ * reaches its head's outputs (one of v: its feature's) from its chunk's start on.
  * workspace: pla_gated_delta_rule_workspace(a, 0) bytes, 256-byte aligned.
  */
 typedef struct pla_delta {

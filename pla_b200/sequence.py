@@ -96,7 +96,10 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     is ``Dk ** -0.5`` if None.  ``state`` is float32 [N, Hv, Dk, Dv] (zeros if
     None).  Dk and Dv are at most 128.  Keys are expected normalised
     (``qk_norm_rotate(..., norm="l2")``): the rule is stable for
-    ``beta * |k|^2 <= 2``.  Returns o, or (o, state after the sequences).
+    ``beta * |k|^2 <= 2``.  A value that is not finite reaches its sequence's
+    outputs from the start of its chunk of 64 tokens on, up to 63 tokens before
+    its own (one of v only its own feature); other sequences and heads never.
+    Returns o, or (o, state after the sequences).
     Differentiable in q, k, v, g, beta and state; the backward pass computes
     the states again and keeps only the inputs.
     """

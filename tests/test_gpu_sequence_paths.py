@@ -343,3 +343,27 @@ def test_the_cases_above_reach_the_kernels_of_large_calls():
                  "qk_norm_forward4<__nv_bfloat16, 16, 4, false>", "qk_norm_forward4<float, 16, 2, false>",
                  "qk_norm_forward4<__nv_bfloat16, 16, 4, true>", "qk_norm_forward4<__half, 8, 4, false>"):
         assert name in names, name
+
+
+# ---- values that are not finite ------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_delta_values_that_are_not_finite_stay_in_their_place(bad, dtype):
+    """They reach their sequence's outputs from the start of their chunk of 64 tokens on: of v its own feature, of k its
+    heads; nothing else."""
+    cu = torch.tensor([0, 10, 190, 200], dtype=torch.int32, device=DEV)
+    q, k, v, g, beta, _, _ = (gpu(t) for t in S.delta_inputs((1, 200, 2, 4, 64, 32, False, None, F32), dtype, seed=181))
+    clean, end = P.gated_delta_rule(q, k, v, g, beta, cu_seqlens=cu, return_state=True)
+    first = 10 + 64  # chunks of the middle sequence start at 10, 74 and 138
+    v2 = v.clone()
+    v2[0, 100, 1, 5] = bad
+    o, state = P.gated_delta_rule(q, k, v2, g, beta, cu_seqlens=cu, return_state=True)
+    assert not torch.isfinite(o[0, 100:190, 1, 5]).any() and not torch.isfinite(state[1, 1, :, 5]).all()
+    o[0, first:190, 1, 5], state[1, 1, :, 5] = clean[0, first:190, 1, 5], end[1, 1, :, 5]
+    assert torch.equal(o, clean) and torch.equal(state, end)
+    k2 = k.clone()
+    k2[0, 100, 1, 5] = bad
+    o, state = P.gated_delta_rule(q, k2, v, g, beta, cu_seqlens=cu, return_state=True)
+    assert not torch.isfinite(o[0, 100:190, 2:]).any()
+    o[0, first:190, 2:], state[1, 2:] = clean[0, first:190, 2:], end[1, 2:]
+    assert torch.equal(o, clean) and torch.equal(state, end)
