@@ -311,11 +311,12 @@ class DepthwiseBase:
     cpu_kind = "reference"
 
     def __init__(self, rank, world, dev):
-        from pla_b200.depthwise import depthwise7x7, depthwise_kxk
-
         self.dev = dev
         self.taps = self.k * self.k
-        self._fn = depthwise7x7 if self.k == 7 else depthwise_kxk
+        if dev is not None:  # (the reference arm's process loads nothing of the package)
+            from pla_b200.depthwise import depthwise7x7, depthwise_kxk
+
+            self._fn = depthwise7x7 if self.k == 7 else depthwise_kxk
         es = torch.tensor([], dtype=self.torch_dtype).element_size()
         self.items = []
         self.bytes = 0
@@ -603,8 +604,6 @@ class DwLnCfg4(DwCfg4):
 
     def __init__(self, rank, world, dev):
         super().__init__(rank, world, dev)
-        from pla_b200.depthwise import depthwise7x7_layernorm
-
         g = torch.Generator().manual_seed(3)
         es = torch.tensor([], dtype=self.torch_dtype).element_size()
         self.norm = []
@@ -618,6 +617,7 @@ class DwLnCfg4(DwCfg4):
         if dev is None:
             return
         from pla_b200 import _lib
+        from pla_b200.depthwise import depthwise7x7_layernorm
 
         self.dev_norm = [(g_.to(dev), b_.to(dev)) for (g_, b_) in self.norm]
         self._ln_fn = depthwise7x7_layernorm
@@ -716,13 +716,15 @@ class IterateCfg5:
     parity_steps = 2
 
     def __init__(self, rank, world, dev, H=32768):
-        from pla_b200.iterate import band_rows
-
         self.H = self.W = H
         self.name = f"iterate7x7_cfg5_{H}x{H}_f32_step"
         self.rank, self.world, self.dev = rank, world, dev
         g = torch.Generator().manual_seed(4)
-        self.r0, self.r1 = band_rows(H, world, rank)
+        self.r0, self.r1 = 0, H
+        if world > 1:  # (the reference arm's process loads nothing of the package)
+            from pla_b200.iterate import band_rows
+
+            self.r0, self.r1 = band_rows(H, world, rank)
         self.rows = self.r1 - self.r0
         # Grid rows [s0, s1) on the host: the band, its 3 halo rows and 3 more
         # on each side (a two-step parity check of an edge row reads 6 rows
