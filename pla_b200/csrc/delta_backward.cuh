@@ -218,7 +218,9 @@ __global__ void __launch_bounds__(VB * 8, PER_SM) delta_sweep_back(DeltaParams p
 // features at a time; 16 warps, each 16 tokens of a quarter of Dk (and of the
 // 64 x 64 matrices).  S0, D, U and dX come as the planes that the sweeps had as
 // operands; their row scales are brought to one by exact powers of two on the
-// way to shared memory, because here the value features are summed over.  The
+// way to shared memory, because here the value features are summed over (an
+// error of about 2^-27 of the head's largest: features far below it keep fewer
+// bits).  The
 // row and column sums over N . (Q K^T) and B . (K K^T) are taken as q . (N K),
 // k . (N^T Q) and so on, so neither Q K^T nor K K^T is needed.
 constexpr int kGradThreads = 512;

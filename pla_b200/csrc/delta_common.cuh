@@ -13,7 +13,7 @@
 // Products run on the tensor cores in fp16 with fp32 accumulators.  An fp32
 // operand is split into planes, hi = fp16(x f), lo = fp16(x f - hi), after
 // multiplying by a power of two f that brings its row's largest value near
-// 2^12: f is exact, nothing overflows whatever the inputs' range, and hi + lo
+// 2^12: f is exact, every finite value has a finite plane, and hi + lo
 // keep 22 bits of a value (values 2^-26 below the row's largest keep fewer,
 // with an error below 2^-38 of the largest).  16-bit inputs fit one plane: a
 // bfloat16 has 8 bits, so only values 2^-22 below the row's largest lose any.
@@ -21,7 +21,7 @@
 // need three of them for the same precision.  Results of 16-bit types are
 // computed like fp32 ones and rounded once.  One plane for what only a bf16
 // result sees takes less time (4096 tokens of 32 heads of 128, forward and
-// backward: 850 us, two planes 1230), but its error, up to 2^-12 of a token's
+// backward: 850 us, two planes 1250), but its error, up to 2^-12 of a token's
 // norm, comes on top of the rounding.
 #pragma once
 

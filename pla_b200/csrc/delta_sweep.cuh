@@ -15,7 +15,7 @@
 // memory as planes (one barrier a step).  One warp that kept all of S^T in
 // registers instead needed no barrier, but its 400 products and 1500 other
 // instructions a chunk took 8.6 us where this took 2.8 us (bf16, Dk = 128, one
-// plane for the outputs; 3.0 us with two).  A chunk's 144 products a warp are
+// plane for the outputs; 3.1 us with two).  A chunk's 144 products a warp are
 // 40 % of that; the rest is the wait for operands and barriers, which more warps
 // an SM or more products at a time do not shorten.
 //

@@ -18,7 +18,7 @@
 // together, the next token's while this one's are worked on, and share the
 // token's cosines and sines.  All arithmetic is fp32 with one rounding at the
 // end.  8192 tokens of 40 heads of 128 in bf16: 45 us, 3.7 TB/s, 57 % of the
-// copy rate; what holds it there is latency (16 warps an SM at 118 registers,
+// copy rate; what holds it there is latency (16 warps an SM at 126 registers,
 // half of the issue slots), not a pipe.  One token a group without the walk and
 // with 64-bit divisions took 68 us; three blocks an SM at 80 registers spill;
 // asynchronous copies through shared memory two tokens ahead leave three blocks

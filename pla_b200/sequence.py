@@ -78,7 +78,8 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     ``positions`` ([T], [1, T] or [B, T] integers; the token's number if
     None).  A position outside the tables gives NaN in the rotated features; a
     head whose squares overflow float32 (values above about 1e19) gives 0.
-    D is at most 256, B at most 65535.  Differentiable in q, k and the weights.
+    D is at most 256, B at most 65535 (for gradients B * T * heads at most
+    2^30).  Differentiable in q, k and the weights.
     """
     if norm not in ("rms", "l2"):
         raise ValueError('norm must be "rms" or "l2"')
