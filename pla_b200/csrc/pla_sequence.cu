@@ -151,8 +151,8 @@ bool causal_vector(const pla_causal* a, int vec, std::initializer_list<const voi
 
 // f(element type, V, K): 8 bytes of channels a thread (backward, which holds
 // five times as much: two channels), or single ones.
-template <typename F>
-int with_causal(int dtype, int taps, bool wide, bool backward, F&& f) {
+template <bool BACK, typename F>
+int with_causal(int dtype, int taps, bool wide, F&& f) {
   return with_type(dtype, [&](auto zero) {
     auto with_taps = [&](auto v) {
       switch (taps) {
@@ -161,9 +161,8 @@ int with_causal(int dtype, int taps, bool wide, bool backward, F&& f) {
         default: return f(zero, v, Int<4>{});
       }
     };
-    constexpr int W = 8 / sizeof(decltype(zero));
-    if (!wide) return with_taps(Int<1>{});
-    return backward ? with_taps(Int<2>{}) : with_taps(Int<W>{});
+    constexpr int W = BACK ? 2 : 8 / sizeof(decltype(zero));
+    return wide ? with_taps(Int<W>{}) : with_taps(Int<1>{});
   });
 }
 
@@ -486,7 +485,7 @@ int pla_causal_depthwise_forward(const pla_causal* a, pla_stream_t stream) {
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
   const bool wide = causal_vector(a, static_cast<int>(8 / es), {a->y, a->state_out});
-  return with_causal(a->dtype, a->taps, wide, false, [&](auto zero, auto v, auto k) {
+  return with_causal<false>(a->dtype, a->taps, wide, [&](auto zero, auto v, auto k) {
     using T = decltype(zero);
     constexpr int V = decltype(v)::value, K = decltype(k)::value;
     CausalParams p = causal_params(a);
@@ -538,7 +537,7 @@ int pla_causal_depthwise_backward(const pla_causal* a, const pla_causal_gradient
   int sms;
   if ((st = current_sm100(&sms)) != PLA_OK) return st;
   const bool wide = causal_vector(a, 2, {g->dy, g->dx, g->dstate_out}) && g->dy_batch % 2 == 0 && g->dy_token % 2 == 0;
-  return with_causal(a->dtype, a->taps, wide, true, [&](auto zero, auto v, auto k) {
+  return with_causal<true>(a->dtype, a->taps, wide, [&](auto zero, auto v, auto k) {
     using T = decltype(zero);
     constexpr int V = decltype(v)::value, K = decltype(k)::value;
     long long rows;
@@ -591,7 +590,7 @@ int pla_causal_depthwise_step(const void* x, int64_t x_row, void* state, int64_t
   const int vec = static_cast<int>(8 / es);
   const bool wide = channels % vec == 0 && x_row % vec == 0 && state_row % vec == 0 && aligned_to(x, 8) &&
                     aligned_to(state, 8) && aligned_to(y, 8) && aligned_to(w, 8) && aligned_to(b, 8);
-  return with_causal(dtype, taps, wide, false, [&](auto zero, auto v, auto k) {
+  return with_causal<false>(dtype, taps, wide, [&](auto zero, auto v, auto k) {
     using T = decltype(zero);
     constexpr int V = decltype(v)::value, K = decltype(k)::value;
     CausalParams p = {};
