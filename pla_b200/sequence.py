@@ -133,7 +133,8 @@ class DeltaMixer(torch.nn.Module):
     a ragged [1, T, dim] with ``cu_seqlens``); ``step`` takes [N, dim] and a
     state from ``new_state`` or ``forward(..., return_state=True)``, which it
     updates in place.  Under ``torch.autocast`` the operators run in its dtype,
-    and so do the convolution's states.
+    and so do the convolution's states.  ``head_dim`` and ``value_dim`` are at
+    most 128 (``step`` alone takes a ``head_dim`` of 256).
     """
 
     def __init__(self, dim: int, num_heads: int, head_dim: int = 128, value_heads: int | None = None,
