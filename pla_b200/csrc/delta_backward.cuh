@@ -236,7 +236,7 @@ struct GradShared {
       __half u[kPlanes][kGradBlock * kChunk], x[kPlanes][kGradBlock * kChunk];                    // U^T, dX^T
       __half o[kPlanes][kChunk * kGradBlock];                                                // do
     } in;
-    alignas(128) __half square[4][kPlanes][kChunk * kChunk];  // N f_k, N f_q (rows), Gamma dA f_k, B f_k (rows)
+    alignas(128) __half square[4][kPlanes][kChunk * kChunk];  // N f_k, N f_q (rows), Gamma dA f_k, B f_k (rows), all below the diagonal
   };
   alignas(16) float krow[kChunk];
   float qrow[kChunk], orow[kChunk];
@@ -245,6 +245,7 @@ struct GradShared {
   float dots[4][4][kChunk];    // quarters of Dk: k.r1, q.dq, k.(r3 + ..), k.Y
   float xv[8][kChunk];         // dX . v, groups of value features
   float warp_sum[16];
+  float diagonal[kChunk];      // of N
   unsigned int common[4], most[4];
 };
 
@@ -608,7 +609,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
         for (int e = 0; e < 4; ++e) {
           const int h = e >> 1, i = r0 + h * 8, j = j0 + (e & 1);
           const float gamma = exp_fast((row_hi[h] - (e & 1 ? hi.y : hi.x)) + (row_lo[h] - (e & 1 ? lo.y : lo.x)));
-          const float nn = j <= i ? gamma * (row_n[h] * a_p[n][e]) : 0.f, ga = j < i ? gamma * (to_a * a_a[n][e]) : 0.f;
+          if (i == j) s.diagonal[i] = row_n[h] * a_p[n][e];
+          const float nn = j < i ? gamma * (row_n[h] * a_p[n][e]) : 0.f, ga = j < i ? gamma * (to_a * a_a[n][e]) : 0.f;
           sq[0][n][e] = nn * (e & 1 ? kj.y : kj.x);
           sq[1][n][e] = nn * q_row[h];
           sq[2][n][e] = ga * (e & 1 ? kj.y : kj.x);
@@ -642,7 +644,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
         }
       }
     __syncthreads();
-    // dq += N K; dk += N^T Q + beta Y + B^T K, Y = (Gamma dA) K; all lower triangular
+    // dq += N K; dk += N^T Q + beta Y + B^T K, Y = (Gamma dA) K; all lower triangular.  N's diagonal gives q . dq and
+    // k . dk the same, which cancel in dG: it is added to dq and dk alone, so that no rest of a rounding stays
     {
       float b_q[NT][4] = {}, b_n[NT][4] = {}, b_y[NT][4] = {}, b_t[NT][4] = {};
       const uint32_t base = shared_u32(s.square);
@@ -696,8 +699,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
             dot[1][h] = fmaf(qv[e], two, dot[1][h]);
             dot[2][h] = fmaf(kv[e], three, dot[2][h]);
             dot[3][h] = fmaf(kv[e], y, dot[3][h]);
-            dq[n][at_e] += two;
-            dk[n][at_e] += fmaf(beta[h], y, three);
+            dq[n][at_e] += fmaf(s.diagonal[i], kv[e], two);
+            dk[n][at_e] += fmaf(beta[h], y, fmaf(s.diagonal[i], qv[e], three));
           }
         }
     }
@@ -717,7 +720,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_gradient(DeltaParams p)
     if (warp == 0) {  // the gates' gradients
       float dg[2], total = 0.f;
 #pragma unroll
-      for (int w = 0; w < 16; ++w) total += s.warp_sum[w];
+      for (int w = 0; w < 4; ++w)  // quarters of Dk as in the dots: a single token's H leaves nothing
+        total += (s.warp_sum[w] + s.warp_sum[4 + w]) + (s.warp_sum[8 + w] + s.warp_sum[12 + w]);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int t = 2 * lane + e;

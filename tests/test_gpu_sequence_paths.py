@@ -367,3 +367,22 @@ def test_delta_values_that_are_not_finite_stay_in_their_place(bad, dtype):
     assert not torch.isfinite(o[0, 100:190, 2:]).any()
     o[0, first:190, 2:], state[1, 2:] = clean[0, first:190, 2:], end[1, 2:]
     assert torch.equal(o, clean) and torch.equal(state, end)
+
+
+# ---- exact zeros ---------------------------------------------------------------
+@pytest.mark.parametrize("dtype,gates", [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 96), (33, 17)])
+def test_delta_decay_of_nothing_has_no_gradient(dtype, gates, dk, dv):
+    """A first token's decay acts on no state, or on one of zeros: dg is 0, not a rounding's rest."""
+    for n, T, cu, zeros in ((3, 1, None, False), (1, 5, [0, 1, 2, 3, 4, 5], False), (2, 1, None, True)):
+        case = (n, T, 2, 4, dk, dv, False, cu, gates)
+        q, k, v, g, beta, _, cu = (gpu(t) for t in S.delta_inputs(case, dtype, seed=191))
+        leaves = [t.requires_grad_() for t in (q, k, v, g, beta)]
+        state = torch.zeros(n, 4, dk, dv, device=DEV) if zeros else None
+        o, last = P.gated_delta_rule(*leaves, cu_seqlens=cu, state=state, return_state=True)
+        gen = torch.Generator().manual_seed(192)
+        d_o, ds = gpu(rand(gen, *o.shape, dtype=dtype)), gpu(rand(gen, *last.shape))
+        for outs, grads in (((o,), (d_o,)), ((o, last), (d_o, ds))):
+            got = torch.autograd.grad(outs, leaves, grads, retain_graph=True)
+            assert not got[3].any(), float(got[3].abs().max())
+            assert all(t.any() for t in (got[0], got[1], got[2], got[4]))
