@@ -400,7 +400,8 @@ typedef struct pla_qk_norm {
   int dtype;
 } pla_qk_norm;
 PLA_API int pla_qk_norm_rotate_forward(const pla_qk_norm* a, pla_stream_t stream);
-/* workspace: pla_qk_norm_rotate_workspace(a) bytes, needed when a dw is wanted. */
+/* workspace: pla_qk_norm_rotate_workspace(a) bytes, needed when a dw is wanted.
+ * batch x tokens x heads is at most 2^30 (forward: batch at most 65535). */
 PLA_API size_t pla_qk_norm_rotate_workspace(const pla_qk_norm* a);
 PLA_API int pla_qk_norm_rotate_backward(const pla_qk_norm* a, void* workspace, size_t workspace_bytes,
                                         pla_stream_t stream);

@@ -1,5 +1,5 @@
-"""Calls of the sequence operators that need no GPU to be judged: what is
-refused, what is laid out, what the sources promise."""
+"""The sequence operators without a GPU: tangents and states that are refused,
+the fault word, and what the kernels' sources have to keep."""
 import glob
 import os
 import re
